@@ -54,7 +54,17 @@ enum {
     QMM_Q8_0 = 8,  /* 34 B / 32:   f16 d, i8 qs[32]                          */
     QMM_Q4K = 12,  /* 144 B / 256: f16 d, f16 dmin, u8 scales[12], u8 qs[128] */
     QMM_Q6K = 14,  /* 210 B / 256: u8 ql[128], u8 qh[64], i8 scales[16], f16 d */
-    QMM_Q8K = 15   /* 292 B / 256: f32 d, i8 qs[256], i16 bsums[16] (activations only) */
+    QMM_Q8K = 15,  /* 292 B / 256: f32 d, i8 qs[256], i16 bsums[16] (activations only) */
+    QMM_MXFP4 = 39,    /* 17 B / 32: u8 e, u8 qs[16]: E2M1 codes times 2^(e - 127), values 0..15 in the
+                        * low nibbles, 16..31 in the high ones (OCP Microscaling MXFP4; GGUF's tag)   */
+    QMM_MXFP6X2 = 256  /* 49 B / 32: u8 e, u8 hi[24], u8 lo[24]: two E2M3 digits of 6 bits a value,
+                        * 2^(e - 127) (hi + lo / 16) (activations only; no GGUF tag)                  */
+};
+
+/* Expert scores (qmm_moe_route_scored, qmm_moe_ffn_scored). */
+enum {
+    QMM_SCORE_SOFTMAX = 0,
+    QMM_SCORE_SIGMOID = 1
 };
 
 typedef struct qmm_qtensor qmm_qtensor;
@@ -73,7 +83,7 @@ int qmm_init(int device);
 void qmm_reload_tuning(void);
 
 /* GGML geometry: elements per block, bytes per block, and the activation type a
- * weight type multiplies against (Q8_0 -> Q8_0, Q4K/Q6K -> Q8K). -1 if unknown.
+ * weight type multiplies against (Q8_0 -> Q8_0, Q4K/Q6K -> Q8K, MXFP4 -> MXFP6X2). -1 if unknown.
  * (GgmlDType::block_size / type_size / vec_dot_type.) */
 int qmm_block_size(int dtype);
 int qmm_type_size(int dtype);
@@ -91,6 +101,16 @@ int qmm_qtensor_from_ggml(int dtype, int64_t n, int64_t k, const void *bytes, in
  * equal those of candle's CPU from_float for the same input. */
 int qmm_qtensor_quantize(int dtype, int64_t n, int64_t k, const float *w, void *stream,
                          qmm_qtensor **out);
+
+/* qmm_qtensor_quantize of a weight of w_dtype QMM_F32, QMM_F16 or QMM_BF16 (MXFP4;
+ * the other types take f32 only). MXFP4: a block's scale is the smallest power of
+ * two at which its largest value does not round past the largest code (6), each
+ * code is rounded to nearest even; a block that holds an infinity or a NaN has the
+ * scale byte 255 and reads back as NaN. w starts on a boundary of four values. The
+ * reference has no such type: the format is the OCP Microscaling specification's,
+ * the block layout GGUF's. */
+int qmm_qtensor_quantize_from(int dtype, int64_t n, int64_t k, const void *w, int w_dtype, void *stream,
+                              qmm_qtensor **out);
 
 /* QTensor::dequantize: n*k f32 into the device buffer `dst`. */
 int qmm_qtensor_dequantize(const qmm_qtensor *t, float *dst, void *stream);
@@ -117,7 +137,12 @@ void qmm_qtensor_free(qmm_qtensor *t);
 /* VecDotType::from_float on the device (replaces launch_mmvq_gguf_quantize_q8_1_f32,
  * ffi.rs:412-419): x is f32 [m, k] with row stride ldx (elements); xq receives
  * m rows of k/block_size blocks of `vdtype` (QMM_Q8_0 or QMM_Q8K), GGML bytes,
- * contiguous. Bytes equal the CPU quantizer's for the same input. */
+ * contiguous. Bytes equal the CPU quantizer's for the same input. QMM_MXFP6X2 (what
+ * MXFP4 weights multiply): a block's scale is the smallest power of two at which its
+ * largest value does not round past 7.5 as one digit, at least 2^-123; hi is the
+ * value rounded to E2M3, lo 16 times what that left, rounded likewise (the error is at
+ * most 2^-9 of the block's largest value). A block that holds an infinity or a NaN has
+ * scale byte 255: its row's products are NaN. */
 int qmm_quantize_rows(int vdtype, const float *x, int64_t m, int64_t k, int64_t ldx, void *xq,
                       void *stream);
 
@@ -148,6 +173,15 @@ int qmm_matmul(const qmm_qtensor *w, const float *x, int64_t m, int64_t ldx, flo
 #define QMM_NOALLOC_SCRATCH_BYTES ((size_t)64 << 20)
 int qmm_matmul_noalloc(const qmm_qtensor *w, const float *x, int64_t m, int64_t ldx, float *y, int64_t ldy,
                        void *stream);
+
+/* QuantizedLinear::forward over typed rows (quant.rs:35-43) for MXFP4 weights:
+ * y = x . W^T (+ bias[n]), the sum rounded once to the output's type. x_dtype,
+ * bias_dtype and y_dtype are QMM_F32, QMM_F16 or QMM_BF16; bias may be NULL. Rows as
+ * for qmm_matmul (the same values, for f32 rows without a bias). ws:
+ * qmm_linear_workspace_size(w, m) bytes. */
+int qmm_linear(const qmm_qtensor *w, const void *x, int x_dtype, int64_t m, int64_t ldx, const void *bias,
+               int bias_dtype, void *y, int y_dtype, int64_t ldy, void *ws, size_t ws_bytes, void *stream);
+size_t qmm_linear_workspace_size(const qmm_qtensor *w, int64_t m);
 
 /* `count` (1..8) QMatMul::forward calls on one input in a single launch:
  * y[j] = x . W[j]^T for weights of one dtype and k (e.g. a layer's q/k/v and
@@ -417,6 +451,29 @@ int qmm_moe_route_ex(const float *logits, int64_t tokens, int experts, int topk,
                      float routed_scaling_factor, int32_t *counts, int32_t *offsets, int32_t *pair_token,
                      float *pair_weight, int32_t *token_pairs, void *stream);
 
+/* Routing with softmax or sigmoid scores, a balance bias, groups of experts and scaled
+ * weights; the same lists as qmm_moe_route. No counterpart in the reference (its
+ * MoeMlp::forward scores by softmax alone, llama.rs:1426-1451).
+ *   score  s = softmax(logits) (QMM_SCORE_SOFTMAX) or 1 / (1 + exp(-logit))
+ *          (QMM_SCORE_SIGMOID). A NaN logit counts as -inf (score 0), +inf as the
+ *          largest finite value; softmax scores without a logit above -inf are all 0.
+ *   choice c = s + bias (f32 [experts], or NULL), which selects and does not weigh.
+ *          A NaN sum comes last.
+ *   groups experts in `groups` runs of equal length; a group's score is the sum of its
+ *          group_top (1 or 2) largest choices; experts outside the topk_groups best
+ *          groups are not selected. Ties: the lower group.
+ *   top-k  the topk largest choices that remain. Ties: the lower expert.
+ *   weight s, divided by the selection's sum when `renormalize` (0 where that sum is 0),
+ *          times routed_scaling_factor.
+ * Scores are held in 64 bits, so close experts are ordered as the exact scores are.
+ * Limits: tokens <= 65536, experts <= 1024, topk <= min(32, experts), groups <= 64.
+ * ws: qmm_moe_route_scored_workspace_size(...) bytes (0: NULL allowed). */
+size_t qmm_moe_route_scored_workspace_size(int64_t tokens, int experts, int topk);
+int qmm_moe_route_scored(const float *logits, int64_t tokens, int experts, int topk, int score, const float *bias,
+                         int groups, int topk_groups, int group_top, int renormalize, float routed_scaling_factor,
+                         int32_t *counts, int32_t *offsets, int32_t *pair_token, float *pair_weight,
+                         int32_t *token_pairs, void *ws, size_t ws_bytes, void *stream);
+
 /* Expert-grouped GEMV (replaces moe_gemm_gguf, ffi.rs:25-39): w[j] (count 1..2)
  * are stacked expert weights [experts*N, K] of one dtype; xq holds `pairs`
  * rows of vec-dot blocks grouped by expert (counts/offsets as produced by
@@ -479,6 +536,24 @@ int qmm_moe_ffn_ex(const float *x, int64_t tokens, int64_t ldx, const float *log
                    const float *shared_gate_weight, float *out, int64_t ldo, void *ws, size_t ws_bytes,
                    void *stream);
 
+/* qmm_moe_ffn_ex with qmm_moe_route_scored's routing. With MXFP4 experts (all three
+ * weights) x and out are of x_dtype / out_dtype QMM_F32, QMM_F16 or QMM_BF16 (a shared
+ * expert in another type than MXFP4 takes f32 rows), topk <= 32, and the activated rows
+ * silu(gate(x)) * up(x) become MXFP6X2 digits without a rounding in between; other
+ * experts take f32 and qmm_moe_ffn's limits. ws:
+ * qmm_moe_ffn_scored_workspace_size(...) bytes. (qmm_moe_ffn and qmm_moe_ffn_ex take
+ * MXFP4 experts too, routed as score QMM_SCORE_SOFTMAX with one group.) */
+size_t qmm_moe_ffn_scored_workspace_size(const qmm_qtensor *gate, const qmm_qtensor *down, int64_t tokens,
+                                         int experts, int topk, const qmm_qtensor *shared_gate,
+                                         const qmm_qtensor *shared_up, const qmm_qtensor *shared_down);
+int qmm_moe_ffn_scored(const void *x, int x_dtype, int64_t tokens, int64_t ldx, const float *logits, int experts,
+                       int topk, int score, const float *bias, int groups, int topk_groups, int group_top,
+                       int norm_topk_prob, float routed_scaling_factor, const qmm_qtensor *gate,
+                       const qmm_qtensor *up, const qmm_qtensor *down, const qmm_qtensor *shared_gate,
+                       const qmm_qtensor *shared_up, const qmm_qtensor *shared_down,
+                       const float *shared_gate_weight, void *out, int out_dtype, int64_t ldo, void *ws,
+                       size_t ws_bytes, void *stream);
+
 /* ---------------------------------------------------------------------------
  * GGUF files (llama.cpp's single-file model container, spec v2/v3).
  * Replaces the reference's GgufFile (crates/llm/mlx-llm/src/gguf/reader.rs:
@@ -532,7 +607,7 @@ int qmm_gguf_meta_i64(const qmm_gguf *g, int64_t i, int64_t elem, int64_t *v);
 int qmm_gguf_meta_f64(const qmm_gguf *g, int64_t i, int64_t elem, double *v);
 int qmm_gguf_meta_string(const qmm_gguf *g, int64_t i, int64_t elem, const char **s, uint64_t *len);
 
-/* Resident load of a 2-D Q8_0 / Q4_K / Q6_K tensor into a device QTensor
+/* Resident load of a 2-D Q8_0 / Q4_K / Q6_K / MXFP4 tensor into a device QTensor
  * (QStorage::from_data + QTensor::new, candle-gen/src/quant/repack.rs:202-203),
  * on the current device, synchronous. unpermute_heads > 0 undoes llama.cpp's
  * q/k row order per head on the quantized rows (unpermute_qk, candle-llm

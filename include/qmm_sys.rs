@@ -29,6 +29,13 @@ pub const QMM_Q8_0: c_int = 8;
 pub const QMM_Q4K: c_int = 12;
 pub const QMM_Q6K: c_int = 14;
 pub const QMM_Q8K: c_int = 15;
+pub const QMM_MXFP4: c_int = 39;
+/// Activations only; not a GGUF tag.
+pub const QMM_MXFP6X2: c_int = 256;
+
+/// Expert scores (qmm_moe_route_scored, qmm_moe_ffn_scored).
+pub const QMM_SCORE_SOFTMAX: c_int = 0;
+pub const QMM_SCORE_SIGMOID: c_int = 1;
 
 /// Workspace bytes held per GPU by `qmm_matmul_noalloc`.
 pub const QMM_NOALLOC_SCRATCH_BYTES: usize = 64 << 20;
@@ -59,7 +66,7 @@ extern "C" {
     pub fn qmm_reload_tuning();
 
     /// GGML geometry: elements per block, bytes per block, and the activation type a
-    /// weight type multiplies against (Q8_0 -> Q8_0, Q4K/Q6K -> Q8K). -1 if unknown.
+    /// weight type multiplies against (Q8_0 -> Q8_0, Q4K/Q6K -> Q8K, MXFP4 -> MXFP6X2). -1 if unknown.
     /// (GgmlDType::block_size / type_size / vec_dot_type.)
     pub fn qmm_block_size(dtype: c_int) -> c_int;
 
@@ -81,6 +88,13 @@ extern "C" {
     /// equal those of candle's CPU from_float for the same input.
     pub fn qmm_qtensor_quantize(
         dtype: c_int, n: i64, k: i64, w: *const f32, stream: *mut c_void, out: *mut *mut QmmQTensor
+    ) -> c_int;
+
+    /// qmm_qtensor_quantize of a weight of w_dtype QMM_F32, QMM_F16 or QMM_BF16 (MXFP4; the other
+    /// types take f32 only). w starts on a boundary of four values.
+    pub fn qmm_qtensor_quantize_from(
+        dtype: c_int, n: i64, k: i64, w: *const c_void, w_dtype: c_int, stream: *mut c_void,
+        out: *mut *mut QmmQTensor
     ) -> c_int;
 
     /// QTensor::dequantize: n*k f32 into the device buffer `dst`.
@@ -138,6 +152,17 @@ extern "C" {
     pub fn qmm_matmul_noalloc(
         w: *const QmmQTensor, x: *const f32, m: i64, ldx: i64, y: *mut f32, ldy: i64, stream: *mut c_void
     ) -> c_int;
+
+    /// QuantizedLinear::forward over typed rows for MXFP4 weights: y = x . W^T (+ bias[n]), the sum
+    /// rounded once to the output's type; x_dtype, bias_dtype and y_dtype are QMM_F32, QMM_F16 or
+    /// QMM_BF16, bias may be NULL. ws: qmm_linear_workspace_size(w, m) bytes.
+    pub fn qmm_linear(
+        w: *const QmmQTensor, x: *const c_void, x_dtype: c_int, m: i64, ldx: i64, bias: *const c_void,
+        bias_dtype: c_int, y: *mut c_void, y_dtype: c_int, ldy: i64, ws: *mut c_void, ws_bytes: usize,
+        stream: *mut c_void
+    ) -> c_int;
+
+    pub fn qmm_linear_workspace_size(w: *const QmmQTensor, m: i64) -> usize;
 
     /// `count` (1..8) QMatMul::forward calls on one input in a single launch:
     /// y[j] = x . W[j]^T for weights of one dtype and k (e.g. a layer's q/k/v and
@@ -420,6 +445,19 @@ extern "C" {
         pair_weight: *mut f32, token_pairs: *mut i32, stream: *mut c_void
     ) -> c_int;
 
+    /// Routing with softmax or sigmoid scores (QMM_SCORE_*), a balance bias (f32 [experts] or NULL;
+    /// it selects and does not weigh), groups of experts and scaled weights; the same lists as
+    /// qmm_moe_route. Scores are held in 64 bits. Limits: tokens <= 65536, experts <= 1024,
+    /// topk <= min(32, experts), groups <= 64.
+    pub fn qmm_moe_route_scored_workspace_size(tokens: i64, experts: c_int, topk: c_int) -> usize;
+
+    pub fn qmm_moe_route_scored(
+        logits: *const f32, tokens: i64, experts: c_int, topk: c_int, score: c_int, bias: *const f32,
+        groups: c_int, topk_groups: c_int, group_top: c_int, renormalize: c_int, routed_scaling_factor: f32,
+        counts: *mut i32, offsets: *mut i32, pair_token: *mut i32, pair_weight: *mut f32,
+        token_pairs: *mut i32, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+
     /// Expert-grouped GEMV (replaces moe_gemm_gguf, ffi.rs:25-39): w[j] (count 1..2)
     /// are stacked expert weights [experts*N, K] of one dtype; xq holds `pairs`
     /// rows of vec-dot blocks grouped by expert (counts/offsets as produced by
@@ -482,6 +520,22 @@ extern "C" {
         down: *const QmmQTensor, shared_gate: *const QmmQTensor, shared_up: *const QmmQTensor,
         shared_down: *const QmmQTensor, shared_gate_weight: *const f32, out: *mut f32, ldo: i64,
         ws: *mut c_void, ws_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+
+    /// qmm_moe_ffn_ex with qmm_moe_route_scored's routing; MXFP4 experts take and give rows of
+    /// x_dtype / out_dtype QMM_F32, QMM_F16 or QMM_BF16, other experts f32.
+    pub fn qmm_moe_ffn_scored_workspace_size(
+        gate: *const QmmQTensor, down: *const QmmQTensor, tokens: i64, experts: c_int, topk: c_int,
+        shared_gate: *const QmmQTensor, shared_up: *const QmmQTensor, shared_down: *const QmmQTensor
+    ) -> usize;
+
+    pub fn qmm_moe_ffn_scored(
+        x: *const c_void, x_dtype: c_int, tokens: i64, ldx: i64, logits: *const f32, experts: c_int,
+        topk: c_int, score: c_int, bias: *const f32, groups: c_int, topk_groups: c_int, group_top: c_int,
+        norm_topk_prob: c_int, routed_scaling_factor: f32, gate: *const QmmQTensor, up: *const QmmQTensor,
+        down: *const QmmQTensor, shared_gate: *const QmmQTensor, shared_up: *const QmmQTensor,
+        shared_down: *const QmmQTensor, shared_gate_weight: *const f32, out: *mut c_void, out_dtype: c_int,
+        ldo: i64, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void
     ) -> c_int;
 
     /// Open a file (memory-mapped, read only) or an in-memory image (copied).

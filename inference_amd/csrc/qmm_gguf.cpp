@@ -66,6 +66,7 @@ bool type_block(int tag, uint64_t* be, uint64_t* bb) {
       {10, 256, 84}, {11, 256, 110}, {12, 256, 144}, {13, 256, 176}, {14, 256, 210},  // Q2_K..Q6_K
       {16, 256, 66}, {17, 256, 74},  {18, 256, 98},  {19, 256, 50},  {20, 32, 18},    // IQ2_XXS..IQ4_NL
       {21, 256, 110}, {22, 256, 82}, {23, 256, 136}, {29, 256, 56},                   // IQ3_S..IQ1_M
+      {39, 32, 17},                                 // MXFP4
   };
   for (const auto& t : table)
     if (t.tag == tag) {
@@ -472,7 +473,8 @@ int qmm_gguf_load_qtensor(const qmm_gguf* g, int64_t i, int unpermute_heads, voi
     case 8: dtype = QMM_Q8_0; break;
     case 12: dtype = QMM_Q4K; break;
     case 14: dtype = QMM_Q6K; break;
-    default: return fail(QMM_ERR_UNSUPPORTED, "gguf: tensor \"%s\" has type %d (resident loads take Q8_0, Q4_K, Q6_K)",
+    case 39: dtype = QMM_MXFP4; break;
+    default: return fail(QMM_ERR_UNSUPPORTED, "gguf: tensor \"%s\" has type %d (resident loads take Q8_0, Q4_K, Q6_K, MXFP4)",
                          t.name.c_str(), t.type);
   }
   if (t.ndims != 2) return fail(QMM_ERR_UNSUPPORTED, "gguf: tensor \"%s\" is %d-D (resident loads take 2-D weights)",

@@ -19,6 +19,7 @@
 
 extern "C" const unsigned char qmm_code_object_start[];
 extern "C" const unsigned char qmm_code_object_end[];
+extern "C" const unsigned char qmm_mx_code_object_start[];
 
 namespace {
 
@@ -77,7 +78,7 @@ struct KernelEntry {
 constexpr int kKernelSlots = 8192;  // > 4x the kernels of the code object
 
 struct Device {
-  hipModule_t module = nullptr;
+  hipModule_t module = nullptr, mx_module = nullptr;  // mx: kernels named qmm_mx_* and qmm_route_*
   std::atomic<const KernelEntry*> slots[kKernelSlots];
   int max_lds = 0;
   int num_cu = 0;
@@ -175,10 +176,18 @@ int current_device(Device** out) {
       return fail(QMM_ERR_NO_KERNEL, "hipModuleLoadData(gfx950 code object) on device %d: %s", dev,
                   hipGetErrorString(e));
     }
+    e = hipModuleLoadData(&d->mx_module, qmm_mx_code_object_start);
+    if (e != hipSuccess) {
+      (void)hipModuleUnload(d->module);
+      delete d;
+      return fail(QMM_ERR_NO_KERNEL, "hipModuleLoadData(second gfx950 code object) on device %d: %s", dev,
+                  hipGetErrorString(e));
+    }
     e = hipDeviceGetAttribute(&d->max_lds, hipDeviceAttributeMaxSharedMemoryPerBlock, dev);
     if (e == hipSuccess) e = hipDeviceGetAttribute(&d->num_cu, hipDeviceAttributeMultiprocessorCount, dev);
     if (e != hipSuccess) {
       (void)hipModuleUnload(d->module);
+      (void)hipModuleUnload(d->mx_module);
       delete d;
       return fail(QMM_ERR_HIP, "hipDeviceGetAttribute: %s", hipGetErrorString(e));
     }
@@ -217,7 +226,8 @@ int kernel(Device* d, const char* name, hipFunction_t* f) {
   }
   if (i == kKernelSlots) return fail(QMM_ERR_NO_KERNEL, "kernel table full looking up %s", name);
   hipFunction_t fn = nullptr;
-  hipError_t err = hipModuleGetFunction(&fn, d->module, name);
+  const bool mx = !strncmp(name, "qmm_mx_", 7) || !strncmp(name, "qmm_route_", 10);
+  hipError_t err = hipModuleGetFunction(&fn, mx ? d->mx_module : d->module, name);
   if (err != hipSuccess || !fn) {
     // The failed lookup also sets the runtime's last error; clear it so the
     // caller's next unrelated HIP call (e.g. a graph capture) does not report it.
@@ -249,6 +259,8 @@ struct qmm_qtensor {
   size_t bytes;  // == GGML bytes of the tensor
 };
 
+#include "qmm_mx_host.h"
+
 extern "C" {
 
 const char* qmm_last_error(void) { return g_err.c_str(); }
@@ -277,7 +289,7 @@ int qmm_init(int device) {
 
 int qmm_block_size(int dtype) {
   switch (dtype) {
-    case QMM_Q8_0: return 32;
+    case QMM_Q8_0: case QMM_MXFP4: case QMM_MXFP6X2: return 32;
     case QMM_Q4K: case QMM_Q6K: case QMM_Q8K: return 256;
     default: return -1;
   }
@@ -289,6 +301,8 @@ int qmm_type_size(int dtype) {
     case QMM_Q4K: return 144;
     case QMM_Q6K: return 210;
     case QMM_Q8K: return 292;
+    case QMM_MXFP4: return 17;
+    case QMM_MXFP6X2: return 49;
     default: return -1;
   }
 }
@@ -297,16 +311,21 @@ int qmm_vec_dot_type(int dtype) {
   switch (dtype) {
     case QMM_Q8_0: return QMM_Q8_0;
     case QMM_Q4K: case QMM_Q6K: return QMM_Q8K;
+    case QMM_MXFP4: return QMM_MXFP6X2;
     default: return -1;
   }
 }
 
 static int check_shape(int dtype, int64_t n, int64_t k) {
-  if (fmt_of(dtype) < 0) return fail(QMM_ERR_INVALID, "unsupported weight dtype %d", dtype);
+  if (fmt_of(dtype) < 0 && !is_mx(dtype)) return fail(QMM_ERR_INVALID, "unsupported weight dtype %d", dtype);
   const int bs = qmm_block_size(dtype);
   if (n <= 0 || k <= 0) return fail(QMM_ERR_INVALID, "empty shape (%lld, %lld)", (long long)n, (long long)k);
   if (k % bs) return fail(QMM_ERR_INVALID, "k = %lld is not a multiple of the block size %d", (long long)k, bs);
   if (n > (1LL << 31) - 1 || k > (1LL << 31) - 1) return fail(QMM_ERR_INVALID, "shape too large");
+  if (is_mx(dtype)) {
+    unsigned units;
+    QMM_TRY(mx_units(n, k, &units));
+  }
   return QMM_OK;
 }
 
@@ -317,7 +336,7 @@ static int alloc_tensor(int dtype, int64_t n, int64_t k, qmm_qtensor** out) {
   t->k = k;
   QMM_HIP(hipGetDevice(&t->device));
   t->bytes = (size_t)(n * (k / qmm_block_size(dtype))) * qmm_type_size(dtype);
-  hipError_t e = hipMalloc(&t->data, t->bytes);
+  hipError_t e = hipMalloc(&t->data, is_mx(dtype) ? mx_weight_bytes(n, k) : t->bytes);
   if (e != hipSuccess) {
     delete t;
     return fail(QMM_ERR_OOM, "hipMalloc(%zu): %s", t->bytes, hipGetErrorString(e));
@@ -329,6 +348,7 @@ static int alloc_tensor(int dtype, int64_t n, int64_t k, qmm_qtensor** out) {
 // Device GGML bytes -> the tensor's device layout.
 static int ggml_to_dev(Device* d, qmm_qtensor* t, const void* src, hipStream_t s) {
   const int fmt = fmt_of(t->dtype);
+  if (is_mx(t->dtype)) return mx_ggml(d, "qmm_mx_from_ggml", src, t->n, t->k, t->data, s);
   if (fmt == kFmtQ4K) {
     QMM_HIP(hipMemcpyAsync(t->data, src, t->bytes, hipMemcpyDeviceToDevice, s));
     return QMM_OK;
@@ -389,9 +409,31 @@ int qmm_qtensor_from_ggml(int dtype, int64_t n, int64_t k, const void* bytes, in
   return QMM_OK;
 }
 
+int qmm_qtensor_quantize_from(int dtype, int64_t n, int64_t k, const void* w, int w_dtype, void* stream,
+                              qmm_qtensor** out) {
+  if (!out || !w) return fail(QMM_ERR_INVALID, "null pointer");
+  *out = nullptr;
+  if (w_dtype == QMM_F32 && !is_mx(dtype)) return qmm_qtensor_quantize(dtype, n, k, (const float*)w, stream, out);
+  if (!is_mx(dtype)) return fail(QMM_ERR_UNSUPPORTED, "quantizing from another type than f32 needs MXFP4");
+  if (!mx_type_name(w_dtype)) return fail(QMM_ERR_INVALID, "quantize: input dtype %d (F32 = 0, F16 = 1, BF16 = 30)", w_dtype);
+  QMM_TRY(check_shape(dtype, n, k));
+  Device* d;
+  QMM_TRY(current_device(&d));
+  qmm_qtensor* t;
+  QMM_TRY(alloc_tensor(dtype, n, k, &t));
+  const int rc = mx_quantize_w(d, w, w_dtype, n, k, t->data, (hipStream_t)stream);
+  if (rc != QMM_OK) {
+    qmm_qtensor_free(t);
+    return rc;
+  }
+  *out = t;
+  return QMM_OK;
+}
+
 int qmm_qtensor_quantize(int dtype, int64_t n, int64_t k, const float* w, void* stream, qmm_qtensor** out) {
   if (!out || !w) return fail(QMM_ERR_INVALID, "null pointer");
   *out = nullptr;
+  if (is_mx(dtype)) return qmm_qtensor_quantize_from(dtype, n, k, w, QMM_F32, stream, out);
   QMM_TRY(check_shape(dtype, n, k));
   Device* d;
   QMM_TRY(current_device(&d));
@@ -431,6 +473,7 @@ int qmm_qtensor_dequantize_to(const qmm_qtensor* t, void* dst, int out_dtype, vo
   if (!name) return fail(QMM_ERR_INVALID, "dequantize: output dtype %d (F32 = 0, F16 = 1, BF16 = 30)", out_dtype);
   Device* d;
   QMM_TRY(current_device(&d));
+  if (is_mx(t->dtype)) return mx_dequantize(d, t->data, t->n, t->k, dst, out_dtype, (hipStream_t)stream);
   const int fmt = fmt_of(t->dtype);
   long long nblocks = t->n * (t->k / qmm_block_size(t->dtype));
   const void* a0 = t->data;
@@ -473,7 +516,8 @@ int qmm_qtensor_to_ggml(const qmm_qtensor* t, void* dst, int dst_on_device, void
   void* a1 = out;
   int f = fmt;
   void* args[] = {&a0, &a1, &nblocks, &f};
-  int rc = launch(d, "qmm_dev_to_ggml", ceil_div(nblocks, 256), 256, 0, s, args);
+  int rc = is_mx(t->dtype) ? mx_ggml(d, "qmm_mx_to_ggml", t->data, t->n, t->k, out, s)
+                           : launch(d, "qmm_dev_to_ggml", ceil_div(nblocks, 256), 256, 0, s, args);
   if (!dst_on_device) {
     if (rc == QMM_OK) {
       hipError_t e = hipMemcpyAsync(dst, out, t->bytes, hipMemcpyDeviceToHost, s);
@@ -511,7 +555,8 @@ void qmm_qtensor_free(qmm_qtensor* t) {
 
 int qmm_quantize_rows(int vdtype, const float* x, int64_t m, int64_t k, int64_t ldx, void* xq, void* stream) {
   if (!x || !xq) return fail(QMM_ERR_INVALID, "null pointer");
-  if (vdtype != QMM_Q8K && vdtype != QMM_Q8_0) return fail(QMM_ERR_INVALID, "vec-dot dtype %d is not Q8_0/Q8K", vdtype);
+  if (vdtype != QMM_Q8K && vdtype != QMM_Q8_0 && vdtype != QMM_MXFP6X2)
+    return fail(QMM_ERR_INVALID, "vec-dot dtype %d is not Q8_0/Q8K/MXFP6X2", vdtype);
   const int bs = qmm_block_size(vdtype);
   if (m <= 0 || k <= 0 || k % bs) return fail(QMM_ERR_INVALID, "bad activation shape (%lld, %lld) for block size %d", (long long)m, (long long)k, bs);
   if (ldx < k) return fail(QMM_ERR_INVALID, "row stride %lld < k %lld", (long long)ldx, (long long)k);
@@ -522,6 +567,12 @@ int qmm_quantize_rows(int vdtype, const float* x, int64_t m, int64_t k, int64_t 
   int kk = (int)k, mm = (int)m;
   void* args[] = {&x, &ld, &xq, &kk, &mm};
   const long long nblocks = m * (k / bs);
+  if (vdtype == QMM_MXFP6X2) {
+    QMM_TRY(mx_check_rows(m, k));
+    int wide = mx_wide(x, QMM_F32, ldx);
+    void* a[] = {&x, &ld, &mm, &kk, &wide, &xq};
+    return launch(d, "qmm_mx_quantize_rows", ceil_div(nblocks, 256), 256, 0, (hipStream_t)stream, a);
+  }
   if (vdtype == QMM_Q8K) return launch(d, "qmm_quantize_q8k", ceil_div(nblocks, 4), 256, 0, (hipStream_t)stream, args);
   return launch(d, "qmm_quantize_q8_0", ceil_div(nblocks * 8, 256), 256, 0, (hipStream_t)stream, args);
 }
@@ -550,6 +601,7 @@ static size_t gemm_split_bytes(const qmm_qtensor* w, int64_t m);
 
 size_t qmm_matmul_workspace_size(const qmm_qtensor* w, int64_t m) {
   if (!w || m <= 0) return 0;
+  if (is_mx(w->dtype)) return mx_planes(m, w->k).total;
   const int vt = qmm_vec_dot_type(w->dtype);
   const size_t ggml = (size_t)m * (size_t)(w->k / qmm_block_size(vt)) * qmm_type_size(vt);
   if (!use_gemm(w, m)) return ggml;
@@ -1111,7 +1163,9 @@ static int check_matmul(const qmm_qtensor* w, int64_t m, const float* y, int64_t
 }
 
 size_t qmm_matmul_q_workspace_size(const qmm_qtensor* w, int64_t m) {
-  if (!w || m <= 0 || !use_gemm(w, m)) return 0;
+  if (!w || m <= 0) return 0;
+  if (is_mx(w->dtype)) return mx_planes(m, w->k).total;
+  if (!use_gemm(w, m)) return 0;
   return mmq_planes(w->dtype, m, w->k).total + gemm_split_bytes(w, m);
 }
 
@@ -1130,10 +1184,39 @@ static int gemm_from_blocks(Device* d, const qmm_qtensor* w, const void* xq, int
   return gemm(d, w, b, m, y, ldy, dump, s, 0, (float*)(b + pb), ws_bytes - pb);
 }
 
+// One or more MXFP4 weights over rows of MXFP6X2 blocks: the blocks become digit
+// planes in the workspace, then a product per weight.
+static int mx_from_blocks(const GemvTarget* tg, int count, const void* xq, int64_t m, int accumulate, void* ws,
+                          size_t ws_bytes, hipStream_t s) {
+  const int64_t k = tg[0].w->k;
+  QMM_TRY(mx_check_rows(m, k));
+  const MxPlanes p = mx_planes(m, k);
+  if (!ws || ws_bytes < p.total)
+    return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed (qmm_matmul_q_workspace_size)", ws ? ws_bytes : 0, p.total);
+  Device* d;
+  QMM_TRY(current_device(&d));
+  uint8_t* b = (uint8_t*)ws;
+  int mm = (int)m, kk = (int)k, kc = (int)mx_chunks(k);
+  void *q = b + p.q, *sc = b + p.s;
+  void* args[] = {&xq, &mm, &kk, &kc, &q, &sc};
+  QMM_TRY(launch(d, "qmm_mx_blocks_to_planes", ceil_div(m * kc * 8, 256), 256, 0, s, args));
+  for (int j = 0; j < count; ++j) {
+    MxOut o = {};
+    o.y = tg[j].y;
+    o.accumulate = accumulate;
+    QMM_TRY(mx_product(d, tg[j].w, b, m, o, tg[j].ldy, s));
+  }
+  return QMM_OK;
+}
+
 int qmm_matmul_q(const qmm_qtensor* w, const void* xq, int64_t m, float* y, int64_t ldy, void* ws, size_t ws_bytes,
                  void* stream) {
   QMM_TRY(check_matmul(w, m, y, ldy));
   if (!xq) return fail(QMM_ERR_INVALID, "null activation");
+  if (is_mx(w->dtype)) {
+    const GemvTarget t = {w, y, ldy};
+    return mx_from_blocks(&t, 1, xq, m, 0, ws, ws_bytes, (hipStream_t)stream);
+  }
   Device* d;
   QMM_TRY(current_device(&d));
   const int vt = qmm_vec_dot_type(w->dtype);
@@ -1167,6 +1250,7 @@ int qmm_matmul_multi_q(const qmm_qtensor* const* w, int count, const void* xq, i
     if (!same_act(w[j], w[0])) return fail(QMM_ERR_INVALID, "weights of one launch must share k and dtype (or be Q4_K/Q6_K)");
     tg[j] = {w[j], y[j], ldy[j]};
   }
+  if (is_mx(w[0]->dtype)) return mx_from_blocks(tg, count, xq, m, 0, ws, ws_bytes, (hipStream_t)stream);
   if (m > 8) {  // the GEMM runs one weight at a time
     for (int j = 0; j < count; ++j) QMM_TRY(qmm_matmul_q(w[j], xq, m, y[j], ldy[j], ws, ws_bytes, stream));
     return QMM_OK;
@@ -1192,6 +1276,10 @@ int qmm_matmul_q_ex(const qmm_qtensor* w, const void* xq, int64_t m, float* y, i
   QMM_TRY(check_matmul(w, m, y, ldy));
   if (!xq) return fail(QMM_ERR_INVALID, "null activation");
   if (!accumulate) return qmm_matmul_q(w, xq, m, y, ldy, ws, ws_bytes, stream);
+  if (is_mx(w->dtype)) {
+    const GemvTarget t = {w, y, ldy};
+    return mx_from_blocks(&t, 1, xq, m, 1, ws, ws_bytes, (hipStream_t)stream);
+  }
   if (m > 8) return fail(QMM_ERR_UNSUPPORTED, "accumulating prequantized matmul is limited to m <= 8");
   Device* d;
   QMM_TRY(current_device(&d));
@@ -1347,6 +1435,32 @@ static int multi_launch(Device* d, const qmm_qtensor* const* w, const MultiPlan&
 }
 
 // Shared by qmm_matmul / qmm_matmul_multi: x f32 [m, k] against `count` weights.
+// One or more MXFP4 weights over typed rows: RMSNorm (f32 rows) if asked, the digit
+// planes in the workspace, then a product per weight.
+static int mx_targets(const GemvTarget* tg, int count, const void* x, int x_dtype, int64_t m, int64_t ldx, void* ws,
+                      size_t ws_bytes, const float* norm_w, float eps, const MxOut& how, hipStream_t s) {
+  const int64_t k = tg[0].w->k;
+  QMM_TRY(mx_check_rows(m, k));
+  const size_t planes = mx_planes(m, k).total, need = planes + (norm_w ? align256((size_t)(m * k) * 4) : 0);
+  if (!ws || ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
+  Device* d;
+  QMM_TRY(current_device(&d));
+  uint8_t* b = (uint8_t*)ws;
+  if (norm_w) {
+    float* xn = (float*)(b + planes);
+    QMM_TRY(qmm_rms_norm((const float*)x, m, k, ldx, norm_w, eps, xn, k, s));
+    x = xn;
+    ldx = k;
+  }
+  QMM_TRY(mx_quantize_x(d, x, x_dtype, m, k, ldx, b, s));
+  for (int j = 0; j < count; ++j) {
+    MxOut o = how;
+    o.y = tg[j].y;
+    QMM_TRY(mx_product(d, tg[j].w, b, m, o, tg[j].ldy, s));
+  }
+  return QMM_OK;
+}
+
 static int matmul_targets(const GemvTarget* tg, int count, const float* x, int64_t m, int64_t ldx, void* ws,
                           size_t ws_bytes, void* stream, const float* norm_w = nullptr, float eps = 0.0f,
                           int accumulate = 0) {
@@ -1356,6 +1470,11 @@ static int matmul_targets(const GemvTarget* tg, int count, const float* x, int64
   Device* d;
   QMM_TRY(current_device(&d));
   hipStream_t s = (hipStream_t)stream;
+  if (is_mx(w->dtype)) {
+    MxOut o = {};
+    o.accumulate = accumulate;
+    return mx_targets(tg, count, x, QMM_F32, m, ldx, ws, ws_bytes, norm_w, eps, o, s);
+  }
   if (m <= 2) {
     // one launch: the activation is (normalised and) quantized in the GEMV prologue
     return gemv(d, tg, count, x, true, ldx, (int)m, nullptr, s, norm_w, eps, accumulate);
@@ -1427,6 +1546,24 @@ int qmm_matmul(const qmm_qtensor* w, const float* x, int64_t m, int64_t ldx, flo
   QMM_TRY(check_matmul(w, m, y, ldy));
   GemvTarget t = {w, y, ldy};
   return matmul_targets(&t, 1, x, m, ldx, ws, ws_bytes, stream);
+}
+
+size_t qmm_linear_workspace_size(const qmm_qtensor* w, int64_t m) { return qmm_matmul_workspace_size(w, m); }
+
+int qmm_linear(const qmm_qtensor* w, const void* x, int x_dtype, int64_t m, int64_t ldx, const void* bias,
+               int bias_dtype, void* y, int y_dtype, int64_t ldy, void* ws, size_t ws_bytes, void* stream) {
+  QMM_TRY(check_matmul(w, m, (const float*)y, ldy));
+  if (!x) return fail(QMM_ERR_INVALID, "null activation");
+  if (!is_mx(w->dtype)) return fail(QMM_ERR_UNSUPPORTED, "linear: MXFP4 weights");
+  if (!mx_type_name(x_dtype) || !mx_type_name(y_dtype) || (bias && !mx_type_name(bias_dtype)))
+    return fail(QMM_ERR_INVALID, "linear: input, bias and output are F32 = 0, F16 = 1 or BF16 = 30");
+  if (ldx < w->k) return fail(QMM_ERR_INVALID, "row stride %lld < k %lld", (long long)ldx, (long long)w->k);
+  MxOut o = {};
+  o.bias = bias;
+  o.bias_type = bias_dtype;
+  o.y_type = y_dtype;
+  const GemvTarget t = {w, (float*)y, ldy};
+  return mx_targets(&t, 1, x, x_dtype, m, ldx, ws, ws_bytes, nullptr, 0.0f, o, (hipStream_t)stream);
 }
 
 int qmm_matmul_multi(const qmm_qtensor* const* w, int count, const float* x, int64_t m, int64_t ldx,
@@ -1567,7 +1704,7 @@ int qmm_matmul_ex(const qmm_qtensor* const* w, int count, const float* x, int64_
 size_t qmm_matmul_ex_workspace_size(const qmm_qtensor* w, int64_t m, int normalize) {
   if (!w || m <= 0) return 0;
   size_t b = qmm_matmul_workspace_size(w, m);
-  if (normalize && m > 2) b += align256((size_t)(m * w->k) * 4);
+  if (normalize && (m > 2 || is_mx(w->dtype))) b += align256((size_t)(m * w->k) * 4);
   return b;
 }
 
@@ -1614,8 +1751,12 @@ struct FfnWs {
 static int ffn_check(const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down, int64_t m) {
   if (!gate || !up || !down) return fail(QMM_ERR_INVALID, "null weight");
   if (m < 1) return fail(QMM_ERR_INVALID, "ffn needs m >= 1 (got %lld)", (long long)m);
-  if (qmm_vec_dot_type(gate->dtype) != QMM_Q8K || qmm_vec_dot_type(down->dtype) != QMM_Q8K || !same_act(gate, up))
-    return fail(QMM_ERR_UNSUPPORTED, "ffn needs Q4_K / Q6_K gate, up and down weights");
+  const bool mx = is_mx(gate->dtype) && is_mx(up->dtype) && is_mx(down->dtype) && same_act(gate, up);
+  if (mx) {
+    QMM_TRY(mx_check_rows(m, gate->k));
+    QMM_TRY(mx_check_rows(m, down->k));
+  } else if (qmm_vec_dot_type(gate->dtype) != QMM_Q8K || qmm_vec_dot_type(down->dtype) != QMM_Q8K || !same_act(gate, up))
+    return fail(QMM_ERR_UNSUPPORTED, "ffn needs Q4_K / Q6_K gate, up and down weights (or all MXFP4)");
   if (gate->n != up->n || down->k != gate->n)
     return fail(QMM_ERR_INVALID, "ffn shapes: gate %lldx%lld, up %lldx%lld, down %lldx%lld", (long long)gate->n,
                 (long long)gate->k, (long long)up->n, (long long)up->k, (long long)down->n, (long long)down->k);
@@ -1657,9 +1798,48 @@ static FfnWs ffn_ws(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, c
   return w;
 }
 
+// The MXFP4 block's workspace: digit planes of the rows and of the activated rows, the
+// normalised rows, gate's and up's outputs.
+struct MxFfnWs {
+  size_t xp, hp, xn, g, u, total;
+};
+static MxFfnWs mx_ffn_ws(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t m, bool normalize) {
+  MxFfnWs w;
+  w.xp = 0;
+  w.hp = mx_planes(m, gate->k).total;
+  w.xn = w.hp + mx_planes(m, down->k).total;
+  w.g = w.xn + (normalize ? align256((size_t)(m * gate->k) * 4) : 0);
+  w.u = w.g + align256((size_t)(m * gate->n) * 4);
+  w.total = w.u + align256((size_t)(m * gate->n) * 4);
+  return w;
+}
+
+static int mx_ffn(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down, const void* x,
+                  int x_dtype, int64_t m, int64_t ldx, const float* norm_w, float eps, int accumulate, float* y,
+                  int64_t ldy, uint8_t* b, hipStream_t s) {
+  const MxFfnWs L = mx_ffn_ws(gate, down, m, norm_w != nullptr);
+  if (norm_w) {
+    float* xn = (float*)(b + L.xn);
+    QMM_TRY(qmm_rms_norm((const float*)x, m, gate->k, ldx, norm_w, eps, xn, gate->k, s));
+    x = xn;
+    ldx = gate->k;
+  }
+  QMM_TRY(mx_quantize_x(d, x, x_dtype, m, gate->k, ldx, b + L.xp, s));
+  MxOut o = {};
+  o.y = b + L.g;
+  QMM_TRY(mx_product(d, gate, b + L.xp, m, o, gate->n, s));
+  o.y = b + L.u;
+  QMM_TRY(mx_product(d, up, b + L.xp, m, o, gate->n, s));
+  QMM_TRY(mx_silu_mul(d, (const float*)(b + L.g), (const float*)(b + L.u), m, gate->n, b + L.hp, s));
+  o.y = y;
+  o.accumulate = accumulate;
+  return mx_product(d, down, b + L.hp, m, o, ldy, s);
+}
+
 size_t qmm_ffn_workspace_size(const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down, int64_t m,
                               int normalize) {
   if (ffn_check(gate, up, down, m) != QMM_OK) return 0;
+  if (is_mx(gate->dtype)) return mx_ffn_ws(gate, down, m, normalize != 0).total;
   Device* d;
   if (current_device(&d) != QMM_OK) return 0;
   return ffn_ws(d, gate, up, down, m, normalize != 0).total;
@@ -1676,6 +1856,11 @@ int qmm_ffn(const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* d
   Device* d;
   QMM_TRY(current_device(&d));
   hipStream_t s = (hipStream_t)stream;
+  if (is_mx(gate->dtype)) {
+    const size_t need = mx_ffn_ws(gate, down, m, norm_weight != nullptr).total;
+    if (!ws || ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
+    return mx_ffn(d, gate, up, down, x, QMM_F32, m, ldx, norm_weight, eps, accumulate ? 1 : 0, y, ldy, (uint8_t*)ws, s);
+  }
   const FfnWs L = ffn_ws(d, gate, up, down, m, norm_weight != nullptr);
   if (!ws || ws_bytes < L.total) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws_bytes, L.total);
   uint8_t* b = (uint8_t*)ws;
@@ -2301,6 +2486,7 @@ int qmm_block_dots(const qmm_qtensor* w, const void* xq, int64_t m, float* y, in
                    size_t ws_bytes, void* stream) {
   QMM_TRY(check_matmul(w, m, y, ldy));
   if (!xq || !dots) return fail(QMM_ERR_INVALID, "null pointer");
+  if (is_mx(w->dtype)) return fail(QMM_ERR_UNSUPPORTED, "block dots: MXFP4 products have no integer block dots");
   Device* d;
   QMM_TRY(current_device(&d));
   if (m > 8) return gemm_from_blocks(d, w, xq, m, y, ldy, dots, ws, ws_bytes, (hipStream_t)stream);
@@ -2338,6 +2524,28 @@ int qmm_moe_route(const float* logits, int64_t tokens, int experts, int topk, in
                   int32_t* offsets, int32_t* pair_token, float* pair_weight, int32_t* token_pairs, void* stream) {
   return qmm_moe_route_ex(logits, tokens, experts, topk, renormalize, 1.0f, counts, offsets, pair_token, pair_weight,
                           token_pairs, stream);
+}
+
+size_t qmm_moe_route_scored_workspace_size(int64_t tokens, int experts, int topk) {
+  if (tokens < 1 || topk < 1 || experts < 1) return 0;
+  return route_scratch(tokens, experts, topk);
+}
+
+int qmm_moe_route_scored(const float* logits, int64_t tokens, int experts, int topk, int score, const float* bias,
+                         int groups, int topk_groups, int group_top, int renormalize, float routed_scaling_factor,
+                         int32_t* counts, int32_t* offsets, int32_t* pair_token, float* pair_weight,
+                         int32_t* token_pairs, void* ws, size_t ws_bytes, void* stream) {
+  if (!logits || !counts || !offsets || !pair_token || !pair_weight || !token_pairs)
+    return fail(QMM_ERR_INVALID, "null pointer");
+  const Routing r = {true, score, groups, topk_groups, group_top, bias, renormalize, routed_scaling_factor};
+  QMM_TRY(check_routing(tokens, experts, topk, r));
+  const size_t need = route_scratch(tokens, experts, topk);
+  if (need && (!ws || ws_bytes < need))
+    return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
+  Device* d;
+  QMM_TRY(current_device(&d));
+  return route_scored(d, logits, tokens, experts, topk, r, counts, offsets, pair_token, pair_weight, token_pairs,
+                      (uint8_t*)ws, (hipStream_t)stream);
 }
 
 // max_count bounds every counts[e] (the token count under top-k routing, else
@@ -2386,6 +2594,7 @@ static int moe_gemv(const qmm_qtensor* const* w, int count, int experts, const v
       return fail(QMM_ERR_INVALID, "stacked expert weights must share dtype and shape");
   }
   if (w[0]->n % experts) return fail(QMM_ERR_INVALID, "rows %lld not divisible by %d experts", (long long)w[0]->n, experts);
+  if (is_mx(w[0]->dtype)) return fail(QMM_ERR_UNSUPPORTED, "expert GEMV: MXFP4 experts run qmm_moe_gemm");
   Device* d;
   QMM_TRY(current_device(&d));
   const int fmt = fmt_of(w[0]->dtype);
@@ -2460,6 +2669,7 @@ int qmm_moe_gemv(const qmm_qtensor* const* w, int count, int experts, const void
 // M tiles (grid z = expert; tiles past an expert's rows exit at once).
 size_t qmm_moe_gemm_workspace_size(const qmm_qtensor* w, int64_t pairs) {
   if (!w || pairs < 1) return 0;
+  if (is_mx(w->dtype)) return mx_planes(pairs, w->k).total;
   return mmq_planes(w->dtype, pairs, w->k).total;
 }
 
@@ -2481,7 +2691,7 @@ int qmm_moe_gemm(const qmm_qtensor* const* w, int count, int experts, const floa
   }
   const qmm_qtensor* w0 = w[0];
   if (w0->n % experts) return fail(QMM_ERR_INVALID, "rows %lld not divisible by %d experts", (long long)w0->n, experts);
-  if (w0->k % 256) return fail(QMM_ERR_UNSUPPORTED, "grouped GEMM needs k %% 256 == 0 (k = %lld)", (long long)w0->k);
+  if (w0->k % 256 && !is_mx(w0->dtype)) return fail(QMM_ERR_UNSUPPORTED, "grouped GEMM needs k %% 256 == 0 (k = %lld)", (long long)w0->k);
   if (pairs < 1 || pairs > (1LL << 24) || ldx < w0->k)
     return fail(QMM_ERR_INVALID, "pairs must be 1..2^24 and ldx >= k");
   if (max_rows < 1 || max_rows > pairs) return fail(QMM_ERR_INVALID, "max_rows must be 1..pairs");
@@ -2491,6 +2701,11 @@ int qmm_moe_gemm(const qmm_qtensor* const* w, int count, int experts, const floa
   QMM_TRY(current_device(&d));
   hipStream_t s = (hipStream_t)stream;
   uint8_t* b = (uint8_t*)ws;
+  if (is_mx(w0->dtype)) {
+    QMM_TRY(mx_check_rows(pairs, w0->k));
+    QMM_TRY(mx_quantize_x(d, x, QMM_F32, pairs, w0->k, ldx, b, s));
+    return mx_expert_product(d, w, count, experts, b, pairs, pairs, max_rows, counts, offsets, nullptr, y, s);
+  }
   QMM_TRY(quantize_planes(d, w0->dtype, x, pairs, w0->k, ldx, b, s));
   return moe_gemm_planes(d, w, count, experts, b, pairs, max_rows, counts, offsets, y, s);
 }
@@ -2633,7 +2848,7 @@ static bool moe_grouped(int64_t pairs, int experts) {
 
 // Workspace of qmm_moe_ffn, carved in this order.
 struct MoeWs {
-  size_t counts, offsets, pair_token, pair_weight, token_pairs, xg, xq, g, u, h, hq, yp, planes;
+  size_t route, counts, offsets, pair_token, pair_weight, token_pairs, xg, xq, g, u, h, hq, yp, planes;
   size_t tails;  // grouped prefill: per expert the GEMM rows, the tail rows and the tails' first row
   size_t shared, sg, shared_ws, shared_ws_bytes;  // the shared expert (qmm_moe_ffn_ex)
   size_t total;
@@ -2645,7 +2860,7 @@ struct MoeShared {
   const float* gate_w = nullptr;  // f32 [hidden] or null (ungated)
 };
 static MoeWs moe_ws(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t T, int E, int k,
-                    const MoeShared* sh = nullptr) {
+                    const MoeShared* sh = nullptr, bool scored = false) {
   MoeWs w = {};
   const int64_t P = T * k, H = gate->k, F = gate->n / E;
   const int vg = qmm_vec_dot_type(gate->dtype), vd = qmm_vec_dot_type(down->dtype);
@@ -2669,6 +2884,7 @@ static MoeWs moe_ws(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t T,
   w.yp = take(4 * P * H);
   w.planes = take(std::max(mmq_planes(gate->dtype, P, H).total, mmq_planes(down->dtype, P, F).total));
   w.tails = take(4 * (3 * (size_t)E + 1));
+  if (scored) w.route = take(route_scratch(T, E, k));
   if (sh != nullptr && sh->gate != nullptr) {
     w.shared = take(4 * T * H);
     w.sg = take(4 * T);
@@ -2681,7 +2897,9 @@ static MoeWs moe_ws(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t T,
 
 static int check_moe(const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down, int E, int k) {
   if (!gate || !up || !down) return fail(QMM_ERR_INVALID, "null expert weight");
-  if (E < 1 || k < 1 || k > 8 || k > E) return fail(QMM_ERR_INVALID, "bad experts/topk %d/%d", E, k);
+  const bool mx = is_mx(gate->dtype);
+  if (E < 1 || k < 1 || k > (mx ? kRouteMaxTopk : 8) || k > E) return fail(QMM_ERR_INVALID, "bad experts/topk %d/%d", E, k);
+  if (mx != is_mx(down->dtype)) return fail(QMM_ERR_UNSUPPORTED, "experts with MXFP4 weights have all three in MXFP4");
   if (gate->dtype != up->dtype || gate->n != up->n || gate->k != up->k)
     return fail(QMM_ERR_INVALID, "gate and up must share dtype and shape");
   if (gate->n % E || down->n % E) return fail(QMM_ERR_INVALID, "stacked rows not divisible by %d experts", E);
@@ -2709,9 +2927,46 @@ static int check_moe_shared(const qmm_qtensor* gate, const MoeShared& sh) {
 // outputs are the whole list's.
 static int64_t moe_chunk(int topk) { return std::min<int64_t>(4096, 8192 / std::max(topk, 1)); }
 
+// MXFP4 experts: workspace of up to mx_moe_chunk(topk) tokens (longer lists run as
+// consecutive chunks: 32768 pairs are far more work than reading the weights again).
+struct MxMoeWs {
+  size_t counts, offsets, pair_token, pair_weight, token_pairs, route, xp, g, u, hp, yp;
+  size_t shared, sg, shared_ws, total;
+};
+static int64_t mx_moe_chunk(int topk) { return std::max<int64_t>(1, 32768 / std::max(topk, 1)); }
+static MxMoeWs mx_moe_ws(const qmm_qtensor* gate, int64_t tokens, int E, int k, const MoeShared& sh) {
+  MxMoeWs w = {};
+  const int64_t T = std::min(tokens, mx_moe_chunk(k)), P = T * k, H = gate->k, F = gate->n / E;
+  size_t o = 0;
+  auto take = [&o](size_t bytes) {
+    const size_t at = o;
+    o += align256(bytes);
+    return at;
+  };
+  w.counts = take(4 * (size_t)E);
+  w.offsets = take(4 * ((size_t)E + 1));
+  w.pair_token = take(4 * P);
+  w.pair_weight = take(4 * P);
+  w.token_pairs = take(4 * P);
+  w.route = take(route_scratch(T, E, k));
+  w.xp = take(mx_planes(T, H).total);
+  w.g = take(4 * (size_t)P * F);
+  w.u = take(4 * (size_t)P * F);
+  w.hp = take(mx_planes(P, F).total);
+  w.yp = take(4 * (size_t)P * H);
+  if (sh.gate) {
+    w.shared = take(4 * (size_t)T * H);
+    w.sg = take(4 * (size_t)T);
+    w.shared_ws = take(qmm_ffn_workspace_size(sh.gate, sh.up, sh.down, T, 0));
+  }
+  w.total = o;
+  return w;
+}
+
 size_t qmm_moe_ffn_workspace_size(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t tokens, int experts,
                                   int topk) {
   if (!gate || !down || tokens < 1 || experts < 1 || topk < 1) return 0;
+  if (is_mx(gate->dtype)) return mx_moe_ws(gate, tokens, experts, topk, MoeShared()).total;
   return moe_ws(gate, down, std::min(tokens, moe_chunk(topk)), experts, topk).total;
 }
 
@@ -2724,6 +2979,7 @@ size_t qmm_moe_ffn_ex_workspace_size(const qmm_qtensor* gate, const qmm_qtensor*
   sh.up = shared_up;
   sh.down = shared_down;
   if (check_moe_shared(gate, sh) != QMM_OK) return 0;
+  if (is_mx(gate->dtype)) return mx_moe_ws(gate, tokens, experts, topk, sh).total;
   return moe_ws(gate, down, std::min(tokens, moe_chunk(topk)), experts, topk, &sh).total;
 }
 
@@ -2775,25 +3031,113 @@ static int moe_gemv_path(Device* d, const MoeWs& L, uint8_t* b, const float* x, 
   return moe_gemv(dw, 1, experts, b + L.hq, P, T, counts, offsets, dy, stream);
 }
 
-static int moe_ffn(const float* x, int64_t tokens, int64_t ldx, const float* logits, int experts, int topk,
-                   int renormalize, float routed_scaling_factor, const qmm_qtensor* gate, const qmm_qtensor* up,
-                   const qmm_qtensor* down, const MoeShared& sh, float* out, int64_t ldo, void* ws, size_t ws_bytes,
-                   void* stream) {
+// The shared expert over a call's tokens into `out`, and its sigmoid gate into `sg`
+// (returned null without one).
+static int moe_shared(Device* d, const MoeShared& sh, const void* x, int x_dtype, int64_t tokens, int64_t ldx, int64_t H,
+                      float* out, float** sg, uint8_t* ws, size_t ws_bytes, hipStream_t s) {
+  if (x_dtype == QMM_F32)
+    QMM_TRY(qmm_ffn(sh.gate, sh.up, sh.down, (const float*)x, tokens, ldx, nullptr, 0.0f, 0, out, H, ws, ws_bytes, s));
+  else
+    QMM_TRY(mx_ffn(d, sh.gate, sh.up, sh.down, x, x_dtype, tokens, ldx, nullptr, 0.0f, 0, out, H, ws, s));
+  if (sh.gate_w == nullptr) {
+    *sg = nullptr;
+    return QMM_OK;
+  }
+  const float* gw = sh.gate_w;
+  long long lx = ldx;
+  int hh = (int)H, tt = (int)tokens, xt = x_dtype;
+  if (x_dtype == QMM_F32) {
+    void* args[] = {&x, &lx, &gw, &hh, &tt, sg};
+    return launch(d, "qmm_moe_shared_gate", ceil_div(tokens, 4), 256, 0, s, args);
+  }
+  void* args[] = {&x, &xt, &lx, &gw, &hh, &tt, sg};
+  return launch(d, "qmm_mx_shared_gate", ceil_div(tokens, 4), 256, 0, s, args);
+}
+
+// The expert FFN with MXFP4 weights: routing, the tokens' digit planes (once a token;
+// the products take routed rows by token), gate and up, silu(g) * u as planes, down,
+// the weighted sums.
+static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const float* logits, int experts, int topk,
+                  const Routing& r, const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down,
+                  const MoeShared& sh, void* out, int out_dtype, int64_t ldo, uint8_t* b, hipStream_t s) {
+  const int64_t H = gate->k, F = gate->n / experts, chunk = mx_moe_chunk(topk);
+  const MxMoeWs L = mx_moe_ws(gate, tokens, experts, topk, sh);
+  Device* d;
+  QMM_TRY(current_device(&d));
+  int32_t *counts = (int32_t*)(b + L.counts), *offsets = (int32_t*)(b + L.offsets);
+  int32_t *ptok = (int32_t*)(b + L.pair_token), *tpairs = (int32_t*)(b + L.token_pairs);
+  float *pw = (float*)(b + L.pair_weight), *g = (float*)(b + L.g), *u = (float*)(b + L.u), *yp = (float*)(b + L.yp);
+  for (int64_t t0 = 0; t0 < tokens; t0 += chunk) {
+    const int64_t T = std::min(chunk, tokens - t0), P = T * topk;
+    const uint8_t* xc = (const uint8_t*)x + t0 * ldx * (int64_t)mx_type_size(x_dtype);
+    QMM_TRY(route_scored(d, logits + t0 * experts, T, experts, topk, r, counts, offsets, ptok, pw, tpairs, b + L.route, s));
+    QMM_TRY(mx_quantize_x(d, xc, x_dtype, T, H, ldx, b + L.xp, s));
+    const qmm_qtensor* gw[2] = {gate, up};
+    float* gy[2] = {g, u};
+    QMM_TRY(mx_expert_product(d, gw, 2, experts, b + L.xp, T, P, T, counts, offsets, ptok, gy, s));
+    QMM_TRY(mx_silu_mul(d, g, u, P, F, b + L.hp, s));
+    QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, P, T, counts, offsets, nullptr, &yp, s));
+    float *shared = nullptr, *sg = nullptr;
+    if (sh.gate) {
+      shared = (float*)(b + L.shared);
+      sg = (float*)(b + L.sg);
+      QMM_TRY(moe_shared(d, sh, xc, x_dtype, T, ldx, H, shared, &sg, b + L.shared_ws,
+                         qmm_ffn_workspace_size(sh.gate, sh.up, sh.down, T, 0), s));
+    }
+    int tt = (int)T, k = topk, n = (int)H, ot = out_dtype;
+    void* oc = (uint8_t*)out + t0 * ldo * (int64_t)mx_type_size(out_dtype);
+    int wide = mx_wide(oc, out_dtype, ldo);
+    long long lo = ldo;
+    void* args[] = {&yp, &pw, &tpairs, &tt, &k, &n, &shared, &sg, &oc, &ot, &lo, &wide};
+    QMM_TRY(launch(d, "qmm_mx_combine", ceil_div(T * (H / 4), 256), 256, 0, s, args));
+  }
+  return QMM_OK;
+}
+
+static int moe_ffn(const void* xv, int x_dtype, int64_t tokens, int64_t ldx, const float* logits, int experts, int topk,
+                   const Routing& route, const qmm_qtensor* gate, const qmm_qtensor* up,
+                   const qmm_qtensor* down, const MoeShared& sh, void* outv, int out_dtype, int64_t ldo, void* ws,
+                   size_t ws_bytes, void* stream) {
   QMM_TRY(check_moe(gate, up, down, experts, topk));
   QMM_TRY(check_moe_shared(gate, sh));
-  if (!x || !logits || !out || !ws) return fail(QMM_ERR_INVALID, "null pointer");
+  if (!xv || !logits || !outv || !ws) return fail(QMM_ERR_INVALID, "null pointer");
   if (tokens < 1) return fail(QMM_ERR_INVALID, "tokens must be >= 1");
   if (ldx < gate->k || ldo < gate->k) return fail(QMM_ERR_INVALID, "row strides must be >= hidden size");
+  if (is_mx(gate->dtype)) {
+    if (!mx_type_name(x_dtype) || !mx_type_name(out_dtype))
+      return fail(QMM_ERR_INVALID, "moe: input and output are F32 = 0, F16 = 1 or BF16 = 30");
+    if (x_dtype != QMM_F32 && sh.gate && !is_mx(sh.gate->dtype))
+      return fail(QMM_ERR_UNSUPPORTED, "a shared expert in another type than MXFP4 takes f32 rows");
+    Routing r = route;
+    if (!r.scored && r.renormalize) r.scale = 1.0f;  // (qmm_moe_route_ex scales without renormalizing only)
+    const int64_t chunk = std::min(tokens, mx_moe_chunk(topk)), pairs = chunk * topk;
+    QMM_TRY(check_routing(chunk, experts, topk, r));
+    QMM_TRY(mx_check_rows(chunk, gate->k));
+    QMM_TRY(mx_check_rows(pairs, down->k));
+    const size_t need = mx_moe_ws(gate, tokens, experts, topk, sh).total;
+    if (ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws_bytes, need);
+    int dev = 0;
+    QMM_HIP(hipGetDevice(&dev));
+    if (dev != gate->device || dev != up->device || dev != down->device)
+      return fail(QMM_ERR_INVALID, "expert weights live on another device than the current one (%d)", dev);
+    return mx_moe(xv, x_dtype, tokens, ldx, logits, experts, topk, r, gate, up, down, sh, outv, out_dtype, ldo,
+                  (uint8_t*)ws, (hipStream_t)stream);
+  }
+  if (x_dtype != QMM_F32 || out_dtype != QMM_F32)
+    return fail(QMM_ERR_UNSUPPORTED, "f16 / bf16 rows need experts with MXFP4 weights");
+  const float* x = (const float*)xv;
+  float* out = (float*)outv;
+  const int renormalize = route.renormalize;
+  const float routed_scaling_factor = route.scale;
   const int64_t chunk = moe_chunk(topk);
   if (tokens > chunk) {  // consecutive chunks through the same workspace, in stream order
     for (int64_t t0 = 0; t0 < tokens; t0 += chunk)
-      QMM_TRY(moe_ffn(x + t0 * ldx, std::min(chunk, tokens - t0), ldx, logits + t0 * experts, experts, topk,
-                      renormalize, routed_scaling_factor, gate, up, down, sh, out + t0 * ldo, ldo, ws, ws_bytes,
-                      stream));
+      QMM_TRY(moe_ffn(x + t0 * ldx, QMM_F32, std::min(chunk, tokens - t0), ldx, logits + t0 * experts, experts, topk,
+                      route, gate, up, down, sh, out + t0 * ldo, QMM_F32, ldo, ws, ws_bytes, stream));
     return QMM_OK;
   }
   const int64_t H = gate->k, F = gate->n / experts, P = tokens * topk;
-  const MoeWs L = moe_ws(gate, down, tokens, experts, topk, &sh);
+  const MoeWs L = moe_ws(gate, down, tokens, experts, topk, &sh, route.scored);
   if (ws_bytes < L.total) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws_bytes, L.total);
   Device* d;
   QMM_TRY(current_device(&d));
@@ -2807,7 +3151,7 @@ static int moe_ffn(const float* x, int64_t tokens, int64_t ldx, const float* log
   const bool grouped = moe_grouped(P, experts) && H % 256 == 0 && F % 256 == 0;
   // decode-sized calls with Q8_K activations: routing and the Q8_K gather of the routed rows in one launch
   // (every workgroup routes the tokens itself; the same lists as qmm_moe_route's)
-  const bool fused_route = !grouped && qmm_vec_dot_type(gate->dtype) == QMM_Q8K && P <= 256;
+  const bool fused_route = !route.scored && !grouped && qmm_vec_dot_type(gate->dtype) == QMM_Q8K && P <= 256;
   if (fused_route) {
     QMM_TRY(route_check(tokens, experts, topk, routed_scaling_factor));
     int T = (int)tokens, E = experts, k = topk, rn = renormalize ? 1 : 0, hh = (int)H;
@@ -2816,6 +3160,9 @@ static int moe_ffn(const float* x, int64_t tokens, int64_t ldx, const float* log
     void* xq = b + L.xq;
     void* args[] = {&logits, &T, &E, &k, &rn, &ps, &counts, &offsets, &ptok, &pw, &tpairs, &x, &lx, &xq, &hh};
     QMM_TRY(launch(d, "qmm_moe_route_gather_q8k", ceil_div(P * (H / 256), 4), 256, 0, s, args));
+  } else if (route.scored) {
+    QMM_TRY(check_routing(tokens, experts, topk, route));
+    QMM_TRY(route_scored(d, logits, tokens, experts, topk, route, counts, offsets, ptok, pw, tpairs, b + L.route, s));
   } else {
     QMM_TRY(qmm_moe_route_ex(logits, tokens, experts, topk, renormalize, routed_scaling_factor, counts, offsets, ptok,
                              pw, tpairs, stream));
@@ -2929,16 +3276,8 @@ static int moe_ffn(const float* x, int64_t tokens, int64_t ldx, const float* log
   float* sg = nullptr;
   if (sh.gate != nullptr) {
     shared = (float*)(b + L.shared);
-    QMM_TRY(qmm_ffn(sh.gate, sh.up, sh.down, x, tokens, ldx, nullptr, 0.0f, 0, shared, H, b + L.shared_ws,
-                    L.shared_ws_bytes, stream));
-    if (sh.gate_w != nullptr) {
-      sg = (float*)(b + L.sg);
-      const float* gw = sh.gate_w;
-      long long lx = ldx;
-      int hh = (int)H, tt = (int)tokens;
-      void* args[] = {&x, &lx, &gw, &hh, &tt, &sg};
-      QMM_TRY(launch(d, "qmm_moe_shared_gate", ceil_div(tokens, 4), 256, 0, s, args));
-    }
+    sg = (float*)(b + L.sg);
+    QMM_TRY(moe_shared(d, sh, x, QMM_F32, tokens, ldx, H, shared, &sg, b + L.shared_ws, L.shared_ws_bytes, s));
   }
   {
     int T = (int)tokens, k = topk, N = (int)H, lo = (int)ldo;
@@ -2951,8 +3290,8 @@ static int moe_ffn(const float* x, int64_t tokens, int64_t ldx, const float* log
 int qmm_moe_ffn(const float* x, int64_t tokens, int64_t ldx, const float* logits, int experts, int topk,
                 const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down, float* out, int64_t ldo,
                 void* ws, size_t ws_bytes, void* stream) {
-  return moe_ffn(x, tokens, ldx, logits, experts, topk, 1, 1.0f, gate, up, down, MoeShared(), out, ldo, ws, ws_bytes,
-                 stream);
+  return moe_ffn(x, QMM_F32, tokens, ldx, logits, experts, topk, Routing(), gate, up, down, MoeShared(), out, QMM_F32, ldo,
+                 ws, ws_bytes, stream);
 }
 
 int qmm_moe_ffn_ex(const float* x, int64_t tokens, int64_t ldx, const float* logits, int experts, int topk,
@@ -2960,13 +3299,34 @@ int qmm_moe_ffn_ex(const float* x, int64_t tokens, int64_t ldx, const float* log
                    const qmm_qtensor* down, const qmm_qtensor* shared_gate, const qmm_qtensor* shared_up,
                    const qmm_qtensor* shared_down, const float* shared_gate_weight, float* out, int64_t ldo, void* ws,
                    size_t ws_bytes, void* stream) {
-  MoeShared sh;
-  sh.gate = shared_gate;
-  sh.up = shared_up;
-  sh.down = shared_down;
-  sh.gate_w = shared_gate_weight;
-  return moe_ffn(x, tokens, ldx, logits, experts, topk, norm_topk_prob, routed_scaling_factor, gate, up, down, sh, out,
-                 ldo, ws, ws_bytes, stream);
+  const MoeShared sh = {shared_gate, shared_up, shared_down, shared_gate_weight};
+  Routing r;
+  r.renormalize = norm_topk_prob;
+  r.scale = routed_scaling_factor;
+  return moe_ffn(x, QMM_F32, tokens, ldx, logits, experts, topk, r, gate, up, down, sh, out, QMM_F32, ldo, ws, ws_bytes,
+                 stream);
+}
+
+size_t qmm_moe_ffn_scored_workspace_size(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t tokens, int experts,
+                                         int topk, const qmm_qtensor* shared_gate, const qmm_qtensor* shared_up,
+                                         const qmm_qtensor* shared_down) {
+  if (!gate || !down || tokens < 1 || experts < 1 || topk < 1) return 0;
+  const MoeShared sh = {shared_gate, shared_up, shared_down, nullptr};
+  if (check_moe_shared(gate, sh) != QMM_OK) return 0;
+  if (is_mx(gate->dtype)) return mx_moe_ws(gate, tokens, experts, topk, sh).total;
+  return moe_ws(gate, down, std::min(tokens, moe_chunk(topk)), experts, topk, &sh, true).total;
+}
+
+int qmm_moe_ffn_scored(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const float* logits, int experts,
+                       int topk, int score, const float* bias, int groups, int topk_groups, int group_top,
+                       int norm_topk_prob, float routed_scaling_factor, const qmm_qtensor* gate, const qmm_qtensor* up,
+                       const qmm_qtensor* down, const qmm_qtensor* shared_gate, const qmm_qtensor* shared_up,
+                       const qmm_qtensor* shared_down, const float* shared_gate_weight, void* out, int out_dtype,
+                       int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
+  const MoeShared sh = {shared_gate, shared_up, shared_down, shared_gate_weight};
+  const Routing r = {true, score, groups, topk_groups, group_top, bias, norm_topk_prob, routed_scaling_factor};
+  return moe_ffn(x, x_dtype, tokens, ldx, logits, experts, topk, r, gate, up, down, sh, out, out_dtype, ldo, ws, ws_bytes,
+                 stream);
 }
 
 }  // extern "C"

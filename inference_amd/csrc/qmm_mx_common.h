@@ -1,0 +1,126 @@
+// Microscaled values: blocks of 32 that share a power-of-two scale byte e
+// (E8M0: 2^(e - 127); 255 marks a block that is not a number).
+//
+//   MXFP4    weights: E2M1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign).
+//   MXFP6x2  activations: two E2M3 digits a value, x = 2^(e - 127) (hi + lo / 16).
+//            E2M3 is sign, two exponent bits, three mantissa bits: steps of 1/8 up
+//            to 2, 1/4 up to 4, 1/2 up to 7.5. The second digit leaves an error of
+//            at most 2^-7 at a block maximum of 3.875 .. 7.75, 2^-9 of the maximum
+//            or less (normal values: 1.1e-3 of their norm; one E4M3 or E2M3 digit
+//            leaves 2.6e-2).
+//
+// Why two six-bit digits. The scaled matrix instruction multiplies either format at
+// the four-bit rate (32x32x64: 8.4 PFLOP/s measured, against 4.7 with an 8-bit
+// operand and 2.3 nominal in bf16), applies the scales of both operands itself,
+// and sums f6 x f4 products exactly (64-bit check, K up to 4096: no difference
+// while the blocks' scales lie within a few binades, 1.5e-7 of the absolute sum
+// with scales over 2^24). With an E4M3 operand its sum loses bits below 2^-13 of
+// the largest product: 4.9e-6 relative on normal data. So one product is two
+// instructions, at 4.2 PFLOP/s, with an error of the activation's rounding only.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace qmm {
+
+// Device layout of an MXFP4 weight [n, k]: units of 32 rows x 256 columns, row
+// tiles outermost (n and k padded with zero codes to whole units). In a unit, step
+// s (64 columns) holds 64 lanes x 16 bytes, lane 32 h + r the codes of row r, block
+// 2 s + h, two values a byte in order: the matrix instruction's operand as it is
+// loaded, 1 KB contiguous a step. Then 64 lanes x 4 scale bytes, byte s the scale of
+// block 2 s + h: one register serves four steps (the instruction selects the byte).
+constexpr int kMxTile = 32;
+constexpr int kMxChunk = 256;
+constexpr int kMxStepBytes = 1024;
+constexpr int kMxScaleOff = 4096;
+constexpr int kMxUnit = 4352;
+// Digit planes of activation rows: per row and chunk 8 blocks x (24 bytes of hi,
+// 24 of lo), and apart from them 8 scale bytes, [h][s] for block 2 s + h.
+constexpr int kMxDigitBlock = 48;
+constexpr int kMxDigitChunk = 8 * kMxDigitBlock;
+constexpr int kMxFp4Bytes = 17;   // GGML block: e, codes 0..15 in low nibbles, 16..31 in high ones
+constexpr int kMxFp6x2Bytes = 49; // block of qmm_quantize_rows: e, hi[24], lo[24]
+constexpr int kMxNan = 255;
+
+typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
+typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
+typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned mx_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned mx_u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned mx_u32x6 __attribute__((ext_vector_type(6)));
+
+// Element types of typed rows: the C ABI's tags.
+constexpr int kF32 = 0, kF16 = 1, kBF16 = 30;
+
+__device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
+// round to nearest even; a NaN stays one
+__device__ __forceinline__ uint16_t f32_to_bf16(float f) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, f);
+  return f != f ? (uint16_t)(u >> 16 | 64) : (uint16_t)((u + 0x7fff + (u >> 16 & 1)) >> 16);
+}
+__device__ __forceinline__ float mx_load(const void* p, int type, long long i) {
+  if (type == kF32) return static_cast<const float*>(p)[i];
+  const uint16_t v = static_cast<const uint16_t*>(p)[i];
+  return type == kF16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_to_f32(v);
+}
+__device__ __forceinline__ uint16_t mx_to16(float v, int type) {
+  return type == kF16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : f32_to_bf16(v);
+}
+__device__ __forceinline__ void mx_store(void* p, int type, long long i, float v) {
+  if (type == kF32) static_cast<float*>(p)[i] = v;
+  else static_cast<uint16_t*>(p)[i] = mx_to16(v, type);
+}
+
+// The scale byte of a block with the largest magnitude amax (as bits, sign clear):
+// the smallest power of two at which amax does not round past the largest code, at
+// least `least`. MAN: the mantissa from which it would (E2M1: 1.75, 7 -> 8; E2M3:
+// 1.9375, 7.75 -> 8). An infinity or NaN gives 255.
+template <uint32_t MAN>
+__device__ __forceinline__ int mx_scale_byte(uint32_t amax, int least) {
+  if (amax >= 0x7f800000u) return kMxNan;
+  const int e = (int)(amax >> 23) - 2 + ((amax & 0x7fffffu) >= MAN ? 1 : 0);
+  return max(e, least);
+}
+constexpr uint32_t kMxMan4 = 0x600000;  // .75
+constexpr uint32_t kMxMan6 = 0x780000;  // .9375
+
+__device__ __forceinline__ int mx_w_byte(uint32_t amax) { return amax == 0 ? 0 : mx_scale_byte<kMxMan4>(amax, 0); }
+// (the second digit's scale is four binades lower)
+__device__ __forceinline__ int mx_x_byte(uint32_t amax) { return mx_scale_byte<kMxMan6>(amax, 4); }
+
+// Both digits of 32 values under scale byte e as 24 + 24 bytes. A block with e = 255
+// gets zero digits (0 * NaN is NaN in the product).
+__device__ __forceinline__ void mx_digits(const float (&x)[32], int e, mx_u32x6& hi, mx_u32x6& lo) {
+  mx_f32x16 a, b;
+  const int up = 127 - e;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {  // the conversion takes even values from one operand, odd ones from the other
+    a[j] = e == kMxNan ? 0.0f : __builtin_ldexpf(x[2 * j], up);
+    b[j] = e == kMxNan ? 0.0f : __builtin_ldexpf(x[2 * j + 1], up);
+  }
+  hi = __builtin_bit_cast(mx_u32x6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 1.0f));
+  typedef float f32x32 __attribute__((ext_vector_type(32)));
+  const f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(hi, 1.0f);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    a[j] = (a[j] - back[2 * j]) * 16.0f;
+    b[j] = (b[j] - back[2 * j + 1]) * 16.0f;
+  }
+  lo = __builtin_bit_cast(mx_u32x6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 1.0f));
+}
+
+// One step (64 columns) of a 32 x 32 tile: weights (A, rows of the result) times
+// both digits of the activations (B, columns). S: the byte of the scale registers.
+template <int S>
+__device__ __forceinline__ mx_f32x16 mx_mfma(const mx_u32x4& w, const mx_u32x6& hi, const mx_u32x6& lo, mx_f32x16 c,
+                                             int sw, int sx, int sx_lo) {
+  const mx_i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+  const mx_i32x8 h = {(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3], (int)hi[4], (int)hi[5], 0, 0};
+  const mx_i32x8 l = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)lo[4], (int)lo[5], 0, 0};
+  c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, h, c, 4, 2, S, sw, S, sx);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, l, c, 4, 2, S, sw, S, sx_lo);
+}
+// (result: lane's column = lane & 31, register r its row 8 (r / 4) + 4 (lane / 32) + r % 4)
+
+}  // namespace qmm

@@ -1,0 +1,218 @@
+// Host side of the microscaled types and of the scored routing (included by
+// qmm_host.cpp after its helpers and qmm_qtensor). Formats and kernels:
+// qmm_mx_common.h, qmm_mx_quant_kernels.h, qmm_mx_gemm_kernels.h, qmm_route_kernels.h.
+#pragma once
+
+namespace {
+
+// qmm_mx_common.h's layout constants.
+constexpr int64_t kMxTile = 32, kMxChunk = 256, kMxUnit = 4352, kMxDigitChunk = 384;
+
+bool is_mx(int dtype) { return dtype == QMM_MXFP4; }
+
+int64_t mx_chunks(int64_t k) { return (k + kMxChunk - 1) / kMxChunk; }
+size_t mx_weight_bytes(int64_t n, int64_t k) {
+  return (size_t)((n + kMxTile - 1) / kMxTile) * (size_t)mx_chunks(k) * (size_t)kMxUnit;
+}
+
+size_t mx_align(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// Digit planes of m rows of k values: digits, then scale bytes.
+struct MxPlanes {
+  size_t q, s, total;
+};
+MxPlanes mx_planes(int64_t m, int64_t k) {
+  MxPlanes p;
+  p.q = 0;
+  p.s = mx_align((size_t)m * (size_t)(mx_chunks(k) * kMxDigitChunk));
+  p.total = p.s + mx_align((size_t)m * (size_t)(mx_chunks(k) * 8));
+  return p;
+}
+
+const char* mx_type_name(int dtype) {
+  return dtype == QMM_F32 ? "f32" : dtype == QMM_F16 ? "f16" : dtype == QMM_BF16 ? "bf16" : nullptr;
+}
+size_t mx_type_size(int dtype) { return dtype == QMM_F32 ? 4 : 2; }
+
+// One workgroup a 32 x 256 unit of the weight.
+int mx_units(int64_t n, int64_t k, unsigned* grid) {
+  const int64_t u = (n + kMxTile - 1) / kMxTile * mx_chunks(k);
+  if (u > (1LL << 31) - 1) return fail(QMM_ERR_INVALID, "MXFP4 tensor too large");
+  *grid = (unsigned)u;
+  return QMM_OK;
+}
+
+int mx_ggml(Device* d, const char* name, const void* src, int64_t n, int64_t k, void* dst, hipStream_t s) {
+  unsigned grid = 0;
+  QMM_TRY(mx_units(n, k, &grid));
+  int nn = (int)n, kk = (int)k, kc = (int)mx_chunks(k);
+  void* args[] = {&src, &nn, &kk, &dst, &kc};
+  return launch(d, name, grid, 256, 0, s, args);
+}
+
+int mx_quantize_w(Device* d, const void* w, int w_dtype, int64_t n, int64_t k, void* out, hipStream_t s) {
+  char name[40];
+  snprintf(name, sizeof(name), "qmm_mx_quantize_w_%s", mx_type_name(w_dtype));
+  // four values a thread and load
+  if ((uintptr_t)w % (4 * mx_type_size(w_dtype))) return fail(QMM_ERR_INVALID, "MXFP4 quantize: the weight must start on a boundary of four values");
+  return mx_ggml(d, name, w, n, k, out, s);
+}
+
+int mx_dequantize(Device* d, const void* w, int64_t n, int64_t k, void* dst, int out_dtype, hipStream_t s) {
+  char name[40];
+  snprintf(name, sizeof(name), "qmm_mx_dequantize_%s", mx_type_name(out_dtype));
+  if ((uintptr_t)dst % (4 * mx_type_size(out_dtype))) return fail(QMM_ERR_INVALID, "MXFP4 dequantize: the output must start on a boundary of four values");
+  return mx_ggml(d, name, w, n, k, dst, s);
+}
+
+// Whether rows of a typed matrix all start on 16-byte boundaries.
+int mx_wide(const void* x, int dtype, int64_t ldx) {
+  return (uintptr_t)x % 16 == 0 && (ldx * (int64_t)mx_type_size(dtype)) % 16 == 0;
+}
+
+// Activation limits: 32-bit offsets within a workgroup's rows, one thread a block.
+int mx_check_rows(int64_t m, int64_t k) {
+  if (m > (1LL << 21) || k > (1LL << 24) || m * mx_chunks(k) > (1LL << 30))
+    return fail(QMM_ERR_INVALID, "activation of %lld x %lld is too large", (long long)m, (long long)k);
+  return QMM_OK;
+}
+
+int mx_quantize_x(Device* d, const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, uint8_t* ws,
+                  hipStream_t s) {
+  const MxPlanes p = mx_planes(m, k);
+  char name[40];
+  snprintf(name, sizeof(name), "qmm_mx_quantize_x_%s", mx_type_name(x_dtype));
+  long long ld = ldx;
+  int mm = (int)m, kk = (int)k, kc = (int)mx_chunks(k), wide = mx_wide(x, x_dtype, ldx);
+  void *q = ws + p.q, *sc = ws + p.s;
+  void* args[] = {&x, &ld, &mm, &kk, &kc, &wide, &q, &sc};
+  return launch(d, name, ceil_div(m * kc * 8, 256), 256, 0, s, args);
+}
+
+// The kernels' by-value argument (qmm::MxOut).
+struct MxOut {
+  const void* w;
+  void* y;
+  const void* bias;
+  int y_type, bias_type, accumulate;
+};
+
+// y = planes . W^T over m dense rows.
+int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, int64_t m, MxOut o, int64_t ldy, hipStream_t s) {
+  const MxPlanes p = mx_planes(m, w->k);
+  o.w = w->data;
+  int mm = (int)m, n = (int)w->n, kc = (int)mx_chunks(w->k), ld = (int)ldy;
+  const void *q = planes + p.q, *sc = planes + p.s;
+  void* args[] = {&o, &mm, &n, &kc, &q, &sc, &ld};
+  hipFunction_t f;
+  if (m <= 32) {
+    QMM_TRY(kernel(d, "qmm_mx_gemv", &f));
+    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 32), 1, 1, 512, 1, 1, 0, s, args, nullptr));
+    return QMM_OK;
+  }
+  QMM_TRY(kernel(d, "qmm_mx_gemm", &f));
+  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 256), ceil_div(m, 64), 1, 256, 1, 1, 0, s, args, nullptr));
+  return QMM_OK;
+}
+
+// The same of expert-ordered rows: row offsets[e] + i of the output takes row
+// src[offsets[e] + i] of the planes (src null: the same row). One or two weights.
+// max_rows bounds every count.
+int mx_expert_product(Device* d, const qmm_qtensor* const* w, int count, int experts, const uint8_t* planes,
+                      int64_t plane_rows, int64_t pairs, int64_t max_rows, const int32_t* counts,
+                      const int32_t* offsets, const int32_t* src, float* const* y, hipStream_t s) {
+  const MxPlanes p = mx_planes(plane_rows, w[0]->k);
+  MxOut o[2] = {};
+  for (int j = 0; j < 2; ++j) {
+    const int i = j < count ? j : 0;
+    o[j].w = w[i]->data;
+    o[j].y = y[i];
+  }
+  int E = experts, P = (int)pairs, n = (int)(w[0]->n / experts), kc = (int)mx_chunks(w[0]->k), ld = n;
+  const void *q = planes + p.q, *sc = planes + p.s;
+  void* args[] = {&o[0], &o[1], &E, &P, &n, &kc, &counts, &offsets, &src, &q, &sc, &ld};
+  const bool gemv = max_rows <= 32;
+  const int64_t bm = gemv ? 32 : 64;
+  const int64_t tiles = std::min<int64_t>(pairs / bm + std::min<int64_t>(experts, pairs), 65535);
+  if (pairs / bm + std::min<int64_t>(experts, pairs) > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
+  hipFunction_t f;
+  QMM_TRY(kernel(d, gemv ? "qmm_mx_expert_gemv" : "qmm_mx_expert_gemm", &f));
+  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, gemv ? 32 : 256), (unsigned)tiles, (unsigned)count, gemv ? 512 : 256, 1, 1,
+                                0, s, args, nullptr));
+  return QMM_OK;
+}
+
+int mx_silu_mul(Device* d, const float* g, const float* u, int64_t m, int64_t k, uint8_t* planes, hipStream_t s) {
+  const MxPlanes p = mx_planes(m, k);
+  int mm = (int)m, kk = (int)k, kc = (int)mx_chunks(k);
+  void *q = planes + p.q, *sc = planes + p.s;
+  void* args[] = {&g, &u, &mm, &kk, &kc, &q, &sc};
+  return launch(d, "qmm_mx_silu_mul", ceil_div(m * kc * 8, 256), 256, 0, s, args);
+}
+
+// How a call routes its tokens.
+struct Routing {
+  bool scored = false;  // qmm_moe_route_scored's rules; else qmm_moe_route_ex's
+  int score = 0, groups = 1, topk_groups = 1, group_top = 1;
+  const float* bias = nullptr;
+  int renormalize = 1;
+  float scale = 1.0f;
+};
+
+struct RouteArgs {  // the kernels' by-value argument (qmm::RouteArgs)
+  int T, E, k, sigmoid, groups, topk_groups, group_top, renorm;
+  float scale;
+};
+
+constexpr int kRouteMaxTokens = 65536, kRouteMaxExperts = 1024, kRouteMaxTopk = 32, kRouteSmall = 16;
+
+int check_routing(int64_t tokens, int experts, int topk, const Routing& r) {
+  if (tokens < 1 || tokens > kRouteMaxTokens || experts < 1 || experts > kRouteMaxExperts || topk < 1 ||
+      topk > kRouteMaxTopk || topk > experts)
+    return fail(QMM_ERR_INVALID, "routing limits: 1 <= tokens <= %d, 1 <= experts <= %d, 1 <= topk <= min(%d, experts)",
+                kRouteMaxTokens, kRouteMaxExperts, kRouteMaxTopk);
+  if (r.score != QMM_SCORE_SOFTMAX && r.score != QMM_SCORE_SIGMOID)
+    return fail(QMM_ERR_INVALID, "routing score %d (softmax = 0, sigmoid = 1)", r.score);
+  if (r.groups < 1 || r.groups > 64 || experts % r.groups || r.topk_groups < 1 || r.topk_groups > r.groups)
+    return fail(QMM_ERR_INVALID, "routing groups: 1 <= topk_groups <= groups <= 64, experts %% groups == 0");
+  if (r.group_top < 1 || r.group_top > 2 || r.group_top > experts / r.groups)
+    return fail(QMM_ERR_INVALID, "a group's score is the sum of its 1 or 2 best experts (group_top %d, groups of %d)",
+                r.group_top, experts / r.groups);
+  if (topk > r.topk_groups * (experts / r.groups))
+    return fail(QMM_ERR_INVALID, "topk %d experts out of %d groups of %d", topk, r.topk_groups, experts / r.groups);
+  if (!(r.scale == r.scale)) return fail(QMM_ERR_INVALID, "routed scaling factor is NaN");
+  return QMM_OK;
+}
+
+// (one launch up to 16 tokens of up to 256 experts)
+bool route_is_small(int64_t tokens, int experts) { return tokens <= kRouteSmall && experts <= 256; }
+
+size_t route_scratch(int64_t tokens, int experts, int topk) {
+  if (route_is_small(tokens, experts)) return 0;
+  return mx_align((size_t)tokens * topk * 2) + mx_align((size_t)tokens * topk * 4);
+}
+
+int route_scored(Device* d, const float* logits, int64_t tokens, int experts, int topk, const Routing& r,
+                 int32_t* counts, int32_t* offsets, int32_t* pair_token, float* pair_weight, int32_t* token_pairs,
+                 uint8_t* ws, hipStream_t s) {
+  RouteArgs a = {(int)tokens, experts, topk, r.score == QMM_SCORE_SIGMOID, r.groups, r.topk_groups, r.group_top,
+                 r.renormalize ? 1 : 0, r.scale};
+  const float* bias = r.bias;
+  const int R = experts <= 64 ? 1 : experts <= 128 ? 2 : experts <= 256 ? 4 : 16;
+  char name[32];
+  // a wave a token: up to 16 tokens are one workgroup, which also makes the lists
+  if (route_is_small(tokens, experts)) {
+    snprintf(name, sizeof(name), "qmm_route_small_r%d", R);
+    void* args[] = {&logits, &bias, &a, &counts, &offsets, &pair_token, &pair_weight, &token_pairs};
+    return launch(d, name, 1, 1024, 0, s, args);
+  }
+  void* ids = ws;
+  void* wts = ws + mx_align((size_t)tokens * topk * 2);
+  snprintf(name, sizeof(name), "qmm_route_tokens_r%d", R);
+  void* a1[] = {&logits, &bias, &a, &ids, &wts};
+  QMM_TRY(launch(d, name, ceil_div(tokens, 4), 256, 0, s, a1));
+  void* a2[] = {&a, &ids, &wts, &counts, &offsets, &pair_token, &pair_weight, &token_pairs};
+  return launch(d, "qmm_route_lists", ceil_div(tokens, 64), 1024, 0, s, a2);
+}
+
+}  // namespace

@@ -1,0 +1,329 @@
+// Quantizers, converters and readers of the microscaled types (formats and layouts:
+// qmm_mx_common.h). All are bound by memory: one pass, each value read once.
+#pragma once
+
+#include "qmm_mx_common.h"
+
+namespace qmm {
+
+// Weight units are made by one workgroup each (32 rows x 256 columns), thread
+// 64 s + 32 h + r the block 2 s + h of row r: its 16 bytes of codes are written where
+// the unit has them, so a wave writes 1 KB at once. The unit's values go through LDS,
+// where a row is 260 floats so that 8 rows' 16-byte reads fall on distinct banks.
+constexpr int kMxLdsRow = kMxChunk + 4;
+
+__device__ __forceinline__ void mx_put_unit(uint8_t* __restrict__ unit, uint8_t (&sc)[256], int t, mx_u32x4 q, int e) {
+  *reinterpret_cast<mx_u32x4*>(unit + 16 * t) = q;
+  sc[4 * (t & 63) + (t >> 6)] = (uint8_t)e;
+  __syncthreads();
+  if (t < 64)
+    *reinterpret_cast<uint32_t*>(unit + kMxScaleOff + 4 * t) = *reinterpret_cast<const uint32_t*>(sc + 4 * t);
+}
+
+// E2M1 codes of 32 values, value j in nibble j.
+__device__ __forceinline__ mx_u32x4 mx_codes(const float (&x)[32], int e) {
+  mx_u32x4 q;
+  const int up = 127 - e;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    int v = 0;
+#define QMM_MX_CVT(B)                                                                                       \
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, e == kMxNan ? 0.0f : __builtin_ldexpf(x[8 * w + 2 * B], up), \
+                                               e == kMxNan ? 0.0f : __builtin_ldexpf(x[8 * w + 2 * B + 1], up), 1.0f, B)
+    QMM_MX_CVT(0);
+    QMM_MX_CVT(1);
+    QMM_MX_CVT(2);
+    QMM_MX_CVT(3);
+#undef QMM_MX_CVT
+    q[w] = (uint32_t)v;
+  }
+  return q;
+}
+
+template <int T>
+__device__ __forceinline__ void mx_quantize_w(const void* __restrict__ w, int n, int k, uint8_t* __restrict__ out,
+                                              int kc) {
+  __shared__ __attribute__((aligned(16))) float buf[kMxTile * kMxLdsRow];
+  __shared__ __attribute__((aligned(16))) uint8_t sc[256];
+  const int t = threadIdx.x;
+  const long long u = blockIdx.x;
+  const int r0 = (int)(u / kc) * kMxTile, c0 = (int)(u % kc) * kMxChunk;
+  // four values a thread and row, whole rows of the unit by a wave (k % 32 == 0)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (t >> 6), c = 4 * (t & 63);
+    mx_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (r0 + r < n && c0 + c < k) {
+      const long long at = (long long)(r0 + r) * k + c0 + c;
+      if constexpr (T == kF32) {
+        v = *reinterpret_cast<const mx_f32x4*>(static_cast<const float*>(w) + at);
+      } else {
+        const mx_u32x2 d = *reinterpret_cast<const mx_u32x2*>(static_cast<const uint16_t*>(w) + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint16_t s = (uint16_t)(d[j >> 1] >> (16 * (j & 1)));
+          v[j] = T == kF16 ? (float)__builtin_bit_cast(_Float16, s) : bf16_to_f32(s);
+        }
+      }
+    }
+    *reinterpret_cast<mx_f32x4*>(buf + r * kMxLdsRow + c) = v;
+  }
+  __syncthreads();
+  const float* p = buf + (t & 31) * kMxLdsRow + 64 * (t >> 6) + (t & 32);
+  float x[32];
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const mx_f32x4 v = *reinterpret_cast<const mx_f32x4*>(p + 4 * j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[4 * j + i] = v[i];  // (a bit cast of the vector's own element would take its first one)
+      amax = max(amax, __builtin_bit_cast(uint32_t, x[4 * j + i]) & 0x7fffffffu);
+    }
+  }
+  const int e = mx_w_byte(amax);
+  mx_put_unit(out + u * kMxUnit, sc, t, mx_codes(x, e), e);
+}
+
+// The code's value of E2M1, doubled.
+__device__ __forceinline__ int mx_twice(uint32_t code) {
+  const int m = (int)((0xC8643210u >> (4 * (code & 7))) & 15u);
+  return code & 8 ? -m : m;
+}
+// twice the value, under scale byte e (255: NaN); exact in f32 down to its smallest subnormal
+__device__ __forceinline__ float mx_value(uint32_t code, int e) {
+  return e == kMxNan ? __builtin_nanf("") : __builtin_ldexpf((float)mx_twice(code), e - 128);
+}
+
+}  // namespace qmm
+
+#define QMM_MX_QUANTIZE_W(NAME, T)                                                                                \
+  extern "C" __global__ void __launch_bounds__(256) qmm_mx_quantize_w_##NAME(                                     \
+      const void* __restrict__ w, int n, int k, uint8_t* __restrict__ out, int kc) {                              \
+    qmm::mx_quantize_w<T>(w, n, k, out, kc);                                                                      \
+  }
+QMM_MX_QUANTIZE_W(f32, qmm::kF32)
+QMM_MX_QUANTIZE_W(f16, qmm::kF16)
+QMM_MX_QUANTIZE_W(bf16, qmm::kBF16)
+
+// GGML blocks -> units, and back. Load time only: byte reads of 17-byte blocks.
+extern "C" __global__ void __launch_bounds__(256) qmm_mx_from_ggml(const uint8_t* __restrict__ src, int n, int k,
+                                                                   uint8_t* __restrict__ out, int kc) {
+  __shared__ __attribute__((aligned(16))) uint8_t sc[256];
+  const int t = threadIdx.x;
+  const long long u = blockIdx.x;
+  const int row = (int)(u / kc) * qmm::kMxTile + (t & 31);
+  const int blk = (int)(u % kc) * 8 + 2 * (t >> 6) + ((t >> 5) & 1);
+  qmm::mx_u32x4 q = {0, 0, 0, 0};
+  int e = 0;
+  if (row < n && blk < k / 32) {
+    const uint8_t* b = src + ((long long)row * (k / 32) + blk) * qmm::kMxFp4Bytes;
+    e = b[0];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {  // byte j: value j low, value j + 16 high
+      const uint32_t v = b[1 + j];
+      q[j >> 3] |= (v & 15u) << (4 * (j & 7));
+      q[2 + (j >> 3)] |= (v >> 4) << (4 * (j & 7));
+    }
+  }
+  qmm::mx_put_unit(out + u * qmm::kMxUnit, sc, t, q, e);
+}
+
+extern "C" __global__ void __launch_bounds__(256) qmm_mx_to_ggml(const uint8_t* __restrict__ w, int n, int k,
+                                                                 uint8_t* __restrict__ dst, int kc) {
+  const int t = threadIdx.x;
+  const long long u = blockIdx.x;
+  const int row = (int)(u / kc) * qmm::kMxTile + (t & 31);
+  const int blk = (int)(u % kc) * 8 + 2 * (t >> 6) + ((t >> 5) & 1);
+  if (row >= n || blk >= k / 32) return;
+  const uint8_t* p = w + u * qmm::kMxUnit;
+  const qmm::mx_u32x4 q = *reinterpret_cast<const qmm::mx_u32x4*>(p + 16 * t);
+  uint8_t* b = dst + ((long long)row * (k / 32) + blk) * qmm::kMxFp4Bytes;
+  b[0] = p[qmm::kMxScaleOff + 4 * (t & 63) + (t >> 6)];
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    b[1 + j] = (uint8_t)((q[j >> 3] >> (4 * (j & 7)) & 15u) | (q[2 + (j >> 3)] >> (4 * (j & 7)) & 15u) << 4);
+}
+
+namespace qmm {
+// Units -> dense [n, k], each value rounded once to the output type. A unit's values go
+// through LDS so that a wave writes whole rows of it.
+template <int T>
+__device__ __forceinline__ void mx_dequantize(const uint8_t* __restrict__ w, int n, int k, void* __restrict__ dst,
+                                              int kc) {
+  __shared__ __attribute__((aligned(16))) float buf[kMxTile * kMxLdsRow];
+  const int t = threadIdx.x;
+  const long long u = blockIdx.x;
+  const uint8_t* p = w + u * kMxUnit;
+  const mx_u32x4 q = *reinterpret_cast<const mx_u32x4*>(p + 16 * t);
+  const int e = p[kMxScaleOff + 4 * (t & 63) + (t >> 6)];
+  float* o = buf + (t & 31) * kMxLdsRow + 64 * (t >> 6) + (t & 32);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    mx_f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = mx_value(q[j >> 1] >> (16 * (j & 1) + 4 * i), e);
+    *reinterpret_cast<mx_f32x4*>(o + 4 * j) = v;
+  }
+  __syncthreads();
+  const int r0 = (int)(u / kc) * kMxTile, c = (int)(u % kc) * kMxChunk + 4 * (t & 63);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (t >> 6);
+    if (r0 + r >= n || c >= k) continue;
+    const mx_f32x4 v = *reinterpret_cast<const mx_f32x4*>(buf + r * kMxLdsRow + 4 * (t & 63));
+    const long long at = (long long)(r0 + r) * k + c;
+    if constexpr (T == kF32) {
+      *reinterpret_cast<mx_f32x4*>(static_cast<float*>(dst) + at) = v;
+    } else {
+      *reinterpret_cast<mx_u32x2*>(static_cast<uint16_t*>(dst) + at) =
+          mx_u32x2{mx_to16(v[0], T) | (uint32_t)mx_to16(v[1], T) << 16, mx_to16(v[2], T) | (uint32_t)mx_to16(v[3], T) << 16};
+    }
+  }
+}
+
+// 32 consecutive values of a typed row. `wide`: the row starts on a 16-byte boundary.
+template <int T>
+__device__ __forceinline__ uint32_t mx_load_block(const void* __restrict__ row, long long at, bool wide, float (&x)[32]) {
+  uint32_t amax = 0;
+  if constexpr (T == kF32) {
+    const float* p = static_cast<const float*>(row) + at;
+    if (wide) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const mx_f32x4 v = reinterpret_cast<const mx_f32x4*>(p)[j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * j + i] = v[i];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] = p[j];
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(row) + at;
+    auto f = [](uint32_t v) {
+      return T == kF16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v) : bf16_to_f32((uint16_t)v);
+    };
+    if (wide) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const mx_u32x4 v = reinterpret_cast<const mx_u32x4*>(p)[j];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[8 * j + i] = f(v[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] = f(p[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) amax = max(amax, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
+  return amax;
+}
+
+__device__ __forceinline__ void mx_put_digits(uint8_t* __restrict__ q, const mx_u32x6& hi, const mx_u32x6& lo) {
+  mx_u32x4* o = reinterpret_cast<mx_u32x4*>(q);
+  o[0] = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
+  o[1] = mx_u32x4{hi[4], hi[5], lo[0], lo[1]};
+  o[2] = mx_u32x4{lo[2], lo[3], lo[4], lo[5]};
+}
+
+// Rows -> digit planes: one thread a block; blocks past k (up to the chunk's end) are zero.
+template <int T>
+__device__ __forceinline__ void mx_quantize_x(const void* __restrict__ x, long long ldx, int m, int k, int kc, int wide,
+                                              uint8_t* __restrict__ q, uint8_t* __restrict__ sc) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int nb = 8 * kc;
+  if (i >= (long long)m * nb) return;
+  const int row = (int)(i / nb), b = (int)(i % nb);
+  mx_u32x6 hi = (mx_u32x6)(0u), lo = (mx_u32x6)(0u);
+  int e = 4;
+  if (32 * b < k) {
+    float v[32];
+    e = mx_x_byte(mx_load_block<T>(x, row * ldx + 32 * b, wide != 0, v));
+    mx_digits(v, e, hi, lo);
+  }
+  mx_put_digits(q + i * kMxDigitBlock, hi, lo);
+  sc[(i & ~7LL) + 4 * (b & 1) + ((b & 7) >> 1)] = (uint8_t)e;
+}
+}  // namespace qmm
+
+#define QMM_MX_TYPED(NAME, T)                                                                                     \
+  extern "C" __global__ void __launch_bounds__(256) qmm_mx_dequantize_##NAME(                                     \
+      const uint8_t* __restrict__ w, int n, int k, void* __restrict__ dst, int kc) {                              \
+    qmm::mx_dequantize<T>(w, n, k, dst, kc);                                                                      \
+  }                                                                                                               \
+  extern "C" __global__ void __launch_bounds__(256) qmm_mx_quantize_x_##NAME(                                     \
+      const void* __restrict__ x, long long ldx, int m, int k, int kc, int wide, uint8_t* __restrict__ q,         \
+      uint8_t* __restrict__ sc) {                                                                                 \
+    qmm::mx_quantize_x<T>(x, ldx, m, k, kc, wide, q, sc);                                                         \
+  }
+QMM_MX_TYPED(f32, qmm::kF32)
+QMM_MX_TYPED(f16, qmm::kF16)
+QMM_MX_TYPED(bf16, qmm::kBF16)
+
+// f32 rows -> 49-byte blocks (qmm_quantize_rows), and those -> digit planes.
+extern "C" __global__ void __launch_bounds__(256) qmm_mx_quantize_rows(const float* __restrict__ x, long long ldx,
+                                                                       int m, int k, int wide,
+                                                                       uint8_t* __restrict__ xq) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int nb = k / 32;
+  if (i >= (long long)m * nb) return;
+  float v[32];
+  qmm::mx_u32x6 hi, lo;
+  const int e = qmm::mx_x_byte(qmm::mx_load_block<qmm::kF32>(x, i / nb * ldx + 32 * (i % nb), wide != 0, v));
+  qmm::mx_digits(v, e, hi, lo);
+  uint8_t* o = xq + i * qmm::kMxFp6x2Bytes;
+  o[0] = (uint8_t)e;
+#pragma unroll
+  for (int j = 0; j < 24; ++j) {
+    o[1 + j] = (uint8_t)(hi[j >> 2] >> (8 * (j & 3)));
+    o[25 + j] = (uint8_t)(lo[j >> 2] >> (8 * (j & 3)));
+  }
+}
+
+extern "C" __global__ void __launch_bounds__(256) qmm_mx_blocks_to_planes(const uint8_t* __restrict__ xq, int m, int k,
+                                                                          int kc, uint8_t* __restrict__ q,
+                                                                          uint8_t* __restrict__ sc) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int nb = 8 * kc;
+  if (i >= (long long)m * nb) return;
+  const int row = (int)(i / nb), b = (int)(i % nb);
+  qmm::mx_u32x6 d[2] = {(qmm::mx_u32x6)(0u), (qmm::mx_u32x6)(0u)};
+  int e = 4;
+  if (32 * b < k) {
+    const uint8_t* p = xq + ((long long)row * (k / 32) + b) * qmm::kMxFp6x2Bytes;
+    e = p[0] < 4 ? qmm::kMxNan : p[0];  // (no quantizer writes one: the second digit's scale would be below 2^-127)
+#pragma unroll
+    for (int j = 0; j < 48; ++j) d[j / 24][j % 24 >> 2] |= (uint32_t)p[1 + j] << (8 * (j & 3));
+  }
+  qmm::mx_put_digits(q + i * qmm::kMxDigitBlock, d[0], d[1]);
+  sc[(i & ~7LL) + 4 * (b & 1) + ((b & 7) >> 1)] = (uint8_t)e;
+}
+
+// silu(g) * u -> digit planes, rows x k f32 (the down projection's input).
+extern "C" __global__ void __launch_bounds__(256) qmm_mx_silu_mul(const float* __restrict__ g,
+                                                                  const float* __restrict__ u, int m, int k, int kc,
+                                                                  uint8_t* __restrict__ q, uint8_t* __restrict__ sc) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int nb = 8 * kc;
+  if (i >= (long long)m * nb) return;
+  const int row = (int)(i / nb), b = (int)(i % nb);
+  qmm::mx_u32x6 hi = (qmm::mx_u32x6)(0u), lo = (qmm::mx_u32x6)(0u);
+  int e = 4;
+  if (32 * b < k) {
+    float a[32], v[32];
+    qmm::mx_load_block<qmm::kF32>(g, (long long)row * k + 32 * b, true, a);
+    qmm::mx_load_block<qmm::kF32>(u, (long long)row * k + 32 * b, true, v);
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      v[j] = a[j] / (1.0f + expf(-a[j])) * v[j];
+      amax = max(amax, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+    }
+    e = qmm::mx_x_byte(amax);
+    qmm::mx_digits(v, e, hi, lo);
+  }
+  qmm::mx_put_digits(q + i * qmm::kMxDigitBlock, hi, lo);
+  sc[(i & ~7LL) + 4 * (b & 1) + ((b & 7) >> 1)] = (uint8_t)e;
+}

@@ -2,7 +2,8 @@
 
 Mirrors the surface the reference engine uses for its quantized projections:
 
-* ``GgmlDType``             -- candle ``quantized::GgmlDType`` (Q8_0, Q4K, Q6K; Q8K as vec-dot type)
+* ``GgmlDType``             -- candle ``quantized::GgmlDType`` (Q8_0, Q4K, Q6K; Q8K as vec-dot type), and MXFP4
+                             with its vec-dot type MXFP6X2 (no counterpart in candle)
 * ``QTensor``               -- ``QTensor::{quantize, new(QStorage::from_data), dequantize, dtype}``
 * ``QMatMul``               -- ``QMatMul::{from_qtensor, forward}``
 * ``QuantSpec``             -- crates/llm/candle-llm/src/primitives/projection.rs:16-52
@@ -63,6 +64,8 @@ EXPORTS = (
     "qmm_silu_mul", "qmm_matmul_q_workspace_size", "qmm_matmul_noalloc",
     "qmm_stream_read", "qmm_reload_tuning", "qmm_moe_route_ex", "qmm_moe_ffn_ex_workspace_size", "qmm_moe_ffn_ex",
     "qmm_decode_rope_attention_warm", "qmm_matmul_grouped",
+    "qmm_qtensor_quantize_from", "qmm_linear", "qmm_linear_workspace_size", "qmm_moe_route_scored",
+    "qmm_moe_route_scored_workspace_size", "qmm_moe_ffn_scored", "qmm_moe_ffn_scored_workspace_size",
 )
 
 
@@ -169,6 +172,15 @@ def lib() -> ctypes.CDLL:
                                          sz, vp], i32),
             "qmm_prefill_attention_o_workspace_size": ([vp, i64], sz),
             "qmm_silu_mul": ([vp, vp, vp, i64, vp], i32),
+            "qmm_qtensor_quantize_from": ([i32, i64, i64, vp, i32, vp, pp], i32),
+            "qmm_linear": ([vp, vp, i32, i64, i64, vp, i32, vp, i32, i64, vp, sz, vp], i32),
+            "qmm_linear_workspace_size": ([vp, i64], sz),
+            "qmm_moe_route_scored": ([vp, i64, i32, i32, i32, vp, i32, i32, i32, i32, ctypes.c_float, vp, vp, vp, vp,
+                                      vp, vp, sz, vp], i32),
+            "qmm_moe_route_scored_workspace_size": ([i64, i32, i32], sz),
+            "qmm_moe_ffn_scored": ([vp, i32, i64, i64, vp, i32, i32, i32, vp, i32, i32, i32, i32, ctypes.c_float, vp,
+                                    vp, vp, vp, vp, vp, vp, vp, i32, i64, vp, sz, vp], i32),
+            "qmm_moe_ffn_scored_workspace_size": ([vp, vp, i64, i32, i32, vp, vp, vp], sz),
             "qmm_stream_read": ([vp, ctypes.c_size_t, vp, i32, i32, vp], i32),
         }
         for name, (args, res) in sig.items():
@@ -205,6 +217,8 @@ class GgmlDType(enum.IntEnum):
     Q4K = 12
     Q6K = 14
     Q8K = 15
+    MXFP4 = 39
+    MXFP6X2 = 256  # activations only; not a GGUF type
 
     def block_size(self) -> int:
         return lib().qmm_block_size(int(self))
@@ -217,6 +231,10 @@ class GgmlDType(enum.IntEnum):
         if v < 0:
             raise QmmError(1, f"{self.name} has no vec-dot type")
         return GgmlDType(v)
+
+
+# C ABI tags of dense types
+_DENSE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
 def _device_of(t: torch.Tensor) -> torch.device:
@@ -259,8 +277,8 @@ class QTensor:
     def quantize(cls, tensor: torch.Tensor, dtype: GgmlDType) -> "QTensor":
         """QTensor::quantize of a dense [n, k] weight, computed on the tensor's GPU."""
         dtype = GgmlDType(dtype)
-        if dtype == GgmlDType.Q8K:
-            raise QmmError(1, "Q8K is an activation-only type")
+        if dtype in (GgmlDType.Q8K, GgmlDType.MXFP6X2):
+            raise QmmError(1, f"{dtype.name} is an activation-only type")
         dev = _device_of(tensor)
         if tensor.dim() != 2:
             raise QmmError(1, f"QTensor::quantize expects a 2-D weight, got shape {tuple(tensor.shape)}")
@@ -268,8 +286,16 @@ class QTensor:
         if k % dtype.block_size():
             raise QmmError(1, f"quantize: the last dim {k} is not a multiple of {dtype.name}'s block size "
                               f"{dtype.block_size()}")
-        w = tensor.to(torch.float32).contiguous()
         h = ctypes.c_void_p()
+        if dtype == GgmlDType.MXFP4:  # f16 and bf16 are read as they are
+            w = tensor.contiguous() if tensor.dtype in _DENSE else tensor.to(torch.float32).contiguous()
+            if w.data_ptr() % (4 * w.element_size()):
+                w = w.clone()
+            with torch.cuda.device(dev):
+                _check(lib().qmm_qtensor_quantize_from(int(dtype), n, k, w.data_ptr(), _DENSE[w.dtype], _stream(dev),
+                                                       ctypes.byref(h)))
+            return cls(h, dev)
+        w = tensor.to(torch.float32).contiguous()
         with torch.cuda.device(dev):
             _check(lib().qmm_qtensor_quantize(int(dtype), n, k, w.data_ptr(), _stream(dev), ctypes.byref(h)))
         return cls(h, dev)
@@ -312,8 +338,8 @@ class QTensor:
             keep = arr
             ptr = arr.ctypes.data
             nbytes = arr.size
-        if dtype == GgmlDType.Q8K:
-            raise QmmError(1, "Q8K is an activation-only type")
+        if dtype in (GgmlDType.Q8K, GgmlDType.MXFP6X2):
+            raise QmmError(1, f"{dtype.name} is an activation-only type")
         if k % dtype.block_size():
             raise QmmError(1, f"k = {k} is not a multiple of {dtype.name}'s block size {dtype.block_size()}")
         expect = n * (k // dtype.block_size()) * dtype.type_size()
@@ -337,7 +363,7 @@ class QTensor:
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """QTensor::dequantize -> [n, k] on the tensor's GPU: f32, or f16 / bf16 rounded once from it
         (QTensor::dequantize_f16; the dequant-dense strategy's to_dtype)."""
-        tag = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(dtype)
+        tag = _DENSE.get(dtype)
         if tag is None:
             raise QmmError(1, f"dequantize to {dtype}: float32, float16 or bfloat16")
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
@@ -400,7 +426,7 @@ class QMatMul:
             L = lib()
             h = qt.handle
             ws, ws_bytes, ws_ptr = None, 0, None
-            if m > 2:  # one and two rows are quantized in the GEMV's prologue
+            if m > 2 or qt._dtype == GgmlDType.MXFP4:  # (one and two rows of the others: in the GEMV's prologue)
                 ws_bytes = int(L.qmm_matmul_workspace_size(h, m))
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
                 ws_ptr = ws.data_ptr()
@@ -414,6 +440,48 @@ class QMatMul:
             if status != QMM_OK:
                 raise QmmError(status, last_error())
         return y if flat else y.reshape(*shape[:-1], n)
+
+    def linear(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x @ W^T (+ bias) in x's type (float32, float16 or bfloat16) for an MXFP4 weight: the sum is
+        rounded once (qmm_linear)."""
+        qt = self.qtensor
+        n, k = qt.shape
+        tag = _DENSE.get(x.dtype)
+        if tag is None:
+            raise QmmError(1, f"QMatMul::linear expects float32, float16 or bfloat16 input, got {x.dtype}")
+        shape = x.shape
+        if shape[-1] != k:
+            raise QmmError(1, f"shape mismatch: input last dim {shape[-1]} vs weight in-dim {k}")
+        dev = x.device
+        if dev != qt.device:
+            raise QmmError(1, f"input on {dev}, weight on {qt.device}")
+        btag, bptr = 0, None
+        if bias is not None:
+            if bias.dim() != 1 or bias.shape[0] != n or bias.device != dev:
+                raise QmmError(1, f"bias must be [{n}] on {dev}, got {tuple(bias.shape)} on {bias.device}")
+            if bias.dtype not in _DENSE:
+                bias = bias.to(torch.float32)
+            bias = bias.contiguous()
+            btag, bptr = _DENSE[bias.dtype], bias.data_ptr()
+        x2 = x if len(shape) == 2 else x.reshape(-1, k)
+        if x2.stride(-1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < k):
+            x2 = x2.contiguous()
+        m = x2.shape[0]
+        y = torch.empty((m, n), dtype=x.dtype, device=dev)
+        if m != 0:
+            L = lib()
+            ws_bytes = int(L.qmm_linear_workspace_size(qt.handle, m))
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            args = (qt.handle, x2.data_ptr(), tag, m, max(x2.stride(0), k), bptr, btag, y.data_ptr(), tag, n,
+                    ws.data_ptr(), ws_bytes, _raw_stream(dev.index))
+            if torch.cuda.current_device() == dev.index:
+                status = L.qmm_linear(*args)
+            else:
+                with torch.cuda.device(dev):
+                    status = L.qmm_linear(*args)
+            if status != QMM_OK:
+                raise QmmError(status, last_error())
+        return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
 
     def forward_via_f16(self, x: torch.Tensor) -> torch.Tensor:
         """QMatMul::forward_via_f16: the weight dequantized to a dense f16 tile, x cast to f16, a dense
@@ -547,18 +615,55 @@ def block_dots(qt: QTensor, xq: torch.Tensor, m: int) -> Tuple[torch.Tensor, tor
     return (dots if per == 2 else dots[..., 0]), y
 
 
-def moe_route(logits: torch.Tensor, topk: int, renormalize: bool = True, routed_scaling_factor: float = 1.0):
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _scored(score, bias, groups, topk_groups, group_top, experts, dev):
+    """(score tag, bias as f32 or None, groups, topk_groups, group_top) of a scored routing's arguments."""
+    if score not in _SCORES:
+        raise QmmError(QMM_ERR_INVALID, f"routing score {score!r} (softmax, sigmoid)")
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != experts or bias.device != dev:
+            raise QmmError(QMM_ERR_INVALID, f"routing bias must be [{experts}] on {dev}, got {tuple(bias.shape)} on "
+                                            f"{bias.device}")
+        bias = bias.to(torch.float32).contiguous()
+    return _SCORES[score], bias, groups, groups if topk_groups is None else topk_groups, group_top
+
+
+def moe_route(logits: torch.Tensor, topk: int, renormalize: bool = True, routed_scaling_factor: float = 1.0,
+              score: Optional[str] = None, bias: Optional[torch.Tensor] = None, groups: int = 1,
+              topk_groups: Optional[int] = None, group_top: int = 1):
     """Device routing: returns (counts, offsets, pair_token, pair_weight, token_pairs). Weights are the
     selected probabilities renormalised over the selection, or (renormalize False) times
-    routed_scaling_factor (MoeMlp::forward, models/llama.rs:1436-1447)."""
+    routed_scaling_factor (MoeMlp::forward, models/llama.rs:1436-1447).
+
+    With `score` ("softmax" or "sigmoid") the routing is qmm_moe_route_scored's: the choice is score + bias
+    (f32 [experts]), limited to the topk_groups (default: all) of `groups` runs of experts whose group_top
+    (1 or 2) best choices sum highest; weights are the scores themselves, renormalised if asked, and times
+    routed_scaling_factor in either case. Scores are held in 64 bits."""
+    if logits.dim() != 2:
+        raise QmmError(QMM_ERR_INVALID, f"router logits must be [tokens, experts], got {tuple(logits.shape)}")
     t, e = logits.shape
     dev = logits.device
+    if score is None and (bias is not None or groups != 1 or topk_groups is not None or group_top != 1):
+        raise QmmError(QMM_ERR_INVALID, "a routing bias or groups need a score (softmax, sigmoid)")
     lg = logits.to(torch.float32).contiguous()
     counts = torch.empty(e, dtype=torch.int32, device=dev)
     offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
     ptok = torch.empty(t * topk, dtype=torch.int32, device=dev)
     pw = torch.empty(t * topk, dtype=torch.float32, device=dev)
     tp = torch.empty(t * topk, dtype=torch.int32, device=dev)
+    if score is not None:
+        L = lib()
+        tag, bias, groups, topk_groups, group_top = _scored(score, bias, groups, topk_groups, group_top, e, dev)
+        nws = int(L.qmm_moe_route_scored_workspace_size(t, e, topk))
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+        with torch.cuda.device(dev):
+            _check(L.qmm_moe_route_scored(lg.data_ptr(), t, e, topk, tag, _ptr(bias), groups, topk_groups, group_top,
+                                          int(renormalize), routed_scaling_factor, counts.data_ptr(),
+                                          offsets.data_ptr(), ptok.data_ptr(), pw.data_ptr(), tp.data_ptr(), _ptr(ws),
+                                          nws, _stream(dev)))
+        return counts, offsets, ptok, pw, tp
     with torch.cuda.device(dev):
         _check(lib().qmm_moe_route_ex(lg.data_ptr(), t, e, topk, int(renormalize), routed_scaling_factor,
                                       counts.data_ptr(), offsets.data_ptr(), ptok.data_ptr(), pw.data_ptr(),
@@ -568,12 +673,23 @@ def moe_route(logits: torch.Tensor, topk: int, renormalize: bool = True, routed_
 
 def moe_ffn(x: torch.Tensor, logits: torch.Tensor, gate: QTensor, up: QTensor, down: QTensor, topk: int,
             norm_topk_prob: bool = True, routed_scaling_factor: float = 1.0, shared=None,
-            shared_gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+            shared_gate: Optional[torch.Tensor] = None, score: Optional[str] = None,
+            bias: Optional[torch.Tensor] = None, groups: int = 1, topk_groups: Optional[int] = None,
+            group_top: int = 1, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Mixture-of-experts FFN (MoeMlp::forward, models/llama.rs:1416-1487) on stacked expert weights:
     top-k routing (renormalised, or scaled by routed_scaling_factor), each expert's gated MLP on its
     tokens, the weighted outputs summed in expert order; then `shared` = (gate, up, down) QTensors of the
     always-on shared expert, added after the routed sum, scaled per token by sigmoid(x . shared_gate)
-    when shared_gate (f32 [hidden]) is given."""
+    when shared_gate (f32 [hidden]) is given. `score`, `bias` and the groups route as in moe_route; the
+    result is of out_dtype. MXFP4 experts read f16 and bf16 rows as they are and round the sum once."""
+    if out_dtype not in _DENSE:
+        raise QmmError(QMM_ERR_INVALID, f"moe_ffn to {out_dtype}: float32, float16 or bfloat16")
+    if score is None and (bias is not None or groups != 1 or topk_groups is not None or group_top != 1):
+        raise QmmError(QMM_ERR_INVALID, "a routing bias or groups need a score (softmax, sigmoid)")
+    mx = gate.dtype() == GgmlDType.MXFP4
+    if mx or score is not None:
+        return _moe_ffn_scored(x, logits, gate, up, down, topk, norm_topk_prob, routed_scaling_factor, shared,
+                               shared_gate, score, bias, groups, topk_groups, group_top, out_dtype)
     t, hdim = x.shape
     e = logits.shape[1]
     dev = x.device
@@ -594,7 +710,46 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, gate: QTensor, up: QTensor, d
                                 routed_scaling_factor, gate.handle, up.handle, down.handle, sg, su, sd,
                                 gw.data_ptr() if gw is not None else None, out.data_ptr(), hdim, ws.data_ptr(), wsb,
                                 _stream(dev)))
-    return out
+    return out.to(out_dtype)
+
+
+def _moe_ffn_scored(x, logits, gate, up, down, topk, norm_topk_prob, routed_scaling_factor, shared, shared_gate, score,
+                    bias, groups, topk_groups, group_top, out_dtype):
+    """moe_ffn through qmm_moe_ffn_scored (MXFP4 experts, or a score given)."""
+    if x.dim() != 2 or logits.dim() != 2 or logits.shape[0] != x.shape[0] or x.shape[1] != gate.shape[1]:
+        raise QmmError(QMM_ERR_INVALID, f"moe_ffn: rows {tuple(x.shape)}, logits {tuple(logits.shape)}, experts of "
+                                        f"width {gate.shape[1]}")
+    t, hdim = x.shape
+    e = logits.shape[1]
+    dev = gate.device
+    if x.device != dev or logits.device != dev:
+        raise QmmError(QMM_ERR_INVALID, f"rows on {x.device}, logits on {logits.device}, experts on {dev}")
+    if score is None:  # qmm_moe_route's rule: scaled where not renormalised
+        score = "softmax"
+        routed_scaling_factor = 1.0 if norm_topk_prob else routed_scaling_factor
+    if shared is None and shared_gate is not None:
+        raise QmmError(QMM_ERR_INVALID, "a shared-expert gate without a shared expert")
+    tag, bias, groups, topk_groups, group_top = _scored(score, bias, groups, topk_groups, group_top, e, dev)
+    typed = gate.dtype() == GgmlDType.MXFP4 and (shared is None or shared[0].dtype() == GgmlDType.MXFP4)
+    xx = (x if typed and x.dtype in _DENSE else x.to(torch.float32)).contiguous()
+    odt = out_dtype if gate.dtype() == GgmlDType.MXFP4 else torch.float32
+    lg = logits.to(torch.float32).contiguous()
+    out = torch.empty((t, hdim), dtype=odt, device=dev)
+    if t == 0:
+        return out.to(out_dtype)
+    L = lib()
+    sg, su, sd = (s.handle for s in shared) if shared is not None else (None, None, None)
+    gw = shared_gate.to(torch.float32).contiguous() if shared_gate is not None else None
+    with torch.cuda.device(dev):
+        wsb = int(L.qmm_moe_ffn_scored_workspace_size(gate.handle, down.handle, t, e, topk, sg, su, sd))
+        if wsb == 0:
+            raise QmmError(QMM_ERR_INVALID, "moe_ffn: " + last_error())
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        _check(L.qmm_moe_ffn_scored(xx.data_ptr(), _DENSE[xx.dtype], t, hdim, lg.data_ptr(), e, topk, tag, _ptr(bias),
+                                    groups, topk_groups, group_top, int(norm_topk_prob), routed_scaling_factor,
+                                    gate.handle, up.handle, down.handle, sg, su, sd, _ptr(gw), out.data_ptr(),
+                                    _DENSE[odt], hdim, ws.data_ptr(), wsb, _stream(dev)))
+    return out.to(out_dtype)
 
 
 # ---------------------------------------------------------------------------
@@ -646,6 +801,8 @@ class QuantizedLinear:
         return cls(QMatMul.from_qtensor(qt), bias)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.inner.qtensor._dtype == GgmlDType.MXFP4 and x.dtype in _DENSE:
+            return self.inner.linear(x, self.bias)
         y = self.inner.forward(x.to(torch.float32)).to(x.dtype)
         if self.bias is not None:
             y = y + self.bias.to(y.dtype)
