@@ -601,7 +601,7 @@ static size_t gemm_split_bytes(const qmm_qtensor* w, int64_t m);
 
 size_t qmm_matmul_workspace_size(const qmm_qtensor* w, int64_t m) {
   if (!w || m <= 0) return 0;
-  if (is_mx(w->dtype)) return mx_planes(m, w->k).total;
+  if (is_mx(w->dtype)) return mx_planes(m, w->k);
   const int vt = qmm_vec_dot_type(w->dtype);
   const size_t ggml = (size_t)m * (size_t)(w->k / qmm_block_size(vt)) * qmm_type_size(vt);
   if (!use_gemm(w, m)) return ggml;
@@ -1164,7 +1164,7 @@ static int check_matmul(const qmm_qtensor* w, int64_t m, const float* y, int64_t
 
 size_t qmm_matmul_q_workspace_size(const qmm_qtensor* w, int64_t m) {
   if (!w || m <= 0) return 0;
-  if (is_mx(w->dtype)) return mx_planes(m, w->k).total;
+  if (is_mx(w->dtype)) return mx_planes(m, w->k);
   if (!use_gemm(w, m)) return 0;
   return mmq_planes(w->dtype, m, w->k).total + gemm_split_bytes(w, m);
 }
@@ -1190,16 +1190,15 @@ static int mx_from_blocks(const GemvTarget* tg, int count, const void* xq, int64
                           size_t ws_bytes, hipStream_t s) {
   const int64_t k = tg[0].w->k;
   QMM_TRY(mx_check_rows(m, k));
-  const MxPlanes p = mx_planes(m, k);
-  if (!ws || ws_bytes < p.total)
-    return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed (qmm_matmul_q_workspace_size)", ws ? ws_bytes : 0, p.total);
+  const size_t need = mx_planes(m, k);
+  if (!ws || ws_bytes < need)
+    return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed (qmm_matmul_q_workspace_size)", ws ? ws_bytes : 0, need);
   Device* d;
   QMM_TRY(current_device(&d));
   uint8_t* b = (uint8_t*)ws;
   int mm = (int)m, kk = (int)k, kc = (int)mx_chunks(k);
-  void *q = b + p.q, *sc = b + p.s;
-  void* args[] = {&xq, &mm, &kk, &kc, &q, &sc};
-  QMM_TRY(launch(d, "qmm_mx_blocks_to_planes", ceil_div(m * kc * 8, 256), 256, 0, s, args));
+  void* args[] = {&xq, &mm, &kk, &kc, &b};
+  QMM_TRY(launch(d, "qmm_mx_blocks_to_planes", mx_plane_units(m, k), 256, 0, s, args));
   for (int j = 0; j < count; ++j) {
     MxOut o = {};
     o.y = tg[j].y;
@@ -1441,7 +1440,7 @@ static int mx_targets(const GemvTarget* tg, int count, const void* x, int x_dtyp
                       size_t ws_bytes, const float* norm_w, float eps, const MxOut& how, hipStream_t s) {
   const int64_t k = tg[0].w->k;
   QMM_TRY(mx_check_rows(m, k));
-  const size_t planes = mx_planes(m, k).total, need = planes + (norm_w ? align256((size_t)(m * k) * 4) : 0);
+  const size_t planes = mx_align(mx_planes(m, k)), need = planes + (norm_w ? align256((size_t)(m * k) * 4) : 0);
   if (!ws || ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
   Device* d;
   QMM_TRY(current_device(&d));
@@ -1452,7 +1451,7 @@ static int mx_targets(const GemvTarget* tg, int count, const void* x, int x_dtyp
     x = xn;
     ldx = k;
   }
-  QMM_TRY(mx_quantize_x(d, x, x_dtype, m, k, ldx, b, s));
+  QMM_TRY(mx_quantize_x(d, x, x_dtype, m, k, ldx, nullptr, b, s));
   for (int j = 0; j < count; ++j) {
     MxOut o = how;
     o.y = tg[j].y;
@@ -1806,8 +1805,8 @@ struct MxFfnWs {
 static MxFfnWs mx_ffn_ws(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t m, bool normalize) {
   MxFfnWs w;
   w.xp = 0;
-  w.hp = mx_planes(m, gate->k).total;
-  w.xn = w.hp + mx_planes(m, down->k).total;
+  w.hp = mx_align(mx_planes(m, gate->k));
+  w.xn = w.hp + mx_align(mx_planes(m, down->k));
   w.g = w.xn + (normalize ? align256((size_t)(m * gate->k) * 4) : 0);
   w.u = w.g + align256((size_t)(m * gate->n) * 4);
   w.total = w.u + align256((size_t)(m * gate->n) * 4);
@@ -1824,7 +1823,7 @@ static int mx_ffn(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, con
     x = xn;
     ldx = gate->k;
   }
-  QMM_TRY(mx_quantize_x(d, x, x_dtype, m, gate->k, ldx, b + L.xp, s));
+  QMM_TRY(mx_quantize_x(d, x, x_dtype, m, gate->k, ldx, nullptr, b + L.xp, s));
   MxOut o = {};
   o.y = b + L.g;
   QMM_TRY(mx_product(d, gate, b + L.xp, m, o, gate->n, s));
@@ -2669,7 +2668,7 @@ int qmm_moe_gemv(const qmm_qtensor* const* w, int count, int experts, const void
 // M tiles (grid z = expert; tiles past an expert's rows exit at once).
 size_t qmm_moe_gemm_workspace_size(const qmm_qtensor* w, int64_t pairs) {
   if (!w || pairs < 1) return 0;
-  if (is_mx(w->dtype)) return mx_planes(pairs, w->k).total;
+  if (is_mx(w->dtype)) return mx_planes(pairs, w->k);
   return mmq_planes(w->dtype, pairs, w->k).total;
 }
 
@@ -2703,8 +2702,8 @@ int qmm_moe_gemm(const qmm_qtensor* const* w, int count, int experts, const floa
   uint8_t* b = (uint8_t*)ws;
   if (is_mx(w0->dtype)) {
     QMM_TRY(mx_check_rows(pairs, w0->k));
-    QMM_TRY(mx_quantize_x(d, x, QMM_F32, pairs, w0->k, ldx, b, s));
-    return mx_expert_product(d, w, count, experts, b, pairs, pairs, max_rows, counts, offsets, nullptr, y, s);
+    QMM_TRY(mx_quantize_x(d, x, QMM_F32, pairs, w0->k, ldx, nullptr, b, s));
+    return mx_expert_product(d, w, count, experts, b, pairs, max_rows, counts, offsets, y, s);
   }
   QMM_TRY(quantize_planes(d, w0->dtype, x, pairs, w0->k, ldx, b, s));
   return moe_gemm_planes(d, w, count, experts, b, pairs, max_rows, counts, offsets, y, s);
@@ -2949,10 +2948,10 @@ static MxMoeWs mx_moe_ws(const qmm_qtensor* gate, int64_t tokens, int E, int k, 
   w.pair_weight = take(4 * P);
   w.token_pairs = take(4 * P);
   w.route = take(route_scratch(T, E, k));
-  w.xp = take(mx_planes(T, H).total);
+  w.xp = take(mx_planes(P, H));
   w.g = take(4 * (size_t)P * F);
   w.u = take(4 * (size_t)P * F);
-  w.hp = take(mx_planes(P, F).total);
+  w.hp = take(mx_planes(P, F));
   w.yp = take(4 * (size_t)P * H);
   if (sh.gate) {
     w.shared = take(4 * (size_t)T * H);
@@ -3054,9 +3053,8 @@ static int moe_shared(Device* d, const MoeShared& sh, const void* x, int x_dtype
   return launch(d, "qmm_mx_shared_gate", ceil_div(tokens, 4), 256, 0, s, args);
 }
 
-// The expert FFN with MXFP4 weights: routing, the tokens' digit planes (once a token;
-// the products take routed rows by token), gate and up, silu(g) * u as planes, down,
-// the weighted sums.
+// The expert FFN with MXFP4 weights: routing, the routed rows' digit planes, gate and up,
+// silu(g) * u as planes, down, the weighted sums.
 static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const float* logits, int experts, int topk,
                   const Routing& r, const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down,
                   const MoeShared& sh, void* out, int out_dtype, int64_t ldo, uint8_t* b, hipStream_t s) {
@@ -3071,12 +3069,12 @@ static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const
     const int64_t T = std::min(chunk, tokens - t0), P = T * topk;
     const uint8_t* xc = (const uint8_t*)x + t0 * ldx * (int64_t)mx_type_size(x_dtype);
     QMM_TRY(route_scored(d, logits + t0 * experts, T, experts, topk, r, counts, offsets, ptok, pw, tpairs, b + L.route, s));
-    QMM_TRY(mx_quantize_x(d, xc, x_dtype, T, H, ldx, b + L.xp, s));
+    QMM_TRY(mx_quantize_x(d, xc, x_dtype, P, H, ldx, ptok, b + L.xp, s));
     const qmm_qtensor* gw[2] = {gate, up};
     float* gy[2] = {g, u};
-    QMM_TRY(mx_expert_product(d, gw, 2, experts, b + L.xp, T, P, T, counts, offsets, ptok, gy, s));
+    QMM_TRY(mx_expert_product(d, gw, 2, experts, b + L.xp, P, T, counts, offsets, gy, s));
     QMM_TRY(mx_silu_mul(d, g, u, P, F, b + L.hp, s));
-    QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, P, T, counts, offsets, nullptr, &yp, s));
+    QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, T, counts, offsets, &yp, s));
     float *shared = nullptr, *sg = nullptr;
     if (sh.gate) {
       shared = (float*)(b + L.shared);
@@ -3112,7 +3110,7 @@ static int moe_ffn(const void* xv, int x_dtype, int64_t tokens, int64_t ldx, con
     if (!r.scored && r.renormalize) r.scale = 1.0f;  // (qmm_moe_route_ex scales without renormalizing only)
     const int64_t chunk = std::min(tokens, mx_moe_chunk(topk)), pairs = chunk * topk;
     QMM_TRY(check_routing(chunk, experts, topk, r));
-    QMM_TRY(mx_check_rows(chunk, gate->k));
+    QMM_TRY(mx_check_rows(pairs, gate->k));
     QMM_TRY(mx_check_rows(pairs, down->k));
     const size_t need = mx_moe_ws(gate, tokens, experts, topk, sh).total;
     if (ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws_bytes, need);

@@ -35,10 +35,16 @@ constexpr int kMxChunk = 256;
 constexpr int kMxStepBytes = 1024;
 constexpr int kMxScaleOff = 4096;
 constexpr int kMxUnit = 4352;
-// Digit planes of activation rows: per row and chunk 8 blocks x (24 bytes of hi,
-// 24 of lo), and apart from them 8 scale bytes, [h][s] for block 2 s + h.
-constexpr int kMxDigitBlock = 48;
-constexpr int kMxDigitChunk = 8 * kMxDigitBlock;
+// Digit planes of activation rows: units of 32 rows x 256 columns in the same order, so
+// that every operand load is contiguous. Step s holds, for 64 lanes (lane 32 h + r:
+// block 2 s + h of row r), the first 16 bytes of hi, the first 16 of lo, the last 8 of
+// hi, the last 8 of lo: a digit is one operand of six registers, loaded by a 16-byte
+// and an 8-byte read (parts that straddled the digits cost a move a register). Then
+// 64 lanes x 4 scale bytes. Rows past the last are left as
+// they are: a column of the product reads its own row only.
+constexpr int kMxXStep = 3072, kMxXLo = 1024, kMxXTail = 2048;
+constexpr int kMxXScaleOff = 4 * kMxXStep;
+constexpr int kMxXUnit = kMxXScaleOff + 256;
 constexpr int kMxFp4Bytes = 17;   // GGML block: e, codes 0..15 in low nibbles, 16..31 in high ones
 constexpr int kMxFp6x2Bytes = 49; // block of qmm_quantize_rows: e, hi[24], lo[24]
 constexpr int kMxNan = 255;
@@ -89,37 +95,55 @@ __device__ __forceinline__ int mx_w_byte(uint32_t amax) { return amax == 0 ? 0 :
 // (the second digit's scale is four binades lower)
 __device__ __forceinline__ int mx_x_byte(uint32_t amax) { return mx_scale_byte<kMxMan6>(amax, 4); }
 
+// 32 values (even ones in `a`, odd ones in `b`) as one E2M3 digit each. The instruction
+// writes its first registers before it has read its last, and the compiler gives the
+// result registers of an operand that ends here: the operands are kept past it.
+__device__ __forceinline__ mx_u32x6 mx_to_digit(const mx_f32x16& a, const mx_f32x16& b) {
+  const auto d = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 1.0f);
+  asm volatile("" ::"v"(a), "v"(b), "v"(d));
+  return __builtin_bit_cast(mx_u32x6, d);
+}
+// and back, in order
+typedef float mx_f32x32 __attribute__((ext_vector_type(32)));
+__device__ __forceinline__ mx_f32x32 mx_from_digit(const mx_u32x6& d) {
+  const mx_f32x32 v = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(d, 1.0f);
+  asm volatile("" ::"v"(d), "v"(v));
+  return v;
+}
+
 // Both digits of 32 values under scale byte e as 24 + 24 bytes. A block with e = 255
 // gets zero digits (0 * NaN is NaN in the product).
 __device__ __forceinline__ void mx_digits(const float (&x)[32], int e, mx_u32x6& hi, mx_u32x6& lo) {
   mx_f32x16 a, b;
   const int up = 127 - e;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {  // the conversion takes even values from one operand, odd ones from the other
+  for (int j = 0; j < 16; ++j) {
     a[j] = e == kMxNan ? 0.0f : __builtin_ldexpf(x[2 * j], up);
     b[j] = e == kMxNan ? 0.0f : __builtin_ldexpf(x[2 * j + 1], up);
   }
-  hi = __builtin_bit_cast(mx_u32x6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 1.0f));
-  typedef float f32x32 __attribute__((ext_vector_type(32)));
-  const f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(hi, 1.0f);
+  hi = mx_to_digit(a, b);
+  const mx_f32x32 back = mx_from_digit(hi);
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     a[j] = (a[j] - back[2 * j]) * 16.0f;
     b[j] = (b[j] - back[2 * j + 1]) * 16.0f;
   }
-  lo = __builtin_bit_cast(mx_u32x6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 1.0f));
+  lo = mx_to_digit(a, b);
 }
 
-// One step (64 columns) of a 32 x 32 tile: weights (A, rows of the result) times
-// both digits of the activations (B, columns). S: the byte of the scale registers.
+// One step (64 columns) of a 32 x 32 tile by one digit: weights (A, rows of the result)
+// times activations (B, columns). S: the byte of the scale registers.
+template <int S>
+__device__ __forceinline__ mx_f32x16 mx_mfma1(const mx_u32x4& w, const mx_u32x6& x, mx_f32x16 c, int sw, int sx) {
+  const mx_i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+  const mx_i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)x[4], (int)x[5], 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 2, S, sw, S, sx);
+}
+// by both digits, the second's scale being sx - 4 in every byte
 template <int S>
 __device__ __forceinline__ mx_f32x16 mx_mfma(const mx_u32x4& w, const mx_u32x6& hi, const mx_u32x6& lo, mx_f32x16 c,
                                              int sw, int sx, int sx_lo) {
-  const mx_i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-  const mx_i32x8 h = {(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3], (int)hi[4], (int)hi[5], 0, 0};
-  const mx_i32x8 l = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)lo[4], (int)lo[5], 0, 0};
-  c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, h, c, 4, 2, S, sw, S, sx);
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, l, c, 4, 2, S, sw, S, sx_lo);
+  return mx_mfma1<S>(w, lo, mx_mfma1<S>(w, hi, c, sw, sx), sw, sx_lo);
 }
 // (result: lane's column = lane & 31, register r its row 8 (r / 4) + 4 (lane / 32) + r % 4)
 

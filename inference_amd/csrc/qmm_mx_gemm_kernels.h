@@ -12,16 +12,15 @@ struct MxOut {
   void* y;
   const void* bias;  // [n] or null
   int y_type, bias_type;
-  int accumulate;    // y += (f32)
+  int accumulate;    // y +=
+  int wide;          // rows of y start on a boundary of four values
 };
 
-// Which rows a workgroup multiplies: rows [first, first + count) of the output, whose
-// activations are rows src[first + i] (or first + i) of the planes, by rows
-// [w0, w0 + n) of the stacked weights.
+// Which rows a workgroup multiplies: rows [first, first + count) of the planes and of
+// the output by rows [w0, w0 + n) of the stacked weights.
 struct MxRows {
   long long w0;
   int first, count;
-  const int* src;
 };
 
 // Tile `y` of an expert-ordered list, BM rows a tile: the expert and the tile's rows.
@@ -29,8 +28,7 @@ struct MxRows {
 // the experts. False past the last tile. Every lane of a wave takes 64 experts' counts
 // at a time. Counts and offsets are the caller's: they are cut to [0, pairs].
 __device__ __forceinline__ bool mx_expert_tile(const int* __restrict__ counts, const int* __restrict__ offsets,
-                                               int experts, int pairs, int n, int bm, int y,
-                                               const int* __restrict__ src, MxRows& r) {
+                                               int experts, int pairs, int n, int bm, int y, MxRows& r) {
   const int lane = threadIdx.x & 63;
   int base = 0;
   for (int e0 = 0; e0 < experts; e0 += 64) {
@@ -55,7 +53,6 @@ __device__ __forceinline__ bool mx_expert_tile(const int* __restrict__ counts, c
       r.w0 = (long long)(e0 + l) * n;
       r.first = o + t * bm;
       r.count = min(c - t * bm, bm);
-      r.src = src;
       return true;
     }
     base += __shfl(sum, 63);
@@ -63,53 +60,101 @@ __device__ __forceinline__ bool mx_expert_tile(const int* __restrict__ counts, c
   return false;
 }
 
-// A lane's place in the weight's units: row `row` (clamped by the caller), lane half h.
+// A lane's place in the units: row `row` of the weight or of the planes (clamped by the
+// caller), lane half h. Rows need not start on a tile: experts' rows follow each other.
 __device__ __forceinline__ long long mx_w_at(long long row, int h, int kc) {
   return (row >> 5) * ((long long)kc * kMxUnit) + 512 * h + 16 * (row & 31);
 }
 __device__ __forceinline__ long long mx_ws_at(long long row, int h, int kc) {
   return (row >> 5) * ((long long)kc * kMxUnit) + kMxScaleOff + 128 * h + 4 * (row & 31);
 }
-
-__device__ __forceinline__ void mx_get_digits(const uint8_t* __restrict__ p, mx_u32x6& hi, mx_u32x6& lo) {
-  const mx_u32x4* q = reinterpret_cast<const mx_u32x4*>(p);
-  const mx_u32x4 a = q[0], b = q[1], c = q[2];
-  hi = mx_u32x6{a[0], a[1], a[2], a[3], b[0], b[1]};
-  lo = mx_u32x6{b[2], b[3], c[0], c[1], c[2], c[3]};
+__device__ __forceinline__ long long mx_x_at(long long row, int kc) { return (row >> 5) * ((long long)kc * kMxXUnit); }
+__device__ __forceinline__ long long mx_xs_at(long long row, int h, int kc) {
+  return (row >> 5) * ((long long)kc * kMxXUnit) + kMxXScaleOff + 128 * h + 4 * (row & 31);
 }
 
-__device__ __forceinline__ void mx_finish(const MxOut& o, long long row, int ldy, int col, float v) {
+// A lane's block of a step as its two digits, from the step's memory or LDS. `l`: the
+// lane's place, 16 (32 h + r).
+struct MxX {
+  mx_u32x6 hi, lo;
+};
+__device__ __forceinline__ mx_u32x6 mx_digit(const uint8_t* p, const uint8_t* tail) {
+  const mx_u32x4 a = *reinterpret_cast<const mx_u32x4*>(p);
+  const mx_u32x2 b = *reinterpret_cast<const mx_u32x2*>(tail);
+  return mx_u32x6{a[0], a[1], a[2], a[3], b[0], b[1]};
+}
+__device__ __forceinline__ MxX mx_get_x(const uint8_t* step, unsigned l) {
+  MxX x;
+  x.hi = mx_digit(step + l, step + kMxXTail + l / 2);
+  x.lo = mx_digit(step + kMxXLo + l, step + kMxXTail + 512 + l / 2);
+  return x;
+}
+
+template <int T>
+struct MxType {
+  static constexpr int value = T;
+};
+
+// Four columns of a row of the output from col on (those below n).
+__device__ __forceinline__ mx_f32x4 mx_bias4(const MxOut& o, int col, int n) {
+  mx_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (o.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < n) v[j] = mx_load(o.bias, o.bias_type, col + j);
+  }
+  return v;
+}
+template <int T>
+__device__ __forceinline__ void mx_put4(const MxOut& o, long long row, int ldy, int col, int n, mx_f32x4 v) {
   const long long at = row * ldy + col;
-  if (o.bias != nullptr) v += mx_load(o.bias, o.bias_type, col);
-  if (o.accumulate) v += mx_load(o.y, o.y_type, at);
-  mx_store(o.y, o.y_type, at, v);
+  if (o.wide && col + 3 < n) {
+    if constexpr (T == kF32) {
+      mx_f32x4* p = reinterpret_cast<mx_f32x4*>(static_cast<float*>(o.y) + at);
+      if (o.accumulate) v += *p;
+      *p = v;
+    } else {
+      *reinterpret_cast<mx_u32x2*>(static_cast<uint16_t*>(o.y) + at) =
+          mx_u32x2{mx_to16(v[0], T) | (uint32_t)mx_to16(v[1], T) << 16, mx_to16(v[2], T) | (uint32_t)mx_to16(v[3], T) << 16};
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (col + j < n) {
+      if constexpr (T == kF32) {
+        float* p = static_cast<float*>(o.y) + at + j;
+        *p = o.accumulate ? *p + v[j] : v[j];
+      } else {
+        static_cast<uint16_t*>(o.y)[at + j] = mx_to16(v[j], T);
+      }
+    }
 }
 
 // Up to 32 rows: a workgroup of W waves takes one 32-column tile of the output and
 // splits K over its waves by chunks; the waves' sums meet in LDS, in wave order.
 template <int W>
 __device__ __forceinline__ void mx_gemv(const MxOut& o, const MxRows& rows, int n, int kc, int tile,
-                                        const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xs, int ldy) {
+                                        const uint8_t* __restrict__ xq, int ldy) {
   __shared__ float red[W][32][33];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, c = lane & 31;
-  const int col = min(kMxTile * tile + c, n - 1);
-  const long long wrow = rows.w0 + col;
-  const int i = rows.first + min(c, rows.count - 1);
-  const long long xrow = rows.src ? rows.src[i] : i;
+  const long long wrow = rows.w0 + min(kMxTile * tile + c, n - 1);
+  const long long xrow = rows.first + min(c, rows.count - 1);
   const uint8_t* wp = o.w + mx_w_at(wrow, h, kc);
   const uint8_t* wsp = o.w + mx_ws_at(wrow, h, kc);
-  const uint8_t* xp = xq + xrow * kc * kMxDigitChunk + kMxDigitBlock * h;
-  const int* sp = reinterpret_cast<const int*>(xs + xrow * kc * 8) + h;
+  const uint8_t* xp = xq + mx_x_at(xrow, kc);
+  const unsigned xl = 512 * h + 16 * (unsigned)(xrow & 31);
+  const uint8_t* xsp = xq + mx_xs_at(xrow, h, kc);
   mx_f32x16 acc = (mx_f32x16)(0.0f);
   for (int k = wave; k < kc; k += W) {
     const uint8_t* wk = wp + (long long)k * kMxUnit;
-    const uint8_t* xk = xp + (long long)k * kMxDigitChunk;
+    const uint8_t* xk = xp + (long long)k * kMxXUnit;
     const int sw = *reinterpret_cast<const int*>(wsp + (long long)k * kMxUnit);
-    const int sx = sp[2 * k], sl = sx - 0x04040404;
-    mx_u32x6 hi, lo;
-#define QMM_MX_STEP(S)                                                    \
-  mx_get_digits(xk + S * 2 * kMxDigitBlock, hi, lo);                      \
-  acc = mx_mfma<S>(*reinterpret_cast<const mx_u32x4*>(wk + S * kMxStepBytes), hi, lo, acc, sw, sx, sl);
+    const int sx = *reinterpret_cast<const int*>(xsp + (long long)k * kMxXUnit), sl = sx - 0x04040404;
+    MxX x;
+#define QMM_MX_STEP(S)                                                                                          \
+  x = mx_get_x(xk + S * kMxXStep, xl);                                                                          \
+  acc = mx_mfma<S>(*reinterpret_cast<const mx_u32x4*>(wk + S * kMxStepBytes), x.hi, x.lo, acc, sw, sx, sl);
     QMM_MX_STEP(0)
     QMM_MX_STEP(1)
     QMM_MX_STEP(2)
@@ -119,79 +164,181 @@ __device__ __forceinline__ void mx_gemv(const MxOut& o, const MxRows& rows, int 
 #pragma unroll
   for (int r = 0; r < 16; ++r) red[wave][c][8 * (r >> 2) + 4 * h + (r & 3)] = acc[r];
   __syncthreads();
-  for (int j = t; j < 32 * rows.count; j += 64 * W) {
-    const int m = j >> 5, q = j & 31;
-    if (kMxTile * tile + q >= n) continue;
-    float v = red[0][m][q];
+  for (int j = t; j < 8 * rows.count; j += 64 * W) {
+    const int m = j >> 3, q = 4 * (j & 7), col = kMxTile * tile + q;
+    mx_f32x4 v;
 #pragma unroll
-    for (int w = 1; w < W; ++w) v += red[w][m][q];
-    mx_finish(o, rows.first + m, ldy, kMxTile * tile + q, v);
+    for (int i = 0; i < 4; ++i) {
+      v[i] = red[0][m][q + i];
+#pragma unroll
+      for (int w = 1; w < W; ++w) v[i] += red[w][m][q + i];
+    }
+    v += mx_bias4(o, col, n);
+    if (o.y_type == kF32) mx_put4<kF32>(o, rows.first + m, ldy, col, n, v);
+    else if (o.y_type == kF16) mx_put4<kF16>(o, rows.first + m, ldy, col, n, v);
+    else mx_put4<kBF16>(o, rows.first + m, ldy, col, n, v);
   }
 }
 
-// 64 rows x 64 columns a wave, straight from memory.
-__device__ __forceinline__ void mx_tile(const MxOut& o, const MxRows& rows, int n, int kc, int col0,
-                                        const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xs, int ldy) {
-  const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
-  const uint8_t *wp[2], *wsp[2], *xp[2];
-  const int* sp[2];
+// A tile of 32 FM WM rows x 32 FN WN columns by WM x WN waves, a wave 32 FM x 32 FN of it.
+// RW steps of weights in registers (this one and those on their way).
+template <int FM, int FN, int WM, int WN, int RW>
+__device__ __forceinline__ void mx_gemm(const MxOut& o, const MxRows& rows, int n, int kc, int n0,
+                                        const uint8_t* __restrict__ xq, int ldy) {
+  constexpr int NW = WM * WN, XF = FM * WM, FW = XF / NW;
+  static_assert(XF % NW == 0, "whole fragments a wave");
+  constexpr int kStage = XF * kMxXStep;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, c = lane & 31, wm = wave % WM, wn = wave / WM;
+  // 64-bit bases at the tile's first row, 32-bit offsets from them
+  const long long xt = rows.first >> 5;
+  const uint8_t* xb = xq + xt * ((long long)kc * kMxXUnit);
+  // the fragments that this wave brings to LDS: a lane's place in the 16-byte and in
+  // the 8-byte parts
+  unsigned xo[FW][2], xso[FM], wo[FN], wso[FN];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const long long wrow = rows.w0 + min(col0 + 32 * j + c, n - 1);
-    const int i = rows.first + min(32 * j + c, rows.count - 1);
-    const long long xrow = rows.src ? rows.src[i] : i;
-    wp[j] = o.w + mx_w_at(wrow, h, kc);
-    wsp[j] = o.w + mx_ws_at(wrow, h, kc);
-    xp[j] = xq + xrow * kc * kMxDigitChunk + kMxDigitBlock * h;
-    sp[j] = reinterpret_cast<const int*>(xs + xrow * kc * 8) + h;
+  for (int j = 0; j < FW; ++j) {
+    const long long r = rows.first + min(32 * (FW * wave + j) + c, rows.count - 1) - 32 * xt;
+    xo[j][0] = (unsigned)mx_x_at(r, kc) + 512 * h + 16 * (unsigned)(r & 31);
+    xo[j][1] = (unsigned)mx_x_at(r, kc) + kMxXTail + 256 * h + 8 * (unsigned)(r & 31);
   }
-  mx_f32x16 acc[2][2] = {{(mx_f32x16)(0.0f), (mx_f32x16)(0.0f)}, {(mx_f32x16)(0.0f), (mx_f32x16)(0.0f)}};
-  for (int k = 0; k < kc; ++k) {
-    int sw[2], sx[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      sw[j] = *reinterpret_cast<const int*>(wsp[j] + (long long)k * kMxUnit);
-      sx[j] = sp[j][2 * k];
+  for (int b = 0; b < FM; ++b)
+    xso[b] = (unsigned)mx_xs_at(rows.first + min(32 * (FM * wm + b) + c, rows.count - 1) - 32 * xt, h, kc);
+  const long long wt = (rows.w0 + n0) >> 5;
+  const uint8_t* wb = o.w + wt * ((long long)kc * kMxUnit);
+#pragma unroll
+  for (int a = 0; a < FN; ++a) {
+    const long long r = rows.w0 + min(n0 + 32 * (FN * wn + a) + c, n - 1) - 32 * wt;
+    wo[a] = (unsigned)mx_w_at(r, h, kc);
+    wso[a] = (unsigned)mx_ws_at(r, h, kc);
+  }
+  mx_f32x16 acc[FN][FM];
+#pragma unroll
+  for (int a = 0; a < FN; ++a)
+#pragma unroll
+    for (int b = 0; b < FM; ++b) acc[a][b] = (mx_f32x16)(0.0f);
+
+  MxX st[FW];            // x on its way to LDS
+  mx_u32x4 w[RW][FN];    // weights of this step and the next ones
+  MxX x[2][FM];          // x of this step and the next
+  int sw[2][FN], sx[2][FM];
+  auto load_x = [&](int k, int s) {
+    const unsigned at = (unsigned)k * kMxXUnit + s * kMxXStep;
+#pragma unroll
+    for (int j = 0; j < FW; ++j) {
+      const uint8_t* p = xb + (xo[j][0] + at);
+      const uint8_t* q = xb + (xo[j][1] + at);
+      st[j].hi = mx_digit(p, q);
+      st[j].lo = mx_digit(p + kMxXLo, q + 512);
     }
-#define QMM_MX_STEP(S)                                                                                               \
-  {                                                                                                                  \
-    mx_u32x4 w[2];                                                                                                   \
-    mx_u32x6 hi[2], lo[2];                                                                                           \
-    _Pragma("unroll") for (int j = 0; j < 2; ++j) {                                                                  \
-      w[j] = *reinterpret_cast<const mx_u32x4*>(wp[j] + (long long)k * kMxUnit + S * kMxStepBytes);                  \
-      mx_get_digits(xp[j] + (long long)k * kMxDigitChunk + S * 2 * kMxDigitBlock, hi[j], lo[j]);                     \
-    }                                                                                                                \
-    _Pragma("unroll") for (int a = 0; a < 2; ++a) _Pragma("unroll") for (int b = 0; b < 2; ++b) acc[a][b] =           \
-        mx_mfma<S>(w[a], hi[b], lo[b], acc[a][b], sw[a], sx[b], sx[b] - 0x04040404);                                 \
+  };
+  auto put_x = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < FW; ++j) {
+      uint8_t* d = &lds[buf][kMxXStep * (FW * wave + j)];
+      const mx_u32x6 u = st[j].hi, v = st[j].lo;
+      *reinterpret_cast<mx_u32x4*>(d + 16 * lane) = mx_u32x4{u[0], u[1], u[2], u[3]};
+      *reinterpret_cast<mx_u32x4*>(d + kMxXLo + 16 * lane) = mx_u32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<mx_u32x2*>(d + kMxXTail + 8 * lane) = mx_u32x2{u[4], u[5]};
+      *reinterpret_cast<mx_u32x2*>(d + kMxXTail + 512 + 8 * lane) = mx_u32x2{v[4], v[5]};
+    }
+  };
+  auto get_x = [&](int buf, MxX (&d)[FM]) {
+#pragma unroll
+    for (int b = 0; b < FM; ++b) d[b] = mx_get_x(&lds[buf][kMxXStep * (FM * wm + b)], 16 * lane);
+  };
+  auto load_w = [&](int k, int s, mx_u32x4 (&d)[FN]) {
+    const unsigned at = (unsigned)k * kMxUnit + s * kMxStepBytes;
+#pragma unroll
+    for (int a = 0; a < FN; ++a) d[a] = *reinterpret_cast<const mx_u32x4*>(wb + (wo[a] + at));
+  };
+  auto load_s = [&](int k, int i) {
+#pragma unroll
+    for (int a = 0; a < FN; ++a) sw[i][a] = *reinterpret_cast<const int*>(wb + (wso[a] + (unsigned)k * kMxUnit));
+#pragma unroll
+    for (int b = 0; b < FM; ++b) sx[i][b] = *reinterpret_cast<const int*>(xb + (xso[b] + (unsigned)k * kMxXUnit));
+  };
+  auto sync = [] {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's writes are in LDS
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  load_s(0, 0);
+  load_x(0, 0);
+#pragma unroll
+  for (int s = 0; s < RW - 1; ++s) load_w(0, s, w[s]);
+  put_x(0);
+  load_x(0, 1);
+  sync();
+  get_x(0, x[0]);
+#define QMM_MX_HALF(S, I, B0, B1)                                                                              \
+  _Pragma("unroll") for (int b = B0; b < B1; ++b) {                                                            \
+    _Pragma("unroll") for (int a = 0; a < FN; ++a) acc[a][b] =                                                 \
+        mx_mfma1<S>(w[S % RW][a], x[S & 1][b].hi, acc[a][b], sw[I][a], sx[I][b]);                              \
+    _Pragma("unroll") for (int a = 0; a < FN; ++a) acc[a][b] =                                                 \
+        mx_mfma1<S>(w[S % RW][a], x[S & 1][b].lo, acc[a][b], sw[I][a], sx[I][b] - 0x04040404);                 \
   }
-    QMM_MX_STEP(0)
-    QMM_MX_STEP(1)
-    QMM_MX_STEP(2)
-    QMM_MX_STEP(3)
+#define QMM_MX_STEP(S, I)                                                                                      \
+  {                                                                                                            \
+    put_x((S + 1) & 1);                                                                                        \
+    load_x(S + 2 < 4 ? k : kn, (S + 2) & 3);                                                                   \
+    load_w(S + RW - 1 < 4 ? k : kn, (S + RW - 1) & 3, w[(S + RW - 1) % RW]);                                   \
+    if (S == 1) load_s(kn, 1 - I);                                                                             \
+    __builtin_amdgcn_sched_barrier(0);                                                                         \
+    QMM_MX_HALF(S, I, 0, FM / 2)                                                                               \
+    sync();                                                                                                    \
+    get_x((S + 1) & 1, x[(S + 1) & 1]);                                                                        \
+    __builtin_amdgcn_sched_barrier(0);                                                                         \
+    QMM_MX_HALF(S, I, FM / 2, FM)                                                                              \
+  }
+  // (past the last chunk the loads read it again, and what they bring is not used)
+#pragma unroll 1
+  for (int k = 0; k < kc; ++k) {
+    const int kn = min(k + 1, kc - 1);
+    QMM_MX_STEP(0, 0)
+    QMM_MX_STEP(1, 0)
+    QMM_MX_STEP(2, 0)
+    QMM_MX_STEP(3, 0)
+#pragma unroll
+    for (int a = 0; a < FN; ++a) sw[0][a] = sw[1][a];
+#pragma unroll
+    for (int b = 0; b < FM; ++b) sx[0][b] = sx[1][b];
+  }
 #undef QMM_MX_STEP
-  }
+#undef QMM_MX_HALF
+  auto put = [&](auto type) {
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int m = 32 * b + c;
-    if (m >= rows.count) continue;
+    for (int a = 0; a < FN; ++a)
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+      for (int q = 0; q < 4; ++q) {
+        const int col = n0 + 32 * (FN * wn + a) + 8 * q + 4 * h;
+        const mx_f32x4 bias = mx_bias4(o, col, n);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int q = col0 + 32 * a + 8 * (r >> 2) + 4 * h + (r & 3);
-        if (q < n) mx_finish(o, rows.first + m, ldy, q, acc[a][b][r]);
+        for (int b = 0; b < FM; ++b) {
+          const int m = 32 * (FM * wm + b) + c;
+          mx_f32x4 v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = acc[a][b][4 * q + j] + bias[j];
+          if (m < rows.count) mx_put4<decltype(type)::value>(o, rows.first + m, ldy, col, n, v);
+        }
       }
-  }
+  };
+  if (o.y_type == kF32) put(MxType<kF32>{});
+  else if (o.y_type == kF16) put(MxType<kF16>{});
+  else put(MxType<kBF16>{});
 }
 }  // namespace qmm
 
 // Dense rows: grid (32-column tiles, 32-row tiles).
 extern "C" __global__ void __launch_bounds__(512) qmm_mx_gemv(qmm::MxOut o, int m, int n, int kc,
-                                                              const uint8_t* __restrict__ xq,
-                                                              const uint8_t* __restrict__ xs, int ldy) {
+                                                              const uint8_t* __restrict__ xq, int ldy) {
   const int first = 32 * blockIdx.y;
-  const qmm::MxRows r = {0, first, min(m - first, 32), nullptr};
-  qmm::mx_gemv<8>(o, r, n, kc, blockIdx.x, xq, xs, ldy);
+  const qmm::MxRows r = {0, first, min(m - first, 32)};
+  qmm::mx_gemv<8>(o, r, n, kc, blockIdx.x, xq, ldy);
 }
 
 // Routed rows: grid (32-column tiles, row tiles, weights).
@@ -199,36 +346,28 @@ extern "C" __global__ void __launch_bounds__(512) qmm_mx_expert_gemv(qmm::MxOut 
                                                                      int pairs, int n, int kc,
                                                                      const int* __restrict__ counts,
                                                                      const int* __restrict__ offsets,
-                                                                     const int* __restrict__ src,
-                                                                     const uint8_t* __restrict__ xq,
-                                                                     const uint8_t* __restrict__ xs, int ldy) {
+                                                                     const uint8_t* __restrict__ xq, int ldy) {
   qmm::MxRows r;
-  if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 32, blockIdx.y, src, r)) return;
-  qmm::mx_gemv<8>(blockIdx.z ? o1 : o0, r, n, kc, blockIdx.x, xq, xs, ldy);
+  if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 32, blockIdx.y, r)) return;
+  qmm::mx_gemv<8>(blockIdx.z ? o1 : o0, r, n, kc, blockIdx.x, xq, ldy);
 }
 
-// Dense rows: grid (256-column tiles, 64-row tiles), a wave 64 of the columns.
-extern "C" __global__ void __launch_bounds__(256) qmm_mx_gemm(qmm::MxOut o, int m, int n, int kc,
-                                                              const uint8_t* __restrict__ xq,
-                                                              const uint8_t* __restrict__ xs, int ldy) {
-  const int first = 64 * blockIdx.y;
-  const qmm::MxRows r = {0, first, min(m - first, 64), nullptr};
-  const int col0 = 256 * blockIdx.x + 64 * (threadIdx.x >> 6);
-  if (col0 < n) qmm::mx_tile(o, r, n, kc, col0, xq, xs, ldy);
-}
-
-extern "C" __global__ void __launch_bounds__(256) qmm_mx_expert_gemm(qmm::MxOut o0, qmm::MxOut o1, int experts,
-                                                                     int pairs, int n, int kc,
-                                                                     const int* __restrict__ counts,
-                                                                     const int* __restrict__ offsets,
-                                                                     const int* __restrict__ src,
-                                                                     const uint8_t* __restrict__ xq,
-                                                                     const uint8_t* __restrict__ xs, int ldy) {
-  qmm::MxRows r;
-  if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 64, blockIdx.y, src, r)) return;
-  const int col0 = 256 * blockIdx.x + 64 * (threadIdx.x >> 6);
-  if (col0 < n) qmm::mx_tile(blockIdx.z ? o1 : o0, r, n, kc, col0, xq, xs, ldy);
-}
+#define QMM_MX_GEMM(NAME, FM, FN, WM, WN, RW, EU)                                                              \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN, EU) qmm_mx_gemm_##NAME(                           \
+      qmm::MxOut o, int m, int n, int kc, const uint8_t* __restrict__ xq, int ldy) {                           \
+    const int first = 32 * FM * WM * blockIdx.y;                                                               \
+    const qmm::MxRows r = {0, first, min(m - first, 32 * FM * WM)};                                            \
+    qmm::mx_gemm<FM, FN, WM, WN, RW>(o, r, n, kc, 32 * FN * WN * blockIdx.x, xq, ldy);                             \
+  }                                                                                                            \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN, EU) qmm_mx_expert_gemm_##NAME(                    \
+      qmm::MxOut o0, qmm::MxOut o1, int experts, int pairs, int n, int kc, const int* __restrict__ counts,     \
+      const int* __restrict__ offsets, const uint8_t* __restrict__ xq, int ldy) {                              \
+    qmm::MxRows r;                                                                                             \
+    if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 32 * FM * WM, blockIdx.y, r)) return;         \
+    qmm::mx_gemm<FM, FN, WM, WN, RW>(blockIdx.z ? o1 : o0, r, n, kc, 32 * FN * WN * blockIdx.x, xq, ldy);          \
+  }
+QMM_MX_GEMM(256x256, 4, 4, 2, 2, 2, 1)
+QMM_MX_GEMM(128x256, 2, 4, 2, 2, 2, 2)
 
 // out[t] = sum over token t's pairs, in increasing expert order, of weight * yp[pair],
 // then + shared[t] (times sg[t] when the shared expert is gated), rounded once to the

@@ -6,7 +6,7 @@
 namespace {
 
 // qmm_mx_common.h's layout constants.
-constexpr int64_t kMxTile = 32, kMxChunk = 256, kMxUnit = 4352, kMxDigitChunk = 384;
+constexpr int64_t kMxTile = 32, kMxChunk = 256, kMxUnit = 4352, kMxXUnit = 12544;
 
 bool is_mx(int dtype) { return dtype == QMM_MXFP4; }
 
@@ -17,16 +17,9 @@ size_t mx_weight_bytes(int64_t n, int64_t k) {
 
 size_t mx_align(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// Digit planes of m rows of k values: digits, then scale bytes.
-struct MxPlanes {
-  size_t q, s, total;
-};
-MxPlanes mx_planes(int64_t m, int64_t k) {
-  MxPlanes p;
-  p.q = 0;
-  p.s = mx_align((size_t)m * (size_t)(mx_chunks(k) * kMxDigitChunk));
-  p.total = p.s + mx_align((size_t)m * (size_t)(mx_chunks(k) * 8));
-  return p;
+// Bytes of the digit planes of m rows of k values.
+size_t mx_planes(int64_t m, int64_t k) {
+  return (size_t)((m + kMxTile - 1) / kMxTile) * (size_t)mx_chunks(k) * (size_t)kMxXUnit;
 }
 
 const char* mx_type_name(int dtype) {
@@ -65,28 +58,31 @@ int mx_dequantize(Device* d, const void* w, int64_t n, int64_t k, void* dst, int
   return mx_ggml(d, name, w, n, k, dst, s);
 }
 
-// Whether rows of a typed matrix all start on 16-byte boundaries.
+// Whether rows of a typed matrix all start on a boundary of four values.
 int mx_wide(const void* x, int dtype, int64_t ldx) {
-  return (uintptr_t)x % 16 == 0 && (ldx * (int64_t)mx_type_size(dtype)) % 16 == 0;
+  const int64_t four = 4 * (int64_t)mx_type_size(dtype);
+  return (uintptr_t)x % four == 0 && ldx % 4 == 0;
 }
 
-// Activation limits: 32-bit offsets within a workgroup's rows, one thread a block.
+// Activation limits: a workgroup's rows are reached by 32-bit offsets (nine 32-row
+// tiles of the planes), a grid has fewer than 2^31 units.
 int mx_check_rows(int64_t m, int64_t k) {
-  if (m > (1LL << 21) || k > (1LL << 24) || m * mx_chunks(k) > (1LL << 30))
+  if (m > (1LL << 21) || k > (1LL << 21) || (m + kMxTile - 1) / kMxTile * mx_chunks(k) > (1LL << 30))
     return fail(QMM_ERR_INVALID, "activation of %lld x %lld is too large", (long long)m, (long long)k);
   return QMM_OK;
 }
 
-int mx_quantize_x(Device* d, const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, uint8_t* ws,
-                  hipStream_t s) {
-  const MxPlanes p = mx_planes(m, k);
+unsigned mx_plane_units(int64_t m, int64_t k) { return (unsigned)((m + kMxTile - 1) / kMxTile * mx_chunks(k)); }
+
+// Planes of m rows: row i is row src[i] of x, or row i (src null).
+int mx_quantize_x(Device* d, const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* src,
+                  uint8_t* planes, hipStream_t s) {
   char name[40];
   snprintf(name, sizeof(name), "qmm_mx_quantize_x_%s", mx_type_name(x_dtype));
   long long ld = ldx;
   int mm = (int)m, kk = (int)k, kc = (int)mx_chunks(k), wide = mx_wide(x, x_dtype, ldx);
-  void *q = ws + p.q, *sc = ws + p.s;
-  void* args[] = {&x, &ld, &mm, &kk, &kc, &wide, &q, &sc};
-  return launch(d, name, ceil_div(m * kc * 8, 256), 256, 0, s, args);
+  void* args[] = {&x, &ld, &mm, &kk, &kc, &wide, &src, &planes};
+  return launch(d, name, mx_plane_units(m, k), 256, 0, s, args);
 }
 
 // The kernels' by-value argument (qmm::MxOut).
@@ -94,60 +90,56 @@ struct MxOut {
   const void* w;
   void* y;
   const void* bias;
-  int y_type, bias_type, accumulate;
+  int y_type, bias_type, accumulate, wide;
 };
 
 // y = planes . W^T over m dense rows.
 int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, int64_t m, MxOut o, int64_t ldy, hipStream_t s) {
-  const MxPlanes p = mx_planes(m, w->k);
   o.w = w->data;
+  o.wide = mx_wide(o.y, o.y_type, ldy);
   int mm = (int)m, n = (int)w->n, kc = (int)mx_chunks(w->k), ld = (int)ldy;
-  const void *q = planes + p.q, *sc = planes + p.s;
-  void* args[] = {&o, &mm, &n, &kc, &q, &sc, &ld};
+  void* args[] = {&o, &mm, &n, &kc, &planes, &ld};
   hipFunction_t f;
   if (m <= 32) {
     QMM_TRY(kernel(d, "qmm_mx_gemv", &f));
     QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 32), 1, 1, 512, 1, 1, 0, s, args, nullptr));
     return QMM_OK;
   }
-  QMM_TRY(kernel(d, "qmm_mx_gemm", &f));
-  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 256), ceil_div(m, 64), 1, 256, 1, 1, 0, s, args, nullptr));
+  const bool big = m > 128;
+  QMM_TRY(kernel(d, big ? "qmm_mx_gemm_256x256" : "qmm_mx_gemm_128x256", &f));
+  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 256), ceil_div(m, big ? 256 : 128), 1, 256, 1, 1, 0, s, args, nullptr));
   return QMM_OK;
 }
 
-// The same of expert-ordered rows: row offsets[e] + i of the output takes row
-// src[offsets[e] + i] of the planes (src null: the same row). One or two weights.
-// max_rows bounds every count.
+// The same of expert-ordered rows: expert e's are rows offsets[e] + i of the planes and
+// of the output. One or two weights. max_rows bounds every count.
 int mx_expert_product(Device* d, const qmm_qtensor* const* w, int count, int experts, const uint8_t* planes,
-                      int64_t plane_rows, int64_t pairs, int64_t max_rows, const int32_t* counts,
-                      const int32_t* offsets, const int32_t* src, float* const* y, hipStream_t s) {
-  const MxPlanes p = mx_planes(plane_rows, w[0]->k);
+                      int64_t pairs, int64_t max_rows, const int32_t* counts, const int32_t* offsets,
+                      float* const* y, hipStream_t s) {
   MxOut o[2] = {};
   for (int j = 0; j < 2; ++j) {
     const int i = j < count ? j : 0;
     o[j].w = w[i]->data;
     o[j].y = y[i];
+    o[j].wide = mx_wide(y[i], QMM_F32, w[0]->n / experts);
   }
   int E = experts, P = (int)pairs, n = (int)(w[0]->n / experts), kc = (int)mx_chunks(w[0]->k), ld = n;
-  const void *q = planes + p.q, *sc = planes + p.s;
-  void* args[] = {&o[0], &o[1], &E, &P, &n, &kc, &counts, &offsets, &src, &q, &sc, &ld};
+  void* args[] = {&o[0], &o[1], &E, &P, &n, &kc, &counts, &offsets, &planes, &ld};
   const bool gemv = max_rows <= 32;
-  const int64_t bm = gemv ? 32 : 64;
-  const int64_t tiles = std::min<int64_t>(pairs / bm + std::min<int64_t>(experts, pairs), 65535);
-  if (pairs / bm + std::min<int64_t>(experts, pairs) > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
+  const int64_t bm = gemv ? 32 : 128;
+  const int64_t tiles = pairs / bm + std::min<int64_t>(experts, pairs);
+  if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
   hipFunction_t f;
-  QMM_TRY(kernel(d, gemv ? "qmm_mx_expert_gemv" : "qmm_mx_expert_gemm", &f));
+  QMM_TRY(kernel(d, gemv ? "qmm_mx_expert_gemv" : "qmm_mx_expert_gemm_128x256", &f));
   QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, gemv ? 32 : 256), (unsigned)tiles, (unsigned)count, gemv ? 512 : 256, 1, 1,
                                 0, s, args, nullptr));
   return QMM_OK;
 }
 
 int mx_silu_mul(Device* d, const float* g, const float* u, int64_t m, int64_t k, uint8_t* planes, hipStream_t s) {
-  const MxPlanes p = mx_planes(m, k);
   int mm = (int)m, kk = (int)k, kc = (int)mx_chunks(k);
-  void *q = planes + p.q, *sc = planes + p.s;
-  void* args[] = {&g, &u, &mm, &kk, &kc, &q, &sc};
-  return launch(d, "qmm_mx_silu_mul", ceil_div(m * kc * 8, 256), 256, 0, s, args);
+  void* args[] = {&g, &u, &mm, &kk, &kc, &planes};
+  return launch(d, "qmm_mx_silu_mul", mx_plane_units(m, k), 256, 0, s, args);
 }
 
 // How a call routes its tokens.

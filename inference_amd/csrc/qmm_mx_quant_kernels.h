@@ -40,6 +40,48 @@ __device__ __forceinline__ mx_u32x4 mx_codes(const float (&x)[32], int e) {
   return q;
 }
 
+// Four values of a typed matrix at element `at`; `wide`: they lie on a boundary of four.
+template <int T>
+__device__ __forceinline__ mx_f32x4 mx_load4(const void* __restrict__ p, long long at, bool wide) {
+  mx_f32x4 v;
+  if constexpr (T == kF32) {
+    const float* q = static_cast<const float*>(p) + at;
+    if (wide) return *reinterpret_cast<const mx_f32x4*>(q);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = q[j];
+  } else {
+    const uint16_t* q = static_cast<const uint16_t*>(p) + at;
+    uint16_t s[4];
+    if (wide) {
+      const mx_u32x2 d = *reinterpret_cast<const mx_u32x2*>(q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = (uint16_t)(d[j >> 1] >> (16 * (j & 1)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = q[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = T == kF16 ? (float)__builtin_bit_cast(_Float16, s[j]) : bf16_to_f32(s[j]);
+  }
+  return v;
+}
+
+// This thread's block of a unit whose rows are in `buf`: its values and largest magnitude.
+__device__ __forceinline__ uint32_t mx_unit_block(const float* buf, int t, float (&x)[32]) {
+  const float* p = buf + (t & 31) * kMxLdsRow + 64 * (t >> 6) + (t & 32);
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const mx_f32x4 v = *reinterpret_cast<const mx_f32x4*>(p + 4 * j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[4 * j + i] = v[i];  // (a bit cast of the vector's own element would take its first one)
+      amax = max(amax, __builtin_bit_cast(uint32_t, x[4 * j + i]) & 0x7fffffffu);
+    }
+  }
+  return amax;
+}
+
 template <int T>
 __device__ __forceinline__ void mx_quantize_w(const void* __restrict__ w, int n, int k, uint8_t* __restrict__ out,
                                               int kc) {
@@ -53,35 +95,12 @@ __device__ __forceinline__ void mx_quantize_w(const void* __restrict__ w, int n,
   for (int i = 0; i < 8; ++i) {
     const int r = 4 * i + (t >> 6), c = 4 * (t & 63);
     mx_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (r0 + r < n && c0 + c < k) {
-      const long long at = (long long)(r0 + r) * k + c0 + c;
-      if constexpr (T == kF32) {
-        v = *reinterpret_cast<const mx_f32x4*>(static_cast<const float*>(w) + at);
-      } else {
-        const mx_u32x2 d = *reinterpret_cast<const mx_u32x2*>(static_cast<const uint16_t*>(w) + at);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint16_t s = (uint16_t)(d[j >> 1] >> (16 * (j & 1)));
-          v[j] = T == kF16 ? (float)__builtin_bit_cast(_Float16, s) : bf16_to_f32(s);
-        }
-      }
-    }
+    if (r0 + r < n && c0 + c < k) v = mx_load4<T>(w, (long long)(r0 + r) * k + c0 + c, true);
     *reinterpret_cast<mx_f32x4*>(buf + r * kMxLdsRow + c) = v;
   }
   __syncthreads();
-  const float* p = buf + (t & 31) * kMxLdsRow + 64 * (t >> 6) + (t & 32);
   float x[32];
-  uint32_t amax = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const mx_f32x4 v = *reinterpret_cast<const mx_f32x4*>(p + 4 * j);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[4 * j + i] = v[i];  // (a bit cast of the vector's own element would take its first one)
-      amax = max(amax, __builtin_bit_cast(uint32_t, x[4 * j + i]) & 0x7fffffffu);
-    }
-  }
-  const int e = mx_w_byte(amax);
+  const int e = mx_w_byte(mx_unit_block(buf, t, x));
   mx_put_unit(out + u * kMxUnit, sc, t, mx_codes(x, e), e);
 }
 
@@ -221,30 +240,43 @@ __device__ __forceinline__ uint32_t mx_load_block(const void* __restrict__ row, 
   return amax;
 }
 
-__device__ __forceinline__ void mx_put_digits(uint8_t* __restrict__ q, const mx_u32x6& hi, const mx_u32x6& lo) {
-  mx_u32x4* o = reinterpret_cast<mx_u32x4*>(q);
-  o[0] = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
-  o[1] = mx_u32x4{hi[4], hi[5], lo[0], lo[1]};
-  o[2] = mx_u32x4{lo[2], lo[3], lo[4], lo[5]};
+// This thread's block of a unit of digit planes.
+__device__ __forceinline__ void mx_put_digits(uint8_t* __restrict__ unit, uint8_t (&sc)[256], int t, int e,
+                                              const mx_u32x6& hi, const mx_u32x6& lo) {
+  uint8_t* o = unit + (t >> 6) * kMxXStep;
+  *reinterpret_cast<mx_u32x4*>(o + 16 * (t & 63)) = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
+  *reinterpret_cast<mx_u32x4*>(o + kMxXLo + 16 * (t & 63)) = mx_u32x4{lo[0], lo[1], lo[2], lo[3]};
+  *reinterpret_cast<mx_u32x2*>(o + kMxXTail + 8 * (t & 63)) = mx_u32x2{hi[4], hi[5]};
+  *reinterpret_cast<mx_u32x2*>(o + kMxXTail + 512 + 8 * (t & 63)) = mx_u32x2{lo[4], lo[5]};
+  sc[4 * (t & 63) + (t >> 6)] = (uint8_t)e;
+  __syncthreads();
+  if (t < 64)
+    *reinterpret_cast<uint32_t*>(unit + kMxXScaleOff + 4 * t) = *reinterpret_cast<const uint32_t*>(sc + 4 * t);
 }
 
-// Rows -> digit planes: one thread a block; blocks past k (up to the chunk's end) are zero.
+// Rows (row i: row src[i], or i) -> digit planes, a workgroup a unit; columns past k (up to the chunk's end) are zero.
 template <int T>
 __device__ __forceinline__ void mx_quantize_x(const void* __restrict__ x, long long ldx, int m, int k, int kc, int wide,
-                                              uint8_t* __restrict__ q, uint8_t* __restrict__ sc) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int nb = 8 * kc;
-  if (i >= (long long)m * nb) return;
-  const int row = (int)(i / nb), b = (int)(i % nb);
-  mx_u32x6 hi = (mx_u32x6)(0u), lo = (mx_u32x6)(0u);
-  int e = 4;
-  if (32 * b < k) {
-    float v[32];
-    e = mx_x_byte(mx_load_block<T>(x, row * ldx + 32 * b, wide != 0, v));
-    mx_digits(v, e, hi, lo);
+                                              const int* __restrict__ src, uint8_t* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) float buf[kMxTile * kMxLdsRow];
+  __shared__ __attribute__((aligned(16))) uint8_t sc[256];
+  const int t = threadIdx.x;
+  const long long u = blockIdx.x;
+  const int r0 = (int)(u / kc) * kMxTile, c0 = (int)(u % kc) * kMxChunk;
+  const int rows = min(m - r0, kMxTile);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (t >> 6), c = 4 * (t & 63);
+    mx_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (r < rows && c0 + c < k) v = mx_load4<T>(x, (src ? src[r0 + r] : r0 + r) * ldx + c0 + c, wide != 0);
+    *reinterpret_cast<mx_f32x4*>(buf + r * kMxLdsRow + c) = v;
   }
-  mx_put_digits(q + i * kMxDigitBlock, hi, lo);
-  sc[(i & ~7LL) + 4 * (b & 1) + ((b & 7) >> 1)] = (uint8_t)e;
+  __syncthreads();
+  float v[32];
+  const int e = mx_x_byte(mx_unit_block(buf, t, v));
+  mx_u32x6 hi, lo;
+  mx_digits(v, e, hi, lo);
+  mx_put_digits(out + u * kMxXUnit, sc, t, e, hi, lo);
 }
 }  // namespace qmm
 
@@ -254,9 +286,9 @@ __device__ __forceinline__ void mx_quantize_x(const void* __restrict__ x, long l
     qmm::mx_dequantize<T>(w, n, k, dst, kc);                                                                      \
   }                                                                                                               \
   extern "C" __global__ void __launch_bounds__(256) qmm_mx_quantize_x_##NAME(                                     \
-      const void* __restrict__ x, long long ldx, int m, int k, int kc, int wide, uint8_t* __restrict__ q,         \
-      uint8_t* __restrict__ sc) {                                                                                 \
-    qmm::mx_quantize_x<T>(x, ldx, m, k, kc, wide, q, sc);                                                         \
+      const void* __restrict__ x, long long ldx, int m, int k, int kc, int wide, const int* __restrict__ src,     \
+      uint8_t* __restrict__ out) {                                                                                \
+    qmm::mx_quantize_x<T>(x, ldx, m, k, kc, wide, src, out);                                                      \
   }
 QMM_MX_TYPED(f32, qmm::kF32)
 QMM_MX_TYPED(f16, qmm::kF16)
@@ -283,47 +315,49 @@ extern "C" __global__ void __launch_bounds__(256) qmm_mx_quantize_rows(const flo
 }
 
 extern "C" __global__ void __launch_bounds__(256) qmm_mx_blocks_to_planes(const uint8_t* __restrict__ xq, int m, int k,
-                                                                          int kc, uint8_t* __restrict__ q,
-                                                                          uint8_t* __restrict__ sc) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int nb = 8 * kc;
-  if (i >= (long long)m * nb) return;
-  const int row = (int)(i / nb), b = (int)(i % nb);
+                                                                          int kc, uint8_t* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) uint8_t sc[256];
+  const int t = threadIdx.x;
+  const long long u = blockIdx.x;
+  const int row = (int)(u / kc) * qmm::kMxTile + (t & 31);
+  const int b = (int)(u % kc) * 8 + 2 * (t >> 6) + ((t >> 5) & 1);
   qmm::mx_u32x6 d[2] = {(qmm::mx_u32x6)(0u), (qmm::mx_u32x6)(0u)};
   int e = 4;
-  if (32 * b < k) {
+  if (row < m && 32 * b < k) {
     const uint8_t* p = xq + ((long long)row * (k / 32) + b) * qmm::kMxFp6x2Bytes;
     e = p[0] < 4 ? qmm::kMxNan : p[0];  // (no quantizer writes one: the second digit's scale would be below 2^-127)
 #pragma unroll
     for (int j = 0; j < 48; ++j) d[j / 24][j % 24 >> 2] |= (uint32_t)p[1 + j] << (8 * (j & 3));
   }
-  qmm::mx_put_digits(q + i * qmm::kMxDigitBlock, d[0], d[1]);
-  sc[(i & ~7LL) + 4 * (b & 1) + ((b & 7) >> 1)] = (uint8_t)e;
+  qmm::mx_put_digits(out + u * qmm::kMxXUnit, sc, t, e, d[0], d[1]);
 }
 
 // silu(g) * u -> digit planes, rows x k f32 (the down projection's input).
 extern "C" __global__ void __launch_bounds__(256) qmm_mx_silu_mul(const float* __restrict__ g,
                                                                   const float* __restrict__ u, int m, int k, int kc,
-                                                                  uint8_t* __restrict__ q, uint8_t* __restrict__ sc) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int nb = 8 * kc;
-  if (i >= (long long)m * nb) return;
-  const int row = (int)(i / nb), b = (int)(i % nb);
-  qmm::mx_u32x6 hi = (qmm::mx_u32x6)(0u), lo = (qmm::mx_u32x6)(0u);
-  int e = 4;
-  if (32 * b < k) {
-    float a[32], v[32];
-    qmm::mx_load_block<qmm::kF32>(g, (long long)row * k + 32 * b, true, a);
-    qmm::mx_load_block<qmm::kF32>(u, (long long)row * k + 32 * b, true, v);
-    uint32_t amax = 0;
+                                                                  uint8_t* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) float buf[qmm::kMxTile * qmm::kMxLdsRow];
+  __shared__ __attribute__((aligned(16))) uint8_t sc[256];
+  const int t = threadIdx.x;
+  const long long unit = blockIdx.x;
+  const int r0 = (int)(unit / kc) * qmm::kMxTile, c0 = (int)(unit % kc) * qmm::kMxChunk;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] = a[j] / (1.0f + expf(-a[j])) * v[j];
-      amax = max(amax, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (t >> 6), c = 4 * (t & 63);
+    qmm::mx_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (r0 + r < m && c0 + c < k) {
+      const long long at = (long long)(r0 + r) * k + c0 + c;
+      const qmm::mx_f32x4 a = *reinterpret_cast<const qmm::mx_f32x4*>(g + at);
+      v = *reinterpret_cast<const qmm::mx_f32x4*>(u + at);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = a[j] / (1.0f + expf(-a[j])) * v[j];
     }
-    e = qmm::mx_x_byte(amax);
-    qmm::mx_digits(v, e, hi, lo);
+    *reinterpret_cast<qmm::mx_f32x4*>(buf + r * qmm::kMxLdsRow + c) = v;
   }
-  qmm::mx_put_digits(q + i * qmm::kMxDigitBlock, hi, lo);
-  sc[(i & ~7LL) + 4 * (b & 1) + ((b & 7) >> 1)] = (uint8_t)e;
+  __syncthreads();
+  float x[32];
+  const int e = qmm::mx_x_byte(qmm::mx_unit_block(buf, t, x));
+  qmm::mx_u32x6 hi, lo;
+  qmm::mx_digits(x, e, hi, lo);
+  qmm::mx_put_digits(out + unit * qmm::kMxXUnit, sc, t, e, hi, lo);
 }
