@@ -1824,12 +1824,8 @@ static int mx_ffn(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, con
     ldx = gate->k;
   }
   QMM_TRY(mx_quantize_x(d, x, x_dtype, m, gate->k, ldx, nullptr, b + L.xp, s));
+  QMM_TRY(mx_glu(d, gate, up, 0, b + L.xp, m, m, nullptr, nullptr, b + L.hp, (float*)(b + L.g), (float*)(b + L.u), s));
   MxOut o = {};
-  o.y = b + L.g;
-  QMM_TRY(mx_product(d, gate, b + L.xp, m, o, gate->n, s));
-  o.y = b + L.u;
-  QMM_TRY(mx_product(d, up, b + L.xp, m, o, gate->n, s));
-  QMM_TRY(mx_silu_mul(d, (const float*)(b + L.g), (const float*)(b + L.u), m, gate->n, b + L.hp, s));
   o.y = y;
   o.accumulate = accumulate;
   return mx_product(d, down, b + L.hp, m, o, ldy, s);
@@ -3070,10 +3066,7 @@ static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const
     const uint8_t* xc = (const uint8_t*)x + t0 * ldx * (int64_t)mx_type_size(x_dtype);
     QMM_TRY(route_scored(d, logits + t0 * experts, T, experts, topk, r, counts, offsets, ptok, pw, tpairs, b + L.route, s));
     QMM_TRY(mx_quantize_x(d, xc, x_dtype, P, H, ldx, ptok, b + L.xp, s));
-    const qmm_qtensor* gw[2] = {gate, up};
-    float* gy[2] = {g, u};
-    QMM_TRY(mx_expert_product(d, gw, 2, experts, b + L.xp, P, T, counts, offsets, gy, s));
-    QMM_TRY(mx_silu_mul(d, g, u, P, F, b + L.hp, s));
+    QMM_TRY(mx_glu(d, gate, up, experts, b + L.xp, P, T, counts, offsets, b + L.hp, g, u, s));
     QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, T, counts, offsets, &yp, s));
     float *shared = nullptr, *sg = nullptr;
     if (sh.gate) {

@@ -36,13 +36,11 @@ constexpr int kMxStepBytes = 1024;
 constexpr int kMxScaleOff = 4096;
 constexpr int kMxUnit = 4352;
 // Digit planes of activation rows: units of 32 rows x 256 columns in the same order, so
-// that every operand load is contiguous. Step s holds, for 64 lanes (lane 32 h + r:
-// block 2 s + h of row r), the first 16 bytes of hi, the first 16 of lo, the last 8 of
-// hi, the last 8 of lo: a digit is one operand of six registers, loaded by a 16-byte
-// and an 8-byte read (parts that straddled the digits cost a move a register). Then
-// 64 lanes x 4 scale bytes. Rows past the last are left as
-// they are: a column of the product reads its own row only.
-constexpr int kMxXStep = 3072, kMxXLo = 1024, kMxXTail = 2048;
+// that every operand load is contiguous. Step s holds three parts of 64 lanes x 16
+// bytes: lane 32 h + r has the 48 bytes of block 2 s + h of row r, 24 of hi and 24 of
+// lo, in the parts' order; then 64 lanes x 4 scale bytes. Rows past the last are left
+// as they are: a column of the product reads its own row only.
+constexpr int kMxXPart = 1024, kMxXStep = 3 * kMxXPart;
 constexpr int kMxXScaleOff = 4 * kMxXStep;
 constexpr int kMxXUnit = kMxXScaleOff + 256;
 constexpr int kMxFp4Bytes = 17;   // GGML block: e, codes 0..15 in low nibbles, 16..31 in high ones
@@ -55,6 +53,8 @@ typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned mx_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned mx_u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned mx_u32x6 __attribute__((ext_vector_type(6)));
+typedef unsigned mx_u32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned mx_u32x12 __attribute__((ext_vector_type(12)));
 
 // Element types of typed rows: the C ABI's tags.
 constexpr int kF32 = 0, kF16 = 1, kBF16 = 30;
@@ -131,20 +131,36 @@ __device__ __forceinline__ void mx_digits(const float (&x)[32], int e, mx_u32x6&
   lo = mx_to_digit(a, b);
 }
 
+// A lane's 48 bytes of a step. As one vector of 12 its two digits are the instruction's
+// operands where the three loads put them, without a move.
+__device__ __forceinline__ mx_u32x12 mx_x(const mx_u32x4& p0, const mx_u32x4& p1, const mx_u32x4& p2) {
+  const mx_u32x8 a = __builtin_shufflevector(p0, p1, 0, 1, 2, 3, 4, 5, 6, 7);
+  const mx_u32x8 b = __builtin_shufflevector(p2, p2, 0, 1, 2, 3, -1, -1, -1, -1);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11);
+}
+__device__ __forceinline__ mx_u32x6 mx_hi(const mx_u32x12& x) { return __builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5); }
+__device__ __forceinline__ mx_u32x6 mx_lo(const mx_u32x12& x) { return __builtin_shufflevector(x, x, 6, 7, 8, 9, 10, 11); }
+
+// Block (step s, lane place l) of a unit of digit planes.
+__device__ __forceinline__ void mx_put_block(uint8_t* unit, int s, int l, int e, const mx_u32x6& hi, const mx_u32x6& lo) {
+  uint8_t* o = unit + s * kMxXStep + 16 * l;
+  *reinterpret_cast<mx_u32x4*>(o) = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
+  *reinterpret_cast<mx_u32x4*>(o + kMxXPart) = mx_u32x4{hi[4], hi[5], lo[0], lo[1]};
+  *reinterpret_cast<mx_u32x4*>(o + 2 * kMxXPart) = mx_u32x4{lo[2], lo[3], lo[4], lo[5]};
+  unit[kMxXScaleOff + 4 * l + s] = (uint8_t)e;
+}
+
 // One step (64 columns) of a 32 x 32 tile by one digit: weights (A, rows of the result)
 // times activations (B, columns). S: the byte of the scale registers.
 template <int S>
-__device__ __forceinline__ mx_f32x16 mx_mfma1(const mx_u32x4& w, const mx_u32x6& x, mx_f32x16 c, int sw, int sx) {
-  const mx_i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-  const mx_i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)x[4], (int)x[5], 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 2, S, sw, S, sx);
+__device__ __forceinline__ mx_f32x16 mx_mfma(const mx_u32x4& w, const mx_u32x6& x, mx_f32x16 c, int sw, int sx) {
+  const mx_u32x8 a = __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
+  const mx_u32x8 b = __builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, -1, -1);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(__builtin_bit_cast(mx_i32x8, a), __builtin_bit_cast(mx_i32x8, b),
+                                                         c, 4, 2, S, sw, S, sx);
 }
-// by both digits, the second's scale being sx - 4 in every byte
-template <int S>
-__device__ __forceinline__ mx_f32x16 mx_mfma(const mx_u32x4& w, const mx_u32x6& hi, const mx_u32x6& lo, mx_f32x16 c,
-                                             int sw, int sx, int sx_lo) {
-  return mx_mfma1<S>(w, lo, mx_mfma1<S>(w, hi, c, sw, sx), sw, sx_lo);
-}
+// (the second digit's scale is the first's less 4 in every byte)
+constexpr int kMxLoScale = 0x04040404;
 // (result: lane's column = lane & 31, register r its row 8 (r / 4) + 4 (lane / 32) + r % 4)
 
 }  // namespace qmm

@@ -13,7 +13,7 @@ struct MxOut {
   const void* bias;  // [n] or null
   int y_type, bias_type;
   int accumulate;    // y +=
-  int wide;          // rows of y start on a boundary of four values
+  int wide;          // rows of y start on 16-byte boundaries
 };
 
 // Which rows a workgroup multiplies: rows [first, first + count) of the planes and of
@@ -50,9 +50,9 @@ __device__ __forceinline__ bool mx_expert_tile(const int* __restrict__ counts, c
       const int l = __builtin_ctzll(hit);
       const int t = y - (base + __shfl(sum, l) - __shfl(tiles, l));
       const int o = __shfl(off, l), c = __shfl(cnt, l);
-      r.w0 = (long long)(e0 + l) * n;
-      r.first = o + t * bm;
-      r.count = min(c - t * bm, bm);
+      r.w0 = (long long)__builtin_amdgcn_readfirstlane(e0 + l) * n;
+      r.first = __builtin_amdgcn_readfirstlane(o + t * bm);
+      r.count = __builtin_amdgcn_readfirstlane(min(c - t * bm, bm));
       return true;
     }
     base += __shfl(sum, 63);
@@ -68,26 +68,16 @@ __device__ __forceinline__ long long mx_w_at(long long row, int h, int kc) {
 __device__ __forceinline__ long long mx_ws_at(long long row, int h, int kc) {
   return (row >> 5) * ((long long)kc * kMxUnit) + kMxScaleOff + 128 * h + 4 * (row & 31);
 }
-__device__ __forceinline__ long long mx_x_at(long long row, int kc) { return (row >> 5) * ((long long)kc * kMxXUnit); }
+__device__ __forceinline__ long long mx_x_at(long long row, int h, int kc) {
+  return (row >> 5) * ((long long)kc * kMxXUnit) + 512 * h + 16 * (row & 31);
+}
 __device__ __forceinline__ long long mx_xs_at(long long row, int h, int kc) {
   return (row >> 5) * ((long long)kc * kMxXUnit) + kMxXScaleOff + 128 * h + 4 * (row & 31);
 }
 
-// A lane's block of a step as its two digits, from the step's memory or LDS. `l`: the
-// lane's place, 16 (32 h + r).
-struct MxX {
-  mx_u32x6 hi, lo;
-};
-__device__ __forceinline__ mx_u32x6 mx_digit(const uint8_t* p, const uint8_t* tail) {
-  const mx_u32x4 a = *reinterpret_cast<const mx_u32x4*>(p);
-  const mx_u32x2 b = *reinterpret_cast<const mx_u32x2*>(tail);
-  return mx_u32x6{a[0], a[1], a[2], a[3], b[0], b[1]};
-}
-__device__ __forceinline__ MxX mx_get_x(const uint8_t* step, unsigned l) {
-  MxX x;
-  x.hi = mx_digit(step + l, step + kMxXTail + l / 2);
-  x.lo = mx_digit(step + kMxXLo + l, step + kMxXTail + 512 + l / 2);
-  return x;
+__device__ __forceinline__ mx_u32x12 mx_get_x(const uint8_t* p) {
+  return mx_x(*reinterpret_cast<const mx_u32x4*>(p), *reinterpret_cast<const mx_u32x4*>(p + kMxXPart),
+              *reinterpret_cast<const mx_u32x4*>(p + 2 * kMxXPart));
 }
 
 template <int T>
@@ -95,40 +85,34 @@ struct MxType {
   static constexpr int value = T;
 };
 
-// Four columns of a row of the output from col on (those below n).
-__device__ __forceinline__ mx_f32x4 mx_bias4(const MxOut& o, int col, int n) {
-  mx_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (o.bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + j < n) v[j] = mx_load(o.bias, o.bias_type, col + j);
-  }
-  return v;
-}
-template <int T>
-__device__ __forceinline__ void mx_put4(const MxOut& o, long long row, int ldy, int col, int n, mx_f32x4 v) {
+// V columns of a row of the output from col on (those below n), 4 f32 or 8 16-bit ones.
+template <int T, int V>
+__device__ __forceinline__ void mx_put(const MxOut& o, long long row, int ldy, int col, int n, const float (&v)[V]) {
   const long long at = row * ldy + col;
-  if (o.wide && col + 3 < n) {
-    if constexpr (T == kF32) {
-      mx_f32x4* p = reinterpret_cast<mx_f32x4*>(static_cast<float*>(o.y) + at);
-      if (o.accumulate) v += *p;
-      *p = v;
+  if constexpr (T == kF32) {
+    float* p = static_cast<float*>(o.y) + at;
+    if (o.wide && col + V <= n) {
+      mx_f32x4 u = {v[0], v[1], v[2], v[3]};
+      if (o.accumulate) u += *reinterpret_cast<const mx_f32x4*>(p);
+      *reinterpret_cast<mx_f32x4*>(p) = u;
     } else {
-      *reinterpret_cast<mx_u32x2*>(static_cast<uint16_t*>(o.y) + at) =
-          mx_u32x2{mx_to16(v[0], T) | (uint32_t)mx_to16(v[1], T) << 16, mx_to16(v[2], T) | (uint32_t)mx_to16(v[3], T) << 16};
-    }
-    return;
-  }
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (col + j < n) {
-      if constexpr (T == kF32) {
-        float* p = static_cast<float*>(o.y) + at + j;
-        *p = o.accumulate ? *p + v[j] : v[j];
-      } else {
-        static_cast<uint16_t*>(o.y)[at + j] = mx_to16(v[j], T);
-      }
+      for (int j = 0; j < V; ++j)
+        if (col + j < n) p[j] = o.accumulate ? p[j] + v[j] : v[j];
     }
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(o.y) + at;
+    if (o.wide && col + V <= n) {
+      mx_u32x4 u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = mx_to16(v[2 * j], T) | (uint32_t)mx_to16(v[2 * j + 1], T) << 16;
+      *reinterpret_cast<mx_u32x4*>(p) = u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (col + j < n) p[j] = mx_to16(v[j], T);
+    }
+  }
 }
 
 // Up to 32 rows: a workgroup of W waves takes one 32-column tile of the output and
@@ -142,19 +126,21 @@ __device__ __forceinline__ void mx_gemv(const MxOut& o, const MxRows& rows, int 
   const long long xrow = rows.first + min(c, rows.count - 1);
   const uint8_t* wp = o.w + mx_w_at(wrow, h, kc);
   const uint8_t* wsp = o.w + mx_ws_at(wrow, h, kc);
-  const uint8_t* xp = xq + mx_x_at(xrow, kc);
-  const unsigned xl = 512 * h + 16 * (unsigned)(xrow & 31);
+  const uint8_t* xp = xq + mx_x_at(xrow, h, kc);
   const uint8_t* xsp = xq + mx_xs_at(xrow, h, kc);
   mx_f32x16 acc = (mx_f32x16)(0.0f);
   for (int k = wave; k < kc; k += W) {
     const uint8_t* wk = wp + (long long)k * kMxUnit;
     const uint8_t* xk = xp + (long long)k * kMxXUnit;
     const int sw = *reinterpret_cast<const int*>(wsp + (long long)k * kMxUnit);
-    const int sx = *reinterpret_cast<const int*>(xsp + (long long)k * kMxXUnit), sl = sx - 0x04040404;
-    MxX x;
-#define QMM_MX_STEP(S)                                                                                          \
-  x = mx_get_x(xk + S * kMxXStep, xl);                                                                          \
-  acc = mx_mfma<S>(*reinterpret_cast<const mx_u32x4*>(wk + S * kMxStepBytes), x.hi, x.lo, acc, sw, sx, sl);
+    const int sx = *reinterpret_cast<const int*>(xsp + (long long)k * kMxXUnit), sl = sx - kMxLoScale;
+#define QMM_MX_STEP(S)                                                                     \
+  {                                                                                        \
+    const mx_u32x12 x = mx_get_x(xk + S * kMxXStep);                                       \
+    const mx_u32x4 w = *reinterpret_cast<const mx_u32x4*>(wk + S * kMxStepBytes);          \
+    acc = mx_mfma<S>(w, mx_hi(x), acc, sw, sx);                                            \
+    acc = mx_mfma<S>(w, mx_lo(x), acc, sw, sl);                                            \
+  }
     QMM_MX_STEP(0)
     QMM_MX_STEP(1)
     QMM_MX_STEP(2)
@@ -164,53 +150,73 @@ __device__ __forceinline__ void mx_gemv(const MxOut& o, const MxRows& rows, int 
 #pragma unroll
   for (int r = 0; r < 16; ++r) red[wave][c][8 * (r >> 2) + 4 * h + (r & 3)] = acc[r];
   __syncthreads();
-  for (int j = t; j < 8 * rows.count; j += 64 * W) {
-    const int m = j >> 3, q = 4 * (j & 7), col = kMxTile * tile + q;
-    mx_f32x4 v;
+  auto put = [&](auto type) {
+    constexpr int T = decltype(type)::value, V = T == kF32 ? 4 : 8, LR = 32 / V;
+    for (int j = t; j < LR * rows.count; j += 64 * W) {
+      const int m = j / LR, q = V * (j % LR), col = kMxTile * tile + q;
+      float v[V];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = red[0][m][q + i];
+      for (int i = 0; i < V; ++i) {
+        v[i] = red[0][m][q + i];
 #pragma unroll
-      for (int w = 1; w < W; ++w) v[i] += red[w][m][q + i];
+        for (int w = 1; w < W; ++w) v[i] += red[w][m][q + i];
+        if (o.bias != nullptr && col + i < n) v[i] += mx_load(o.bias, o.bias_type, col + i);
+      }
+      mx_put<T, V>(o, rows.first + m, ldy, col, n, v);
     }
-    v += mx_bias4(o, col, n);
-    if (o.y_type == kF32) mx_put4<kF32>(o, rows.first + m, ldy, col, n, v);
-    else if (o.y_type == kF16) mx_put4<kF16>(o, rows.first + m, ldy, col, n, v);
-    else mx_put4<kBF16>(o, rows.first + m, ldy, col, n, v);
-  }
+  };
+  if (o.y_type == kF32) put(MxType<kF32>{});
+  else if (o.y_type == kF16) put(MxType<kF16>{});
+  else put(MxType<kBF16>{});
 }
 
-// A tile of 32 FM WM rows x 32 FN WN columns by WM x WN waves, a wave 32 FM x 32 FN of it.
-// RW steps of weights in registers (this one and those on their way).
-template <int FM, int FN, int WM, int WN, int RW>
-__device__ __forceinline__ void mx_gemm(const MxOut& o, const MxRows& rows, int n, int kc, int n0,
-                                        const uint8_t* __restrict__ xq, int ldy) {
+// A tile of 32 FM WM rows x 32 FN WN columns by WM x WN waves, a wave FM x FN fragments;
+// WK such groups of waves share the columns of x (K) by chunks and join their sums.
+// GLU: half of a wave's column fragments are rows of o.w, half the same rows of `up`, and
+// silu(first) * second becomes digit planes (o.y), the down product's input.
+//
+// What bounds it: the matrix cores' power. 4096 rows x 16384 x 8192 takes 564 us, 1.95
+// PFLOP/s of products and twice that of instructions; without any loads or LDS the same
+// instructions take 414 us on random values (and 272 us on zeros: the clock falls with
+// the values' toggling). Per step (64 columns) a wave issues 2 FM FN instructions of 32
+// cycles. x goes through LDS (two buffers, one barrier a step): the waves of a column
+// of the tile share it. The weights go straight to registers: a step's operand is 1 KB
+// contiguous, and the LDS has no time for them (reads of x alone take 384 of the 1024
+// cycles of a step on a CU). The first half of a step's fragments of x is read in the
+// second half of the step before, the second half in the first: neither waits. Two
+// workgroups a CU, so that one's barrier and epilogue fall into the other's products:
+// 327 us at K = 4096 against 360 with one 256 x 256 workgroup of four waves (128 x 128
+// a wave, sums in the second register file). x straight to LDS without registers
+// measured the same (339 us, and two steps ahead in four buffers 339 us).
+template <int FM, int FN, int WM, int WN, int WK, bool GLU>
+__device__ __forceinline__ void mx_gemm(const MxOut& o, const uint8_t* __restrict__ up, const MxRows& rows, int n, int kc,
+                                        int n0, const uint8_t* __restrict__ xq, int ldy) {
   constexpr int NW = WM * WN, XF = FM * WM, FW = XF / NW;
-  static_assert(XF % NW == 0, "whole fragments a wave");
+  constexpr int FC = GLU ? FN / 2 : FN;  // column fragments of a wave's output
+  static_assert(XF % NW == 0 && FM % 2 == 0 && (!GLU || (FN == 4 && WK == 1)), "whole fragments a wave");
   constexpr int kStage = XF * kMxXStep;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][kStage];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the epilogue's 32 rows of a wave's columns, a row padded by 16 bytes
+  constexpr int kRow = 32 * FC + 4, kLoop = 2 * WK * kStage, kEpi = WK * NW * 32 * kRow * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kLoop > kEpi ? kLoop : kEpi];
+  const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = all / NW, wave = all % NW;
+  auto lds = reinterpret_cast<uint8_t(*)[kStage]>(smem + 2 * kStage * wk);
   const int h = lane >> 5, c = lane & 31, wm = wave % WM, wn = wave / WM;
   // 64-bit bases at the tile's first row, 32-bit offsets from them
   const long long xt = rows.first >> 5;
   const uint8_t* xb = xq + xt * ((long long)kc * kMxXUnit);
-  // the fragments that this wave brings to LDS: a lane's place in the 16-byte and in
-  // the 8-byte parts
-  unsigned xo[FW][2], xso[FM], wo[FN], wso[FN];
+  unsigned xo[FW], xso[FM], wo[FC], wso[FC];
 #pragma unroll
-  for (int j = 0; j < FW; ++j) {
-    const long long r = rows.first + min(32 * (FW * wave + j) + c, rows.count - 1) - 32 * xt;
-    xo[j][0] = (unsigned)mx_x_at(r, kc) + 512 * h + 16 * (unsigned)(r & 31);
-    xo[j][1] = (unsigned)mx_x_at(r, kc) + kMxXTail + 256 * h + 8 * (unsigned)(r & 31);
-  }
+  for (int j = 0; j < FW; ++j)  // the fragments that this wave brings to LDS
+    xo[j] = (unsigned)mx_x_at(rows.first + min(32 * (FW * wave + j) + c, rows.count - 1) - 32 * xt, h, kc);
 #pragma unroll
   for (int b = 0; b < FM; ++b)
-    xso[b] = (unsigned)mx_xs_at(rows.first + min(32 * (FM * wm + b) + c, rows.count - 1) - 32 * xt, h, kc);
+    xso[b] = (unsigned)mx_xs_at(rows.first + min(32 * (WM * b + wm) + c, rows.count - 1) - 32 * xt, h, kc);
   const long long wt = (rows.w0 + n0) >> 5;
-  const uint8_t* wb = o.w + wt * ((long long)kc * kMxUnit);
+  const uint8_t* wb[2] = {o.w + wt * ((long long)kc * kMxUnit), GLU ? up + wt * ((long long)kc * kMxUnit) : nullptr};
 #pragma unroll
-  for (int a = 0; a < FN; ++a) {
-    const long long r = rows.w0 + min(n0 + 32 * (FN * wn + a) + c, n - 1) - 32 * wt;
+  for (int a = 0; a < FC; ++a) {
+    const long long r = rows.w0 + min(n0 + 32 * (FC * wn + a) + c, n - 1) - 32 * wt;
     wo[a] = (unsigned)mx_w_at(r, h, kc);
     wso[a] = (unsigned)mx_ws_at(r, h, kc);
   }
@@ -220,43 +226,34 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const MxRows& rows, int 
 #pragma unroll
     for (int b = 0; b < FM; ++b) acc[a][b] = (mx_f32x16)(0.0f);
 
-  MxX st[FW];            // x on its way to LDS
-  mx_u32x4 w[RW][FN];    // weights of this step and the next ones
-  MxX x[2][FM];          // x of this step and the next
+  mx_u32x4 st[3 * FW];   // x on its way to LDS
+  mx_u32x4 w[2][FN];     // weights of this step and the next
+  mx_u32x12 x[FM];       // x of this step
   int sw[2][FN], sx[2][FM];
   auto load_x = [&](int k, int s) {
     const unsigned at = (unsigned)k * kMxXUnit + s * kMxXStep;
 #pragma unroll
-    for (int j = 0; j < FW; ++j) {
-      const uint8_t* p = xb + (xo[j][0] + at);
-      const uint8_t* q = xb + (xo[j][1] + at);
-      st[j].hi = mx_digit(p, q);
-      st[j].lo = mx_digit(p + kMxXLo, q + 512);
-    }
+    for (int i = 0; i < 3 * FW; ++i)
+      st[i] = *reinterpret_cast<const mx_u32x4*>(xb + (xo[i / 3] + at) + kMxXPart * (i % 3));
   };
   auto put_x = [&](int buf) {
 #pragma unroll
-    for (int j = 0; j < FW; ++j) {
-      uint8_t* d = &lds[buf][kMxXStep * (FW * wave + j)];
-      const mx_u32x6 u = st[j].hi, v = st[j].lo;
-      *reinterpret_cast<mx_u32x4*>(d + 16 * lane) = mx_u32x4{u[0], u[1], u[2], u[3]};
-      *reinterpret_cast<mx_u32x4*>(d + kMxXLo + 16 * lane) = mx_u32x4{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<mx_u32x2*>(d + kMxXTail + 8 * lane) = mx_u32x2{u[4], u[5]};
-      *reinterpret_cast<mx_u32x2*>(d + kMxXTail + 512 + 8 * lane) = mx_u32x2{v[4], v[5]};
-    }
+    for (int i = 0; i < 3 * FW; ++i)
+      *reinterpret_cast<mx_u32x4*>(&lds[buf][kMxXPart * (3 * FW * wave + i) + 16 * lane]) = st[i];
   };
-  auto get_x = [&](int buf, MxX (&d)[FM]) {
+  auto get_x = [&](int buf, int b0, int b1) {
 #pragma unroll
-    for (int b = 0; b < FM; ++b) d[b] = mx_get_x(&lds[buf][kMxXStep * (FM * wm + b)], 16 * lane);
+    for (int b = b0; b < b1; ++b) x[b] = mx_get_x(&lds[buf][kMxXStep * (WM * b + wm) + 16 * lane]);
   };
   auto load_w = [&](int k, int s, mx_u32x4 (&d)[FN]) {
     const unsigned at = (unsigned)k * kMxUnit + s * kMxStepBytes;
 #pragma unroll
-    for (int a = 0; a < FN; ++a) d[a] = *reinterpret_cast<const mx_u32x4*>(wb + (wo[a] + at));
+    for (int a = 0; a < FN; ++a) d[a] = *reinterpret_cast<const mx_u32x4*>(wb[a / FC] + (wo[a % FC] + at));
   };
   auto load_s = [&](int k, int i) {
 #pragma unroll
-    for (int a = 0; a < FN; ++a) sw[i][a] = *reinterpret_cast<const int*>(wb + (wso[a] + (unsigned)k * kMxUnit));
+    for (int a = 0; a < FN; ++a)
+      sw[i][a] = *reinterpret_cast<const int*>(wb[a / FC] + (wso[a % FC] + (unsigned)k * kMxUnit));
 #pragma unroll
     for (int b = 0; b < FM; ++b) sx[i][b] = *reinterpret_cast<const int*>(xb + (xso[b] + (unsigned)k * kMxXUnit));
   };
@@ -267,42 +264,50 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const MxRows& rows, int 
     asm volatile("" ::: "memory");
   };
 
-  load_s(0, 0);
-  load_x(0, 0);
-#pragma unroll
-  for (int s = 0; s < RW - 1; ++s) load_w(0, s, w[s]);
+  // this group's chunks; every group makes as many rounds, so that the barriers match
+  const int per = (kc + WK - 1) / WK, k0 = min(per * wk, kc - 1), live = min(per, kc - per * wk);
+  // A wave's fragments of rows are wm, wm + WM, ...: a tile with few rows is spread over
+  // its waves, and fragments without rows are left out.
+  const int full = min((rows.count + 32 * (WM - wm) - 1) / (32 * WM), FM);
+  load_s(k0, 0);
+  load_x(k0, 0);
+  load_w(k0, 0, w[0]);
   put_x(0);
-  load_x(0, 1);
+  load_x(k0, 1);
   sync();
-  get_x(0, x[0]);
-#define QMM_MX_HALF(S, I, B0, B1)                                                                              \
-  _Pragma("unroll") for (int b = B0; b < B1; ++b) {                                                            \
+  get_x(0, 0, FM / 2);
+#define QMM_MX_HALF(S, B0, B1)                                                                                 \
+  _Pragma("unroll") for (int b = B0; b < B1; ++b) if (b < have) {                                              \
     _Pragma("unroll") for (int a = 0; a < FN; ++a) acc[a][b] =                                                 \
-        mx_mfma1<S>(w[S % RW][a], x[S & 1][b].hi, acc[a][b], sw[I][a], sx[I][b]);                              \
+        mx_mfma<S>(w[S & 1][a], mx_hi(x[b]), acc[a][b], sw[0][a], sx[0][b]);                                   \
     _Pragma("unroll") for (int a = 0; a < FN; ++a) acc[a][b] =                                                 \
-        mx_mfma1<S>(w[S % RW][a], x[S & 1][b].lo, acc[a][b], sw[I][a], sx[I][b] - 0x04040404);                 \
+        mx_mfma<S>(w[S & 1][a], mx_lo(x[b]), acc[a][b], sw[0][a], sx[0][b] - kMxLoScale);                      \
   }
-#define QMM_MX_STEP(S, I)                                                                                      \
+#define QMM_MX_STEP(S)                                                                                         \
   {                                                                                                            \
     put_x((S + 1) & 1);                                                                                        \
     load_x(S + 2 < 4 ? k : kn, (S + 2) & 3);                                                                   \
-    load_w(S + RW - 1 < 4 ? k : kn, (S + RW - 1) & 3, w[(S + RW - 1) % RW]);                                   \
-    if (S == 1) load_s(kn, 1 - I);                                                                             \
+    load_w(S + 1 < 4 ? k : kn, (S + 1) & 3, w[(S + 1) & 1]);                                                   \
+    if (S == 1) load_s(kn, 1);                                                                                 \
+    get_x(S & 1, FM / 2, FM);                                                                                  \
     __builtin_amdgcn_sched_barrier(0);                                                                         \
-    QMM_MX_HALF(S, I, 0, FM / 2)                                                                               \
+    QMM_MX_HALF(S, 0, FM / 2)                                                                                  \
+    __builtin_amdgcn_sched_barrier(0);                                                                         \
     sync();                                                                                                    \
-    get_x((S + 1) & 1, x[(S + 1) & 1]);                                                                        \
+    get_x((S + 1) & 1, 0, FM / 2);                                                                             \
     __builtin_amdgcn_sched_barrier(0);                                                                         \
-    QMM_MX_HALF(S, I, FM / 2, FM)                                                                              \
+    QMM_MX_HALF(S, FM / 2, FM)                                                                                 \
+    __builtin_amdgcn_sched_barrier(0);                                                                         \
   }
   // (past the last chunk the loads read it again, and what they bring is not used)
 #pragma unroll 1
-  for (int k = 0; k < kc; ++k) {
-    const int kn = min(k + 1, kc - 1);
-    QMM_MX_STEP(0, 0)
-    QMM_MX_STEP(1, 0)
-    QMM_MX_STEP(2, 0)
-    QMM_MX_STEP(3, 0)
+  for (int i = 0; i < per; ++i) {
+    const int k = min(k0 + i, kc - 1), kn = min(k0 + i + 1, kc - 1);
+    const int have = WK == 1 || i < live ? full : 0;
+    QMM_MX_STEP(0)
+    QMM_MX_STEP(1)
+    QMM_MX_STEP(2)
+    QMM_MX_STEP(3)
 #pragma unroll
     for (int a = 0; a < FN; ++a) sw[0][a] = sw[1][a];
 #pragma unroll
@@ -310,22 +315,99 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const MxRows& rows, int 
   }
 #undef QMM_MX_STEP
 #undef QMM_MX_HALF
-  auto put = [&](auto type) {
+  sync();
+  float* e = reinterpret_cast<float*>(smem) + all * 32 * kRow;
+  const int col0 = n0 + 32 * FC * wn;
+  if constexpr (GLU) {
+    // silu(g) * u of 64 columns: one step of a chunk of the planes, a block a lane
+    if (col0 >= n) return;
+    const int hb = h, kf = (n + kMxChunk - 1) / kMxChunk, s = col0 % kMxChunk / 64;
+    const bool last = col0 + 64 >= n;
 #pragma unroll
-    for (int a = 0; a < FN; ++a)
+    for (int b = 0; b < FM; ++b) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = n0 + 32 * (FN * wn + a) + 8 * q + 4 * h;
-        const mx_f32x4 bias = mx_bias4(o, col, n);
+      for (int a = 0; a < FC; ++a)
 #pragma unroll
-        for (int b = 0; b < FM; ++b) {
-          const int m = 32 * (FM * wm + b) + c;
+        for (int i = 0; i < 4; ++i) {
           mx_f32x4 v;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = acc[a][b][4 * q + j] + bias[j];
-          if (m < rows.count) mx_put4<decltype(type)::value>(o, rows.first + m, ldy, col, n, v);
+          for (int j = 0; j < 4; ++j) {
+            const float g = acc[a][b][4 * i + j];
+            v[j] = g / (1.0f + expf(-g)) * acc[a + FC][b][4 * i + j];
+          }
+          *reinterpret_cast<mx_f32x4*>(e + c * kRow + 32 * a + 8 * i + 4 * h) = v;
+        }
+      __builtin_amdgcn_wave_barrier();
+      const int m = 32 * (WM * b + wm) + c;
+      float v[32];
+      uint32_t amax = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const mx_f32x4 t = *reinterpret_cast<const mx_f32x4*>(e + c * kRow + 32 * hb + 4 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[4 * j + i] = t[i];
+          amax = max(amax, __builtin_bit_cast(uint32_t, v[4 * j + i]) & 0x7fffffffu);
         }
       }
+      __builtin_amdgcn_wave_barrier();
+      mx_u32x6 hi = (mx_u32x6)(0u), lo = (mx_u32x6)(0u);
+      int byte = 4;
+      if (col0 + 32 * hb < n) {
+        byte = mx_x_byte(amax);
+        mx_digits(v, byte, hi, lo);
+      }
+      if (m < rows.count) {
+        const long long r = rows.first + m;
+        uint8_t* u = static_cast<uint8_t*>(o.y) + ((r >> 5) * kf + col0 / kMxChunk) * kMxXUnit;
+        const int l = 32 * hb + (int)(r & 31);
+        mx_put_block(u, s, l, byte, hi, lo);
+        if (last)  // the rest of the chunk: the product reads whole ones
+          for (int z = s + 1; z < 4; ++z) mx_put_block(u, z, l, 4, (mx_u32x6)(0u), (mx_u32x6)(0u));
+      }
+    }
+    return;
+  }
+  // The accumulators hold four columns of a row a lane; through LDS a wave writes 16
+  // bytes a lane, whole runs of a row's 32 FN columns (writing them as they are, 8 bytes
+  // a lane over 32 rows, took 36 us a 256 x 256 tile).
+  auto put = [&](auto type) {
+    constexpr int T = decltype(type)::value;
+    constexpr int V = T == kF32 ? 4 : 8, LR = 32 * FN / V;  // columns and lanes of a 16-byte run and of a row
+    constexpr int R = 32 / WK;  // rows that this group joins and writes
+    const int q = V * (lane % LR);
+    float bias[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      bias[j] = o.bias != nullptr && col0 + q + j < n ? mx_load(o.bias, o.bias_type, col0 + q + j) : 0.0f;
+#pragma unroll
+    for (int b = 0; b < FM; ++b) {
+#pragma unroll
+      for (int a = 0; a < FN; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<mx_f32x4*>(e + c * kRow + 32 * a + 8 * i + 4 * h) =
+              mx_f32x4{acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
+      if constexpr (WK == 1) __builtin_amdgcn_wave_barrier();
+      else sync();
+#pragma unroll 4
+      for (int r = R * wk + lane / LR; r < R * wk + R; r += 64 / LR) {
+        const int m = 32 * (WM * b + wm) + r;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          mx_f32x4 t = (mx_f32x4)(0.0f);
+#pragma unroll
+          for (int g = 0; g < WK; ++g)  // the groups' sums in order
+            t += *reinterpret_cast<const mx_f32x4*>(e + (g - wk) * (NW * 32 * kRow) + r * kRow + q + j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[j + i] = t[i] + bias[j + i];
+        }
+        if (m < rows.count) mx_put<T, V>(o, rows.first + m, ldy, col0 + q, n, v);
+      }
+      if constexpr (WK == 1) __builtin_amdgcn_wave_barrier();
+      else sync();
+    }
   };
   if (o.y_type == kF32) put(MxType<kF32>{});
   else if (o.y_type == kF16) put(MxType<kF16>{});
@@ -352,22 +434,41 @@ extern "C" __global__ void __launch_bounds__(512) qmm_mx_expert_gemv(qmm::MxOut 
   qmm::mx_gemv<8>(blockIdx.z ? o1 : o0, r, n, kc, blockIdx.x, xq, ldy);
 }
 
-#define QMM_MX_GEMM(NAME, FM, FN, WM, WN, RW, EU)                                                              \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN, EU) qmm_mx_gemm_##NAME(                           \
+#define QMM_MX_GEMM(NAME, FM, FN, WM, WN, WK, EU)                                                              \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK, EU) qmm_mx_gemm_##NAME(                      \
       qmm::MxOut o, int m, int n, int kc, const uint8_t* __restrict__ xq, int ldy) {                           \
     const int first = 32 * FM * WM * blockIdx.y;                                                               \
     const qmm::MxRows r = {0, first, min(m - first, 32 * FM * WM)};                                            \
-    qmm::mx_gemm<FM, FN, WM, WN, RW>(o, r, n, kc, 32 * FN * WN * blockIdx.x, xq, ldy);                             \
+    qmm::mx_gemm<FM, FN, WM, WN, WK, false>(o, nullptr, r, n, kc, 32 * FN * WN * blockIdx.x, xq, ldy);         \
   }                                                                                                            \
-  extern "C" __global__ void __launch_bounds__(64 * WM * WN, EU) qmm_mx_expert_gemm_##NAME(                    \
+  extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK, EU) qmm_mx_expert_gemm_##NAME(               \
       qmm::MxOut o0, qmm::MxOut o1, int experts, int pairs, int n, int kc, const int* __restrict__ counts,     \
       const int* __restrict__ offsets, const uint8_t* __restrict__ xq, int ldy) {                              \
     qmm::MxRows r;                                                                                             \
     if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 32 * FM * WM, blockIdx.y, r)) return;         \
-    qmm::mx_gemm<FM, FN, WM, WN, RW>(blockIdx.z ? o1 : o0, r, n, kc, 32 * FN * WN * blockIdx.x, xq, ldy);          \
+    qmm::mx_gemm<FM, FN, WM, WN, WK, false>(blockIdx.z ? o1 : o0, nullptr, r, n, kc, 32 * FN * WN * blockIdx.x, xq,  \
+                                            ldy);                                                              \
   }
-QMM_MX_GEMM(256x256, 4, 4, 2, 2, 2, 1)
-QMM_MX_GEMM(128x256, 2, 4, 2, 2, 2, 2)
+QMM_MX_GEMM(128x256, 2, 4, 2, 2, 1, 2)
+QMM_MX_GEMM(128x128, 2, 2, 2, 2, 1, 2)
+QMM_MX_GEMM(64x128k4, 2, 2, 1, 2, 4, 2)
+
+// Gate and up with the activation, into the planes of the down product's rows: dense
+// rows, or routed ones.
+extern "C" __global__ void __launch_bounds__(256, 2) qmm_mx_glu_128x128(qmm::MxOut o, const uint8_t* __restrict__ up,
+                                                                       int m, int n, int kc,
+                                                                       const uint8_t* __restrict__ xq) {
+  const int first = 128 * blockIdx.y;
+  const qmm::MxRows r = {0, first, min(m - first, 128)};
+  qmm::mx_gemm<2, 4, 2, 2, 1, true>(o, up, r, n, kc, 128 * blockIdx.x, xq, 0);
+}
+extern "C" __global__ void __launch_bounds__(256, 2) qmm_mx_expert_glu_128x128(
+    qmm::MxOut o, const uint8_t* __restrict__ up, int experts, int pairs, int n, int kc, const int* __restrict__ counts,
+    const int* __restrict__ offsets, const uint8_t* __restrict__ xq) {
+  qmm::MxRows r;
+  if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 128, blockIdx.y, r)) return;
+  qmm::mx_gemm<2, 4, 2, 2, 1, true>(o, up, r, n, kc, 128 * blockIdx.x, xq, 0);
+}
 
 // out[t] = sum over token t's pairs, in increasing expert order, of weight * yp[pair],
 // then + shared[t] (times sg[t] when the shared expert is gated), rounded once to the

@@ -64,6 +64,11 @@ int mx_wide(const void* x, int dtype, int64_t ldx) {
   return (uintptr_t)x % four == 0 && ldx % 4 == 0;
 }
 
+// Whether rows of a typed output all start on 16-byte boundaries.
+int mx_wide16(const void* y, int dtype, int64_t ldy) {
+  return (uintptr_t)y % 16 == 0 && ldy * (int64_t)mx_type_size(dtype) % 16 == 0;
+}
+
 // Activation limits: a workgroup's rows are reached by 32-bit offsets (nine 32-row
 // tiles of the planes), a grid has fewer than 2^31 units.
 int mx_check_rows(int64_t m, int64_t k) {
@@ -93,10 +98,37 @@ struct MxOut {
   int y_type, bias_type, accumulate, wide;
 };
 
+// The product's tiles (kernels qmm_mx_gemm_<name>): rows, columns, threads, and the time
+// of one on a CU at k = 4096, measured with every CU busy (us; two of the first run side
+// by side, so it counts once for each).
+struct MxTileCfg {
+  const char* name;
+  int rows, cols, threads;
+  double us;
+};
+constexpr MxTileCfg kMxTiles[] = {{"128x256", 128, 256, 256, 41.0}, {"128x128", 128, 128, 256, 24.0}, {"64x128k4", 64, 128, 512, 13.4}};
+
+// The tile with the least rounds x time: the wide ones do more per byte, the narrow one
+// (which splits K over its waves) fills the chip with few rows or columns (333 x 4096 x
+// 4096: 41.6, 27.7 and 14.2 us; 512 x 14336 x 4096: 48.9, 47.0 and 54.2).
+const MxTileCfg& mx_tile_for(const Device* d, int64_t row_tiles64, int64_t row_tiles128, int64_t n) {
+  const MxTileCfg* best = nullptr;
+  double least = 0.0;
+  for (const MxTileCfg& c : kMxTiles) {
+    const int64_t tiles = (c.rows == 64 ? row_tiles64 : row_tiles128) * ((n + c.cols - 1) / c.cols);
+    const double us = (double)((tiles + d->num_cu - 1) / d->num_cu) * c.us;
+    if (!best || us < least) {
+      best = &c;
+      least = us;
+    }
+  }
+  return *best;
+}
+
 // y = planes . W^T over m dense rows.
 int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, int64_t m, MxOut o, int64_t ldy, hipStream_t s) {
   o.w = w->data;
-  o.wide = mx_wide(o.y, o.y_type, ldy);
+  o.wide = mx_wide16(o.y, o.y_type, ldy);
   int mm = (int)m, n = (int)w->n, kc = (int)mx_chunks(w->k), ld = (int)ldy;
   void* args[] = {&o, &mm, &n, &kc, &planes, &ld};
   hipFunction_t f;
@@ -105,9 +137,11 @@ int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, int64_t m
     QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 32), 1, 1, 512, 1, 1, 0, s, args, nullptr));
     return QMM_OK;
   }
-  const bool big = m > 128;
-  QMM_TRY(kernel(d, big ? "qmm_mx_gemm_256x256" : "qmm_mx_gemm_128x256", &f));
-  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 256), ceil_div(m, big ? 256 : 128), 1, 256, 1, 1, 0, s, args, nullptr));
+  const MxTileCfg& c = mx_tile_for(d, ceil_div(m, 64), ceil_div(m, 128), n);
+  char name[40];
+  snprintf(name, sizeof(name), "qmm_mx_gemm_%s", c.name);
+  QMM_TRY(kernel(d, name, &f));
+  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, c.cols), ceil_div(m, c.rows), 1, c.threads, 1, 1, 0, s, args, nullptr));
   return QMM_OK;
 }
 
@@ -121,18 +155,27 @@ int mx_expert_product(Device* d, const qmm_qtensor* const* w, int count, int exp
     const int i = j < count ? j : 0;
     o[j].w = w[i]->data;
     o[j].y = y[i];
-    o[j].wide = mx_wide(y[i], QMM_F32, w[0]->n / experts);
+    o[j].wide = mx_wide16(y[i], QMM_F32, w[0]->n / experts);
   }
   int E = experts, P = (int)pairs, n = (int)(w[0]->n / experts), kc = (int)mx_chunks(w[0]->k), ld = n;
   void* args[] = {&o[0], &o[1], &E, &P, &n, &kc, &counts, &offsets, &planes, &ld};
-  const bool gemv = max_rows <= 32;
-  const int64_t bm = gemv ? 32 : 128;
-  const int64_t tiles = pairs / bm + std::min<int64_t>(experts, pairs);
-  if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
   hipFunction_t f;
-  QMM_TRY(kernel(d, gemv ? "qmm_mx_expert_gemv" : "qmm_mx_expert_gemm_128x256", &f));
-  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, gemv ? 32 : 256), (unsigned)tiles, (unsigned)count, gemv ? 512 : 256, 1, 1,
-                                0, s, args, nullptr));
+  const int64_t active = std::min<int64_t>(experts, pairs);
+  if (max_rows <= 32) {
+    const int64_t tiles = pairs / 32 + active;
+    if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
+    QMM_TRY(kernel(d, "qmm_mx_expert_gemv", &f));
+    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 32), (unsigned)tiles, (unsigned)count, 512, 1, 1, 0, s, args, nullptr));
+    return QMM_OK;
+  }
+  // (the tiles that there will be, each expert's last one half full)
+  const MxTileCfg& c = mx_tile_for(d, pairs / 64 + (active + 1) / 2, pairs / 128 + (active + 1) / 2, (int64_t)n * count);
+  const int64_t tiles = pairs / c.rows + active;
+  if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
+  char name[40];
+  snprintf(name, sizeof(name), "qmm_mx_expert_gemm_%s", c.name);
+  QMM_TRY(kernel(d, name, &f));
+  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, c.cols), (unsigned)tiles, (unsigned)count, c.threads, 1, 1, 0, s, args, nullptr));
   return QMM_OK;
 }
 
@@ -140,6 +183,45 @@ int mx_silu_mul(Device* d, const float* g, const float* u, int64_t m, int64_t k,
   int mm = (int)m, kk = (int)k, kc = (int)mx_chunks(k);
   void* args[] = {&g, &u, &mm, &kk, &kc, &planes};
   return launch(d, "qmm_mx_silu_mul", mx_plane_units(m, k), 256, 0, s, args);
+}
+
+// silu(gate) * up of the planes' rows, as the planes of the down product's rows: dense
+// rows (experts 0) or routed ones.
+int mx_glu(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, int experts, const uint8_t* planes, int64_t m,
+           int64_t max_rows, const int32_t* counts, const int32_t* offsets, uint8_t* out, float* g, float* u, hipStream_t s) {
+  const int64_t F = gate->n / std::max(experts, 1);
+  const int64_t tiles = experts ? m / 128 + std::min<int64_t>(experts, m) : ceil_div(m, 128);
+  if (max_rows <= 32) {
+    if (experts) {
+      const qmm_qtensor* w[2] = {gate, up};
+      float* y[2] = {g, u};
+      QMM_TRY(mx_expert_product(d, w, 2, experts, planes, m, max_rows, counts, offsets, y, s));
+    } else {
+      MxOut o = {};
+      o.y = g;
+      QMM_TRY(mx_product(d, gate, planes, m, o, F, s));
+      o.y = u;
+      QMM_TRY(mx_product(d, up, planes, m, o, F, s));
+    }
+    return mx_silu_mul(d, g, u, m, F, out, s);
+  }
+  if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many rows");
+  MxOut o = {};
+  o.w = gate->data;
+  o.y = out;
+  const void* uw = up->data;
+  int E = experts, P = (int)m, n = (int)F, kc = (int)mx_chunks(gate->k);
+  hipFunction_t f;
+  if (!experts) {
+    void* args[] = {&o, &uw, &P, &n, &kc, &planes};
+    QMM_TRY(kernel(d, "qmm_mx_glu_128x128", &f));
+    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 128), (unsigned)tiles, 1, 256, 1, 1, 0, s, args, nullptr));
+    return QMM_OK;
+  }
+  void* args[] = {&o, &uw, &E, &P, &n, &kc, &counts, &offsets, &planes};
+  QMM_TRY(kernel(d, "qmm_mx_expert_glu_128x128", &f));
+  QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 128), (unsigned)tiles, 1, 256, 1, 1, 0, s, args, nullptr));
+  return QMM_OK;
 }
 
 // How a call routes its tokens.

@@ -243,11 +243,10 @@ __device__ __forceinline__ uint32_t mx_load_block(const void* __restrict__ row, 
 // This thread's block of a unit of digit planes.
 __device__ __forceinline__ void mx_put_digits(uint8_t* __restrict__ unit, uint8_t (&sc)[256], int t, int e,
                                               const mx_u32x6& hi, const mx_u32x6& lo) {
-  uint8_t* o = unit + (t >> 6) * kMxXStep;
-  *reinterpret_cast<mx_u32x4*>(o + 16 * (t & 63)) = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
-  *reinterpret_cast<mx_u32x4*>(o + kMxXLo + 16 * (t & 63)) = mx_u32x4{lo[0], lo[1], lo[2], lo[3]};
-  *reinterpret_cast<mx_u32x2*>(o + kMxXTail + 8 * (t & 63)) = mx_u32x2{hi[4], hi[5]};
-  *reinterpret_cast<mx_u32x2*>(o + kMxXTail + 512 + 8 * (t & 63)) = mx_u32x2{lo[4], lo[5]};
+  uint8_t* o = unit + (t >> 6) * kMxXStep + 16 * (t & 63);
+  *reinterpret_cast<mx_u32x4*>(o) = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
+  *reinterpret_cast<mx_u32x4*>(o + kMxXPart) = mx_u32x4{hi[4], hi[5], lo[0], lo[1]};
+  *reinterpret_cast<mx_u32x4*>(o + 2 * kMxXPart) = mx_u32x4{lo[2], lo[3], lo[4], lo[5]};
   sc[4 * (t & 63) + (t >> 6)] = (uint8_t)e;
   __syncthreads();
   if (t < 64)
