@@ -601,7 +601,7 @@ static size_t gemm_split_bytes(const qmm_qtensor* w, int64_t m);
 
 size_t qmm_matmul_workspace_size(const qmm_qtensor* w, int64_t m) {
   if (!w || m <= 0) return 0;
-  if (is_mx(w->dtype)) return mx_planes(m, w->k);
+  if (is_mx(w->dtype)) return m <= kMxRawRows ? 0 : align256(mx_planes(m, w->k));
   const int vt = qmm_vec_dot_type(w->dtype);
   const size_t ggml = (size_t)m * (size_t)(w->k / qmm_block_size(vt)) * qmm_type_size(vt);
   if (!use_gemm(w, m)) return ggml;
@@ -1203,7 +1203,7 @@ static int mx_from_blocks(const GemvTarget* tg, int count, const void* xq, int64
     MxOut o = {};
     o.y = tg[j].y;
     o.accumulate = accumulate;
-    QMM_TRY(mx_product(d, tg[j].w, b, m, o, tg[j].ldy, s));
+    QMM_TRY(mx_product(d, tg[j].w, b, nullptr, m, o, tg[j].ldy, s));
   }
   return QMM_OK;
 }
@@ -1435,13 +1435,17 @@ static int multi_launch(Device* d, const qmm_qtensor* const* w, const MultiPlan&
 
 // Shared by qmm_matmul / qmm_matmul_multi: x f32 [m, k] against `count` weights.
 // One or more MXFP4 weights over typed rows: RMSNorm (f32 rows) if asked, the digit
-// planes in the workspace, then a product per weight.
+// planes in the workspace, then a product per weight. Up to two rows are quantized in
+// the product's own launch and need no workspace.
 static int mx_targets(const GemvTarget* tg, int count, const void* x, int x_dtype, int64_t m, int64_t ldx, void* ws,
                       size_t ws_bytes, const float* norm_w, float eps, const MxOut& how, hipStream_t s) {
   const int64_t k = tg[0].w->k;
   QMM_TRY(mx_check_rows(m, k));
-  const size_t planes = mx_align(mx_planes(m, k)), need = planes + (norm_w ? align256((size_t)(m * k) * 4) : 0);
-  if (!ws || ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
+  const bool direct = m <= kMxRawRows;
+  const size_t planes = direct ? 0 : align256(mx_planes(m, k));
+  const size_t need = planes + (norm_w ? align256((size_t)(m * k) * 4) : 0);
+  if (need && (!ws || ws_bytes < need))
+    return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
   Device* d;
   QMM_TRY(current_device(&d));
   uint8_t* b = (uint8_t*)ws;
@@ -1451,11 +1455,12 @@ static int mx_targets(const GemvTarget* tg, int count, const void* x, int x_dtyp
     x = xn;
     ldx = k;
   }
-  QMM_TRY(mx_quantize_x(d, x, x_dtype, m, k, ldx, nullptr, b, s));
+  const MxRaw raw = {x, ldx, nullptr, x_dtype, mx_wide16(x, x_dtype, ldx)};
+  if (!direct) QMM_TRY(mx_quantize_x(d, x, x_dtype, m, k, ldx, nullptr, b, s));
   for (int j = 0; j < count; ++j) {
     MxOut o = how;
     o.y = tg[j].y;
-    QMM_TRY(mx_product(d, tg[j].w, b, m, o, tg[j].ldy, s));
+    QMM_TRY(mx_product(d, tg[j].w, b, direct ? &raw : nullptr, m, o, tg[j].ldy, s));
   }
   return QMM_OK;
 }
@@ -1798,18 +1803,16 @@ static FfnWs ffn_ws(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, c
 }
 
 // The MXFP4 block's workspace: digit planes of the rows and of the activated rows, the
-// normalised rows, gate's and up's outputs.
+// normalised rows.
 struct MxFfnWs {
-  size_t xp, hp, xn, g, u, total;
+  size_t xp, hp, xn, total;
 };
 static MxFfnWs mx_ffn_ws(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t m, bool normalize) {
   MxFfnWs w;
   w.xp = 0;
-  w.hp = mx_align(mx_planes(m, gate->k));
-  w.xn = w.hp + mx_align(mx_planes(m, down->k));
-  w.g = w.xn + (normalize ? align256((size_t)(m * gate->k) * 4) : 0);
-  w.u = w.g + align256((size_t)(m * gate->n) * 4);
-  w.total = w.u + align256((size_t)(m * gate->n) * 4);
+  w.hp = m <= kMxRawRows ? 0 : align256(mx_planes(m, gate->k));
+  w.xn = w.hp + align256(mx_planes(m, down->k));
+  w.total = w.xn + (normalize ? align256((size_t)(m * gate->k) * 4) : 0);
   return w;
 }
 
@@ -1823,12 +1826,14 @@ static int mx_ffn(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, con
     x = xn;
     ldx = gate->k;
   }
-  QMM_TRY(mx_quantize_x(d, x, x_dtype, m, gate->k, ldx, nullptr, b + L.xp, s));
-  QMM_TRY(mx_glu(d, gate, up, 0, b + L.xp, m, m, nullptr, nullptr, b + L.hp, (float*)(b + L.g), (float*)(b + L.u), s));
+  const MxRaw raw = {x, ldx, nullptr, x_dtype, mx_wide16(x, x_dtype, ldx)};
+  const bool direct = m <= kMxRawRows;
+  if (!direct) QMM_TRY(mx_quantize_x(d, x, x_dtype, m, gate->k, ldx, nullptr, b + L.xp, s));
+  QMM_TRY(mx_glu(d, gate, up, 0, b + L.xp, direct ? &raw : nullptr, m, m, nullptr, nullptr, b + L.hp, s));
   MxOut o = {};
   o.y = y;
   o.accumulate = accumulate;
-  return mx_product(d, down, b + L.hp, m, o, ldy, s);
+  return mx_product(d, down, b + L.hp, nullptr, m, o, ldy, s);
 }
 
 size_t qmm_ffn_workspace_size(const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down, int64_t m,
@@ -2925,7 +2930,7 @@ static int64_t moe_chunk(int topk) { return std::min<int64_t>(4096, 8192 / std::
 // MXFP4 experts: workspace of up to mx_moe_chunk(topk) tokens (longer lists run as
 // consecutive chunks: 32768 pairs are far more work than reading the weights again).
 struct MxMoeWs {
-  size_t counts, offsets, pair_token, pair_weight, token_pairs, route, xp, g, u, hp, yp;
+  size_t counts, offsets, pair_token, pair_weight, token_pairs, route, xp, hp, yp;
   size_t shared, sg, shared_ws, total;
 };
 static int64_t mx_moe_chunk(int topk) { return std::max<int64_t>(1, 32768 / std::max(topk, 1)); }
@@ -2944,9 +2949,7 @@ static MxMoeWs mx_moe_ws(const qmm_qtensor* gate, int64_t tokens, int E, int k, 
   w.pair_weight = take(4 * P);
   w.token_pairs = take(4 * P);
   w.route = take(route_scratch(T, E, k));
-  w.xp = take(mx_planes(P, H));
-  w.g = take(4 * (size_t)P * F);
-  w.u = take(4 * (size_t)P * F);
+  w.xp = take(tokens <= kMxRawRows ? 0 : mx_planes(P, H));
   w.hp = take(mx_planes(P, F));
   w.yp = take(4 * (size_t)P * H);
   if (sh.gate) {
@@ -3060,13 +3063,16 @@ static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const
   QMM_TRY(current_device(&d));
   int32_t *counts = (int32_t*)(b + L.counts), *offsets = (int32_t*)(b + L.offsets);
   int32_t *ptok = (int32_t*)(b + L.pair_token), *tpairs = (int32_t*)(b + L.token_pairs);
-  float *pw = (float*)(b + L.pair_weight), *g = (float*)(b + L.g), *u = (float*)(b + L.u), *yp = (float*)(b + L.yp);
+  float *pw = (float*)(b + L.pair_weight), *yp = (float*)(b + L.yp);
   for (int64_t t0 = 0; t0 < tokens; t0 += chunk) {
     const int64_t T = std::min(chunk, tokens - t0), P = T * topk;
     const uint8_t* xc = (const uint8_t*)x + t0 * ldx * (int64_t)mx_type_size(x_dtype);
     QMM_TRY(route_scored(d, logits + t0 * experts, T, experts, topk, r, counts, offsets, ptok, pw, tpairs, b + L.route, s));
-    QMM_TRY(mx_quantize_x(d, xc, x_dtype, P, H, ldx, ptok, b + L.xp, s));
-    QMM_TRY(mx_glu(d, gate, up, experts, b + L.xp, P, T, counts, offsets, b + L.hp, g, u, s));
+    // (an expert has a token's row once at most: up to two tokens need no planes)
+    const MxRaw raw = {xc, ldx, ptok, x_dtype, mx_wide16(xc, x_dtype, ldx)};
+    const bool direct = T <= kMxRawRows && tokens <= kMxRawRows;
+    if (!direct) QMM_TRY(mx_quantize_x(d, xc, x_dtype, P, H, ldx, ptok, b + L.xp, s));
+    QMM_TRY(mx_glu(d, gate, up, experts, b + L.xp, direct ? &raw : nullptr, P, T, counts, offsets, b + L.hp, s));
     QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, T, counts, offsets, &yp, s));
     float *shared = nullptr, *sg = nullptr;
     if (sh.gate) {

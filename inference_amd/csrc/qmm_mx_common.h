@@ -159,6 +159,19 @@ __device__ __forceinline__ mx_f32x16 mx_mfma(const mx_u32x4& w, const mx_u32x6& 
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(__builtin_bit_cast(mx_i32x8, a), __builtin_bit_cast(mx_i32x8, b),
                                                          c, 4, 2, S, sw, S, sx);
 }
+// One step of 128 columns of a 16 x 16 tile: lane 16 g + r holds block g of row r, the
+// result's column is lane & 15, its rows 4 (lane / 16) + register. The result must not
+// share registers with an operand (the compiler allows it for this size; the sums were
+// wrong): the operands are kept past it.
+template <int S>
+__device__ __forceinline__ mx_f32x4 mx_mfma16(const mx_u32x4& w, const mx_u32x6& x, mx_f32x4 c, int sw, int sx) {
+  const mx_u32x8 a = __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
+  const mx_u32x8 b = __builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, -1, -1);
+  const mx_f32x4 d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      __builtin_bit_cast(mx_i32x8, a), __builtin_bit_cast(mx_i32x8, b), c, 4, 2, S, sw, S, sx);
+  asm volatile("" ::"v"(w), "v"(x), "v"(sw), "v"(sx), "v"(d));
+  return d;
+}
 // (the second digit's scale is the first's less 4 in every byte)
 constexpr int kMxLoScale = 0x04040404;
 // (result: lane's column = lane & 31, register r its row 8 (r / 4) + 4 (lane / 32) + r % 4)

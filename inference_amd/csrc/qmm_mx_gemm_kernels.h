@@ -3,6 +3,7 @@
 #pragma once
 
 #include "qmm_mx_common.h"
+#include "qmm_mx_quant_kernels.h"
 
 namespace qmm {
 
@@ -115,51 +116,187 @@ __device__ __forceinline__ void mx_put(const MxOut& o, long long row, int ldy, i
   }
 }
 
-// Up to 32 rows: a workgroup of W waves takes one 32-column tile of the output and
-// splits K over its waves by chunks; the waves' sums meet in LDS, in wave order.
-template <int W>
-__device__ __forceinline__ void mx_gemv(const MxOut& o, const MxRows& rows, int n, int kc, int tile,
-                                        const uint8_t* __restrict__ xq, int ldy) {
-  __shared__ float red[W][32][33];
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, c = lane & 31;
-  const long long wrow = rows.w0 + min(kMxTile * tile + c, n - 1);
-  const long long xrow = rows.first + min(c, rows.count - 1);
-  const uint8_t* wp = o.w + mx_w_at(wrow, h, kc);
-  const uint8_t* wsp = o.w + mx_ws_at(wrow, h, kc);
-  const uint8_t* xp = xq + mx_x_at(xrow, h, kc);
-  const uint8_t* xsp = xq + mx_xs_at(xrow, h, kc);
-  mx_f32x16 acc = (mx_f32x16)(0.0f);
-  for (int k = wave; k < kc; k += W) {
-    const uint8_t* wk = wp + (long long)k * kMxUnit;
-    const uint8_t* xk = xp + (long long)k * kMxXUnit;
-    const int sw = *reinterpret_cast<const int*>(wsp + (long long)k * kMxUnit);
-    const int sx = *reinterpret_cast<const int*>(xsp + (long long)k * kMxXUnit), sl = sx - kMxLoScale;
-#define QMM_MX_STEP(S)                                                                     \
-  {                                                                                        \
-    const mx_u32x12 x = mx_get_x(xk + S * kMxXStep);                                       \
-    const mx_u32x4 w = *reinterpret_cast<const mx_u32x4*>(wk + S * kMxStepBytes);          \
-    acc = mx_mfma<S>(w, mx_hi(x), acc, sw, sx);                                            \
-    acc = mx_mfma<S>(w, mx_lo(x), acc, sw, sl);                                            \
-  }
-    QMM_MX_STEP(0)
-    QMM_MX_STEP(1)
-    QMM_MX_STEP(2)
-    QMM_MX_STEP(3)
-#undef QMM_MX_STEP
-  }
+// Unquantized rows: row i of the product is row src[i] of x (or i), of type T.
+struct MxRaw {
+  const void* x;
+  long long ldx;
+  const int* src;
+  int type, wide;
+};
+
+// Up to 16 rows: a workgroup of W waves takes NT 16-column tiles of the output and splits
+// K over its waves by chunks; the waves' sums meet in LDS, in wave order. GLU: half of
+// the tiles are rows of o.w, half the same rows of `up`, and silu(first) * second of
+// their 32 columns becomes one block of the digit planes o.y.
+// RAW: up to two rows, quantized here (each wave its own chunks, a block a lane); else
+// digit planes.
+//
+// What bounds it: the weights' stream. A wave loads a chunk of a tile (2 KB) in two
+// instructions, U of them in flight; 16 waves a CU ask for far more than a round trip's
+// worth. One matrix instruction takes 16 columns x 128 of K by up to 16 rows, so rows
+// cost nothing until their digits' reads show. Rows of x are read by every workgroup:
+// quantized ahead into planes (1.5 bytes a value) above two rows, in place below, where
+// a launch of its own costs more than it takes (2.4 us and the gap).
+template <int W, int NT, bool GLU, bool RAW>
+__device__ __forceinline__ void mx_gemv(const MxOut& o, const uint8_t* __restrict__ up, const MxRows& rows, int n, int k,
+                                        int n0, const uint8_t* __restrict__ xq, const MxRaw& raw, int ldy) {
+  constexpr int U = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // chunks of a wave in flight
+  constexpr int NC = GLU ? NT / 2 : NT;             // 16-column tiles of the output
+  static_assert(!GLU || NT == 4, "a block of 32 columns");
+  constexpr int kRowF = 16 * NT + 4;                // floats of a row of sums, padded
+  constexpr int kRed = W * 16 * kRowF * 4, kRaw = RAW ? W * U * 16 * 64 : 0;
+  // a raw block: 48 bytes of digits, its scale byte in the last of 16 more
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kRed > kRaw ? kRed : kRaw];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int c = lane & 15, g = lane >> 4, h = g & 1;
+  const int kc = (k + kMxChunk - 1) / kMxChunk;
+  const uint8_t *wp[NT], *ws[NT];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) red[wave][c][8 * (r >> 2) + 4 * h + (r & 3)] = acc[r];
+  for (int j = 0; j < NT; ++j) {
+    const long long r = rows.w0 + min(n0 + 16 * (j % NC) + c, n - 1);
+    const uint8_t* b = j < NC ? o.w : up;
+    wp[j] = b + mx_w_at(r, h, kc) + (g >> 1) * kMxStepBytes;
+    ws[j] = b + mx_ws_at(r, h, kc);
+  }
+  const int xc = min(c, rows.count - 1);
+  const uint8_t *xp = nullptr, *xs = nullptr;
+  if constexpr (!RAW) {
+    xp = xq + mx_x_at(rows.first + xc, h, kc) + (g >> 1) * kMxXStep;
+    xs = xq + mx_xs_at(rows.first + xc, h, kc);
+  }
+  uint8_t* mine = smem + wave * (U * 16 * 64);  // RAW: this wave's blocks, [chunk][row][block]
+  mx_f32x4 acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = (mx_f32x4)(0.0f);
+  for (int k0 = wave; k0 < kc; k0 += W * U) {
+    mx_u32x4 w[U][NT][2];
+    int sw[U][NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long at = (long long)min(k0 + W * u, kc - 1) * kMxUnit;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        w[u][j][0] = *reinterpret_cast<const mx_u32x4*>(wp[j] + at);
+        w[u][j][1] = *reinterpret_cast<const mx_u32x4*>(wp[j] + at + 2 * kMxStepBytes);
+        sw[u][j] = *reinterpret_cast<const int*>(ws[j] + at);
+      }
+    }
+    if constexpr (RAW) {
+      // lane 16 u + 8 row + block
+      const int u = lane >> 4, row = (lane >> 3) & 1, b = lane & 7, kk = k0 + W * u;
+      if (u < U && row < rows.count && kk < kc) {
+        mx_u32x6 hi = (mx_u32x6)(0u), lo = (mx_u32x6)(0u);
+        int e = 4;
+        const int col = kMxChunk * kk + 32 * b;
+        if (col < k) {
+          float v[32];
+          const int r = rows.first + row;
+          const long long at = (raw.src ? raw.src[r] : r) * raw.ldx + col;
+          const uint32_t amax = raw.type == kF32   ? mx_load_block<kF32>(raw.x, at, raw.wide, v)
+                                : raw.type == kF16 ? mx_load_block<kF16>(raw.x, at, raw.wide, v)
+                                                   : mx_load_block<kBF16>(raw.x, at, raw.wide, v);
+          e = mx_x_byte(amax);
+          mx_digits(v, e, hi, lo);
+        }
+        uint8_t* d = mine + 64 * lane;
+        *reinterpret_cast<mx_u32x4*>(d) = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
+        *reinterpret_cast<mx_u32x4*>(d + 16) = mx_u32x4{hi[4], hi[5], lo[0], lo[1]};
+        *reinterpret_cast<mx_u32x4*>(d + 32) = mx_u32x4{lo[2], lo[3], lo[4], lo[5]};
+        *reinterpret_cast<int*>(d + 48) = e;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int kk = k0 + W * u;
+      if (kk >= kc) break;
+      mx_u32x12 x[2];
+      int sx[2];
+      if constexpr (RAW) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint8_t* d = mine + 64 * (16 * u + 8 * xc + 4 * s + g);
+          x[s] = mx_x(*reinterpret_cast<const mx_u32x4*>(d), *reinterpret_cast<const mx_u32x4*>(d + 16),
+                      *reinterpret_cast<const mx_u32x4*>(d + 32));
+          sx[s] = *reinterpret_cast<const int*>(d + 48);
+        }
+      } else {
+        const uint8_t* p = xp + (long long)kk * kMxXUnit;
+        x[0] = mx_get_x(p);
+        x[1] = mx_get_x(p + 2 * kMxXStep);
+        const int b = *reinterpret_cast<const int*>(xs + (long long)kk * kMxXUnit) >> (8 * (g >> 1));
+        sx[0] = b & 255;
+        sx[1] = b >> 16 & 255;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int b = sw[u][j] >> (8 * (g >> 1));  // block 2 s + h of steps s = g / 2 and 2 + g / 2
+        acc[j] = mx_mfma16<0>(w[u][j][0], mx_hi(x[0]), acc[j], b, sx[0]);
+        acc[j] = mx_mfma16<0>(w[u][j][0], mx_lo(x[0]), acc[j], b, sx[0] - 4);
+        acc[j] = mx_mfma16<0>(w[u][j][1], mx_hi(x[1]), acc[j], b >> 16, sx[1]);
+        acc[j] = mx_mfma16<0>(w[u][j][1], mx_lo(x[1]), acc[j], b >> 16, sx[1] - 4);
+      }
+    }
+    if constexpr (RAW) __builtin_amdgcn_wave_barrier();
+  }
+  if constexpr (RAW) __syncthreads();  // the sums take the blocks' place
+  float(*red)[16][kRowF] = reinterpret_cast<float(*)[16][kRowF]>(smem);
+#pragma unroll
+  for (int j = 0; j < NT; ++j) *reinterpret_cast<mx_f32x4*>(&red[wave][c][16 * j + 4 * g]) = acc[j];
   __syncthreads();
+  auto total = [&](int m, int q) {
+    float v = red[0][m][q];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v += red[i][m][q];
+    return v;
+  };
+  if constexpr (GLU) {
+    // h over the first wave's sums, then a lane a row
+    const int cols = min(32, n - n0);
+    float act[(32 * 16 + 64 * W - 1) / (64 * W)];
+#pragma unroll
+    for (int i = 0; i * 64 * W < 512; ++i) {
+      const int j = t + i * 64 * W, m = j >> 5, q = j & 31;
+      if (m < rows.count) {
+        const float a = total(m, q), b = total(m, 32 + q);
+        act[i] = a / (1.0f + expf(-a)) * b;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i * 64 * W < 512; ++i) {
+      const int j = t + i * 64 * W;
+      if (j >> 5 < rows.count) red[0][j >> 5][j & 31] = act[i];
+    }
+    __syncthreads();
+    if (t >= rows.count) return;
+    float v[32];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      v[j] = red[0][t][j];
+      amax = max(amax, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+    }
+    mx_u32x6 hi, lo;
+    const int e = mx_x_byte(amax);
+    mx_digits(v, e, hi, lo);
+    const long long r = rows.first + t;
+    const int kf = (n + kMxChunk - 1) / kMxChunk, blk = n0 % kMxChunk / 32;
+    uint8_t* unit = static_cast<uint8_t*>(o.y) + ((r >> 5) * kf + n0 / kMxChunk) * kMxXUnit;
+    mx_put_block(unit, blk >> 1, 32 * (blk & 1) + (int)(r & 31), e, hi, lo);
+    if (n0 + cols >= n)  // the rest of the chunk: the product reads whole ones
+      for (int z = blk + 1; z < 8; ++z)
+        mx_put_block(unit, z >> 1, 32 * (z & 1) + (int)(r & 31), 4, (mx_u32x6)(0u), (mx_u32x6)(0u));
+    return;
+  }
   auto put = [&](auto type) {
-    constexpr int T = decltype(type)::value, V = T == kF32 ? 4 : 8, LR = 32 / V;
+    constexpr int T = decltype(type)::value, V = T == kF32 ? 4 : 8, LR = 16 * NT / V;
     for (int j = t; j < LR * rows.count; j += 64 * W) {
-      const int m = j / LR, q = V * (j % LR), col = kMxTile * tile + q;
+      const int m = j / LR, q = V * (j % LR), col = n0 + q;
       float v[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[i] = red[0][m][q + i];
-#pragma unroll
-        for (int w = 1; w < W; ++w) v[i] += red[w][m][q + i];
+        v[i] = total(m, q + i);
         if (o.bias != nullptr && col + i < n) v[i] += mx_load(o.bias, o.bias_type, col + i);
       }
       mx_put<T, V>(o, rows.first + m, ldy, col, n, v);
@@ -415,24 +552,50 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const uint8_t* __restric
 }
 }  // namespace qmm
 
-// Dense rows: grid (32-column tiles, 32-row tiles).
-extern "C" __global__ void __launch_bounds__(512) qmm_mx_gemv(qmm::MxOut o, int m, int n, int kc,
-                                                              const uint8_t* __restrict__ xq, int ldy) {
-  const int first = 32 * blockIdx.y;
-  const qmm::MxRows r = {0, first, min(m - first, 32)};
-  qmm::mx_gemv<8>(o, r, n, kc, blockIdx.x, xq, ldy);
-}
+// Up to 16 rows. Dense: grid (16 NT-column tiles). Routed: grid (column tiles, row tiles).
+#define QMM_MX_GEMV(W, NT, NAME, RAW)                                                                          \
+  extern "C" __global__ void __launch_bounds__(64 * W) qmm_mx_gemv##NAME##_w##W##_t##NT(                       \
+      qmm::MxOut o, int m, int n, int k, const uint8_t* __restrict__ xq, qmm::MxRaw raw, int ldy) {            \
+    const qmm::MxRows r = {0, 0, m};                                                                           \
+    qmm::mx_gemv<W, NT, false, RAW>(o, nullptr, r, n, k, 16 * NT * blockIdx.x, xq, raw, ldy);                  \
+  }
+#define QMM_MX_GEMVS(W)         \
+  QMM_MX_GEMV(W, 1, , false)    \
+  QMM_MX_GEMV(W, 2, , false)    \
+  QMM_MX_GEMV(W, 1, _raw, true) \
+  QMM_MX_GEMV(W, 2, _raw, true)
+QMM_MX_GEMVS(4)
+QMM_MX_GEMVS(8)
+QMM_MX_GEMVS(16)
 
-// Routed rows: grid (32-column tiles, row tiles, weights).
-extern "C" __global__ void __launch_bounds__(512) qmm_mx_expert_gemv(qmm::MxOut o0, qmm::MxOut o1, int experts,
-                                                                     int pairs, int n, int kc,
-                                                                     const int* __restrict__ counts,
-                                                                     const int* __restrict__ offsets,
-                                                                     const uint8_t* __restrict__ xq, int ldy) {
-  qmm::MxRows r;
-  if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 32, blockIdx.y, r)) return;
-  qmm::mx_gemv<8>(blockIdx.z ? o1 : o0, r, n, kc, blockIdx.x, xq, ldy);
-}
+#define QMM_MX_EXPERT_GEMV(W)                                                                                  \
+  extern "C" __global__ void __launch_bounds__(64 * W) qmm_mx_expert_gemv_w##W(                                \
+      qmm::MxOut o0, qmm::MxOut o1, int experts, int pairs, int n, int k, const int* __restrict__ counts,      \
+      const int* __restrict__ offsets, const uint8_t* __restrict__ xq, int ldy) {                              \
+    qmm::MxRows r;                                                                                             \
+    if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 16, blockIdx.y, r)) return;                   \
+    qmm::mx_gemv<W, 1, false, false>(blockIdx.z ? o1 : o0, nullptr, r, n, k, 16 * blockIdx.x, xq, qmm::MxRaw{}, ldy);  \
+  }
+QMM_MX_EXPERT_GEMV(4)
+QMM_MX_EXPERT_GEMV(8)
+QMM_MX_EXPERT_GEMV(16)
+
+// Gate and up with the activation: dense rows (experts 0) or routed ones.
+#define QMM_MX_GLU_GEMV(W, NAME, RAW)                                                                          \
+  extern "C" __global__ void __launch_bounds__(64 * W) qmm_mx_glu_gemv##NAME##_w##W(                           \
+      qmm::MxOut o, const uint8_t* __restrict__ up, int experts, int pairs, int n, int k,                      \
+      const int* __restrict__ counts, const int* __restrict__ offsets, const uint8_t* __restrict__ xq,         \
+      qmm::MxRaw raw) {                                                                                        \
+    qmm::MxRows r = {0, 0, pairs};                                                                             \
+    if (experts > 0 && !qmm::mx_expert_tile(counts, offsets, experts, pairs, n, RAW ? 2 : 16, blockIdx.y, r)) return;  \
+    qmm::mx_gemv<W, 4, true, RAW>(o, up, r, n, k, 32 * blockIdx.x, xq, raw, 0);                                \
+  }
+#define QMM_MX_GLU_GEMVS(W)        \
+  QMM_MX_GLU_GEMV(W, , false)      \
+  QMM_MX_GLU_GEMV(W, _raw, true)
+QMM_MX_GLU_GEMVS(4)
+QMM_MX_GLU_GEMVS(8)
+QMM_MX_GLU_GEMVS(16)
 
 #define QMM_MX_GEMM(NAME, FM, FN, WM, WN, WK, EU)                                                              \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK, EU) qmm_mx_gemm_##NAME(                      \

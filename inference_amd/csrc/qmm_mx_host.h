@@ -125,20 +125,44 @@ const MxTileCfg& mx_tile_for(const Device* d, int64_t row_tiles64, int64_t row_t
   return *best;
 }
 
-// y = planes . W^T over m dense rows.
-int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, int64_t m, MxOut o, int64_t ldy, hipStream_t s) {
+// Unquantized rows of a product (qmm::MxRaw).
+struct MxRaw {
+  const void* x;
+  long long ldx;
+  const int32_t* src;
+  int type, wide;
+};
+
+// Rows of the narrow kernels: of a tile, of unquantized rows, of an expert (two tiles,
+// the second of which finds the weights in cache).
+constexpr int64_t kMxGemvRows = 16, kMxRawRows = 2, kMxExpertGemvRows = 32;
+
+// Waves that split K: a chunk of 256 columns each at least.
+int mx_gemv_waves(int64_t k) {
+  const int64_t kc = mx_chunks(k);
+  return kc >= 16 ? 16 : kc >= 8 ? 8 : 4;
+}
+
+// y = x . W^T over m dense rows: of digit planes, or (up to two rows) of raw ones.
+int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, const MxRaw* raw, int64_t m, MxOut o, int64_t ldy,
+               hipStream_t s) {
   o.w = w->data;
   o.wide = mx_wide16(o.y, o.y_type, ldy);
-  int mm = (int)m, n = (int)w->n, kc = (int)mx_chunks(w->k), ld = (int)ldy;
-  void* args[] = {&o, &mm, &n, &kc, &planes, &ld};
+  int mm = (int)m, n = (int)w->n, k = (int)w->k, ld = (int)ldy;
   hipFunction_t f;
-  if (m <= 32) {
-    QMM_TRY(kernel(d, "qmm_mx_gemv", &f));
-    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 32), 1, 1, 512, 1, 1, 0, s, args, nullptr));
+  char name[40];
+  if (m <= kMxGemvRows) {
+    MxRaw r = raw ? *raw : MxRaw();
+    const int waves = mx_gemv_waves(k), nt = ceil_div(n, 16) > 2u * (unsigned)d->num_cu ? 2 : 1;
+    snprintf(name, sizeof(name), "qmm_mx_gemv%s_w%d_t%d", raw ? "_raw" : "", waves, nt);
+    void* args[] = {&o, &mm, &n, &k, &planes, &r, &ld};
+    QMM_TRY(kernel(d, name, &f));
+    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 16 * nt), 1, 1, 64 * waves, 1, 1, 0, s, args, nullptr));
     return QMM_OK;
   }
+  int kc = (int)mx_chunks(k);
+  void* args[] = {&o, &mm, &n, &kc, &planes, &ld};
   const MxTileCfg& c = mx_tile_for(d, ceil_div(m, 64), ceil_div(m, 128), n);
-  char name[40];
   snprintf(name, sizeof(name), "qmm_mx_gemm_%s", c.name);
   QMM_TRY(kernel(d, name, &f));
   QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, c.cols), ceil_div(m, c.rows), 1, c.threads, 1, 1, 0, s, args, nullptr));
@@ -157,61 +181,57 @@ int mx_expert_product(Device* d, const qmm_qtensor* const* w, int count, int exp
     o[j].y = y[i];
     o[j].wide = mx_wide16(y[i], QMM_F32, w[0]->n / experts);
   }
-  int E = experts, P = (int)pairs, n = (int)(w[0]->n / experts), kc = (int)mx_chunks(w[0]->k), ld = n;
-  void* args[] = {&o[0], &o[1], &E, &P, &n, &kc, &counts, &offsets, &planes, &ld};
+  int E = experts, P = (int)pairs, n = (int)(w[0]->n / experts), k = (int)w[0]->k, kc = (int)mx_chunks(k), ld = n;
   hipFunction_t f;
   const int64_t active = std::min<int64_t>(experts, pairs);
-  if (max_rows <= 32) {
-    const int64_t tiles = pairs / 32 + active;
+  char name[40];
+  if (max_rows <= kMxExpertGemvRows) {
+    const int64_t tiles = pairs / kMxGemvRows + active;
     if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
-    QMM_TRY(kernel(d, "qmm_mx_expert_gemv", &f));
-    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 32), (unsigned)tiles, (unsigned)count, 512, 1, 1, 0, s, args, nullptr));
+    const int waves = mx_gemv_waves(k);
+    snprintf(name, sizeof(name), "qmm_mx_expert_gemv_w%d", waves);
+    void* args[] = {&o[0], &o[1], &E, &P, &n, &k, &counts, &offsets, &planes, &ld};
+    QMM_TRY(kernel(d, name, &f));
+    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 16), (unsigned)tiles, (unsigned)count, 64 * waves, 1, 1, 0, s, args, nullptr));
     return QMM_OK;
   }
+  void* args[] = {&o[0], &o[1], &E, &P, &n, &kc, &counts, &offsets, &planes, &ld};
   // (the tiles that there will be, each expert's last one half full)
   const MxTileCfg& c = mx_tile_for(d, pairs / 64 + (active + 1) / 2, pairs / 128 + (active + 1) / 2, (int64_t)n * count);
   const int64_t tiles = pairs / c.rows + active;
   if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
-  char name[40];
   snprintf(name, sizeof(name), "qmm_mx_expert_gemm_%s", c.name);
   QMM_TRY(kernel(d, name, &f));
   QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, c.cols), (unsigned)tiles, (unsigned)count, c.threads, 1, 1, 0, s, args, nullptr));
   return QMM_OK;
 }
 
-int mx_silu_mul(Device* d, const float* g, const float* u, int64_t m, int64_t k, uint8_t* planes, hipStream_t s) {
-  int mm = (int)m, kk = (int)k, kc = (int)mx_chunks(k);
-  void* args[] = {&g, &u, &mm, &kk, &kc, &planes};
-  return launch(d, "qmm_mx_silu_mul", mx_plane_units(m, k), 256, 0, s, args);
-}
-
-// silu(gate) * up of the planes' rows, as the planes of the down product's rows: dense
-// rows (experts 0) or routed ones.
-int mx_glu(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, int experts, const uint8_t* planes, int64_t m,
-           int64_t max_rows, const int32_t* counts, const int32_t* offsets, uint8_t* out, float* g, float* u, hipStream_t s) {
-  const int64_t F = gate->n / std::max(experts, 1);
-  const int64_t tiles = experts ? m / 128 + std::min<int64_t>(experts, m) : ceil_div(m, 128);
-  if (max_rows <= 32) {
-    if (experts) {
-      const qmm_qtensor* w[2] = {gate, up};
-      float* y[2] = {g, u};
-      QMM_TRY(mx_expert_product(d, w, 2, experts, planes, m, max_rows, counts, offsets, y, s));
-    } else {
-      MxOut o = {};
-      o.y = g;
-      QMM_TRY(mx_product(d, gate, planes, m, o, F, s));
-      o.y = u;
-      QMM_TRY(mx_product(d, up, planes, m, o, F, s));
-    }
-    return mx_silu_mul(d, g, u, m, F, out, s);
-  }
-  if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many rows");
+// silu(gate) * up of m rows as the digit planes of the down product's rows: dense rows
+// (experts 0) or routed ones, of planes or (up to kMxRawRows an expert) raw.
+int mx_glu(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, int experts, const uint8_t* planes,
+           const MxRaw* raw, int64_t m, int64_t max_rows, const int32_t* counts, const int32_t* offsets, uint8_t* out,
+           hipStream_t s) {
+  const int64_t F = gate->n / std::max(experts, 1), active = std::min<int64_t>(experts, m);
   MxOut o = {};
   o.w = gate->data;
   o.y = out;
   const void* uw = up->data;
-  int E = experts, P = (int)m, n = (int)F, kc = (int)mx_chunks(gate->k);
+  int E = experts, P = (int)m, n = (int)F, k = (int)gate->k, kc = (int)mx_chunks(k);
   hipFunction_t f;
+  char name[40];
+  const bool gemv = max_rows <= (experts ? kMxExpertGemvRows : kMxGemvRows);
+  const int64_t bm = gemv ? (raw ? kMxRawRows : kMxGemvRows) : 128;
+  const int64_t tiles = experts ? m / bm + active : ceil_div(m, bm);
+  if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many rows");
+  if (gemv) {
+    MxRaw r = raw ? *raw : MxRaw();
+    const int waves = mx_gemv_waves(k);
+    snprintf(name, sizeof(name), "qmm_mx_glu_gemv%s_w%d", raw ? "_raw" : "", waves);
+    void* args[] = {&o, &uw, &E, &P, &n, &k, &counts, &offsets, &planes, &r};
+    QMM_TRY(kernel(d, name, &f));
+    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 32), (unsigned)tiles, 1, 64 * waves, 1, 1, 0, s, args, nullptr));
+    return QMM_OK;
+  }
   if (!experts) {
     void* args[] = {&o, &uw, &P, &n, &kc, &planes};
     QMM_TRY(kernel(d, "qmm_mx_glu_128x128", &f));

@@ -330,33 +330,3 @@ extern "C" __global__ void __launch_bounds__(256) qmm_mx_blocks_to_planes(const 
   }
   qmm::mx_put_digits(out + u * qmm::kMxXUnit, sc, t, e, d[0], d[1]);
 }
-
-// silu(g) * u -> digit planes, rows x k f32 (the down projection's input).
-extern "C" __global__ void __launch_bounds__(256) qmm_mx_silu_mul(const float* __restrict__ g,
-                                                                  const float* __restrict__ u, int m, int k, int kc,
-                                                                  uint8_t* __restrict__ out) {
-  __shared__ __attribute__((aligned(16))) float buf[qmm::kMxTile * qmm::kMxLdsRow];
-  __shared__ __attribute__((aligned(16))) uint8_t sc[256];
-  const int t = threadIdx.x;
-  const long long unit = blockIdx.x;
-  const int r0 = (int)(unit / kc) * qmm::kMxTile, c0 = (int)(unit % kc) * qmm::kMxChunk;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 4 * i + (t >> 6), c = 4 * (t & 63);
-    qmm::mx_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (r0 + r < m && c0 + c < k) {
-      const long long at = (long long)(r0 + r) * k + c0 + c;
-      const qmm::mx_f32x4 a = *reinterpret_cast<const qmm::mx_f32x4*>(g + at);
-      v = *reinterpret_cast<const qmm::mx_f32x4*>(u + at);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = a[j] / (1.0f + expf(-a[j])) * v[j];
-    }
-    *reinterpret_cast<qmm::mx_f32x4*>(buf + r * qmm::kMxLdsRow + c) = v;
-  }
-  __syncthreads();
-  float x[32];
-  const int e = qmm::mx_x_byte(qmm::mx_unit_block(buf, t, x));
-  qmm::mx_u32x6 hi, lo;
-  qmm::mx_digits(x, e, hi, lo);
-  qmm::mx_put_digits(out + unit * qmm::kMxXUnit, sc, t, e, hi, lo);
-}

@@ -426,7 +426,7 @@ class QMatMul:
             L = lib()
             h = qt.handle
             ws, ws_bytes, ws_ptr = None, 0, None
-            if m > 2 or qt._dtype == GgmlDType.MXFP4:  # (one and two rows of the others: in the GEMV's prologue)
+            if m > 2:  # one and two rows are quantized in the GEMV's prologue
                 ws_bytes = int(L.qmm_matmul_workspace_size(h, m))
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
                 ws_ptr = ws.data_ptr()
@@ -470,10 +470,13 @@ class QMatMul:
         y = torch.empty((m, n), dtype=x.dtype, device=dev)
         if m != 0:
             L = lib()
-            ws_bytes = int(L.qmm_linear_workspace_size(qt.handle, m))
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            args = (qt.handle, x2.data_ptr(), tag, m, max(x2.stride(0), k), bptr, btag, y.data_ptr(), tag, n,
-                    ws.data_ptr(), ws_bytes, _raw_stream(dev.index))
+            ws, ws_bytes, ws_ptr = None, 0, None
+            if m > 2:
+                ws_bytes = int(L.qmm_linear_workspace_size(qt.handle, m))
+                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+                ws_ptr = ws.data_ptr()
+            args = (qt.handle, x2.data_ptr(), tag, m, max(x2.stride(0), k), bptr, btag, y.data_ptr(), tag, n, ws_ptr,
+                    ws_bytes, _raw_stream(dev.index))
             if torch.cuda.current_device() == dev.index:
                 status = L.qmm_linear(*args)
             else:
