@@ -601,7 +601,7 @@ static size_t gemm_split_bytes(const qmm_qtensor* w, int64_t m);
 
 size_t qmm_matmul_workspace_size(const qmm_qtensor* w, int64_t m) {
   if (!w || m <= 0) return 0;
-  if (is_mx(w->dtype)) return m <= kMxRawRows ? 0 : align256(mx_planes(m, w->k));
+  if (is_mx(w->dtype)) return mx_raw_fits(m, w->k) ? 0 : align256(mx_planes(m, w->k));
   const int vt = qmm_vec_dot_type(w->dtype);
   const size_t ggml = (size_t)m * (size_t)(w->k / qmm_block_size(vt)) * qmm_type_size(vt);
   if (!use_gemm(w, m)) return ggml;
@@ -1441,7 +1441,7 @@ static int mx_targets(const GemvTarget* tg, int count, const void* x, int x_dtyp
                       size_t ws_bytes, const float* norm_w, float eps, const MxOut& how, hipStream_t s) {
   const int64_t k = tg[0].w->k;
   QMM_TRY(mx_check_rows(m, k));
-  const bool direct = m <= kMxRawRows;
+  const bool direct = mx_raw_fits(m, k);
   const size_t planes = direct ? 0 : align256(mx_planes(m, k));
   const size_t need = planes + (norm_w ? align256((size_t)(m * k) * 4) : 0);
   if (need && (!ws || ws_bytes < need))
@@ -1810,7 +1810,7 @@ struct MxFfnWs {
 static MxFfnWs mx_ffn_ws(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t m, bool normalize) {
   MxFfnWs w;
   w.xp = 0;
-  w.hp = m <= kMxRawRows ? 0 : align256(mx_planes(m, gate->k));
+  w.hp = mx_raw_fits(m, gate->k) ? 0 : align256(mx_planes(m, gate->k));
   w.xn = w.hp + align256(mx_planes(m, down->k));
   w.total = w.xn + (normalize ? align256((size_t)(m * gate->k) * 4) : 0);
   return w;
@@ -1827,7 +1827,7 @@ static int mx_ffn(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, con
     ldx = gate->k;
   }
   const MxRaw raw = {x, ldx, nullptr, x_dtype, mx_wide16(x, x_dtype, ldx)};
-  const bool direct = m <= kMxRawRows;
+  const bool direct = mx_raw_fits(m, gate->k);
   if (!direct) QMM_TRY(mx_quantize_x(d, x, x_dtype, m, gate->k, ldx, nullptr, b + L.xp, s));
   QMM_TRY(mx_glu(d, gate, up, 0, b + L.xp, direct ? &raw : nullptr, m, m, nullptr, nullptr, b + L.hp, s));
   MxOut o = {};
@@ -2949,7 +2949,7 @@ static MxMoeWs mx_moe_ws(const qmm_qtensor* gate, int64_t tokens, int E, int k, 
   w.pair_weight = take(4 * P);
   w.token_pairs = take(4 * P);
   w.route = take(route_scratch(T, E, k));
-  w.xp = take(tokens <= kMxRawRows ? 0 : mx_planes(P, H));
+  w.xp = take(mx_raw_fits(tokens, H) ? 0 : mx_planes(P, H));
   w.hp = take(mx_planes(P, F));
   w.yp = take(4 * (size_t)P * H);
   if (sh.gate) {
@@ -3070,7 +3070,7 @@ static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const
     QMM_TRY(route_scored(d, logits + t0 * experts, T, experts, topk, r, counts, offsets, ptok, pw, tpairs, b + L.route, s));
     // (an expert has a token's row once at most: up to two tokens need no planes)
     const MxRaw raw = {xc, ldx, ptok, x_dtype, mx_wide16(xc, x_dtype, ldx)};
-    const bool direct = T <= kMxRawRows && tokens <= kMxRawRows;
+    const bool direct = mx_raw_fits(tokens, H);
     if (!direct) QMM_TRY(mx_quantize_x(d, xc, x_dtype, P, H, ldx, ptok, b + L.xp, s));
     QMM_TRY(mx_glu(d, gate, up, experts, b + L.xp, direct ? &raw : nullptr, P, T, counts, offsets, b + L.hp, s));
     QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, T, counts, offsets, &yp, s));

@@ -124,126 +124,11 @@ struct MxRaw {
   int type, wide;
 };
 
-// Up to 16 rows: a workgroup of W waves takes NT 16-column tiles of the output and splits
-// K over its waves by chunks; the waves' sums meet in LDS, in wave order. GLU: half of
-// the tiles are rows of o.w, half the same rows of `up`, and silu(first) * second of
-// their 32 columns becomes one block of the digit planes o.y.
-// RAW: up to two rows, quantized here (each wave its own chunks, a block a lane); else
-// digit planes.
-//
-// What bounds it: the weights' stream. A wave loads a chunk of a tile (2 KB) in two
-// instructions, U of them in flight; 16 waves a CU ask for far more than a round trip's
-// worth. One matrix instruction takes 16 columns x 128 of K by up to 16 rows, so rows
-// cost nothing until their digits' reads show. Rows of x are read by every workgroup:
-// quantized ahead into planes (1.5 bytes a value) above two rows, in place below, where
-// a launch of its own costs more than it takes (2.4 us and the gap).
-template <int W, int NT, bool GLU, bool RAW>
-__device__ __forceinline__ void mx_gemv(const MxOut& o, const uint8_t* __restrict__ up, const MxRows& rows, int n, int k,
-                                        int n0, const uint8_t* __restrict__ xq, const MxRaw& raw, int ldy) {
-  constexpr int U = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // chunks of a wave in flight
-  constexpr int NC = GLU ? NT / 2 : NT;             // 16-column tiles of the output
-  static_assert(!GLU || NT == 4, "a block of 32 columns");
-  constexpr int kRowF = 16 * NT + 4;                // floats of a row of sums, padded
-  constexpr int kRed = W * 16 * kRowF * 4, kRaw = RAW ? W * U * 16 * 64 : 0;
-  // a raw block: 48 bytes of digits, its scale byte in the last of 16 more
-  __shared__ __attribute__((aligned(16))) uint8_t smem[kRed > kRaw ? kRed : kRaw];
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int c = lane & 15, g = lane >> 4, h = g & 1;
-  const int kc = (k + kMxChunk - 1) / kMxChunk;
-  const uint8_t *wp[NT], *ws[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const long long r = rows.w0 + min(n0 + 16 * (j % NC) + c, n - 1);
-    const uint8_t* b = j < NC ? o.w : up;
-    wp[j] = b + mx_w_at(r, h, kc) + (g >> 1) * kMxStepBytes;
-    ws[j] = b + mx_ws_at(r, h, kc);
-  }
-  const int xc = min(c, rows.count - 1);
-  const uint8_t *xp = nullptr, *xs = nullptr;
-  if constexpr (!RAW) {
-    xp = xq + mx_x_at(rows.first + xc, h, kc) + (g >> 1) * kMxXStep;
-    xs = xq + mx_xs_at(rows.first + xc, h, kc);
-  }
-  uint8_t* mine = smem + wave * (U * 16 * 64);  // RAW: this wave's blocks, [chunk][row][block]
-  mx_f32x4 acc[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j] = (mx_f32x4)(0.0f);
-  for (int k0 = wave; k0 < kc; k0 += W * U) {
-    mx_u32x4 w[U][NT][2];
-    int sw[U][NT];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long at = (long long)min(k0 + W * u, kc - 1) * kMxUnit;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        w[u][j][0] = *reinterpret_cast<const mx_u32x4*>(wp[j] + at);
-        w[u][j][1] = *reinterpret_cast<const mx_u32x4*>(wp[j] + at + 2 * kMxStepBytes);
-        sw[u][j] = *reinterpret_cast<const int*>(ws[j] + at);
-      }
-    }
-    if constexpr (RAW) {
-      // lane 16 u + 8 row + block
-      const int u = lane >> 4, row = (lane >> 3) & 1, b = lane & 7, kk = k0 + W * u;
-      if (u < U && row < rows.count && kk < kc) {
-        mx_u32x6 hi = (mx_u32x6)(0u), lo = (mx_u32x6)(0u);
-        int e = 4;
-        const int col = kMxChunk * kk + 32 * b;
-        if (col < k) {
-          float v[32];
-          const int r = rows.first + row;
-          const long long at = (raw.src ? raw.src[r] : r) * raw.ldx + col;
-          const uint32_t amax = raw.type == kF32   ? mx_load_block<kF32>(raw.x, at, raw.wide, v)
-                                : raw.type == kF16 ? mx_load_block<kF16>(raw.x, at, raw.wide, v)
-                                                   : mx_load_block<kBF16>(raw.x, at, raw.wide, v);
-          e = mx_x_byte(amax);
-          mx_digits(v, e, hi, lo);
-        }
-        uint8_t* d = mine + 64 * lane;
-        *reinterpret_cast<mx_u32x4*>(d) = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
-        *reinterpret_cast<mx_u32x4*>(d + 16) = mx_u32x4{hi[4], hi[5], lo[0], lo[1]};
-        *reinterpret_cast<mx_u32x4*>(d + 32) = mx_u32x4{lo[2], lo[3], lo[4], lo[5]};
-        *reinterpret_cast<int*>(d + 48) = e;
-      }
-      __builtin_amdgcn_wave_barrier();
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int kk = k0 + W * u;
-      if (kk >= kc) break;
-      mx_u32x12 x[2];
-      int sx[2];
-      if constexpr (RAW) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint8_t* d = mine + 64 * (16 * u + 8 * xc + 4 * s + g);
-          x[s] = mx_x(*reinterpret_cast<const mx_u32x4*>(d), *reinterpret_cast<const mx_u32x4*>(d + 16),
-                      *reinterpret_cast<const mx_u32x4*>(d + 32));
-          sx[s] = *reinterpret_cast<const int*>(d + 48);
-        }
-      } else {
-        const uint8_t* p = xp + (long long)kk * kMxXUnit;
-        x[0] = mx_get_x(p);
-        x[1] = mx_get_x(p + 2 * kMxXStep);
-        const int b = *reinterpret_cast<const int*>(xs + (long long)kk * kMxXUnit) >> (8 * (g >> 1));
-        sx[0] = b & 255;
-        sx[1] = b >> 16 & 255;
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int b = sw[u][j] >> (8 * (g >> 1));  // block 2 s + h of steps s = g / 2 and 2 + g / 2
-        acc[j] = mx_mfma16<0>(w[u][j][0], mx_hi(x[0]), acc[j], b, sx[0]);
-        acc[j] = mx_mfma16<0>(w[u][j][0], mx_lo(x[0]), acc[j], b, sx[0] - 4);
-        acc[j] = mx_mfma16<0>(w[u][j][1], mx_hi(x[1]), acc[j], b >> 16, sx[1]);
-        acc[j] = mx_mfma16<0>(w[u][j][1], mx_lo(x[1]), acc[j], b >> 16, sx[1] - 4);
-      }
-    }
-    if constexpr (RAW) __builtin_amdgcn_wave_barrier();
-  }
-  if constexpr (RAW) __syncthreads();  // the sums take the blocks' place
-  float(*red)[16][kRowF] = reinterpret_cast<float(*)[16][kRowF]>(smem);
-#pragma unroll
-  for (int j = 0; j < NT; ++j) *reinterpret_cast<mx_f32x4*>(&red[wave][c][16 * j + 4 * g]) = acc[j];
-  __syncthreads();
+// The waves' sums of NT 16-column tiles, joined in wave order and written.
+template <int W, int NT, bool GLU>
+__device__ __forceinline__ void mx_gemv_join(const MxOut& o, const MxRows& rows, int n, int n0,
+                                             float (&red)[W][16][16 * NT + 4], int ldy) {
+  const int t = threadIdx.x;
   auto total = [&](int m, int q) {
     float v = red[0][m][q];
 #pragma unroll
@@ -305,6 +190,178 @@ __device__ __forceinline__ void mx_gemv(const MxOut& o, const uint8_t* __restric
   if (o.y_type == kF32) put(MxType<kF32>{});
   else if (o.y_type == kF16) put(MxType<kF16>{});
   else put(MxType<kBF16>{});
+}
+
+// Up to 16 rows: a workgroup of W waves takes every gridDim.x-th group of NT 16-column
+// tiles of the output and splits K over its waves by chunks (wave i: chunks i, i + W,
+// ..., U of them in flight); the waves' sums meet in LDS, in wave order. GLU: half of the
+// tiles are rows of o.w, half the same rows of `up`, and silu(first) * second of their 32
+// columns becomes one block of the digit planes o.y.
+// RAW: up to two rows, f32 (1) or 16 bits (2), quantized here (each wave its own chunks, a
+// block a lane) into LDS; else digit planes.
+//
+// What bounds it: the weights' stream. A wave loads a chunk of a tile (2 KB) in two
+// instructions, 16 waves a CU (128 registers a lane) ask for 32 KB at least at a time, and
+// the next group's weights are on their way while this one's sums are joined. Keeping a
+// wave's digits in registers from group to group took 156 registers and a second
+// workgroup's place: 37 us against 24 for the gate and up of 24 tokens with 6 of 64 experts
+// each, 2048 x 1408. One matrix instruction
+// takes 16 columns x 128 of K by up to 16 rows, so rows cost nothing until their digits'
+// reads show. Rows of x are read by every workgroup: quantized ahead into planes (1.5
+// bytes a value) above two rows, in place below, where a launch of its own costs more
+// than it takes (2.4 us and the gap).
+template <int W, int NT, int U, bool GLU, int RAW>
+__device__ __forceinline__ void mx_gemv(const MxOut& o, const uint8_t* __restrict__ up, const MxRows& rows, int n, int k,
+                                        const uint8_t* __restrict__ xq, const MxRaw& raw, int ldy) {
+  constexpr int NC = GLU ? NT / 2 : NT;  // 16-column tiles of the output
+  static_assert(!GLU || NT == 4, "a block of 32 columns");
+  constexpr int kRowF = 16 * NT + 4;     // floats of a row of sums, padded
+  __shared__ __attribute__((aligned(16))) float red[W][16][kRowF];
+  // RAW: [chunk][row][block] of 48 bytes of digits and a scale; a wave's chunks are its own
+  extern __shared__ __attribute__((aligned(16))) uint8_t blocks[];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int c = lane & 15, g = lane >> 4, h = g & 1;
+  const int kc = (k + kMxChunk - 1) / kMxChunk;
+  const int groups = (n + 16 * NC - 1) / (16 * NC);
+  const int xc = min(c, rows.count - 1);
+  const uint8_t *xp = nullptr, *xs = nullptr;
+  if constexpr (!RAW) {
+    xp = xq + mx_x_at(rows.first + xc, h, kc) + (g >> 1) * kMxXStep;
+    xs = xq + mx_xs_at(rows.first + xc, h, kc);
+  }
+  mx_u32x4 w[U][NT][2];
+  int sw[U][NT];
+  auto load_w = [&](int grp, int k0) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const long long r = rows.w0 + min(16 * (NC * grp + j % NC) + c, n - 1);
+      const uint8_t* b = j < NC ? o.w : up;
+      const uint8_t* wp = b + mx_w_at(r, h, kc) + (g >> 1) * kMxStepBytes;
+      const uint8_t* ws = b + mx_ws_at(r, h, kc);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long at = (long long)min(k0 + W * u, kc - 1) * kMxUnit;
+        w[u][j][0] = *reinterpret_cast<const mx_u32x4*>(wp + at);
+        w[u][j][1] = *reinterpret_cast<const mx_u32x4*>(wp + at + 2 * kMxStepBytes);
+        sw[u][j] = *reinterpret_cast<const int*>(ws + at);
+      }
+    }
+  };
+  int grp = blockIdx.x;
+  if constexpr (RAW) {
+    // Lane 16 u + 8 row + block of four chunks. The first chunks' values are asked for
+    // before the weights: loads return in order, and the weights come from afar.
+    const int row = (lane >> 3) & 1, blk = lane & 7;
+    const int r = rows.first + min(row, rows.count - 1);
+    const long long src = (raw.src ? raw.src[r] : r) * raw.ldx;
+    mx_u32x4 v[RAW == 1 ? 8 : 4];
+    auto load = [&](int k0) {
+      const int col = min(kMxChunk * (k0 + W * (lane >> 4)) + 32 * blk, k - 32);
+      if (raw.wide) {
+        const uint8_t* p = static_cast<const uint8_t*>(raw.x) + (src + col) * (RAW == 1 ? 4 : 2);
+#pragma unroll
+        for (int i = 0; i < (RAW == 1 ? 8 : 4); ++i) v[i] = reinterpret_cast<const mx_u32x4*>(p)[i];
+      } else if constexpr (RAW == 1) {
+        const uint32_t* p = static_cast<const uint32_t*>(raw.x) + src + col;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i / 4][i % 4] = p[i];
+      } else {
+        const uint16_t* p = static_cast<const uint16_t*>(raw.x) + src + col;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i / 4][i % 4] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+      }
+    };
+    load(wave);
+    load_w(grp, wave);
+    for (int k0 = wave; k0 < kc; k0 += 4 * W) {
+      if (k0 != wave) load(k0);
+      const int kk = k0 + W * (lane >> 4);
+      if (row < rows.count && kk < kc) {
+        float f[32];
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if constexpr (RAW == 1) {
+            const uint32_t u = v[i / 4][i % 4];
+            f[i] = __builtin_bit_cast(float, u);
+          } else {
+            const uint16_t u = (uint16_t)(v[i / 8][i % 8 / 2] >> (16 * (i & 1)));
+            f[i] = raw.type == kF16 ? (float)__builtin_bit_cast(_Float16, u) : bf16_to_f32(u);
+          }
+          amax = max(amax, __builtin_bit_cast(uint32_t, f[i]) & 0x7fffffffu);
+        }
+        const bool in = kMxChunk * kk + 32 * blk < k;  // (the last chunk's blocks past k are zero)
+        if (!in) {
+          amax = 0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+        }
+        mx_u32x6 hi, lo;
+        const int e = mx_x_byte(amax);
+        mx_digits(f, e, hi, lo);
+        uint8_t* d = blocks + 64 * (16 * kk + 8 * row + blk);
+        *reinterpret_cast<mx_u32x4*>(d) = mx_u32x4{hi[0], hi[1], hi[2], hi[3]};
+        *reinterpret_cast<mx_u32x4*>(d + 16) = mx_u32x4{hi[4], hi[5], lo[0], lo[1]};
+        *reinterpret_cast<mx_u32x4*>(d + 32) = mx_u32x4{lo[2], lo[3], lo[4], lo[5]};
+        *reinterpret_cast<int*>(d + 48) = e;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    load_w(grp, wave);
+  }
+  auto get_x = [&](int kk, mx_u32x12 (&x)[2], int (&sx)[2]) {
+    if constexpr (RAW) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint8_t* d = blocks + 64 * (16 * kk + 8 * xc + 4 * s + g);
+        x[s] = mx_x(*reinterpret_cast<const mx_u32x4*>(d), *reinterpret_cast<const mx_u32x4*>(d + 16),
+                    *reinterpret_cast<const mx_u32x4*>(d + 32));
+        sx[s] = *reinterpret_cast<const int*>(d + 48);
+      }
+    } else {
+      const uint8_t* p = xp + (long long)kk * kMxXUnit;
+      x[0] = mx_get_x(p);
+      x[1] = mx_get_x(p + 2 * kMxXStep);
+      const int b = *reinterpret_cast<const int*>(xs + (long long)kk * kMxXUnit) >> (8 * (g >> 1));
+      sx[0] = b & 255;
+      sx[1] = b >> 16 & 255;
+    }
+  };
+#pragma unroll 1
+  for (; grp < groups; grp += gridDim.x) {
+    mx_f32x4 acc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = (mx_f32x4)(0.0f);
+#pragma unroll 1
+    for (int k0 = wave; k0 < kc; k0 += W * U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int kk = k0 + W * u;
+        if (kk < kc) {
+          mx_u32x12 x[2];
+          int sx[2];
+          get_x(kk, x, sx);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const int b = sw[u][j] >> (8 * (g >> 1));  // block 2 s + h of steps s = g / 2 and 2 + g / 2
+            acc[j] = mx_mfma16<0>(w[u][j][0], mx_hi(x[0]), acc[j], b, sx[0]);
+            acc[j] = mx_mfma16<0>(w[u][j][0], mx_lo(x[0]), acc[j], b, sx[0] - 4);
+            acc[j] = mx_mfma16<0>(w[u][j][1], mx_hi(x[1]), acc[j], b >> 16, sx[1]);
+            acc[j] = mx_mfma16<0>(w[u][j][1], mx_lo(x[1]), acc[j], b >> 16, sx[1] - 4);
+          }
+        }
+      }
+      // the next chunks of this group or the next group's first
+      const bool more = k0 + W * U < kc;
+      if (more || grp + (int)gridDim.x < groups) load_w(more ? grp : grp + (int)gridDim.x, more ? k0 + W * U : wave);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *reinterpret_cast<mx_f32x4*>(&red[wave][c][16 * j + 4 * g]) = acc[j];
+    __syncthreads();
+    mx_gemv_join<W, NT, GLU>(o, rows, n, 16 * NC * grp, red, ldy);
+    __syncthreads();
+  }
 }
 
 // A tile of 32 FM WM rows x 32 FN WN columns by WM x WN waves, a wave FM x FN fragments;
@@ -552,50 +609,46 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const uint8_t* __restric
 }
 }  // namespace qmm
 
-// Up to 16 rows. Dense: grid (16 NT-column tiles). Routed: grid (column tiles, row tiles).
-#define QMM_MX_GEMV(W, NT, NAME, RAW)                                                                          \
-  extern "C" __global__ void __launch_bounds__(64 * W) qmm_mx_gemv##NAME##_w##W##_t##NT(                       \
+// Up to 16 rows. Grid: workgroups that share the columns (and, routed, row tiles).
+#define QMM_MX_GEMV(W, U, NAME, RAW)                                                                           \
+  extern "C" __global__ void __launch_bounds__(64 * W, 4) qmm_mx_gemv##NAME##_w##W##_u##U(                     \
       qmm::MxOut o, int m, int n, int k, const uint8_t* __restrict__ xq, qmm::MxRaw raw, int ldy) {            \
     const qmm::MxRows r = {0, 0, m};                                                                           \
-    qmm::mx_gemv<W, NT, false, RAW>(o, nullptr, r, n, k, 16 * NT * blockIdx.x, xq, raw, ldy);                  \
+    qmm::mx_gemv<W, 1, U, false, RAW>(o, nullptr, r, n, k, xq, raw, ldy);                                      \
   }
-#define QMM_MX_GEMVS(W)         \
-  QMM_MX_GEMV(W, 1, , false)    \
-  QMM_MX_GEMV(W, 2, , false)    \
-  QMM_MX_GEMV(W, 1, _raw, true) \
-  QMM_MX_GEMV(W, 2, _raw, true)
-QMM_MX_GEMVS(4)
-QMM_MX_GEMVS(8)
-QMM_MX_GEMVS(16)
-
-#define QMM_MX_EXPERT_GEMV(W)                                                                                  \
-  extern "C" __global__ void __launch_bounds__(64 * W) qmm_mx_expert_gemv_w##W(                                \
+#define QMM_MX_EXPERT_GEMV(W, U)                                                                               \
+  extern "C" __global__ void __launch_bounds__(64 * W, 4) qmm_mx_expert_gemv_w##W##_u##U(                      \
       qmm::MxOut o0, qmm::MxOut o1, int experts, int pairs, int n, int k, const int* __restrict__ counts,      \
       const int* __restrict__ offsets, const uint8_t* __restrict__ xq, int ldy) {                              \
     qmm::MxRows r;                                                                                             \
     if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 16, blockIdx.y, r)) return;                   \
-    qmm::mx_gemv<W, 1, false, false>(blockIdx.z ? o1 : o0, nullptr, r, n, k, 16 * blockIdx.x, xq, qmm::MxRaw{}, ldy);  \
+    qmm::mx_gemv<W, 1, U, false, 0>(blockIdx.z ? o1 : o0, nullptr, r, n, k, xq, qmm::MxRaw{}, ldy);            \
   }
-QMM_MX_EXPERT_GEMV(4)
-QMM_MX_EXPERT_GEMV(8)
-QMM_MX_EXPERT_GEMV(16)
-
 // Gate and up with the activation: dense rows (experts 0) or routed ones.
 #define QMM_MX_GLU_GEMV(W, NAME, RAW)                                                                          \
-  extern "C" __global__ void __launch_bounds__(64 * W) qmm_mx_glu_gemv##NAME##_w##W(                           \
+  extern "C" __global__ void __launch_bounds__(64 * W, 4) qmm_mx_glu_gemv##NAME##_w##W(                        \
       qmm::MxOut o, const uint8_t* __restrict__ up, int experts, int pairs, int n, int k,                      \
       const int* __restrict__ counts, const int* __restrict__ offsets, const uint8_t* __restrict__ xq,         \
       qmm::MxRaw raw) {                                                                                        \
     qmm::MxRows r = {0, 0, pairs};                                                                             \
     if (experts > 0 && !qmm::mx_expert_tile(counts, offsets, experts, pairs, n, RAW ? 2 : 16, blockIdx.y, r)) return;  \
-    qmm::mx_gemv<W, 4, true, RAW>(o, up, r, n, k, 32 * blockIdx.x, xq, raw, 0);                                \
+    qmm::mx_gemv<W, 4, 1, true, RAW>(o, up, r, n, k, xq, raw, 0);                                              \
   }
-#define QMM_MX_GLU_GEMVS(W)        \
-  QMM_MX_GLU_GEMV(W, , false)      \
-  QMM_MX_GLU_GEMV(W, _raw, true)
-QMM_MX_GLU_GEMVS(4)
-QMM_MX_GLU_GEMVS(8)
-QMM_MX_GLU_GEMVS(16)
+#define QMM_MX_GEMVS(W, U)        \
+  QMM_MX_GEMV(W, U, , 0)          \
+  QMM_MX_GEMV(W, U, _raw32, 1)    \
+  QMM_MX_GEMV(W, U, _raw16, 2)    \
+  QMM_MX_EXPERT_GEMV(W, U)
+#define QMM_MX_GEMVS_W(W)         \
+  QMM_MX_GEMVS(W, 1)              \
+  QMM_MX_GEMVS(W, 2)              \
+  QMM_MX_GEMVS(W, 4)              \
+  QMM_MX_GLU_GEMV(W, , 0)         \
+  QMM_MX_GLU_GEMV(W, _raw32, 1)   \
+  QMM_MX_GLU_GEMV(W, _raw16, 2)
+QMM_MX_GEMVS_W(4)
+QMM_MX_GEMVS_W(8)
+QMM_MX_GEMVS_W(16)
 
 #define QMM_MX_GEMM(NAME, FM, FN, WM, WN, WK, EU)                                                              \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK, EU) qmm_mx_gemm_##NAME(                      \

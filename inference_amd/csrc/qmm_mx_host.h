@@ -137,11 +137,35 @@ struct MxRaw {
 // the second of which finds the weights in cache).
 constexpr int64_t kMxGemvRows = 16, kMxRawRows = 2, kMxExpertGemvRows = 32;
 
-// Waves that split K: a chunk of 256 columns each at least.
-int mx_gemv_waves(int64_t k) {
-  const int64_t kc = mx_chunks(k);
-  return kc >= 16 ? 16 : kc >= 8 ? 8 : 4;
+// The narrow kernels' launch: `groups` column groups of each of `row_tiles`. Four waves
+// split K where that fills the chip with 16 waves a CU, else 8 or 16, at a chunk of 256
+// columns each at least; up to four chunks of a wave are in flight. Planes: a workgroup
+// a group. Raw rows, which every workgroup quantizes for itself: 16 waves a CU in all,
+// each workgroup as many groups as any other but one.
+struct MxGemv {
+  int waves, depth;
+  unsigned grid;
+};
+MxGemv mx_gemv_plan(const Device* d, int64_t k, int64_t groups, int64_t row_tiles, bool raw) {
+  const int64_t kc = mx_chunks(k), fill = (int64_t)d->num_cu * 16;
+  MxGemv p;
+  p.waves = 4;
+  while (p.waves < 16 && p.waves < kc && groups * row_tiles * p.waves < fill) p.waves *= 2;
+  const int64_t mine = (kc + p.waves - 1) / p.waves;
+  p.depth = mine > 2 ? 4 : (int)mine;
+  p.grid = (unsigned)groups;
+  if (raw) {
+    const int64_t want = std::max<int64_t>(fill / p.waves / row_tiles, 1), per = (groups + want - 1) / want;
+    p.grid = (unsigned)((groups + per - 1) / per);
+  }
+  return p;
 }
+const char* mx_raw_name(const MxRaw* raw) { return !raw ? "" : raw->type == QMM_F32 ? "_raw32" : "_raw16"; }
+
+// LDS of unquantized rows' digits, and the widest rows that take that way.
+unsigned mx_raw_lds(int64_t k) { return (unsigned)(mx_chunks(k) * 1024); }
+constexpr int64_t kMxRawCols = 16384;
+bool mx_raw_fits(int64_t m, int64_t k) { return m <= kMxRawRows && k <= kMxRawCols; }
 
 // y = x . W^T over m dense rows: of digit planes, or (up to two rows) of raw ones.
 int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, const MxRaw* raw, int64_t m, MxOut o, int64_t ldy,
@@ -153,11 +177,11 @@ int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, const MxR
   char name[40];
   if (m <= kMxGemvRows) {
     MxRaw r = raw ? *raw : MxRaw();
-    const int waves = mx_gemv_waves(k), nt = ceil_div(n, 16) > 2u * (unsigned)d->num_cu ? 2 : 1;
-    snprintf(name, sizeof(name), "qmm_mx_gemv%s_w%d_t%d", raw ? "_raw" : "", waves, nt);
+    const MxGemv p = mx_gemv_plan(d, k, ceil_div(n, 16), 1, raw);
+    snprintf(name, sizeof(name), "qmm_mx_gemv%s_w%d_u%d", mx_raw_name(raw), p.waves, p.depth);
     void* args[] = {&o, &mm, &n, &k, &planes, &r, &ld};
     QMM_TRY(kernel(d, name, &f));
-    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 16 * nt), 1, 1, 64 * waves, 1, 1, 0, s, args, nullptr));
+    QMM_HIP(hipModuleLaunchKernel(f, p.grid, 1, 1, 64 * p.waves, 1, 1, raw ? mx_raw_lds(k) : 0, s, args, nullptr));
     return QMM_OK;
   }
   int kc = (int)mx_chunks(k);
@@ -188,11 +212,11 @@ int mx_expert_product(Device* d, const qmm_qtensor* const* w, int count, int exp
   if (max_rows <= kMxExpertGemvRows) {
     const int64_t tiles = pairs / kMxGemvRows + active;
     if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
-    const int waves = mx_gemv_waves(k);
-    snprintf(name, sizeof(name), "qmm_mx_expert_gemv_w%d", waves);
+    const MxGemv p = mx_gemv_plan(d, k, ceil_div(n, 16), active * count, false);
+    snprintf(name, sizeof(name), "qmm_mx_expert_gemv_w%d_u%d", p.waves, p.depth);
     void* args[] = {&o[0], &o[1], &E, &P, &n, &k, &counts, &offsets, &planes, &ld};
     QMM_TRY(kernel(d, name, &f));
-    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 16), (unsigned)tiles, (unsigned)count, 64 * waves, 1, 1, 0, s, args, nullptr));
+    QMM_HIP(hipModuleLaunchKernel(f, p.grid, (unsigned)tiles, (unsigned)count, 64 * p.waves, 1, 1, 0, s, args, nullptr));
     return QMM_OK;
   }
   void* args[] = {&o[0], &o[1], &E, &P, &n, &kc, &counts, &offsets, &planes, &ld};
@@ -225,11 +249,12 @@ int mx_glu(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, int expert
   if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many rows");
   if (gemv) {
     MxRaw r = raw ? *raw : MxRaw();
-    const int waves = mx_gemv_waves(k);
-    snprintf(name, sizeof(name), "qmm_mx_glu_gemv%s_w%d", raw ? "_raw" : "", waves);
+    const MxGemv p = mx_gemv_plan(d, k, ceil_div(n, 32), std::max<int64_t>(active, 1), raw);
+    snprintf(name, sizeof(name), "qmm_mx_glu_gemv%s_w%d", mx_raw_name(raw), p.waves);
     void* args[] = {&o, &uw, &E, &P, &n, &k, &counts, &offsets, &planes, &r};
     QMM_TRY(kernel(d, name, &f));
-    QMM_HIP(hipModuleLaunchKernel(f, ceil_div(n, 32), (unsigned)tiles, 1, 64 * waves, 1, 1, 0, s, args, nullptr));
+    QMM_HIP(hipModuleLaunchKernel(f, p.grid, (unsigned)tiles, 1, 64 * p.waves, 1, 1, raw ? mx_raw_lds(k) : 0, s, args,
+                                  nullptr));
     return QMM_OK;
   }
   if (!experts) {

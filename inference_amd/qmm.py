@@ -426,7 +426,7 @@ class QMatMul:
             L = lib()
             h = qt.handle
             ws, ws_bytes, ws_ptr = None, 0, None
-            if m > 2:  # one and two rows are quantized in the GEMV's prologue
+            if m > 2 or k > 16384:  # one and two rows are quantized in the GEMV's prologue
                 ws_bytes = int(L.qmm_matmul_workspace_size(h, m))
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
                 ws_ptr = ws.data_ptr()
@@ -471,7 +471,7 @@ class QMatMul:
         if m != 0:
             L = lib()
             ws, ws_bytes, ws_ptr = None, 0, None
-            if m > 2:
+            if m > 2 or k > 16384:
                 ws_bytes = int(L.qmm_linear_workspace_size(qt.handle, m))
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
                 ws_ptr = ws.data_ptr()
