@@ -231,21 +231,45 @@ __device__ __forceinline__ void mx_gemv(const MxOut& o, const uint8_t* __restric
   }
   mx_u32x4 w[U][NT][2];
   int sw[U][NT];
-  auto load_w = [&](int grp, int k0) {
+  // x of chunk kk into slot u: planes are asked for together with the weights (loads return
+  // in order), except by GLU, whose weights leave no registers for them
+  constexpr bool kAhead = !RAW && !GLU;
+  mx_u32x12 x[kAhead ? U : 1][2];
+  int sx[kAhead ? U : 1][2];
+  auto load_x = [&](int u, int kk) {
+    if constexpr (RAW) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint8_t* d = blocks + 64 * (16 * kk + 8 * xc + 4 * q + g);
+        x[u][q] = mx_x(*reinterpret_cast<const mx_u32x4*>(d), *reinterpret_cast<const mx_u32x4*>(d + 16),
+                       *reinterpret_cast<const mx_u32x4*>(d + 32));
+        sx[u][q] = *reinterpret_cast<const int*>(d + 48);
+      }
+    } else {
+      const uint8_t* p = xp + (long long)kk * kMxXUnit;
+      x[u][0] = mx_get_x(p);
+      x[u][1] = mx_get_x(p + 2 * kMxXStep);
+      sx[u][0] = *reinterpret_cast<const int*>(xs + (long long)kk * kMxXUnit) >> (8 * (g >> 1));
+      sx[u][1] = sx[u][0] >> 16;
+    }
+  };
+  auto load_one = [&](int grp, int kk, int u) {
+    if (kAhead && kk >= kc) return;
+    if constexpr (kAhead) load_x(u, kk);
+    else kk = min(kk, kc - 1);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const long long r = rows.w0 + min(16 * (NC * grp + j % NC) + c, n - 1);
       const uint8_t* b = j < NC ? o.w : up;
-      const uint8_t* wp = b + mx_w_at(r, h, kc) + (g >> 1) * kMxStepBytes;
-      const uint8_t* ws = b + mx_ws_at(r, h, kc);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const long long at = (long long)min(k0 + W * u, kc - 1) * kMxUnit;
-        w[u][j][0] = *reinterpret_cast<const mx_u32x4*>(wp + at);
-        w[u][j][1] = *reinterpret_cast<const mx_u32x4*>(wp + at + 2 * kMxStepBytes);
-        sw[u][j] = *reinterpret_cast<const int*>(ws + at);
-      }
+      const uint8_t* wp = b + mx_w_at(r, h, kc) + (g >> 1) * kMxStepBytes + (long long)kk * kMxUnit;
+      w[u][j][0] = *reinterpret_cast<const mx_u32x4*>(wp);
+      w[u][j][1] = *reinterpret_cast<const mx_u32x4*>(wp + 2 * kMxStepBytes);
+      sw[u][j] = *reinterpret_cast<const int*>(b + mx_ws_at(r, h, kc) + (long long)kk * kMxUnit);
     }
+  };
+  auto load_w = [&](int grp, int k0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_one(grp, k0 + W * u, u);
   };
   int grp = blockIdx.x;
   if constexpr (RAW) {
@@ -310,24 +334,6 @@ __device__ __forceinline__ void mx_gemv(const MxOut& o, const uint8_t* __restric
   } else {
     load_w(grp, wave);
   }
-  auto get_x = [&](int kk, mx_u32x12 (&x)[2], int (&sx)[2]) {
-    if constexpr (RAW) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const uint8_t* d = blocks + 64 * (16 * kk + 8 * xc + 4 * s + g);
-        x[s] = mx_x(*reinterpret_cast<const mx_u32x4*>(d), *reinterpret_cast<const mx_u32x4*>(d + 16),
-                    *reinterpret_cast<const mx_u32x4*>(d + 32));
-        sx[s] = *reinterpret_cast<const int*>(d + 48);
-      }
-    } else {
-      const uint8_t* p = xp + (long long)kk * kMxXUnit;
-      x[0] = mx_get_x(p);
-      x[1] = mx_get_x(p + 2 * kMxXStep);
-      const int b = *reinterpret_cast<const int*>(xs + (long long)kk * kMxXUnit) >> (8 * (g >> 1));
-      sx[0] = b & 255;
-      sx[1] = b >> 16 & 255;
-    }
-  };
 #pragma unroll 1
   for (; grp < groups; grp += gridDim.x) {
     mx_f32x4 acc[NT];
@@ -335,26 +341,27 @@ __device__ __forceinline__ void mx_gemv(const MxOut& o, const uint8_t* __restric
     for (int j = 0; j < NT; ++j) acc[j] = (mx_f32x4)(0.0f);
 #pragma unroll 1
     for (int k0 = wave; k0 < kc; k0 += W * U) {
+      // the next chunks of this group or the next group's first
+      const bool more = k0 + W * U < kc;
+      const bool any = more || grp + (int)gridDim.x < groups;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int kk = k0 + W * u;
         if (kk < kc) {
-          mx_u32x12 x[2];
-          int sx[2];
-          get_x(kk, x, sx);
+          constexpr int X = kAhead ? 1 : 0;
+          if constexpr (!kAhead) load_x(0, kk);
+          const int s0 = sx[X * u][0] & 255, s1 = sx[X * u][1] & 255;
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             const int b = sw[u][j] >> (8 * (g >> 1));  // block 2 s + h of steps s = g / 2 and 2 + g / 2
-            acc[j] = mx_mfma16<0>(w[u][j][0], mx_hi(x[0]), acc[j], b, sx[0]);
-            acc[j] = mx_mfma16<0>(w[u][j][0], mx_lo(x[0]), acc[j], b, sx[0] - 4);
-            acc[j] = mx_mfma16<0>(w[u][j][1], mx_hi(x[1]), acc[j], b >> 16, sx[1]);
-            acc[j] = mx_mfma16<0>(w[u][j][1], mx_lo(x[1]), acc[j], b >> 16, sx[1] - 4);
+            acc[j] = mx_mfma16<0>(w[u][j][0], mx_hi(x[X * u][0]), acc[j], b, s0);
+            acc[j] = mx_mfma16<0>(w[u][j][0], mx_lo(x[X * u][0]), acc[j], b, s0 - 4);
+            acc[j] = mx_mfma16<0>(w[u][j][1], mx_hi(x[X * u][1]), acc[j], b >> 16, s1);
+            acc[j] = mx_mfma16<0>(w[u][j][1], mx_lo(x[X * u][1]), acc[j], b >> 16, s1 - 4);
           }
         }
+        if (any) load_one(more ? grp : grp + (int)gridDim.x, (more ? k0 + W * U : wave) + W * u, u);
       }
-      // the next chunks of this group or the next group's first
-      const bool more = k0 + W * U < kc;
-      if (more || grp + (int)gridDim.x < groups) load_w(more ? grp : grp + (int)gridDim.x, more ? k0 + W * U : wave);
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) *reinterpret_cast<mx_f32x4*>(&red[wave][c][16 * j + 4 * g]) = acc[j];
@@ -642,7 +649,6 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const uint8_t* __restric
 #define QMM_MX_GEMVS_W(W)         \
   QMM_MX_GEMVS(W, 1)              \
   QMM_MX_GEMVS(W, 2)              \
-  QMM_MX_GEMVS(W, 4)              \
   QMM_MX_GLU_GEMV(W, , 0)         \
   QMM_MX_GLU_GEMV(W, _raw32, 1)   \
   QMM_MX_GLU_GEMV(W, _raw16, 2)
