@@ -1829,7 +1829,7 @@ static int mx_ffn(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, con
   const MxRaw raw = {x, ldx, nullptr, x_dtype, mx_wide16(x, x_dtype, ldx)};
   const bool direct = mx_raw_fits(m, gate->k);
   if (!direct) QMM_TRY(mx_quantize_x(d, x, x_dtype, m, gate->k, ldx, nullptr, b + L.xp, s));
-  QMM_TRY(mx_glu(d, gate, up, 0, b + L.xp, direct ? &raw : nullptr, m, m, nullptr, nullptr, b + L.hp, s));
+  QMM_TRY(mx_glu(d, gate, up, 0, b + L.xp, direct ? &raw : nullptr, m, nullptr, nullptr, b + L.hp, s));
   MxOut o = {};
   o.y = y;
   o.accumulate = accumulate;
@@ -2704,7 +2704,7 @@ int qmm_moe_gemm(const qmm_qtensor* const* w, int count, int experts, const floa
   if (is_mx(w0->dtype)) {
     QMM_TRY(mx_check_rows(pairs, w0->k));
     QMM_TRY(mx_quantize_x(d, x, QMM_F32, pairs, w0->k, ldx, nullptr, b, s));
-    return mx_expert_product(d, w, count, experts, b, pairs, max_rows, counts, offsets, y, s);
+    return mx_expert_product(d, w, count, experts, b, pairs, counts, offsets, y, s);
   }
   QMM_TRY(quantize_planes(d, w0->dtype, x, pairs, w0->k, ldx, b, s));
   return moe_gemm_planes(d, w, count, experts, b, pairs, max_rows, counts, offsets, y, s);
@@ -3072,8 +3072,8 @@ static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const
     const MxRaw raw = {xc, ldx, ptok, x_dtype, mx_wide16(xc, x_dtype, ldx)};
     const bool direct = mx_raw_fits(tokens, H);
     if (!direct) QMM_TRY(mx_quantize_x(d, xc, x_dtype, P, H, ldx, ptok, b + L.xp, s));
-    QMM_TRY(mx_glu(d, gate, up, experts, b + L.xp, direct ? &raw : nullptr, P, T, counts, offsets, b + L.hp, s));
-    QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, T, counts, offsets, &yp, s));
+    QMM_TRY(mx_glu(d, gate, up, experts, b + L.xp, direct ? &raw : nullptr, P, counts, offsets, b + L.hp, s));
+    QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, counts, offsets, &yp, s));
     float *shared = nullptr, *sg = nullptr;
     if (sh.gate) {
       shared = (float*)(b + L.shared);

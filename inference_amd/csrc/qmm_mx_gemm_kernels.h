@@ -192,7 +192,7 @@ __device__ __forceinline__ void mx_gemv_join(const MxOut& o, const MxRows& rows,
   else put(MxType<kBF16>{});
 }
 
-// Up to 16 rows: a workgroup of W waves takes every gridDim.x-th group of NT 16-column
+// Tiles of up to 16 rows: a workgroup of W waves takes every gridDim.x-th group of NT 16-column
 // tiles of the output and splits K over its waves by chunks (wave i: chunks i, i + W,
 // ..., U of them in flight); the waves' sums meet in LDS, in wave order. GLU: half of the
 // tiles are rows of o.w, half the same rows of `up`, and silu(first) * second of their 32
@@ -232,8 +232,8 @@ __device__ __forceinline__ void mx_gemv(const MxOut& o, const uint8_t* __restric
   mx_u32x4 w[U][NT][2];
   int sw[U][NT];
   // x of chunk kk into slot u: planes are asked for together with the weights (loads return
-  // in order), except by GLU, whose weights leave no registers for them
-  constexpr bool kAhead = !RAW && !GLU;
+  // in order), except with four tiles, whose weights leave no registers for them
+  constexpr bool kAhead = !RAW && NT == 1;
   mx_u32x12 x[kAhead ? U : 1][2];
   int sx[kAhead ? U : 1][2];
   auto load_x = [&](int u, int kk) {
@@ -616,20 +616,20 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const uint8_t* __restric
 }
 }  // namespace qmm
 
-// Up to 16 rows. Grid: workgroups that share the columns (and, routed, row tiles).
-#define QMM_MX_GEMV(W, U, NAME, RAW)                                                                           \
-  extern "C" __global__ void __launch_bounds__(64 * W, 4) qmm_mx_gemv##NAME##_w##W##_u##U(                     \
+// Grid: workgroups that share the columns, row tiles.
+#define QMM_MX_GEMV(W, NT, U, NAME, RAW)                                                                       \
+  extern "C" __global__ void __launch_bounds__(64 * W, 4) qmm_mx_gemv##NAME##_w##W##_n##NT##_u##U(             \
       qmm::MxOut o, int m, int n, int k, const uint8_t* __restrict__ xq, qmm::MxRaw raw, int ldy) {            \
-    const qmm::MxRows r = {0, 0, m};                                                                           \
-    qmm::mx_gemv<W, 1, U, false, RAW>(o, nullptr, r, n, k, xq, raw, ldy);                                      \
+    const qmm::MxRows r = {0, 16 * (int)blockIdx.y, min(16, m - 16 * (int)blockIdx.y)};                        \
+    qmm::mx_gemv<W, NT, U, false, RAW>(o, nullptr, r, n, k, xq, raw, ldy);                                     \
   }
-#define QMM_MX_EXPERT_GEMV(W, U)                                                                               \
-  extern "C" __global__ void __launch_bounds__(64 * W, 4) qmm_mx_expert_gemv_w##W##_u##U(                      \
+#define QMM_MX_EXPERT_GEMV(W, NT, U)                                                                           \
+  extern "C" __global__ void __launch_bounds__(64 * W, 4) qmm_mx_expert_gemv_w##W##_n##NT##_u##U(              \
       qmm::MxOut o0, qmm::MxOut o1, int experts, int pairs, int n, int k, const int* __restrict__ counts,      \
       const int* __restrict__ offsets, const uint8_t* __restrict__ xq, int ldy) {                              \
     qmm::MxRows r;                                                                                             \
     if (!qmm::mx_expert_tile(counts, offsets, experts, pairs, n, 16, blockIdx.y, r)) return;                   \
-    qmm::mx_gemv<W, 1, U, false, 0>(blockIdx.z ? o1 : o0, nullptr, r, n, k, xq, qmm::MxRaw{}, ldy);            \
+    qmm::mx_gemv<W, NT, U, false, 0>(blockIdx.z ? o1 : o0, nullptr, r, n, k, xq, qmm::MxRaw{}, ldy);           \
   }
 // Gate and up with the activation: dense rows (experts 0) or routed ones.
 #define QMM_MX_GLU_GEMV(W, NAME, RAW)                                                                          \
@@ -637,20 +637,23 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const uint8_t* __restric
       qmm::MxOut o, const uint8_t* __restrict__ up, int experts, int pairs, int n, int k,                      \
       const int* __restrict__ counts, const int* __restrict__ offsets, const uint8_t* __restrict__ xq,         \
       qmm::MxRaw raw) {                                                                                        \
-    qmm::MxRows r = {0, 0, pairs};                                                                             \
+    qmm::MxRows r = {0, 16 * (int)blockIdx.y, min(16, pairs - 16 * (int)blockIdx.y)};                          \
     if (experts > 0 && !qmm::mx_expert_tile(counts, offsets, experts, pairs, n, RAW ? 2 : 16, blockIdx.y, r)) return;  \
     qmm::mx_gemv<W, 4, 1, true, RAW>(o, up, r, n, k, xq, raw, 0);                                              \
   }
-#define QMM_MX_GEMVS(W, U)        \
-  QMM_MX_GEMV(W, U, , 0)          \
-  QMM_MX_GEMV(W, U, _raw32, 1)    \
-  QMM_MX_GEMV(W, U, _raw16, 2)    \
-  QMM_MX_EXPERT_GEMV(W, U)
-#define QMM_MX_GEMVS_W(W)         \
-  QMM_MX_GEMVS(W, 1)              \
-  QMM_MX_GEMVS(W, 2)              \
-  QMM_MX_GLU_GEMV(W, , 0)         \
-  QMM_MX_GLU_GEMV(W, _raw32, 1)   \
+#define QMM_MX_GEMVS_W(W)            \
+  QMM_MX_GEMV(W, 1, 1, , 0)          \
+  QMM_MX_GEMV(W, 1, 2, , 0)          \
+  QMM_MX_GEMV(W, 4, 1, , 0)          \
+  QMM_MX_GEMV(W, 1, 1, _raw32, 1)    \
+  QMM_MX_GEMV(W, 1, 2, _raw32, 1)    \
+  QMM_MX_GEMV(W, 1, 1, _raw16, 2)    \
+  QMM_MX_GEMV(W, 1, 2, _raw16, 2)    \
+  QMM_MX_EXPERT_GEMV(W, 1, 1)        \
+  QMM_MX_EXPERT_GEMV(W, 1, 2)        \
+  QMM_MX_EXPERT_GEMV(W, 4, 1)        \
+  QMM_MX_GLU_GEMV(W, , 0)            \
+  QMM_MX_GLU_GEMV(W, _raw32, 1)      \
   QMM_MX_GLU_GEMV(W, _raw16, 2)
 QMM_MX_GEMVS_W(4)
 QMM_MX_GEMVS_W(8)

@@ -133,34 +133,51 @@ struct MxRaw {
   int type, wide;
 };
 
-// Rows of the narrow kernels: of a tile, of unquantized rows, of an expert (two tiles,
-// the second of which finds the weights in cache).
-constexpr int64_t kMxGemvRows = 16, kMxRawRows = 2, kMxExpertGemvRows = 32;
+// Rows of the narrow kernels: of a tile, of unquantized rows.
+constexpr int64_t kMxGemvRows = 16, kMxRawRows = 2;
 
-// The narrow kernels' launch: `groups` column groups of each of `row_tiles`. Four waves
-// split K where that fills the chip with 16 waves a CU, else 8 or 16, at a chunk of 256
-// columns each at least; a wave has two chunks in flight where it has two. A workgroup a
-// group, or, `share`: 16 waves a CU in all, each workgroup as many groups as any other but
-// one. Raw rows share, since each workgroup quantizes them for itself; so do experts'
-// products (57 experts of 2048 x 1408: 19.5 us against 22.5), but not those of dense planes
-// (16 rows x 14336 x 4096: 16.1 us against 15.0) nor gate and up (26.6 us against 25.7).
+// Dense rows that the narrow kernels take: one tile, or tiles of rows by 64 columns that
+// are two a CU at most (128 rows x 4096 x 4096: 13.6 us against 17.8 by the wide ones, 32 x
+// 4096 x 14336 22.4 against 40.1, 32 x 14336 x 4096 17.6 against 19.1; at 3.5 a CU, 64 x
+// 14336 x 4096, 22.8 against 21.6).
+bool mx_gemv_rows(const Device* d, int64_t m, int64_t n) {
+  return m <= kMxGemvRows || ceil_div(m, kMxGemvRows) * (int64_t)ceil_div(n, 64) <= 2 * (int64_t)d->num_cu;
+}
+// Routed rows: one tile an expert or less (gate and up, and down: 512 rows over 64 experts
+// of 2048 x 1408 43 and 23 us against 54 and 37, 1024 rows 48 and 30 against 56 and 38;
+// 128 rows over 8 experts of 4096 x 14336 125 and 60 against 123 and 50).
+bool mx_gemv_experts(int64_t pairs, int64_t active) { return pairs <= kMxGemvRows * active; }
+
+// The narrow kernels' launch over `row_tiles` tiles of rows: a workgroup takes a group of
+// `tiles` 16-column tiles (raw rows, which every workgroup quantizes for itself: as many
+// groups as any other but one, 16 waves a CU in all). Four waves split K where that fills
+// the chip with 16 waves a CU, else 8 or 16, at a chunk of 256 columns each at least; a
+// wave has two chunks in flight (of one tile) where it has two.
 struct MxGemv {
-  int waves, depth;
+  int waves, tiles, depth;
   unsigned grid;
 };
-MxGemv mx_gemv_plan(const Device* d, int64_t k, int64_t groups, int64_t row_tiles, bool share) {
-  const int64_t kc = mx_chunks(k), fill = (int64_t)d->num_cu * 16;
+MxGemv mx_gemv_plan(const Device* d, int64_t n, int64_t k, int64_t row_tiles, int tiles, bool raw) {
+  const int64_t kc = mx_chunks(k), fill = (int64_t)d->num_cu * 16, groups = ceil_div(n, 16 * tiles);
   MxGemv p;
+  p.tiles = tiles;
   p.waves = 4;
   while (p.waves < 16 && p.waves < kc && groups * row_tiles * p.waves < fill) p.waves *= 2;
-  const int64_t mine = (kc + p.waves - 1) / p.waves;
-  p.depth = mine > 1 ? 2 : 1;
+  p.depth = tiles == 1 && kc > p.waves ? 2 : 1;
   p.grid = (unsigned)groups;
-  if (share) {
+  if (raw) {
     const int64_t want = std::max<int64_t>(fill / p.waves / row_tiles, 1), per = (groups + want - 1) / want;
     p.grid = (unsigned)((groups + per - 1) / per);
   }
   return p;
+}
+// Planes: four tiles a group, since every group reads the rows' digits (16 rows x 65536 x
+// 4096: 32.3 us against 44.3; 24 tokens' down products over 64 experts of 2048 x 1408 18.5
+// against 25.3), unless that leaves half of the chip idle with 16 waves a group (16 x 4096 x
+// 4096: 10.3 us against 9.5).
+MxGemv mx_planes_plan(const Device* d, int64_t n, int64_t k, int64_t row_tiles) {
+  const bool wide = ceil_div(n, 64) * row_tiles * 32 >= (int64_t)d->num_cu * 16;
+  return mx_gemv_plan(d, n, k, row_tiles, wide ? 4 : 1, false);
 }
 const char* mx_raw_name(const MxRaw* raw) { return !raw ? "" : raw->type == QMM_F32 ? "_raw32" : "_raw16"; }
 
@@ -177,13 +194,13 @@ int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, const MxR
   int mm = (int)m, n = (int)w->n, k = (int)w->k, ld = (int)ldy;
   hipFunction_t f;
   char name[40];
-  if (m <= kMxGemvRows) {
+  if (mx_gemv_rows(d, m, n)) {
     MxRaw r = raw ? *raw : MxRaw();
-    const MxGemv p = mx_gemv_plan(d, k, ceil_div(n, 16), 1, raw);
-    snprintf(name, sizeof(name), "qmm_mx_gemv%s_w%d_u%d", mx_raw_name(raw), p.waves, p.depth);
+    const MxGemv p = raw ? mx_gemv_plan(d, n, k, 1, 1, true) : mx_planes_plan(d, n, k, ceil_div(m, kMxGemvRows));
+    snprintf(name, sizeof(name), "qmm_mx_gemv%s_w%d_n%d_u%d", mx_raw_name(raw), p.waves, p.tiles, p.depth);
     void* args[] = {&o, &mm, &n, &k, &planes, &r, &ld};
     QMM_TRY(kernel(d, name, &f));
-    QMM_HIP(hipModuleLaunchKernel(f, p.grid, 1, 1, 64 * p.waves, 1, 1, raw ? mx_raw_lds(k) : 0, s, args, nullptr));
+    QMM_HIP(hipModuleLaunchKernel(f, p.grid, ceil_div(m, kMxGemvRows), 1, 64 * p.waves, 1, 1, raw ? mx_raw_lds(k) : 0, s, args, nullptr));
     return QMM_OK;
   }
   int kc = (int)mx_chunks(k);
@@ -196,9 +213,9 @@ int mx_product(Device* d, const qmm_qtensor* w, const uint8_t* planes, const MxR
 }
 
 // The same of expert-ordered rows: expert e's are rows offsets[e] + i of the planes and
-// of the output. One or two weights. max_rows bounds every count.
+// of the output. One or two weights.
 int mx_expert_product(Device* d, const qmm_qtensor* const* w, int count, int experts, const uint8_t* planes,
-                      int64_t pairs, int64_t max_rows, const int32_t* counts, const int32_t* offsets,
+                      int64_t pairs, const int32_t* counts, const int32_t* offsets,
                       float* const* y, hipStream_t s) {
   MxOut o[2] = {};
   for (int j = 0; j < 2; ++j) {
@@ -211,11 +228,11 @@ int mx_expert_product(Device* d, const qmm_qtensor* const* w, int count, int exp
   hipFunction_t f;
   const int64_t active = std::min<int64_t>(experts, pairs);
   char name[40];
-  if (max_rows <= kMxExpertGemvRows) {
+  if (mx_gemv_experts(pairs, active)) {
     const int64_t tiles = pairs / kMxGemvRows + active;
     if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many routed rows");
-    const MxGemv p = mx_gemv_plan(d, k, ceil_div(n, 16), active * count, true);
-    snprintf(name, sizeof(name), "qmm_mx_expert_gemv_w%d_u%d", p.waves, p.depth);
+    const MxGemv p = mx_planes_plan(d, n, k, active * count);
+    snprintf(name, sizeof(name), "qmm_mx_expert_gemv_w%d_n%d_u%d", p.waves, p.tiles, p.depth);
     void* args[] = {&o[0], &o[1], &E, &P, &n, &k, &counts, &offsets, &planes, &ld};
     QMM_TRY(kernel(d, name, &f));
     QMM_HIP(hipModuleLaunchKernel(f, p.grid, (unsigned)tiles, (unsigned)count, 64 * p.waves, 1, 1, 0, s, args, nullptr));
@@ -235,7 +252,7 @@ int mx_expert_product(Device* d, const qmm_qtensor* const* w, int count, int exp
 // silu(gate) * up of m rows as the digit planes of the down product's rows: dense rows
 // (experts 0) or routed ones, of planes or (up to kMxRawRows an expert) raw.
 int mx_glu(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, int experts, const uint8_t* planes,
-           const MxRaw* raw, int64_t m, int64_t max_rows, const int32_t* counts, const int32_t* offsets, uint8_t* out,
+           const MxRaw* raw, int64_t m, const int32_t* counts, const int32_t* offsets, uint8_t* out,
            hipStream_t s) {
   const int64_t F = gate->n / std::max(experts, 1), active = std::min<int64_t>(experts, m);
   MxOut o = {};
@@ -245,13 +262,13 @@ int mx_glu(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, int expert
   int E = experts, P = (int)m, n = (int)F, k = (int)gate->k, kc = (int)mx_chunks(k);
   hipFunction_t f;
   char name[40];
-  const bool gemv = max_rows <= (experts ? kMxExpertGemvRows : kMxGemvRows);
+  const bool gemv = experts ? mx_gemv_experts(m, active) : mx_gemv_rows(d, m, 2 * F);
   const int64_t bm = gemv ? (raw ? kMxRawRows : kMxGemvRows) : 128;
   const int64_t tiles = experts ? m / bm + active : ceil_div(m, bm);
   if (tiles > 65535) return fail(QMM_ERR_INVALID, "too many rows");
   if (gemv) {
     MxRaw r = raw ? *raw : MxRaw();
-    const MxGemv p = mx_gemv_plan(d, k, ceil_div(n, 32), std::max<int64_t>(active, 1), raw);
+    const MxGemv p = mx_gemv_plan(d, n, k, experts ? active : ceil_div(m, bm), 2, raw);
     snprintf(name, sizeof(name), "qmm_mx_glu_gemv%s_w%d", mx_raw_name(raw), p.waves);
     void* args[] = {&o, &uw, &E, &P, &n, &k, &counts, &offsets, &planes, &r};
     QMM_TRY(kernel(d, name, &f));

@@ -210,6 +210,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _call(dev: torch.device, fn, *args) -> int:
+    """fn(*args, the current stream of dev) with dev as the current device."""
+    if torch.cuda.current_device() == dev.index:
+        return fn(*args, _raw_stream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev.index))
+
+
 class GgmlDType(enum.IntEnum):
     """GGML block types of the quantized path (GGUF numbering)."""
 
@@ -475,13 +483,8 @@ class QMatMul:
                 ws_bytes = int(L.qmm_linear_workspace_size(qt.handle, m))
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
                 ws_ptr = ws.data_ptr()
-            args = (qt.handle, x2.data_ptr(), tag, m, max(x2.stride(0), k), bptr, btag, y.data_ptr(), tag, n, ws_ptr,
-                    ws_bytes, _raw_stream(dev.index))
-            if torch.cuda.current_device() == dev.index:
-                status = L.qmm_linear(*args)
-            else:
-                with torch.cuda.device(dev):
-                    status = L.qmm_linear(*args)
+            status = _call(dev, L.qmm_linear, qt.handle, x2.data_ptr(), tag, m, max(x2.stride(0), k), bptr, btag,
+                           y.data_ptr(), tag, n, ws_ptr, ws_bytes)
             if status != QMM_OK:
                 raise QmmError(status, last_error())
         return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
@@ -651,22 +654,26 @@ def moe_route(logits: torch.Tensor, topk: int, renormalize: bool = True, routed_
     if score is None and (bias is not None or groups != 1 or topk_groups is not None or group_top != 1):
         raise QmmError(QMM_ERR_INVALID, "a routing bias or groups need a score (softmax, sigmoid)")
     lg = logits.to(torch.float32).contiguous()
+    if score is not None:
+        L = lib()
+        tag, bias, groups, topk_groups, group_top = _scored(score, bias, groups, topk_groups, group_top, e, dev)
+        # A few tokens are 4 us of kernel: the host's part sets the pace, so the results are one allocation and
+        # there is no device context or Stream object (11.8 us a call; with those and one allocation each 16.4 us).
+        pairs = max(t * topk, 0)
+        counts, offsets, ptok, pw, tp = torch.empty(2 * e + 1 + 3 * pairs, dtype=torch.int32, device=dev).split(
+            (e, e + 1, pairs, pairs, pairs))
+        pw = pw.view(torch.float32)
+        nws = int(L.qmm_moe_route_scored_workspace_size(t, e, topk))
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+        _check(_call(dev, L.qmm_moe_route_scored, lg.data_ptr(), t, e, topk, tag, _ptr(bias), groups, topk_groups,
+                     group_top, int(renormalize), routed_scaling_factor, counts.data_ptr(), offsets.data_ptr(),
+                     ptok.data_ptr(), pw.data_ptr(), tp.data_ptr(), _ptr(ws), nws))
+        return counts, offsets, ptok, pw, tp
     counts = torch.empty(e, dtype=torch.int32, device=dev)
     offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
     ptok = torch.empty(t * topk, dtype=torch.int32, device=dev)
     pw = torch.empty(t * topk, dtype=torch.float32, device=dev)
     tp = torch.empty(t * topk, dtype=torch.int32, device=dev)
-    if score is not None:
-        L = lib()
-        tag, bias, groups, topk_groups, group_top = _scored(score, bias, groups, topk_groups, group_top, e, dev)
-        nws = int(L.qmm_moe_route_scored_workspace_size(t, e, topk))
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-        with torch.cuda.device(dev):
-            _check(L.qmm_moe_route_scored(lg.data_ptr(), t, e, topk, tag, _ptr(bias), groups, topk_groups, group_top,
-                                          int(renormalize), routed_scaling_factor, counts.data_ptr(),
-                                          offsets.data_ptr(), ptok.data_ptr(), pw.data_ptr(), tp.data_ptr(), _ptr(ws),
-                                          nws, _stream(dev)))
-        return counts, offsets, ptok, pw, tp
     with torch.cuda.device(dev):
         _check(lib().qmm_moe_route_ex(lg.data_ptr(), t, e, topk, int(renormalize), routed_scaling_factor,
                                       counts.data_ptr(), offsets.data_ptr(), ptok.data_ptr(), pw.data_ptr(),
@@ -743,15 +750,13 @@ def _moe_ffn_scored(x, logits, gate, up, down, topk, norm_topk_prob, routed_scal
     L = lib()
     sg, su, sd = (s.handle for s in shared) if shared is not None else (None, None, None)
     gw = shared_gate.to(torch.float32).contiguous() if shared_gate is not None else None
-    with torch.cuda.device(dev):
-        wsb = int(L.qmm_moe_ffn_scored_workspace_size(gate.handle, down.handle, t, e, topk, sg, su, sd))
-        if wsb == 0:
-            raise QmmError(QMM_ERR_INVALID, "moe_ffn: " + last_error())
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-        _check(L.qmm_moe_ffn_scored(xx.data_ptr(), _DENSE[xx.dtype], t, hdim, lg.data_ptr(), e, topk, tag, _ptr(bias),
-                                    groups, topk_groups, group_top, int(norm_topk_prob), routed_scaling_factor,
-                                    gate.handle, up.handle, down.handle, sg, su, sd, _ptr(gw), out.data_ptr(),
-                                    _DENSE[odt], hdim, ws.data_ptr(), wsb, _stream(dev)))
+    wsb = int(L.qmm_moe_ffn_scored_workspace_size(gate.handle, down.handle, t, e, topk, sg, su, sd))
+    if wsb == 0:
+        raise QmmError(QMM_ERR_INVALID, "moe_ffn: " + last_error())
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    _check(_call(dev, L.qmm_moe_ffn_scored, xx.data_ptr(), _DENSE[xx.dtype], t, hdim, lg.data_ptr(), e, topk, tag,
+                 _ptr(bias), groups, topk_groups, group_top, int(norm_topk_prob), routed_scaling_factor, gate.handle,
+                 up.handle, down.handle, sg, su, sd, _ptr(gw), out.data_ptr(), _DENSE[odt], hdim, ws.data_ptr(), wsb))
     return out.to(out_dtype)
 
 
