@@ -641,23 +641,24 @@ __device__ __forceinline__ void mx_gemm(const MxOut& o, const uint8_t* __restric
     if (experts > 0 && !qmm::mx_expert_tile(counts, offsets, experts, pairs, n, RAW ? 2 : 16, blockIdx.y, r)) return;  \
     qmm::mx_gemv<W, 4, 1, true, RAW>(o, up, r, n, k, xq, raw, 0);                                              \
   }
-#define QMM_MX_GEMVS_W(W)            \
+#define QMM_MX_GEMVS(W)              \
   QMM_MX_GEMV(W, 1, 1, , 0)          \
-  QMM_MX_GEMV(W, 1, 2, , 0)          \
   QMM_MX_GEMV(W, 4, 1, , 0)          \
   QMM_MX_GEMV(W, 1, 1, _raw32, 1)    \
   QMM_MX_GEMV(W, 1, 2, _raw32, 1)    \
   QMM_MX_GEMV(W, 1, 1, _raw16, 2)    \
   QMM_MX_GEMV(W, 1, 2, _raw16, 2)    \
   QMM_MX_EXPERT_GEMV(W, 1, 1)        \
-  QMM_MX_EXPERT_GEMV(W, 1, 2)        \
   QMM_MX_EXPERT_GEMV(W, 4, 1)        \
   QMM_MX_GLU_GEMV(W, , 0)            \
   QMM_MX_GLU_GEMV(W, _raw32, 1)      \
   QMM_MX_GLU_GEMV(W, _raw16, 2)
-QMM_MX_GEMVS_W(4)
-QMM_MX_GEMVS_W(8)
-QMM_MX_GEMVS_W(16)
+QMM_MX_GEMVS(4)
+QMM_MX_GEMVS(8)
+QMM_MX_GEMVS(16)
+// (planes of one column tile a group that has more chunks than waves get all 16)
+QMM_MX_GEMV(16, 1, 2, , 0)
+QMM_MX_EXPERT_GEMV(16, 1, 2)
 
 #define QMM_MX_GEMM(NAME, FM, FN, WM, WN, WK, EU)                                                              \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN * WK, EU) qmm_mx_gemm_##NAME(                      \
