@@ -3073,7 +3073,9 @@ static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const
     const bool direct = mx_raw_fits(tokens, H);
     if (!direct) QMM_TRY(mx_quantize_x(d, xc, x_dtype, P, H, ldx, ptok, b + L.xp, s));
     QMM_TRY(mx_glu(d, gate, up, experts, b + L.xp, direct ? &raw : nullptr, P, counts, offsets, b + L.hp, s));
-    QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, counts, offsets, &yp, s));
+    // (a token or two: the down products and their sums are one launch, below)
+    if (T > kMxRawRows)
+      QMM_TRY(mx_expert_product(d, &down, 1, experts, b + L.hp, P, counts, offsets, &yp, s));
     float *shared = nullptr, *sg = nullptr;
     if (sh.gate) {
       shared = (float*)(b + L.shared);
@@ -3085,6 +3087,19 @@ static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const
     void* oc = (uint8_t*)out + t0 * ldo * (int64_t)mx_type_size(out_dtype);
     int wide = mx_wide(oc, out_dtype, ldo);
     long long lo = ldo;
+    if (T <= kMxRawRows) {
+      MxOut o = {};
+      o.w = down->data;
+      o.y = oc;
+      o.y_type = out_dtype;
+      int E = experts, ff = (int)F;
+      const uint8_t* hq = b + L.hp;
+      void* args[] = {&o, &E, &k, &n, &ff, &counts, &offsets, &tpairs, &pw, &hq, &shared, &sg, &lo};
+      hipFunction_t f;
+      QMM_TRY(kernel(d, "qmm_mx_down_sum", &f));
+      QMM_HIP(hipModuleLaunchKernel(f, ceil_div(H, 16), (unsigned)T, 1, 1024, 1, 1, 0, s, args, nullptr));
+      continue;
+    }
     void* args[] = {&yp, &pw, &tpairs, &tt, &k, &n, &shared, &sg, &oc, &ot, &lo, &wide};
     QMM_TRY(launch(d, "qmm_mx_combine", ceil_div(T * (H / 4), 256), 256, 0, s, args));
   }

@@ -696,6 +696,104 @@ extern "C" __global__ void __launch_bounds__(256, 2) qmm_mx_expert_glu_128x128(
   qmm::mx_gemm<2, 4, 2, 2, 1, true>(o, up, r, n, kc, 128 * blockIdx.x, xq, 0);
 }
 
+// The down products of a token's experts and their weighted sum in one launch, for a
+// token or two: out[t] = sum over t's pairs, in increasing expert order, of weight *
+// down(h[pair]), then + shared[t] (times sg[t]), rounded once. Grid: 16-column groups,
+// tokens. The pairs' chunks are one list that 16 waves split (wave i: chunks i, i + 16, ...,
+// two in flight), a wave's sums of a pair are scaled when the list leaves it, and the waves'
+// sums meet in LDS, in wave order.
+//
+// What bounds it: the weights' stream and its beginning. One token's two experts of 4096 x
+// 14336 (62 MB): 13.7 us, against 12.9 and 3.9 of products by pair and their sum; the call
+// 43.7 us against 45.7, with 6 of 64 experts of 2048 x 1408 23.3 against 26.2. Two tokens read
+// an expert that both chose twice: 67.0 us against 64.8, and 32.6 against 37.2 (8 of 64).
+extern "C" __global__ void __launch_bounds__(1024, 4)
+    qmm_mx_down_sum(qmm::MxOut o, int experts, int topk, int n, int k, const int* __restrict__ counts,
+                    const int* __restrict__ offsets, const int* __restrict__ token_pairs,
+                    const float* __restrict__ pair_weight, const uint8_t* __restrict__ hq,
+                    const float* __restrict__ shared, const float* __restrict__ sg, long long ldo) {
+  using namespace qmm;
+  constexpr int W = 16, U = 2, kPairs = 32;
+  __shared__ int expert[kPairs];
+  __shared__ __attribute__((aligned(16))) float red[W][16];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int c = lane & 15, g = lane >> 4, h = g & 1, token = blockIdx.y;
+  const int* pairs = token_pairs + (long long)token * topk;
+  for (int s = wave; s < topk; s += W) {  // the expert that holds row p of the list
+    const int p = pairs[s];
+    if (lane == 0) expert[s] = 0;
+    for (int e0 = 0; e0 < experts; e0 += 64) {
+      const int e = e0 + lane;
+      if (e < experts && p >= offsets[e] && p < offsets[e] + counts[e]) expert[s] = e;
+    }
+  }
+  __syncthreads();
+  const int kc = (k + kMxChunk - 1) / kMxChunk, col = min(16 * (int)blockIdx.x + c, n - 1);
+  mx_u32x4 w[U][2];
+  mx_u32x12 x[U][2];
+  int sw[U], sx[U];
+  auto load = [&](int u, int s, int kk) {
+    const int p = __builtin_amdgcn_readfirstlane(pairs[s]);
+    const long long r = (long long)__builtin_amdgcn_readfirstlane(expert[s]) * n + col;
+    const uint8_t* xp = hq + mx_x_at(p, h, kc) + (g >> 1) * kMxXStep + (long long)kk * kMxXUnit;
+    x[u][0] = mx_get_x(xp);
+    x[u][1] = mx_get_x(xp + 2 * kMxXStep);
+    sx[u] = *reinterpret_cast<const int*>(hq + mx_xs_at(p, h, kc) + (long long)kk * kMxXUnit);
+    const uint8_t* wp = o.w + mx_w_at(r, h, kc) + (g >> 1) * kMxStepBytes + (long long)kk * kMxUnit;
+    w[u][0] = *reinterpret_cast<const mx_u32x4*>(wp);
+    w[u][1] = *reinterpret_cast<const mx_u32x4*>(wp + 2 * kMxStepBytes);
+    sw[u] = *reinterpret_cast<const int*>(o.w + mx_ws_at(r, h, kc) + (long long)kk * kMxUnit);
+  };
+  int s = wave / kc, kk = wave % kc;  // the chunk in turn, and the one to load
+  int sl = s, kl = kk;
+  auto next = [&](int& s, int& kk) {
+    kk += W;
+    while (kk >= kc) {
+      kk -= kc;
+      ++s;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (sl < topk) load(u, sl, kl);
+    next(sl, kl);
+  }
+  mx_f32x4 sum = (mx_f32x4)(0.0f), acc = (mx_f32x4)(0.0f);
+  auto weight = [&](int s) { return pair_weight[__builtin_amdgcn_readfirstlane(pairs[s])]; };
+  int cur = s;
+#pragma unroll 1
+  while (s < topk) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s >= topk) break;
+      if (s != cur) {
+        sum += weight(cur) * acc;
+        acc = (mx_f32x4)(0.0f);
+        cur = s;
+      }
+      const int b = sw[u] >> (8 * (g >> 1)), e = sx[u] >> (8 * (g >> 1));
+      const int s0 = e & 255, s1 = e >> 16 & 255;
+      acc = mx_mfma16<0>(w[u][0], mx_hi(x[u][0]), acc, b, s0);
+      acc = mx_mfma16<0>(w[u][0], mx_lo(x[u][0]), acc, b, s0 - 4);
+      acc = mx_mfma16<0>(w[u][1], mx_hi(x[u][1]), acc, b >> 16, s1);
+      acc = mx_mfma16<0>(w[u][1], mx_lo(x[u][1]), acc, b >> 16, s1 - 4);
+      next(s, kk);
+      if (sl < topk) load(u, sl, kl);
+      next(sl, kl);
+    }
+  }
+  if (cur < topk) sum += weight(cur) * acc;
+  if (c == 0) *reinterpret_cast<mx_f32x4*>(&red[wave][4 * g]) = sum;
+  __syncthreads();
+  const int q = 16 * (int)blockIdx.x + t;
+  if (t >= 16 || q >= n) return;
+  float v = red[0][t];
+#pragma unroll
+  for (int i = 1; i < W; ++i) v += red[i][t];
+  if (shared != nullptr) v += (sg != nullptr ? sg[token] : 1.0f) * shared[(long long)token * n + q];
+  mx_store(o.y, o.y_type, token * ldo + q, v);
+}
+
 // out[t] = sum over token t's pairs, in increasing expert order, of weight * yp[pair],
 // then + shared[t] (times sg[t] when the shared expert is gated), rounded once to the
 // output's type. Four columns a thread (n is a multiple of 32).

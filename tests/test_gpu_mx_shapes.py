@@ -110,6 +110,8 @@ def test_rows_longer_than_a_workgroup_holds(m):
 @pytest.mark.parametrize("counts,n,k", [
     ([50, 0, 0, 1, 0, 0, 0, 0], 100, 288),       # four row tiles of one expert, one column tile a group
     ([50, 0, 0, 1, 0, 0, 0, 0], 2060, 2400),     # four column tiles, 16 and 8 waves
+    ([3, 0, 2], 100, 2400),                      # 16 waves, a chunk each
+    ([1] * 8, 1030, 1312),                       # four column tiles, 8 waves
     ([2, 0, 33, 5] * 16, 1040, 1312),            # four waves, two chunks each
     ([100, 0, 250], 500, 352),                   # 64-row tiles
     ([500, 524], 3570, 96),                      # 128 x 128
@@ -140,7 +142,7 @@ def ffn_reference(x, rows, g, u, d):
 
 @pytest.mark.parametrize("t,e,k,h,f", [
     (1, 8, 2, 4128, 160), (2, 4, 2, 2080, 96), (2, 64, 6, 288, 1056), (1, 4, 1, 96, 8224), (1, 2, 2, 16416, 64),
-    (1, 2, 1, 16384, 64),
+    (1, 2, 1, 16384, 64), (1, 8, 2, 1312, 64),
     (5, 8, 2, 4128, 96), (20, 8, 3, 1312, 288), (9, 8, 2, 544, 4128), (120, 16, 2, 96, 1056), (120, 4, 4, 544, 416),
     (700, 3, 2, 288, 1120)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
