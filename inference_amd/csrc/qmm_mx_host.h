@@ -350,7 +350,7 @@ int route_scored(Device* d, const float* logits, int64_t tokens, int experts, in
   void* a1[] = {&logits, &bias, &a, &ids, &wts};
   QMM_TRY(launch(d, name, ceil_div(tokens, 4), 256, 0, s, a1));
   void* a2[] = {&a, &ids, &wts, &counts, &offsets, &pair_token, &pair_weight, &token_pairs};
-  return launch(d, "qmm_route_lists", ceil_div(tokens, 64), 1024, 0, s, a2);
+  return launch(d, "qmm_route_lists", experts, 1024, 0, s, a2);
 }
 
 }  // namespace

@@ -24,17 +24,37 @@ struct RouteArgs {
   float scale;
 };
 
+// A lane's value as a scalar, and a value of another lane of a row of 16 by its pattern:
+// a wave's maximum and sum are chains of these, a tenth of the latency of a shuffle each.
+__device__ __forceinline__ int route_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ float route_lane(float v, int l) { return __int_as_float(route_lane(__float_as_int(v), l)); }
+__device__ __forceinline__ double route_lane(double v, int l) {
+  return __hiloint2double(route_lane(__double2hiint(v), l), route_lane(__double2loint(v), l));
+}
+template <int P>
+__device__ __forceinline__ double route_row(double v) {
+  const int lo = __double2loint(v), hi = __double2hiint(v);
+  return __hiloint2double(__builtin_amdgcn_update_dpp(hi, hi, P, 0xf, 0xf, true),
+                          __builtin_amdgcn_update_dpp(lo, lo, P, 0xf, 0xf, true));
+}
+template <typename F>
+__device__ __forceinline__ double route_wave(double v, F f) {
+  v = f(v, route_row<0xb1>(v));   // lanes 1 0 3 2 of four
+  v = f(v, route_row<0x4e>(v));   // 2 3 0 1
+  v = f(v, route_row<0x141>(v));  // eight, mirrored
+  v = f(v, route_row<0x140>(v));  // sixteen, mirrored
+  return f(f(route_lane(v, 0), route_lane(v, 16)), f(route_lane(v, 32), route_lane(v, 48)));
+}
 __device__ __forceinline__ double route_wave_max(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v = fmax(v, __shfl_xor(v, d));
-  return v;
+  return route_wave(v, [](double a, double b) { return fmax(a, b); });
 }
 __device__ __forceinline__ double route_wave_sum(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  return v;
+  return route_wave(v, [](double a, double b) { return a + b; });
 }
 
+// What bounds it: the f64 exponentials (and quotients) of all experts and the chain of k
+// maxima over the wave. 4096 tokens of 256 experts, 8 of 8 groups' 4 with sigmoid scores:
+// 13.7 us, 16.4 with the maxima, sums and group scores by shuffles.
 // One token by one wave, expert e = 64 i + lane in register i. Lane j < k returns the
 // token's j-th expert in increasing order, and its weight. `ch`: E doubles of LDS, this
 // wave's own.
@@ -84,17 +104,27 @@ __device__ __forceinline__ void route_token(const float* __restrict__ logits, co
       if (64 * i + lane < a.E) ch[64 * i + lane] = c[i];
     // (one wave writes and reads its own part: the LDS keeps the order)
     __builtin_amdgcn_wave_barrier();
+    // `sub` lanes a group, then lane g has group g's score
+    int sub = 64;
+    while (sub * a.groups > 64) sub /= 2;
+    const int mine = lane / sub;
     double best = -INFINITY, second = -INFINITY;
-    if (lane < a.groups)
-      for (int j = 0; j < gs; ++j) {
-        const double v = ch[lane * gs + j];
+    if (mine < a.groups)
+      for (int j = lane % sub; j < gs; j += sub) {
+        const double v = ch[mine * gs + j];
         second = fmax(second, fmin(best, v));
         best = fmax(best, v);
       }
-    const double score = a.group_top == 2 ? best + second : best;
+    for (int d = 1; d < sub; d *= 2) {
+      const double b = __shfl_xor(best, d), n = __shfl_xor(second, d);
+      second = fmax(fmax(second, n), fmin(best, b));
+      best = fmax(best, b);
+    }
+    const double part = a.group_top == 2 ? best + second : best;
+    const double score = __shfl(part, lane * sub & 63);
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
-      const double o = __shfl(score, g);
+      const double o = route_lane(part, g * sub);
       rank += o > score || (o == score && g < lane);
     }
     const unsigned long long kept = __ballot(lane < a.groups && rank < a.topk_groups);
@@ -121,7 +151,7 @@ __device__ __forceinline__ void route_token(const float* __restrict__ logits, co
       if (e < 0 && b) {
         const int l = __builtin_ctzll(b);
         e = 64 * i + l;
-        sc = __shfl(s[i], l);
+        sc = route_lane(s[i], l);
         if (lane == l) c[i] = -INFINITY;
       }
     }
@@ -134,14 +164,14 @@ __device__ __forceinline__ void route_token(const float* __restrict__ logits, co
   double w = ms;
   if (a.renorm) w = sum > 0.0 ? ms / sum : 0.0;
   const float wf = (float)(w * (double)a.scale);
-  int place = 0;  // increasing expert order
-  for (int j = 0; j < a.k; ++j) place += __shfl(mine, j) < mine;
-  // lane p takes the selection whose place is p
+  // lane p takes the selection whose place in increasing expert order is p
+  int place = 0;
+  for (int j = 0; j < a.k; ++j) place += route_lane(mine, j) < mine;
   expert = 0;
   weight = 0.0f;
   for (int j = 0; j < a.k; ++j) {
-    const int p = __shfl(place, j), e = __shfl(mine, j);
-    const float v = __shfl(wf, j);
+    const int p = route_lane(place, j), e = route_lane(mine, j);
+    const float v = route_lane(wf, j);
     if (lane == p) {
       expert = e;
       weight = v;
@@ -149,21 +179,18 @@ __device__ __forceinline__ void route_token(const float* __restrict__ logits, co
   }
 }
 
-constexpr int kRouteMaxE = 1024, kRouteMaxK = 32;
+constexpr int kRouteMaxK = 32;
 
-// The lists of one group of up to 64 tokens [t0, t0 + nt), of which sel_e / sel_w (LDS)
-// hold the selections in expert order: `before` and `total` are the counts of each
-// expert over the tokens before t0 and over all of them. A pair's place is its expert's
-// offset, plus `before`, plus the number of the group's earlier tokens that selected it
-// (a bit mask of tokens per expert: any order of the ORs gives the same mask).
-template <int NT>
-__device__ __forceinline__ void route_lists(const RouteArgs& a, int t0, int nt, const uint16_t* sel_e,
-                                            const float* sel_w, const int* before, const int* total, int* offs,
-                                            unsigned long long* mask, int* __restrict__ counts,
+// The lists of up to 16 tokens, by one workgroup: sel_e / sel_w (LDS) hold the selections
+// in expert order, `total` each expert's count. A pair's place is its expert's offset plus
+// the number of earlier tokens that selected it (a bit mask of tokens per expert: any
+// order of the ORs gives the same mask).
+__device__ __forceinline__ void route_lists(const RouteArgs& a, const uint16_t* sel_e, const float* sel_w,
+                                            const int* total, int* offs, unsigned* mask, int* __restrict__ counts,
                                             int* __restrict__ offsets, int* __restrict__ pair_token,
                                             float* __restrict__ pair_weight, int* __restrict__ token_pairs) {
   const int t = threadIdx.x;
-  for (int e = t; e < a.E; e += NT) mask[e] = 0;
+  if (t < a.E) mask[t] = 0;
   if (t < 64) {  // exclusive prefix of the totals
     int base = 0;
     for (int e0 = 0; e0 < a.E; e0 += 64) {
@@ -175,25 +202,21 @@ __device__ __forceinline__ void route_lists(const RouteArgs& a, int t0, int nt, 
         if (t >= d) sum += o;
       }
       if (e < a.E) offs[e] = base + sum - v;
-      base += __shfl(sum, 63);
+      base += route_lane(sum, 63);
     }
     if (t == 0) offs[a.E] = base;
   }
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int e = t; e <= a.E; e += NT) {
-      offsets[e] = offs[e];
-      if (e < a.E) counts[e] = total[e];
-    }
-  const int np = nt * a.k;
-  for (int p = t; p < np; p += NT) atomicOr(&mask[sel_e[p]], 1ull << (p / a.k));
+  if (t <= a.E) offsets[t] = offs[t];
+  if (t < a.E) counts[t] = total[t];
+  const int i = t / a.k, e = i < a.T ? sel_e[t] : 0;
+  if (i < a.T) atomicOr(&mask[e], 1u << i);
   __syncthreads();
-  for (int p = t; p < np; p += NT) {
-    const int i = p / a.k, e = sel_e[p];
-    const int at = offs[e] + before[e] + __popcll(mask[e] & ((1ull << i) - 1ull));
-    pair_token[at] = t0 + i;
-    pair_weight[at] = sel_w[p];
-    token_pairs[(long long)t0 * a.k + p] = at;
+  if (i < a.T) {
+    const int at = offs[e] + __popc(mask[e] & ((1u << i) - 1u));
+    pair_token[at] = i;
+    pair_weight[at] = sel_w[t];
+    token_pairs[t] = at;
   }
 }
 
@@ -208,10 +231,10 @@ __device__ __forceinline__ void route_lists(const RouteArgs& a, int t0, int nt, 
     __shared__ double ch[16][64 * R];                                                                             \
     __shared__ uint16_t sel_e[16 * qmm::kRouteMaxK];                                                              \
     __shared__ float sel_w[16 * qmm::kRouteMaxK];                                                                 \
-    __shared__ int before[64 * R], total[64 * R], offs[64 * R + 1];                                               \
-    __shared__ unsigned long long mask[64 * R];                                                                   \
+    __shared__ int total[64 * R], offs[64 * R + 1];                                                               \
+    __shared__ unsigned mask[64 * R];                                                                             \
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;                                                   \
-    for (int e = threadIdx.x; e < a.E; e += 1024) before[e] = total[e] = 0;                                       \
+    for (int e = threadIdx.x; e < a.E; e += 1024) total[e] = 0;                                                   \
     __syncthreads();                                                                                              \
     if (wave < a.T) {                                                                                             \
       int e;                                                                                                      \
@@ -224,8 +247,7 @@ __device__ __forceinline__ void route_lists(const RouteArgs& a, int t0, int nt, 
       }                                                                                                           \
     }                                                                                                             \
     __syncthreads();                                                                                              \
-    qmm::route_lists<1024>(a, 0, a.T, sel_e, sel_w, before, total, offs, mask, counts, offsets, pair_token,       \
-                           pair_weight, token_pairs);                                                             \
+    qmm::route_lists(a, sel_e, sel_w, total, offs, mask, counts, offsets, pair_token, pair_weight, token_pairs);  \
   }
 QMM_ROUTE_SMALL(1)
 QMM_ROUTE_SMALL(2)
@@ -253,41 +275,83 @@ QMM_ROUTE_TOKENS(2)
 QMM_ROUTE_TOKENS(4)
 QMM_ROUTE_TOKENS(16)
 
-// The lists from all tokens' selections, 64 tokens a workgroup. Every workgroup counts
-// the selections before its tokens and the rest by itself (LDS counters, eight copies
-// by lane where experts are few, so that a wave's adds fall on distinct words); integer
-// adds, so their order does not matter.
+// The lists from all tokens' selections, a workgroup an expert: it counts the selections
+// of lower experts (its offset) and its own, each thread over a run of the list, and
+// writes its own pairs in the list's order. Every workgroup reads the whole list (2 bytes
+// a selection), 64 selections a thread in flight; no atomics and no other launch. 32768
+// selections of 256 experts: 6.9 us (11.8 by workgroups of 64 tokens that count every
+// expert in LDS; 11.5 with one load of 8 selections after another).
 extern "C" __global__ void __launch_bounds__(1024) qmm_route_lists(
     qmm::RouteArgs a, const uint16_t* __restrict__ ids, const float* __restrict__ wts, int* __restrict__ counts,
     int* __restrict__ offsets, int* __restrict__ pair_token, float* __restrict__ pair_weight,
     int* __restrict__ token_pairs) {
-  __shared__ uint16_t sel_e[64 * qmm::kRouteMaxK];
-  __shared__ float sel_w[64 * qmm::kRouteMaxK];
-  __shared__ int cnt[2][qmm::kRouteMaxE];
-  __shared__ int before[qmm::kRouteMaxE], total[qmm::kRouteMaxE], offs[qmm::kRouteMaxE + 1];
-  __shared__ unsigned long long mask[qmm::kRouteMaxE];
-  const int t = threadIdx.x, t0 = 64 * blockIdx.x, nt = min(64, a.T - t0);
-  const int copies = a.E <= 128 ? 8 : 1;
-  for (int i = t; i < a.E * copies; i += 1024) cnt[0][i] = cnt[1][i] = 0;
-  __syncthreads();
-  const long long first = (long long)t0 * a.k, all = (long long)a.T * a.k;
-  for (long long p = t; p < all; p += 1024)
-    atomicAdd(&cnt[p < first ? 0 : 1][ids[p] * copies + (t & (copies - 1))], 1);
-  for (int p = t; p < nt * a.k; p += 1024) {
-    sel_e[p] = ids[first + p];
-    sel_w[p] = wts[first + p];
-  }
-  __syncthreads();
-  for (int e = t; e < a.E; e += 1024) {
-    int b = 0, r = 0;
-    for (int c = 0; c < copies; ++c) {
-      b += cnt[0][e * copies + c];
-      r += cnt[1][e * copies + c];
+  __shared__ int wave_eq[16], wave_lt[16];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, e = blockIdx.x;
+  const int all = a.T * a.k, run = ((all + 1023) / 1024 + 7) & ~7;  // runs of 16-byte pieces
+  const int p0 = min(t * run, all), p1 = min(p0 + run, all);
+  // 64 selections of a run at a time: bit j of the masks is selection j's
+  auto masks = [&](int p, unsigned long long& is, unsigned long long& less) {
+    qmm::mx_u32x4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (p + 8 * i < p1) v[i] = *reinterpret_cast<const qmm::mx_u32x4*>(ids + p + 8 * i);
+    is = less = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (p + 8 * i < p1) {
+        unsigned a8 = 0, b8 = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int id = (int)(v[i][j >> 1] >> (16 * (j & 1)) & 0xffff);
+          a8 |= (unsigned)(id == e) << j;
+          b8 |= (unsigned)(id < e) << j;
+        }
+        is |= (unsigned long long)a8 << (8 * i);
+        less |= (unsigned long long)b8 << (8 * i);
+      }
+    if (p1 - p < 64) {  // (the list's last piece may be read past its end, within its workspace)
+      is &= (1ull << (p1 - p)) - 1;
+      less &= (1ull << (p1 - p)) - 1;
     }
-    before[e] = b;
-    total[e] = b + r;
+  };
+  unsigned long long is = 0, less = 0;
+  int eq = 0, lt = 0;
+  for (int p = p0; p < p1; p += 64) {
+    masks(p, is, less);
+    eq += __popcll(is);
+    lt += __popcll(less);
+  }
+  int pre = eq, low = lt;  // inclusive prefix of eq, sum of lt, over the wave
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(pre, d);
+    if (lane >= d) pre += o;
+    low += __shfl_xor(low, d);
+  }
+  if (lane == 63) {
+    wave_eq[wave] = pre;
+    wave_lt[wave] = low;
   }
   __syncthreads();
-  qmm::route_lists<1024>(a, t0, nt, sel_e, sel_w, before, total, offs, mask, counts, offsets, pair_token, pair_weight,
-                         token_pairs);
+  int at = pre - eq, total = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    at += wave_lt[i] + (i < wave ? wave_eq[i] : 0);
+    total += wave_eq[i];
+  }
+  if (t == 0) {  // (its own run is empty before it: `at` is the expert's offset)
+    counts[e] = total;
+    offsets[e] = at;
+    if (e == a.E - 1) offsets[a.E] = at + total;
+  }
+  if (eq == 0) return;
+  for (int p = p0; p < p1; p += 64) {
+    if (run > 64) masks(p, is, less);
+    for (; is; is &= is - 1) {
+      const int q = p + __builtin_ctzll(is);
+      pair_token[at] = q / a.k;
+      pair_weight[at] = wts[q];
+      token_pairs[q] = at++;
+    }
+  }
 }
