@@ -1191,8 +1191,7 @@ static int mx_from_blocks(const GemvTarget* tg, int count, const void* xq, int64
   const int64_t k = tg[0].w->k;
   QMM_TRY(mx_check_rows(m, k));
   const size_t need = mx_planes(m, k);
-  if (!ws || ws_bytes < need)
-    return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed (qmm_matmul_q_workspace_size)", ws ? ws_bytes : 0, need);
+  QMM_TRY(mx_check_ws(ws, ws_bytes, need));
   Device* d;
   QMM_TRY(current_device(&d));
   uint8_t* b = (uint8_t*)ws;
@@ -1444,8 +1443,7 @@ static int mx_targets(const GemvTarget* tg, int count, const void* x, int x_dtyp
   const bool direct = mx_raw_fits(m, k);
   const size_t planes = direct ? 0 : align256(mx_planes(m, k));
   const size_t need = planes + (norm_w ? align256((size_t)(m * k) * 4) : 0);
-  if (need && (!ws || ws_bytes < need))
-    return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
+  QMM_TRY(mx_check_ws(ws, ws_bytes, need));
   Device* d;
   QMM_TRY(current_device(&d));
   uint8_t* b = (uint8_t*)ws;
@@ -1819,6 +1817,9 @@ static MxFfnWs mx_ffn_ws(const qmm_qtensor* gate, const qmm_qtensor* down, int64
 static int mx_ffn(Device* d, const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* down, const void* x,
                   int x_dtype, int64_t m, int64_t ldx, const float* norm_w, float eps, int accumulate, float* y,
                   int64_t ldy, uint8_t* b, hipStream_t s) {
+  QMM_TRY(mx_here(gate));
+  QMM_TRY(mx_here(up));
+  QMM_TRY(mx_here(down));
   const MxFfnWs L = mx_ffn_ws(gate, down, m, norm_w != nullptr);
   if (norm_w) {
     float* xn = (float*)(b + L.xn);
@@ -1857,8 +1858,7 @@ int qmm_ffn(const qmm_qtensor* gate, const qmm_qtensor* up, const qmm_qtensor* d
   QMM_TRY(current_device(&d));
   hipStream_t s = (hipStream_t)stream;
   if (is_mx(gate->dtype)) {
-    const size_t need = mx_ffn_ws(gate, down, m, norm_weight != nullptr).total;
-    if (!ws || ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
+    QMM_TRY(mx_check_ws(ws, ws_bytes, mx_ffn_ws(gate, down, m, norm_weight != nullptr).total));
     return mx_ffn(d, gate, up, down, x, QMM_F32, m, ldx, norm_weight, eps, accumulate ? 1 : 0, y, ldy, (uint8_t*)ws, s);
   }
   const FfnWs L = ffn_ws(d, gate, up, down, m, norm_weight != nullptr);
@@ -2135,7 +2135,7 @@ static int warm_plan(const Device* d, const qmm_qtensor* const* warm, const int*
       if (i == count) break;
     }
     const qmm_qtensor* w = warm[i];
-    if (!w || fmt_of(w->dtype) == kFmtQ80) return fail(QMM_ERR_INVALID, "L2 warming takes Q4_K / Q6_K weights");
+    if (!w || (w->dtype != QMM_Q4K && w->dtype != QMM_Q6K)) return fail(QMM_ERR_INVALID, "L2 warming takes Q4_K / Q6_K weights");
     if (warm_launch[i] < launch || warm_launch[i] < 0) return fail(QMM_ERR_INVALID, "warm_launch must not decrease");
     launch = warm_launch[i];
     const int rpw = warm_rows[launch];
@@ -2361,7 +2361,7 @@ int qmm_prefill_attention(const float* q, int64_t ldq, const float* kcache, cons
 size_t qmm_prefill_attention_o_workspace_size(const qmm_qtensor* wo, int64_t count) {
   if (!wo || count < 1) return 0;
   const size_t mm = qmm_matmul_ex_workspace_size(wo, count, 0);
-  if (mm == 0) return 0;
+  if (mm == 0 && !is_mx(wo->dtype)) return 0;  // (a row or two of MXFP4 need none)
   return align256((size_t)count * (size_t)wo->k * 4) + mm;
 }
 
@@ -2539,9 +2539,7 @@ int qmm_moe_route_scored(const float* logits, int64_t tokens, int experts, int t
     return fail(QMM_ERR_INVALID, "null pointer");
   const Routing r = {true, score, groups, topk_groups, group_top, bias, renormalize, routed_scaling_factor};
   QMM_TRY(check_routing(tokens, experts, topk, r));
-  const size_t need = route_scratch(tokens, experts, topk);
-  if (need && (!ws || ws_bytes < need))
-    return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? ws_bytes : 0, need);
+  QMM_TRY(mx_check_ws(ws, ws_bytes, route_scratch(tokens, experts, topk)));
   Device* d;
   QMM_TRY(current_device(&d));
   return route_scored(d, logits, tokens, experts, topk, r, counts, offsets, pair_token, pair_weight, token_pairs,
@@ -2703,6 +2701,8 @@ int qmm_moe_gemm(const qmm_qtensor* const* w, int count, int experts, const floa
   uint8_t* b = (uint8_t*)ws;
   if (is_mx(w0->dtype)) {
     QMM_TRY(mx_check_rows(pairs, w0->k));
+    QMM_TRY(mx_check_ws(ws, ws_bytes, mx_planes(pairs, w0->k)));
+    for (int j = 0; j < count; ++j) QMM_TRY(mx_here(w[j]));
     QMM_TRY(mx_quantize_x(d, x, QMM_F32, pairs, w0->k, ldx, nullptr, b, s));
     return mx_expert_product(d, w, count, experts, b, pairs, counts, offsets, y, s);
   }
@@ -3126,12 +3126,10 @@ static int moe_ffn(const void* xv, int x_dtype, int64_t tokens, int64_t ldx, con
     QMM_TRY(check_routing(chunk, experts, topk, r));
     QMM_TRY(mx_check_rows(pairs, gate->k));
     QMM_TRY(mx_check_rows(pairs, down->k));
-    const size_t need = mx_moe_ws(gate, tokens, experts, topk, sh).total;
-    if (ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws_bytes, need);
-    int dev = 0;
-    QMM_HIP(hipGetDevice(&dev));
-    if (dev != gate->device || dev != up->device || dev != down->device)
-      return fail(QMM_ERR_INVALID, "expert weights live on another device than the current one (%d)", dev);
+    QMM_TRY(mx_check_ws(ws, ws_bytes, mx_moe_ws(gate, tokens, experts, topk, sh).total));
+    QMM_TRY(mx_here(gate));
+    QMM_TRY(mx_here(up));
+    QMM_TRY(mx_here(down));
     return mx_moe(xv, x_dtype, tokens, ldx, logits, experts, topk, r, gate, up, down, sh, outv, out_dtype, ldo,
                   (uint8_t*)ws, (hipStream_t)stream);
   }

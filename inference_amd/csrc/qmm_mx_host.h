@@ -77,6 +77,21 @@ int mx_check_rows(int64_t m, int64_t k) {
   return QMM_OK;
 }
 
+// A workspace of `need` bytes (0: none); its parts are read 16 bytes at a time.
+int mx_check_ws(const void* ws, size_t bytes, size_t need) {
+  if (need == 0) return QMM_OK;
+  if (!ws || bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws ? bytes : 0, need);
+  if ((uintptr_t)ws % 16) return fail(QMM_ERR_INVALID, "workspaces must be 16-byte aligned");
+  return QMM_OK;
+}
+
+int mx_here(const qmm_qtensor* w) {
+  int dev = 0;
+  QMM_HIP(hipGetDevice(&dev));
+  if (dev != w->device) return fail(QMM_ERR_INVALID, "tensor lives on device %d, current device is %d", w->device, dev);
+  return QMM_OK;
+}
+
 unsigned mx_plane_units(int64_t m, int64_t k) { return (unsigned)((m + kMxTile - 1) / kMxTile * mx_chunks(k)); }
 
 // Planes of m rows: row i is row src[i] of x, or row i (src null).

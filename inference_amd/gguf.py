@@ -31,7 +31,7 @@ _UNSIGNED = (T_UINT8, T_UINT16, T_UINT32, T_UINT64)
 _SIGNED = (T_INT8, T_INT16, T_INT32, T_INT64)
 
 # GGML type tags of the formats a resident load takes
-GGML_F32, GGML_F16, GGML_Q8_0, GGML_Q4K, GGML_Q6K, GGML_BF16 = 0, 1, 8, 12, 14, 30
+GGML_F32, GGML_F16, GGML_Q8_0, GGML_Q4K, GGML_Q6K, GGML_BF16, GGML_MXFP4 = 0, 1, 8, 12, 14, 30, 39
 
 
 @dataclass(frozen=True)
@@ -214,7 +214,7 @@ class GgufFile:
         return a
 
     def load_qtensor(self, info: TensorInfo, device: torch.device, unpermute_heads: int = 0) -> QTensor:
-        """Resident load of a 2-D Q8_0 / Q4_K / Q6_K tensor into a device QTensor (blocks copied as is;
+        """Resident load of a 2-D Q8_0 / Q4_K / Q6_K / MXFP4 tensor into a device QTensor (blocks copied as is;
         unpermute_heads > 0 restores the half-split q/k row order of llama.cpp files)."""
         with torch.cuda.device(device):
             h = ctypes.c_void_p()
@@ -223,8 +223,8 @@ class GgufFile:
         return QTensor(h, device)
 
     def load_dense(self, info: TensorInfo, device: torch.device) -> torch.Tensor:
-        """F32 / F16 / BF16 tensor as f32 on the device; Q8_0 / Q4_K / Q6_K dequantized on the device."""
-        if info.ggml_type in (GGML_Q8_0, GGML_Q4K, GGML_Q6K):
+        """F32 / F16 / BF16 tensor as f32 on the device; Q8_0 / Q4_K / Q6_K / MXFP4 dequantized on the device."""
+        if info.ggml_type in (GGML_Q8_0, GGML_Q4K, GGML_Q6K, GGML_MXFP4):
             qt = self.load_qtensor(info, device)
             return qt.dequantize().reshape(info.shape)
         raw = self.tensor_data(info)

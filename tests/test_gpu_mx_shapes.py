@@ -215,3 +215,73 @@ def test_mixed_types_are_refused():
     w = weight(1, 64, 64)
     with pytest.raises(QmmError):
         QMatMul(w).forward(torch.zeros(2, 64, device=DEV, dtype=torch.float16))
+
+
+@pytest.mark.parametrize("m", [1, 2, 20])
+def test_attention_output_projection(m):
+    """qmm_prefill_attention_o with an MXFP4 projection: the attention, then the product added to the residual."""
+    heads, kv, hd, max_seq, n = 4, 2, 64, 32, 100
+    h = heads * hd
+    wo = weight(1, n, h)
+    q, kc, vc = (torch.from_numpy(randn(i, *s)).to(DEV) for i, s in enumerate(
+        ((m, h), (kv, max_seq, hd), (kv, max_seq, hd))))
+    L, s, scale = qmm.lib(), qmm._stream(DEV), ctypes.c_float(0.125)
+    att = torch.empty(m, h, device=DEV)
+    qmm._check(L.qmm_prefill_attention(q.data_ptr(), h, kc.data_ptr(), vc.data_ptr(), 3, m, att.data_ptr(), h, heads, kv,
+                                       hd, max_seq, scale, s))
+    res = torch.from_numpy(randn(9, m, n)).to(DEV)
+    x = res.clone()
+    nws = L.qmm_prefill_attention_o_workspace_size(wo.handle, m)
+    ws = torch.empty(nws, dtype=torch.uint8, device=DEV)
+    qmm._check(L.qmm_prefill_attention_o(q.data_ptr(), h, kc.data_ptr(), vc.data_ptr(), 3, m, heads, kv, hd, max_seq,
+                                         scale, wo.handle, x.data_ptr(), n, ws.data_ptr(), nws, s))
+    assert torch.equal(x, QMatMul(wo).forward(att) + res)
+
+
+def test_cache_warming_refuses_the_type():
+    """qmm_decode_rope_attention_warm knows the row bytes of Q4_K and Q6_K only."""
+    w = weight(1, 256, 256)
+    b = torch.zeros(1 << 16, device=DEV)
+    p = [b.data_ptr()] * 5 + [torch.zeros(1, dtype=torch.int32, device=DEV).data_ptr()] + [b.data_ptr()] * 3
+    L = qmm.lib()
+    ws = torch.empty(L.qmm_decode_attention_workspace_size(4, 2, 64, 32), dtype=torch.uint8, device=DEV)
+    assert L.qmm_decode_rope_attention_warm(*p, 4, 2, 64, 32, ctypes.c_float(1), ws.data_ptr(), ws.numel(),
+                                            (ctypes.c_void_p * 1)(w.handle.value), (ctypes.c_int * 1)(0), 1,
+                                            (ctypes.c_int * 1)(1), qmm._stream(DEV)) == 1
+    assert "Q4_K / Q6_K" in qmm.last_error()
+
+
+def test_unaligned_workspaces_are_refused():
+    e, h, f = 4, 64, 96
+    wg, wu, wd = weight(1, e * f, h), weight(2, e * f, h), weight(3, e * h, f)
+    x, lg, y = torch.zeros(20, h, device=DEV), torch.zeros(20, e, device=DEV), torch.zeros(20, e * f, device=DEV)
+    L, s = qmm.lib(), qmm._stream(DEV)
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
+    c = torch.zeros(256, dtype=torch.int32, device=DEV)
+    a, n = ws.data_ptr() + 4, ws.numel() - 4
+    hp, yp = (ctypes.c_void_p * 1)(wg.handle.value), (ctypes.c_void_p * 1)(y.data_ptr())
+    fg, fu, fd = weight(4, f, h), weight(5, f, h), weight(6, h, f)
+    calls = [
+        (L.qmm_matmul, wg.handle, x.data_ptr(), 20, h, y.data_ptr(), e * f),
+        (L.qmm_linear, wg.handle, x.data_ptr(), 0, 20, h, None, 0, y.data_ptr(), 0, e * f),
+        (L.qmm_matmul_q, wg.handle, x.data_ptr(), 20, y.data_ptr(), e * f),
+        (L.qmm_ffn, fg.handle, fu.handle, fd.handle, x.data_ptr(), 20, h, None, 0.0, 0, y.data_ptr(), h),
+        (L.qmm_moe_gemm, hp, 1, e, x.data_ptr(), 20, h, 20, c.data_ptr(), c.data_ptr(), yp),
+        (L.qmm_moe_route_scored, lg.data_ptr(), 20, e, 2, 0, None, 1, 1, 1, 1, 1.0, c.data_ptr(), c.data_ptr(),
+         c.data_ptr(), y.data_ptr(), c.data_ptr()),
+        (L.qmm_moe_ffn_scored, x.data_ptr(), 0, 20, h, lg.data_ptr(), e, 2, 0, None, 1, 1, 1, 1, 1.0, wg.handle,
+         wu.handle, wd.handle, None, None, None, None, y.data_ptr(), 0, h)]
+    for fn, *args in calls:
+        assert fn(*args, a, n, s) == 1 and "aligned" in qmm.last_error(), (args, qmm.last_error())
+
+
+def test_gguf_dense_load(tmp_path):
+    import gguf_writer as W
+    from inference_amd.gguf import GgufFile
+    b = mx.to_mxfp4(randn(5, 64, 96))
+    p = tmp_path / "w.gguf"
+    p.write_bytes(W.build([("general.architecture", W.T_STRING, "llama")], [("w", (64, 96), 39, b.tobytes())]))
+    f = GgufFile.open(p)
+    got = f.load_dense(f.tensors[0], DEV)
+    assert got.shape == (64, 96) and got.dtype == torch.float32
+    np.testing.assert_array_equal(got.double().cpu().numpy(), mx.from_mxfp4(b))
