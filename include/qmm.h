@@ -155,9 +155,11 @@ size_t qmm_matmul_workspace_size(const qmm_qtensor *w, int64_t m);
  * quantized to W's vec-dot type first (as Candle's CPU path does).
  * x: f32 [m, k] (row stride ldx); y: f32 [m, n] (row stride ldy); ws: device
  * scratch of qmm_matmul_workspace_size(w, m) bytes (may be NULL for m <= 2,
- * where one kernel quantizes x in its prologue). m = 1..8 runs the decode
+ * where one kernel quantizes x in its prologue; of an MXFP4 weight for k <= 16384,
+ * where the workspace is of 0 bytes). m = 1..8 runs the decode
  * GEMV (replaces launch_mmvq_gguf_quantize_q8_1_f32 + launch_mmvq_gguf_*_f32_plain);
- * larger m runs the GEMM path (replaces launch_mmq_gguf_*). */
+ * larger m runs the GEMM path (replaces launch_mmq_gguf_*). An MXFP4 weight takes
+ * any m and n and k <= 2^21 (a multiple of 32) on kernels of its own. */
 int qmm_matmul(const qmm_qtensor *w, const float *x, int64_t m, int64_t ldx, float *y, int64_t ldy,
                void *ws, size_t ws_bytes, void *stream);
 
@@ -178,7 +180,8 @@ int qmm_matmul_noalloc(const qmm_qtensor *w, const float *x, int64_t m, int64_t 
  * y = x . W^T (+ bias[n]), the sum rounded once to the output's type. x_dtype,
  * bias_dtype and y_dtype are QMM_F32, QMM_F16 or QMM_BF16; bias may be NULL. Rows as
  * for qmm_matmul (the same values, for f32 rows without a bias). ws:
- * qmm_linear_workspace_size(w, m) bytes. */
+ * qmm_linear_workspace_size(w, m) bytes on a 16-byte boundary (0 for m <= 2 and
+ * k <= 16384: NULL). */
 int qmm_linear(const qmm_qtensor *w, const void *x, int x_dtype, int64_t m, int64_t ldx, const void *bias,
                int bias_dtype, void *y, int y_dtype, int64_t ldy, void *ws, size_t ws_bytes, void *stream);
 size_t qmm_linear_workspace_size(const qmm_qtensor *w, int64_t m);

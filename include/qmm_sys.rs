@@ -141,9 +141,11 @@ extern "C" {
     /// quantized to W's vec-dot type first (as Candle's CPU path does).
     /// x: f32 [m, k] (row stride ldx); y: f32 [m, n] (row stride ldy); ws: device
     /// scratch of qmm_matmul_workspace_size(w, m) bytes (may be NULL for m <= 2,
-    /// where one kernel quantizes x in its prologue). m = 1..8 runs the decode
+    /// where one kernel quantizes x in its prologue; of an MXFP4 weight for k <= 16384,
+    /// where the workspace is of 0 bytes). m = 1..8 runs the decode
     /// GEMV (replaces launch_mmvq_gguf_quantize_q8_1_f32 + launch_mmvq_gguf_*_f32_plain);
-    /// larger m runs the GEMM path (replaces launch_mmq_gguf_*).
+    /// larger m runs the GEMM path (replaces launch_mmq_gguf_*). An MXFP4 weight takes
+    /// any m and n and k <= 2^21 (a multiple of 32) on kernels of its own.
     pub fn qmm_matmul(
         w: *const QmmQTensor, x: *const f32, m: i64, ldx: i64, y: *mut f32, ldy: i64, ws: *mut c_void,
         ws_bytes: usize, stream: *mut c_void
@@ -155,7 +157,8 @@ extern "C" {
 
     /// QuantizedLinear::forward over typed rows for MXFP4 weights: y = x . W^T (+ bias[n]), the sum
     /// rounded once to the output's type; x_dtype, bias_dtype and y_dtype are QMM_F32, QMM_F16 or
-    /// QMM_BF16, bias may be NULL. ws: qmm_linear_workspace_size(w, m) bytes.
+    /// QMM_BF16, bias may be NULL. ws: qmm_linear_workspace_size(w, m) bytes on a 16-byte
+    /// boundary (0 for m <= 2 and k <= 16384: NULL).
     pub fn qmm_linear(
         w: *const QmmQTensor, x: *const c_void, x_dtype: c_int, m: i64, ldx: i64, bias: *const c_void,
         bias_dtype: c_int, y: *mut c_void, y_dtype: c_int, ldy: i64, ws: *mut c_void, ws_bytes: usize,
