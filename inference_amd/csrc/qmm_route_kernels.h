@@ -222,7 +222,7 @@ __device__ __forceinline__ void route_lists(const RouteArgs& a, const uint16_t* 
 
 }  // namespace qmm
 
-// Up to 16 tokens of up to 256 experts: one launch, a wave a token.
+// Up to 16 tokens: one launch, a wave a token.
 #define QMM_ROUTE_SMALL(R)                                                                                             \
   extern "C" __global__ void __launch_bounds__(1024) qmm_route_small_r##R(                                        \
       const float* __restrict__ logits, const float* __restrict__ bias, qmm::RouteArgs a, int* __restrict__ counts,  \

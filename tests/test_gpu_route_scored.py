@@ -30,7 +30,8 @@ def check(lg, k, bias=None, **kw):
 
 CASES = [(1, 1, 1, 1, 1, 1), (1, 8, 2, 1, 1, 1), (5, 8, 8, 1, 1, 1), (16, 64, 6, 8, 3, 1), (17, 64, 6, 8, 3, 2),
          (33, 60, 4, 4, 2, 2), (64, 96, 8, 8, 4, 2), (65, 128, 1, 64, 1, 2), (100, 160, 8, 8, 5, 1), (257, 256, 8, 8, 4, 2),
-         (12, 300, 10, 10, 4, 2), (9, 100, 4, 4, 2, 2), (16, 256, 8, 1, 1, 1), (70, 1024, 32, 64, 3, 2),
+         (12, 300, 10, 10, 4, 2), (9, 100, 4, 4, 2, 2), (16, 256, 8, 1, 1, 1), (8, 100, 4, 4, 2, 2),
+         (4, 256, 8, 8, 4, 2), (1, 300, 10, 10, 4, 2), (70, 1024, 32, 64, 3, 2),
          (1000, 16, 4, 1, 1, 1), (3, 7, 3, 7, 3, 1)]
 
 
