@@ -285,3 +285,59 @@ def test_gguf_dense_load(tmp_path):
     got = f.load_dense(f.tensors[0], DEV)
     assert got.shape == (64, 96) and got.dtype == torch.float32
     np.testing.assert_array_equal(got.double().cpu().numpy(), mx.from_mxfp4(b))
+
+
+@pytest.mark.parametrize("t", [1, 2, 5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pad", [0, 3, 8])
+def test_moe_rows_keep_their_padding(t, dtype, pad):
+    """Strided rows in and out of the C call: the Python call's values, nothing written past a row."""
+    e, k, h, f = 6, 3, 96, 160
+    wg, wu, wd = weight(1, e * f, h), weight(2, e * f, h), weight(3, e * h, f)
+    x = torch.from_numpy(randn(t, t, h + pad)).to(dtype).to(DEV)
+    lg = torch.from_numpy(randn(4, t, e)).to(DEV)
+    want = moe_ffn(x[:, :h], lg, wg, wu, wd, k, score="softmax", out_dtype=dtype)
+    L, tag = qmm.lib(), qmm._DENSE[dtype]
+    out = torch.full((t, h + pad), 5.0, dtype=dtype, device=DEV)
+    ws = torch.empty(L.qmm_moe_ffn_scored_workspace_size(wg.handle, wd.handle, t, e, k, None, None, None),
+                     dtype=torch.uint8, device=DEV)
+    qmm._check(L.qmm_moe_ffn_scored(x.data_ptr(), tag, t, h + pad, lg.data_ptr(), e, k, 0, None, 1, 1, 1, 1, 1.0,
+                                    wg.handle, wu.handle, wd.handle, None, None, None, None, out.data_ptr(), tag, h + pad,
+                                    ws.data_ptr(), ws.numel(), qmm._stream(DEV)))
+    assert torch.equal(out[:, :h], want) and bool((out[:, h:] == 5).all())
+
+
+@pytest.mark.parametrize("t", [1, 2])
+def test_moe_token_captured_and_on_two_streams(t):
+    """The decode form: replayed between eager calls on other inputs, and two calls at once."""
+    e, k, h, f = 16, 4, 288, 160
+    wg, wu, wd = weight(1, e * f, h), weight(2, e * f, h), weight(3, e * h, f)
+    bias = torch.from_numpy(randn(6, e, std=0.1)).to(DEV)
+    xs = [torch.from_numpy(randn(s, t, h)).to(DEV).bfloat16() for s in range(3)]
+    ls = [torch.from_numpy(randn(s + 9, t, e)).to(DEV) for s in range(3)]
+
+    def call(x, lg):
+        return moe_ffn(x, lg, wg, wu, wd, k, score="sigmoid", bias=bias, groups=4, topk_groups=2, group_top=2,
+                       out_dtype=torch.bfloat16)
+
+    want = [call(x, lg) for x, lg in zip(xs, ls)]
+    x, lg = xs[0].clone(), ls[0].clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = call(x, lg)
+    for i in (1, 2, 0, 1):
+        x.copy_(xs[i])
+        lg.copy_(ls[i])
+        g.replay()
+        eager = call(xs[(i + 1) % 3], ls[(i + 1) % 3])
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i]) and torch.equal(eager, want[(i + 1) % 3])
+    got = []
+    for i in range(2):
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            got.append(call(xs[i], ls[i]))
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
