@@ -63,11 +63,13 @@ __device__ __forceinline__ void route_token(const float* __restrict__ logits, co
                                             const RouteArgs& a, double* ch, int& expert, float& weight) {
   const int lane = threadIdx.x & 63;
   double s[R], c[R];
+  float add[R];  // (asked for together with the logits)
   double mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int e = 64 * i + lane;
     float l = e < a.E ? logits[e] : -INFINITY;
+    add[i] = bias != nullptr && e < a.E ? bias[e] : 0.0f;
     l = l != l ? -INFINITY : fminf(l, 3.40282347e38f);
     s[i] = l;
     mx = fmax(mx, s[i]);
@@ -92,7 +94,7 @@ __device__ __forceinline__ void route_token(const float* __restrict__ logits, co
     const int e = 64 * i + lane;
     c[i] = s[i];
     if (bias != nullptr && e < a.E) {
-      const double v = s[i] + (double)bias[e];
+      const double v = s[i] + (double)add[i];
       c[i] = v != v ? -1e300 : fmin(fmax(v, -1e300), 1e300);
     }
     if (e >= a.E) c[i] = -INFINITY;
@@ -186,29 +188,30 @@ constexpr int kRouteMaxK = 32;
 // the number of earlier tokens that selected it (a bit mask of tokens per expert: any
 // order of the ORs gives the same mask).
 __device__ __forceinline__ void route_lists(const RouteArgs& a, const uint16_t* sel_e, const float* sel_w,
-                                            const int* total, int* offs, unsigned* mask, int* __restrict__ counts,
+                                            const int* total, int* offs, int (&sums)[4], unsigned* mask,
+                                            int* __restrict__ counts,
                                             int* __restrict__ offsets, int* __restrict__ pair_token,
                                             float* __restrict__ pair_weight, int* __restrict__ token_pairs) {
   const int t = threadIdx.x;
   if (t < a.E) mask[t] = 0;
-  if (t < 64) {  // exclusive prefix of the totals
-    int base = 0;
-    for (int e0 = 0; e0 < a.E; e0 += 64) {
-      const int e = e0 + t, v = e < a.E ? total[e] : 0;
-      int sum = v;
+  int sum = 0, cnt = 0;  // prefix of the totals: of 64 experts a wave, then of the waves
+  if (t < 256) {
+    sum = cnt = t < a.E ? total[t] : 0;
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int o = __shfl_up(sum, d);
-        if (t >= d) sum += o;
-      }
-      if (e < a.E) offs[e] = base + sum - v;
-      base += route_lane(sum, 63);
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(sum, d);
+      if ((t & 63) >= d) sum += o;
     }
-    if (t == 0) offs[a.E] = base;
+    if ((t & 63) == 63) sums[t >> 6] = sum;
   }
   __syncthreads();
-  if (t <= a.E) offsets[t] = offs[t];
-  if (t < a.E) counts[t] = total[t];
+  if (t < a.E) {
+    for (int i = 0; i < t >> 6; ++i) sum += sums[i];
+    offs[t] = sum - cnt;
+    offsets[t] = sum - cnt;
+    counts[t] = cnt;
+    if (t == a.E - 1) offsets[a.E] = sum;
+  }
   const int i = t / a.k, e = i < a.T ? sel_e[t] : 0;
   if (i < a.T) atomicOr(&mask[e], 1u << i);
   __syncthreads();
@@ -231,7 +234,7 @@ __device__ __forceinline__ void route_lists(const RouteArgs& a, const uint16_t* 
     __shared__ double ch[16][64 * R];                                                                             \
     __shared__ uint16_t sel_e[16 * qmm::kRouteMaxK];                                                              \
     __shared__ float sel_w[16 * qmm::kRouteMaxK];                                                                 \
-    __shared__ int total[64 * R], offs[64 * R + 1];                                                               \
+    __shared__ int total[64 * R], offs[64 * R], sums[4];                                                          \
     __shared__ unsigned mask[64 * R];                                                                             \
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;                                                   \
     for (int e = threadIdx.x; e < a.E; e += 1024) total[e] = 0;                                                   \
@@ -247,7 +250,8 @@ __device__ __forceinline__ void route_lists(const RouteArgs& a, const uint16_t* 
       }                                                                                                           \
     }                                                                                                             \
     __syncthreads();                                                                                              \
-    qmm::route_lists(a, sel_e, sel_w, total, offs, mask, counts, offsets, pair_token, pair_weight, token_pairs);  \
+    qmm::route_lists(a, sel_e, sel_w, total, offs, sums, mask, counts, offsets, pair_token, pair_weight,          \
+                     token_pairs);                                                                                \
   }
 QMM_ROUTE_SMALL(1)
 QMM_ROUTE_SMALL(2)
