@@ -37,34 +37,42 @@ __device__ __forceinline__ double route_row(double v) {
   return __hiloint2double(__builtin_amdgcn_update_dpp(hi, hi, P, 0xf, 0xf, true),
                           __builtin_amdgcn_update_dpp(lo, lo, P, 0xf, 0xf, true));
 }
-template <typename F>
-__device__ __forceinline__ double route_wave(double v, F f) {
+template <int P>
+__device__ __forceinline__ int route_row(int v) {
+  return __builtin_amdgcn_update_dpp(v, v, P, 0xf, 0xf, true);
+}
+template <typename T, typename F>
+__device__ __forceinline__ T route_wave(T v, F f) {
   v = f(v, route_row<0xb1>(v));   // lanes 1 0 3 2 of four
   v = f(v, route_row<0x4e>(v));   // 2 3 0 1
   v = f(v, route_row<0x141>(v));  // eight, mirrored
   v = f(v, route_row<0x140>(v));  // sixteen, mirrored
   return f(f(route_lane(v, 0), route_lane(v, 16)), f(route_lane(v, 32), route_lane(v, 48)));
 }
-__device__ __forceinline__ double route_wave_max(double v) {
-  return route_wave(v, [](double a, double b) { return fmax(a, b); });
+__device__ __forceinline__ int route_wave_max(int v) {
+  return route_wave(v, [](int a, int b) { return max(a, b); });
 }
 __device__ __forceinline__ double route_wave_sum(double v) {
   return route_wave(v, [](double a, double b) { return a + b; });
 }
+// A word whose order as a signed integer is that of a float's bits (its own inverse).
+__device__ __forceinline__ int route_order(int bits) { return bits ^ (bits >> 31 & 0x7fffffff); }
 
-// What bounds it: the f64 exponentials (and quotients) of all experts and the chain of k
-// maxima over the wave. 4096 tokens of 256 experts, 8 of 8 groups' 4 with sigmoid scores:
-// 13.7 us, 16.4 with the maxima, sums and group scores by shuffles.
 // One token by one wave, expert e = 64 i + lane in register i. Lane j < k returns the
 // token's j-th expert in increasing order, and its weight. `ch`: E doubles of LDS, this
 // wave's own.
+//
+// What bounds it: instruction issue, of the f64 exponentials and quotients of all experts,
+// the groups' scores and the k maxima over the wave. 4096 tokens of 256 experts, 8 of 8
+// groups' 4 with sigmoid scores: 12.7 us; 13.5 with 64-bit maxima, 16.4 with maxima, sums
+// and group scores by shuffles.
 template <int R>
 __device__ __forceinline__ void route_token(const float* __restrict__ logits, const float* __restrict__ bias,
                                             const RouteArgs& a, double* ch, int& expert, float& weight) {
   const int lane = threadIdx.x & 63;
   double s[R], c[R];
   float add[R];  // (asked for together with the logits)
-  double mx = -INFINITY;
+  float mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int e = 64 * i + lane;
@@ -72,17 +80,17 @@ __device__ __forceinline__ void route_token(const float* __restrict__ logits, co
     add[i] = bias != nullptr && e < a.E ? bias[e] : 0.0f;
     l = l != l ? -INFINITY : fminf(l, 3.40282347e38f);
     s[i] = l;
-    mx = fmax(mx, s[i]);
+    mx = fmaxf(mx, l);
   }
   if (a.sigmoid) {
 #pragma unroll
     for (int i = 0; i < R; ++i) s[i] = 1.0 / (1.0 + exp(-s[i]));
   } else {
-    mx = route_wave_max(mx);
+    mx = __int_as_float(route_order(route_wave_max(route_order(__float_as_int(mx)))));
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      s[i] = mx == -INFINITY ? 0.0 : exp(s[i] - mx);
+      s[i] = mx == -INFINITY ? 0.0 : exp(s[i] - (double)mx);
       sum += s[i];
     }
     sum = route_wave_sum(sum);
@@ -137,26 +145,52 @@ __device__ __forceinline__ void route_token(const float* __restrict__ logits, co
     }
     __builtin_amdgcn_wave_barrier();
   }
-  // top-k: the largest choice, then the lowest expert that has it
+  // top-k: the largest choice, then the lowest expert that has it. The choices as two words
+  // that are ordered like them: the maximum of the high ones decides but for close choices.
+  int hi[R];
+  unsigned lo[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int b = __double2hiint(c[i]), sign = b >> 31;
+    hi[i] = route_order(b);
+    lo[i] = (unsigned)(__double2loint(c[i]) ^ sign);
+  }
   int mine = 0x7fffffff;  // lane j < k: the j-th selected expert
   double ms = 0.0;        // its score
   for (int j = 0; j < a.k; ++j) {
-    double top = c[0];
+    int high = hi[0];
 #pragma unroll
-    for (int i = 1; i < R; ++i) top = fmax(top, c[i]);
-    top = route_wave_max(top);
+    for (int i = 1; i < R; ++i) high = max(high, hi[i]);
+    high = route_wave_max(high);
+    unsigned long long b[R];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      b[i] = __ballot(hi[i] == high);
+      n += __popcll(b[i]);
+    }
+    if (n > 1) {
+      int low = INT_MIN;  // (unsigned words, their top bit flipped)
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (hi[i] == high) low = max(low, (int)(lo[i] ^ 0x80000000u));
+      low = route_wave_max(low);
+#pragma unroll
+      for (int i = 0; i < R; ++i) b[i] = __ballot(hi[i] == high && (int)(lo[i] ^ 0x80000000u) == low);
+    }
     int e = -1;
     double sc = 0.0;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const unsigned long long b = __ballot(c[i] == top);
-      if (e < 0 && b) {
-        const int l = __builtin_ctzll(b);
+    for (int i = 0; i < R; ++i)
+      if (e < 0 && b[i]) {
+        const int l = __builtin_ctzll(b[i]);
         e = 64 * i + l;
         sc = route_lane(s[i], l);
-        if (lane == l) c[i] = -INFINITY;
+        if (lane == l) {  // below every choice
+          hi[i] = INT_MIN;
+          lo[i] = 0;
+        }
       }
-    }
     if (lane == j) {
       mine = e;
       ms = sc;
@@ -284,7 +318,9 @@ QMM_ROUTE_TOKENS(16)
 // writes its own pairs in the list's order. Every workgroup reads the whole list (2 bytes
 // a selection), 64 selections a thread in flight; no atomics and no other launch. 32768
 // selections of 256 experts: 6.9 us (11.8 by workgroups of 64 tokens that count every
-// expert in LDS; 11.5 with one load of 8 selections after another).
+// expert in LDS; 11.5 with one load of 8 selections after another; 14.4 with ranks by
+// ballots over a wave's neighbouring selections, which is faster only where one expert has
+// nearly all of them).
 extern "C" __global__ void __launch_bounds__(1024) qmm_route_lists(
     qmm::RouteArgs a, const uint16_t* __restrict__ ids, const float* __restrict__ wts, int* __restrict__ counts,
     int* __restrict__ offsets, int* __restrict__ pair_token, float* __restrict__ pair_weight,

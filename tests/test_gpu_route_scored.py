@@ -148,3 +148,16 @@ def test_graph_replays():
             torch.cuda.synchronize()
             for a, b in zip(out, want[i]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n", [16, 100, 256, 300])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("t", [1, 40])
+def test_close_choices_of_either_sign(n, sign, t):
+    """Choices that differ beyond their first 21 significant bits alone, above and below zero, some of them equal."""
+    rng = np.random.default_rng(n)
+    bias = np.float32(sign * 2) + np.float32(sign * 2.0 ** -22) * rng.integers(0, 8, n).astype(np.float32)
+    lg = np.full((t, n), -60, np.float32)
+    lg[:, rng.integers(0, n)] = -59.5
+    check(lg, 6, bias, score="sigmoid")
+    check(lg, 6, bias, score="sigmoid", groups=2, topk_groups=1, group_top=2)
