@@ -112,7 +112,8 @@ int qmm_qtensor_quantize(int dtype, int64_t n, int64_t k, const float *w, void *
 int qmm_qtensor_quantize_from(int dtype, int64_t n, int64_t k, const void *w, int w_dtype, void *stream,
                               qmm_qtensor **out);
 
-/* QTensor::dequantize: n*k f32 into the device buffer `dst`. */
+/* QTensor::dequantize: n*k f32 into the device buffer `dst` (of an MXFP4 tensor on a
+ * 16-byte boundary). */
 int qmm_qtensor_dequantize(const qmm_qtensor *t, float *dst, void *stream);
 
 /* qmm_qtensor_dequantize to a dense [n, k] of out_dtype QMM_F32, QMM_F16 or
@@ -120,7 +121,7 @@ int qmm_qtensor_dequantize(const qmm_qtensor *t, float *dst, void *stream);
  * candle's QTensor::dequantize_f16 and the dequant-dense matmul strategy's
  * weight.dequantize(device).to_dtype(x.dtype) (candle-gen/src/quant/mod.rs:
  * 515-533; QMatMul::forward_via_f16 at candle-gen-lens/src/text_encoder.rs:
- * 518-529). */
+ * 518-529). Of an MXFP4 tensor dst starts on a boundary of four values. */
 int qmm_qtensor_dequantize_to(const qmm_qtensor *t, void *dst, int out_dtype, void *stream);
 
 /* Export the tensor as GGML block bytes (qmm_qtensor_ggml_bytes() of them) into

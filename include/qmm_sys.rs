@@ -105,7 +105,7 @@ extern "C" {
     /// candle's QTensor::dequantize_f16 and the dequant-dense matmul strategy's
     /// weight.dequantize(device).to_dtype(x.dtype) (candle-gen/src/quant/mod.rs:
     /// 515-533; QMatMul::forward_via_f16 at candle-gen-lens/src/text_encoder.rs:
-    /// 518-529).
+    /// 518-529). Of an MXFP4 tensor dst starts on a boundary of four values.
     pub fn qmm_qtensor_dequantize_to(
         t: *const QmmQTensor, dst: *mut c_void, out_dtype: c_int, stream: *mut c_void
     ) -> c_int;

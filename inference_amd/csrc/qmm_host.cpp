@@ -3172,6 +3172,7 @@ static int moe_ffn(const void* xv, int x_dtype, int64_t tokens, int64_t ldx, con
     QMM_TRY(launch(d, "qmm_moe_route_gather_q8k", ceil_div(P * (H / 256), 4), 256, 0, s, args));
   } else if (route.scored) {
     QMM_TRY(check_routing(tokens, experts, topk, route));
+    QMM_TRY(mx_check_ws(ws, ws_bytes, L.total));
     QMM_TRY(route_scored(d, logits, tokens, experts, topk, route, counts, offsets, ptok, pw, tpairs, b + L.route, s));
   } else {
     QMM_TRY(qmm_moe_route_ex(logits, tokens, experts, topk, renormalize, routed_scaling_factor, counts, offsets, ptok,

@@ -111,7 +111,7 @@ def test_route_refusals(L, bad):
 
 def test_route_workspace(L):
     buf = (ctypes.c_uint8 * 64)()
-    assert L.qmm_moe_route_scored_workspace_size(16, 256, 8) == 0
+    assert L.qmm_moe_route_scored_workspace_size(4, 256, 8) == 0 and L.qmm_moe_route_scored_workspace_size(16, 64, 8) == 0
     need = L.qmm_moe_route_scored_workspace_size(17, 256, 8)
     assert need >= 17 * 8 * 6 and L.qmm_moe_route_scored_workspace_size(1, 257, 8) > 0
     assert L.qmm_moe_route_scored_workspace_size(0, 256, 8) == 0
