@@ -341,3 +341,23 @@ def test_moe_token_captured_and_on_two_streams(t):
             got.append(call(xs[i], ls[i]))
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_offsets_past_32_bits():
+    """A weight of 4.6 GB, products of 2.3 G values and a dense form of 8.6 G: the last rows and columns."""
+    n, k, tail = 2100000, 4096, 100
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    b = torch.randint(0, 256, (n, k // 32, 17), dtype=torch.uint8, device=DEV, generator=g)
+    b[..., 0] = 118
+    w = QTensor.from_ggml(b.reshape(-1), MX, (n, k), device=DEV)
+    end = QTensor.from_ggml(b[-tail:].contiguous().reshape(-1), MX, (tail, k), device=DEV)
+    del b
+    v = end.dequantize()
+    assert torch.equal(w.dequantize(torch.bfloat16)[-tail:].float(), v)
+    for m in (1, 5, 20, 1100):
+        x = torch.from_numpy(randn(m, m, k)).to(DEV)
+        y = QMatMul(w).forward(x)
+        check(y[-3:, -tail:], x[-3:], v)
+        del y
+    torch.cuda.empty_cache()
