@@ -2931,12 +2931,12 @@ static int64_t moe_chunk(int topk) { return std::min<int64_t>(4096, 8192 / std::
 // consecutive chunks: 32768 pairs are far more work than reading the weights again).
 struct MxMoeWs {
   size_t counts, offsets, pair_token, pair_weight, token_pairs, route, xp, hp, yp;
-  size_t shared, sg, shared_ws, total;
+  size_t shared, sg, shared_ws, shared_ws_bytes, total;
 };
 static int64_t mx_moe_chunk(int topk) { return std::max<int64_t>(1, 32768 / std::max(topk, 1)); }
 static MxMoeWs mx_moe_ws(const qmm_qtensor* gate, int64_t tokens, int E, int k, const MoeShared& sh) {
   MxMoeWs w = {};
-  const int64_t T = std::min(tokens, mx_moe_chunk(k)), P = T * k, H = gate->k, F = gate->n / E;
+  const int64_t chunk = mx_moe_chunk(k), T = std::min(tokens, chunk), P = T * k, H = gate->k, F = gate->n / E;
   size_t o = 0;
   auto take = [&o](size_t bytes) {
     const size_t at = o;
@@ -2955,7 +2955,11 @@ static MxMoeWs mx_moe_ws(const qmm_qtensor* gate, int64_t tokens, int E, int k, 
   if (sh.gate) {
     w.shared = take(4 * (size_t)T * H);
     w.sg = take(4 * (size_t)T);
-    w.shared_ws = take(qmm_ffn_workspace_size(sh.gate, sh.up, sh.down, T, 0));
+    // (the last chunk's fewer rows may need more: Q4_K / Q6_K products that split K)
+    const int64_t last = tokens > chunk ? tokens % chunk : 0;
+    w.shared_ws_bytes = std::max(qmm_ffn_workspace_size(sh.gate, sh.up, sh.down, T, 0),
+                                 last ? qmm_ffn_workspace_size(sh.gate, sh.up, sh.down, last, 0) : 0);
+    w.shared_ws = take(w.shared_ws_bytes);
   }
   w.total = o;
   return w;
@@ -3033,10 +3037,12 @@ static int moe_gemv_path(Device* d, const MoeWs& L, uint8_t* b, const float* x, 
 // (returned null without one).
 static int moe_shared(Device* d, const MoeShared& sh, const void* x, int x_dtype, int64_t tokens, int64_t ldx, int64_t H,
                       float* out, float** sg, uint8_t* ws, size_t ws_bytes, hipStream_t s) {
-  if (x_dtype == QMM_F32)
+  if (x_dtype == QMM_F32) {
     QMM_TRY(qmm_ffn(sh.gate, sh.up, sh.down, (const float*)x, tokens, ldx, nullptr, 0.0f, 0, out, H, ws, ws_bytes, s));
-  else
+  } else {
+    QMM_TRY(mx_check_ws(ws, ws_bytes, mx_ffn_ws(sh.gate, sh.down, tokens, false).total));
     QMM_TRY(mx_ffn(d, sh.gate, sh.up, sh.down, x, x_dtype, tokens, ldx, nullptr, 0.0f, 0, out, H, ws, s));
+  }
   if (sh.gate_w == nullptr) {
     *sg = nullptr;
     return QMM_OK;
@@ -3080,8 +3086,7 @@ static int mx_moe(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const
     if (sh.gate) {
       shared = (float*)(b + L.shared);
       sg = (float*)(b + L.sg);
-      QMM_TRY(moe_shared(d, sh, xc, x_dtype, T, ldx, H, shared, &sg, b + L.shared_ws,
-                         qmm_ffn_workspace_size(sh.gate, sh.up, sh.down, T, 0), s));
+      QMM_TRY(moe_shared(d, sh, xc, x_dtype, T, ldx, H, shared, &sg, b + L.shared_ws, L.shared_ws_bytes, s));
     }
     int tt = (int)T, k = topk, n = (int)H, ot = out_dtype;
     void* oc = (uint8_t*)out + t0 * ldo * (int64_t)mx_type_size(out_dtype);
