@@ -511,7 +511,7 @@ int qmm_moe_gemm(const qmm_qtensor *const *w, int count, int experts, const floa
  * topk) tokens) runs as consecutive chunks of that many tokens, in stream
  * order through the same workspace; tokens are routed and combined
  * independently, so the result is the whole list's.
- * ws: device scratch of qmm_moe_ffn_workspace_size() bytes (one chunk's). */
+ * ws: device scratch of qmm_moe_ffn_workspace_size() bytes (the largest chunk's). */
 size_t qmm_moe_ffn_workspace_size(const qmm_qtensor *gate, const qmm_qtensor *down, int64_t tokens,
                                   int experts, int topk);
 int qmm_moe_ffn(const float *x, int64_t tokens, int64_t ldx, const float *logits, int experts, int topk,

@@ -499,7 +499,7 @@ extern "C" {
     /// topk) tokens) runs as consecutive chunks of that many tokens, in stream
     /// order through the same workspace; tokens are routed and combined
     /// independently, so the result is the whole list's.
-    /// ws: device scratch of qmm_moe_ffn_workspace_size() bytes (one chunk's).
+    /// ws: device scratch of qmm_moe_ffn_workspace_size() bytes (the largest chunk's).
     pub fn qmm_moe_ffn_workspace_size(
         gate: *const QmmQTensor, down: *const QmmQTensor, tokens: i64, experts: c_int, topk: c_int
     ) -> usize;

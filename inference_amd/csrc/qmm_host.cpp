@@ -2927,6 +2927,15 @@ static int check_moe_shared(const qmm_qtensor* gate, const MoeShared& sh) {
 // outputs are the whole list's.
 static int64_t moe_chunk(int topk) { return std::min<int64_t>(4096, 8192 / std::max(topk, 1)); }
 
+// Workspace of a list of any length: a whole chunk's, or the last chunk's where that is
+// more (its shared expert's products may split K, with a plane of partial sums a split).
+static size_t moe_ws_bytes(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t tokens, int E, int k,
+                           const MoeShared* sh, bool scored) {
+  const int64_t chunk = moe_chunk(k), last = tokens > chunk ? tokens % chunk : 0;
+  const size_t b = moe_ws(gate, down, std::min(tokens, chunk), E, k, sh, scored).total;
+  return last ? std::max(b, moe_ws(gate, down, last, E, k, sh, scored).total) : b;
+}
+
 // MXFP4 experts: workspace of up to mx_moe_chunk(topk) tokens (longer lists run as
 // consecutive chunks: 32768 pairs are far more work than reading the weights again).
 struct MxMoeWs {
@@ -2969,7 +2978,7 @@ size_t qmm_moe_ffn_workspace_size(const qmm_qtensor* gate, const qmm_qtensor* do
                                   int topk) {
   if (!gate || !down || tokens < 1 || experts < 1 || topk < 1) return 0;
   if (is_mx(gate->dtype)) return mx_moe_ws(gate, tokens, experts, topk, MoeShared()).total;
-  return moe_ws(gate, down, std::min(tokens, moe_chunk(topk)), experts, topk).total;
+  return moe_ws_bytes(gate, down, tokens, experts, topk, nullptr, false);
 }
 
 size_t qmm_moe_ffn_ex_workspace_size(const qmm_qtensor* gate, const qmm_qtensor* down, int64_t tokens, int experts,
@@ -2982,7 +2991,7 @@ size_t qmm_moe_ffn_ex_workspace_size(const qmm_qtensor* gate, const qmm_qtensor*
   sh.down = shared_down;
   if (check_moe_shared(gate, sh) != QMM_OK) return 0;
   if (is_mx(gate->dtype)) return mx_moe_ws(gate, tokens, experts, topk, sh).total;
-  return moe_ws(gate, down, std::min(tokens, moe_chunk(topk)), experts, topk, &sh).total;
+  return moe_ws_bytes(gate, down, tokens, experts, topk, &sh, false);
 }
 
 // Decode-sized MoE: gathered Q8_K rows through the expert GEMVs.
@@ -3146,6 +3155,8 @@ static int moe_ffn(const void* xv, int x_dtype, int64_t tokens, int64_t ldx, con
   const float routed_scaling_factor = route.scale;
   const int64_t chunk = moe_chunk(topk);
   if (tokens > chunk) {  // consecutive chunks through the same workspace, in stream order
+    const size_t need = moe_ws_bytes(gate, down, tokens, experts, topk, &sh, route.scored);
+    if (ws_bytes < need) return fail(QMM_ERR_INVALID, "workspace of %zu B < %zu B needed", ws_bytes, need);
     for (int64_t t0 = 0; t0 < tokens; t0 += chunk)
       QMM_TRY(moe_ffn(x + t0 * ldx, QMM_F32, std::min(chunk, tokens - t0), ldx, logits + t0 * experts, experts, topk,
                       route, gate, up, down, sh, out + t0 * ldo, QMM_F32, ldo, ws, ws_bytes, stream));
@@ -3330,7 +3341,7 @@ size_t qmm_moe_ffn_scored_workspace_size(const qmm_qtensor* gate, const qmm_qten
   const MoeShared sh = {shared_gate, shared_up, shared_down, nullptr};
   if (check_moe_shared(gate, sh) != QMM_OK) return 0;
   if (is_mx(gate->dtype)) return mx_moe_ws(gate, tokens, experts, topk, sh).total;
-  return moe_ws(gate, down, std::min(tokens, moe_chunk(topk)), experts, topk, &sh, true).total;
+  return moe_ws_bytes(gate, down, tokens, experts, topk, &sh, true);
 }
 
 int qmm_moe_ffn_scored(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const float* logits, int experts,

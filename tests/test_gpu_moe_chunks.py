@@ -59,3 +59,18 @@ def test_mxfp4_experts_and_a_q4k_shared_expert():
         for a, b in ((0, chunk), (chunk, t)):
             part = moe_ffn(x[a:b], lg[a:b], *w, k, shared=tuple(shared), score="sigmoid" if score else None)
             assert torch.equal(y[a:b], part)
+
+
+@pytest.mark.parametrize("score", [False, True])
+def test_q4k_experts_and_a_wide_shared_expert(score):
+    e, k, h, f, fs, chunk, rest = 8, 1, 512, 256, 8192, 4096, 3584
+    q = (GgmlDType.Q4K, GgmlDType.Q6K)
+    w, shared, g = experts(q, e, h, f, fs, q)
+    L, hs = qmm.lib(), [v.handle for v in shared]
+    size = [L.qmm_moe_ffn_ex_workspace_size(w[0].handle, w[2].handle, t, e, k, *hs) for t in (chunk, rest, chunk + rest)]
+    assert size[1] > size[0] and size[2] == size[1]
+    t = chunk + rest
+    x, lg = torch.randn(t, h, generator=g, device=DEV), torch.randn(t, e, generator=g, device=DEV)
+    y = guarded_call(x, lg, k, w, shared, score)
+    for a, b in ((0, chunk), (chunk, t)):
+        assert torch.equal(y[a:b], moe_ffn(x[a:b], lg[a:b], *w, k, shared=tuple(shared), score="sigmoid" if score else None))

@@ -81,6 +81,33 @@ def check_mxfp4(so):
     assert last < whole  # (and a case in which the full chunk is the larger one)
 
 
+def check_other_types(so):
+    host = Host(so)
+    L = host.L
+    e = 8
+    for topk, hidden, ffn, chunk, rest, more in ((1, 512, 8192, 4096, 3584, True), (8, 2048, 8192, 1024, 896, True),
+                                                 (4, 1024, 8192, 2048, 1792, True), (2, 2048, 1024, 4096, 976, False)):
+        x = [host.weight(*s) for s in ((Q4K, e * 256, hidden), (Q4K, e * 256, hidden), (Q6K, e * hidden, 256))]
+        shared = [host.weight(*s) for s in ((Q4K, ffn, hidden), (Q4K, ffn, hidden), (Q6K, hidden, ffn))]
+        whole, last = (L.qmm_moe_ffn_ex_workspace_size(x[0], x[2], ctypes.c_int64(t), e, topk, *shared) for t in (chunk, rest))
+        assert (last > whole) == more
+        for t in (chunk, chunk + rest, 2 * chunk + rest):
+            args = (x[0], x[2], ctypes.c_int64(t), e, topk)
+            for score, size in ((True, L.qmm_moe_ffn_scored_workspace_size), (False, L.qmm_moe_ffn_ex_workspace_size)):
+                total = size(*args, *shared)
+                rc, names = host.call(t, e, topk, hidden, x, shared, score, total)
+                assert rc == 0, (topk, t, score, L.qmm_last_error())
+                assert names.count("qmm_moe_combine") == -(-t // chunk)
+                assert host.call(t, e, topk, hidden, x, shared, score, total - 1) == (1, [])
+        # without a shared expert a whole chunk's workspace covers every shorter one
+        total = L.qmm_moe_ffn_workspace_size(*args)
+        assert total == L.qmm_moe_ffn_workspace_size(x[0], x[2], ctypes.c_int64(chunk), e, topk)
+        for score in (False, True):
+            total = (L.qmm_moe_ffn_scored_workspace_size if score else L.qmm_moe_ffn_ex_workspace_size)(*args, *(None,) * 3)
+            assert host.call(t, e, topk, hidden, x, (None,) * 3, score, total)[0] == 0
+            assert host.call(t, e, topk, hidden, x, (None,) * 3, score, total - 1) == (1, [])
+
+
 def run(check, so):
     """A check of this file in a process of its own: the stand-in must not meet a GPU's runtime."""
     code = f"import sys; sys.path.insert(0, {HERE!r}); import test_moe_workspace as t; t.{check}({so!r})"
@@ -90,3 +117,7 @@ def run(check, so):
 
 def test_mxfp4_experts_with_a_shared_expert_of_another_type(runtime):
     run("check_mxfp4", runtime)
+
+
+def test_other_experts_with_a_shared_expert(runtime):
+    run("check_other_types", runtime)
