@@ -434,7 +434,8 @@ class QMatMul:
             L = lib()
             h = qt.handle
             ws, ws_bytes, ws_ptr = None, 0, None
-            if m > 2 or k > 16384:  # one and two rows are quantized in the GEMV's prologue
+            # one and two rows are quantized in the GEMV's prologue (an MXFP4 weight's up to 16384 values)
+            if m > 2 or (k > 16384 and qt._dtype == GgmlDType.MXFP4):
                 ws_bytes = int(L.qmm_matmul_workspace_size(h, m))
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
                 ws_ptr = ws.data_ptr()
