@@ -145,10 +145,11 @@ class LlamaWeights:
         crates/llm/candle-llm/src/gguf.rs:63-170, without its dequantize -> re-quantize): projections
         go straight into device QTensors (q/k rows un-permuted from llama.cpp's order on the quantized
         rows), the token embedding is dequantized to f32 on the device, norms are read as f32, and a
-        missing output.weight ties the head to the embedding's quantized tensor. The configuration
+        missing output.weight ties the head to the embedding's quantized tensor (an MXFP4 head is
+        refused; an MXFP4 embedding with a head of its own is not). The configuration
         follows reconstruct_config (gguf.rs:361-428): absent llama3 RoPE-scaling keys mean standard
         RoPE (factor 1)."""
-        from .gguf import GgufFile, GGML_Q4K, GGML_Q6K
+        from .gguf import GgufFile, GGML_MXFP4, GGML_Q4K, GGML_Q6K
         f = path if isinstance(path, GgufFile) else GgufFile.open(path)
         arch = f.meta_str("general.architecture")
         if arch != "llama":
@@ -167,6 +168,11 @@ class LlamaWeights:
         infos = {t.name: t for t in f.tensors}
         if "token_embd.weight" not in infos:
             raise qmm.QmmError(qmm.QMM_ERR_INVALID, "gguf: no token embedding tensor")
+        emb_info = infos["token_embd.weight"]
+        head_info = infos.get("output.weight", emb_info)
+        if head_info.ggml_type == GGML_MXFP4:  # (a step gives the head no workspace for its normalised row)
+            raise qmm.QmmError(qmm.QMM_ERR_UNSUPPORTED,
+                               f"gguf: the head's {head_info.name} has GGML type {GGML_MXFP4} (MXFP4 heads are not taken)")
         low = f.meta_f64(f"{arch}.rope.scaling.low_freq_factor")
         high = f.meta_f64(f"{arch}.rope.scaling.high_freq_factor")
         llama3 = f.meta_str(f"{arch}.rope.scaling.type") == "llama3" or low is not None or high is not None
@@ -199,9 +205,7 @@ class LlamaWeights:
             layers.append(lw)
             attn_norm.append(f.load_dense(tensor(f"blk.{li}.attn_norm.weight"), device).float())
             ffn_norm.append(f.load_dense(tensor(f"blk.{li}.ffn_norm.weight"), device).float())
-        emb_info = infos["token_embd.weight"]
         embed = f.load_dense(emb_info, device).float().contiguous()
-        head_info = infos.get("output.weight", emb_info)
         head = f.load_qtensor(head_info, device)
         cfg.dtypes = {k: v.dtype() for k, v in layers[0].items()}
         cfg.dtypes["head"] = head.dtype()
