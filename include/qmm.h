@@ -469,7 +469,9 @@ int qmm_moe_route_ex(const float *logits, int64_t tokens, int experts, int topk,
  *   top-k  the topk largest choices that remain. Ties: the lower expert.
  *   weight s, divided by the selection's sum when `renormalize` (0 where that sum is 0),
  *          times routed_scaling_factor.
- * Scores are held in 64 bits, so close experts are ordered as the exact scores are.
+ * Scores are held in 64 bits: choices that lie further apart than a rounding to 64 bits
+ * are ordered as the exact ones are. Sigmoid scores near 1 are steps of 2^-53, and equal
+ * to 1 for logits above 36.8 (0 for those below -709.8): such experts tie.
  * Limits: tokens <= 65536, experts <= 1024, topk <= min(32, experts), groups <= 64.
  * ws: qmm_moe_route_scored_workspace_size(...) bytes (0: NULL allowed). */
 size_t qmm_moe_route_scored_workspace_size(int64_t tokens, int experts, int topk);

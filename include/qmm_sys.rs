@@ -450,7 +450,8 @@ extern "C" {
 
     /// Routing with softmax or sigmoid scores (QMM_SCORE_*), a balance bias (f32 [experts] or NULL;
     /// it selects and does not weigh), groups of experts and scaled weights; the same lists as
-    /// qmm_moe_route. Scores are held in 64 bits. Limits: tokens <= 65536, experts <= 1024,
+    /// qmm_moe_route. Scores are held in 64 bits (sigmoid scores are 1 for logits above 36.8: such
+    /// experts tie, and the lower one goes first). Limits: tokens <= 65536, experts <= 1024,
     /// topk <= min(32, experts), groups <= 64.
     pub fn qmm_moe_route_scored_workspace_size(tokens: i64, experts: c_int, topk: c_int) -> usize;
 

@@ -647,7 +647,8 @@ def moe_route(logits: torch.Tensor, topk: int, renormalize: bool = True, routed_
     With `score` ("softmax" or "sigmoid") the routing is qmm_moe_route_scored's: the choice is score + bias
     (f32 [experts]), limited to the topk_groups (default: all) of `groups` runs of experts whose group_top
     (1 or 2) best choices sum highest; weights are the scores themselves, renormalised if asked, and times
-    routed_scaling_factor in either case. Scores are held in 64 bits."""
+    routed_scaling_factor in either case. Scores are held in 64 bits (sigmoid scores are 1 for logits above
+    36.8); ties go to the lower expert."""
     if logits.dim() != 2:
         raise QmmError(QMM_ERR_INVALID, f"router logits must be [tokens, experts], got {tuple(logits.shape)}")
     t, e = logits.shape
