@@ -698,6 +698,9 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, gate: QTensor, up: QTensor, d
         raise QmmError(QMM_ERR_INVALID, f"moe_ffn to {out_dtype}: float32, float16 or bfloat16")
     if score is None and (bias is not None or groups != 1 or topk_groups is not None or group_top != 1):
         raise QmmError(QMM_ERR_INVALID, "a routing bias or groups need a score (softmax, sigmoid)")
+    if shared_gate is not None and (shared_gate.numel() != x.shape[-1] or shared_gate.device != x.device):
+        raise QmmError(QMM_ERR_INVALID, f"the shared expert's gate must be [{x.shape[-1]}] on {x.device}, got "
+                                        f"{tuple(shared_gate.shape)} on {shared_gate.device}")
     mx = gate.dtype() == GgmlDType.MXFP4
     if mx or score is not None:
         return _moe_ffn_scored(x, logits, gate, up, down, topk, norm_topk_prob, routed_scaling_factor, shared,
