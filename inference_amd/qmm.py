@@ -705,9 +705,14 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, gate: QTensor, up: QTensor, d
     if mx or score is not None:
         return _moe_ffn_scored(x, logits, gate, up, down, topk, norm_topk_prob, routed_scaling_factor, shared,
                                shared_gate, score, bias, groups, topk_groups, group_top, out_dtype)
+    if x.dim() != 2 or logits.dim() != 2 or logits.shape[0] < x.shape[0] or x.shape[1] != gate.shape[1]:
+        raise QmmError(QMM_ERR_INVALID, f"moe_ffn: rows {tuple(x.shape)}, logits {tuple(logits.shape)}, experts of "
+                                        f"width {gate.shape[1]}")
     t, hdim = x.shape
     e = logits.shape[1]
     dev = x.device
+    if logits.device != dev:
+        raise QmmError(QMM_ERR_INVALID, f"rows on {dev}, logits on {logits.device}")
     xx = x.to(torch.float32).contiguous()
     lg = logits.to(torch.float32).contiguous()
     out = torch.empty((t, hdim), dtype=torch.float32, device=dev)

@@ -1,4 +1,5 @@
-"""moe_ffn refuses operands that its kernels would read past, before any call of the library."""
+"""moe_ffn refuses operands that its kernels would read past, before any call of the library: fewer rows of logits than
+tokens, rows of another width than the experts', a shared expert's gate of another length or device."""
 from types import SimpleNamespace
 
 import pytest
@@ -16,7 +17,8 @@ def stack(dtype, n, k):
 @pytest.mark.parametrize("dtype", [GgmlDType.Q4K, GgmlDType.Q8_0, GgmlDType.MXFP4])
 @pytest.mark.parametrize("score", [None, "sigmoid"])
 @pytest.mark.parametrize("case,match", [
-    (dict(gate=(H - 1,)), "gate must"),
+    (dict(x=(T, H + 256)), "rows"), (dict(x=(T, H - 32)), "rows"), (dict(x=(H,)), "rows"), (dict(logits=(T - 1, E)), "logits"),
+    (dict(logits=(T * E,)), "logits"), (dict(logits_device="meta"), "logits on meta"), (dict(gate=(H - 1,)), "gate must"),
     (dict(gate=(H + 1,)), "gate must"), (dict(gate=(0,)), "gate must"), (dict(gate=(H,), gate_device="meta"), "gate must")])
 def test_refused_on_the_host(monkeypatch, dtype, score, case, match):
     def lib():
