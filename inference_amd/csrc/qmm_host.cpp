@@ -1432,7 +1432,6 @@ static int multi_launch(Device* d, const qmm_qtensor* const* w, const MultiPlan&
   return launch(d, "qmm_mmqs_multi", (unsigned)start, 512, lds, s, args);
 }
 
-// Shared by qmm_matmul / qmm_matmul_multi: x f32 [m, k] against `count` weights.
 // One or more MXFP4 weights over typed rows: RMSNorm (f32 rows) if asked, the digit
 // planes in the workspace, then a product per weight. Up to two rows are quantized in
 // the product's own launch and need no workspace.
@@ -1463,6 +1462,7 @@ static int mx_targets(const GemvTarget* tg, int count, const void* x, int x_dtyp
   return QMM_OK;
 }
 
+// Shared by qmm_matmul / qmm_matmul_multi: x f32 [m, k] against `count` weights.
 static int matmul_targets(const GemvTarget* tg, int count, const float* x, int64_t m, int64_t ldx, void* ws,
                           size_t ws_bytes, void* stream, const float* norm_w = nullptr, float eps = 0.0f,
                           int accumulate = 0) {

@@ -69,8 +69,9 @@ int mx_wide16(const void* y, int dtype, int64_t ldy) {
   return (uintptr_t)y % 16 == 0 && ldy * (int64_t)mx_type_size(dtype) % 16 == 0;
 }
 
-// Activation limits: a workgroup's rows are reached by 32-bit offsets (nine 32-row
-// tiles of the planes), a grid has fewer than 2^31 units.
+// Activation limits: a workgroup's rows are reached by 32-bit offsets (128 rows, five
+// 32-row tiles of the planes where routed rows do not start on one: 514 MB of 2^21
+// columns), and a grid has fewer than 2^31 units.
 int mx_check_rows(int64_t m, int64_t k) {
   if (m > (1LL << 21) || k > (1LL << 21) || (m + kMxTile - 1) / kMxTile * mx_chunks(k) > (1LL << 30))
     return fail(QMM_ERR_INVALID, "activation of %lld x %lld is too large", (long long)m, (long long)k);
@@ -337,12 +338,12 @@ int check_routing(int64_t tokens, int experts, int topk, const Routing& r) {
   return QMM_OK;
 }
 
-// (one launch up to 16 tokens of up to 256 experts)
 // Registers of 64 experts that a wave holds.
 int route_regs(int experts) { return experts <= 64 ? 1 : experts <= 128 ? 2 : experts <= 256 ? 4 : 16; }
-// One launch on one CU, or the selections on all and then the lists: 16 tokens of 64
-// experts 7.9 us against 7.5, 8 of 128 7.6 against 8.8, 16 of 128 10.1 against 8.8, 4 of 256
-// 9.0 against 10.5, 16 of 256 12.9 against 10.5.
+// One launch on one CU (16 tokens of up to 64 experts, 8 of 128, 4 of 256), or the
+// selections on all and then the lists: 16 tokens of 64 experts 7.9 us against 7.5, 8 of
+// 128 7.6 against 8.8, 16 of 128 10.1 against 8.8, 4 of 256 9.0 against 10.5, 16 of 256
+// 12.9 against 10.5.
 bool route_is_small(int64_t tokens, int experts) {
   return experts <= 256 && tokens * route_regs(experts) <= kRouteSmall;
 }

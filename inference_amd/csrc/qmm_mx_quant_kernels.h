@@ -201,39 +201,19 @@ __device__ __forceinline__ void mx_dequantize(const uint8_t* __restrict__ w, int
   }
 }
 
-// 32 consecutive values of a typed row. `wide`: the row starts on a 16-byte boundary.
-template <int T>
-__device__ __forceinline__ uint32_t mx_load_block(const void* __restrict__ row, long long at, bool wide, float (&x)[32]) {
+// 32 consecutive f32 values. `wide`: they start on a 16-byte boundary.
+__device__ __forceinline__ uint32_t mx_load_block(const float* __restrict__ p, bool wide, float (&x)[32]) {
   uint32_t amax = 0;
-  if constexpr (T == kF32) {
-    const float* p = static_cast<const float*>(row) + at;
-    if (wide) {
+  if (wide) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const mx_f32x4 v = reinterpret_cast<const mx_f32x4*>(p)[j];
+    for (int j = 0; j < 8; ++j) {
+      const mx_f32x4 v = reinterpret_cast<const mx_f32x4*>(p)[j];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * j + i] = v[i];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] = p[j];
+      for (int i = 0; i < 4; ++i) x[4 * j + i] = v[i];
     }
   } else {
-    const uint16_t* p = static_cast<const uint16_t*>(row) + at;
-    auto f = [](uint32_t v) {
-      return T == kF16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)v) : bf16_to_f32((uint16_t)v);
-    };
-    if (wide) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const mx_u32x4 v = reinterpret_cast<const mx_u32x4*>(p)[j];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[8 * j + i] = f(v[i >> 1] >> (16 * (i & 1)) & 0xffffu);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] = f(p[j]);
-    }
+    for (int j = 0; j < 32; ++j) x[j] = p[j];
   }
 #pragma unroll
   for (int j = 0; j < 32; ++j) amax = max(amax, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
@@ -302,7 +282,7 @@ extern "C" __global__ void __launch_bounds__(256) qmm_mx_quantize_rows(const flo
   if (i >= (long long)m * nb) return;
   float v[32];
   qmm::mx_u32x6 hi, lo;
-  const int e = qmm::mx_x_byte(qmm::mx_load_block<qmm::kF32>(x, i / nb * ldx + 32 * (i % nb), wide != 0, v));
+  const int e = qmm::mx_x_byte(qmm::mx_load_block(x + i / nb * ldx + 32 * (i % nb), wide != 0, v));
   qmm::mx_digits(v, e, hi, lo);
   uint8_t* o = xq + i * qmm::kMxFp6x2Bytes;
   o[0] = (uint8_t)e;

@@ -12,7 +12,8 @@
 // Scores are formed in 64 bits. Experts' scores are close together (256 of them in
 // [0, 1]), a token in a few thousand has two within an f32 rounding of each other at
 // its top-k border, and the list must not hang on which exponential made them; the
-// f64 work is a few microseconds of a few thousand tokens'.
+// f64 work is a few microseconds of a few thousand tokens'. Sigmoid scores of logits
+// above 53 ln 2 = 36.74 are 1 in 64 bits as well, and tie.
 #pragma once
 
 #include "qmm_mx_common.h"
@@ -259,7 +260,7 @@ __device__ __forceinline__ void route_lists(const RouteArgs& a, const uint16_t* 
 
 }  // namespace qmm
 
-// Up to 16 tokens: one launch, a wave a token.
+// Up to 16 tokens, and fewer of more experts (route_is_small): one launch, a wave a token.
 #define QMM_ROUTE_SMALL(R)                                                                                             \
   extern "C" __global__ void __launch_bounds__(1024) qmm_route_small_r##R(                                        \
       const float* __restrict__ logits, const float* __restrict__ bias, qmm::RouteArgs a, int* __restrict__ counts,  \
