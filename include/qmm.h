@@ -160,7 +160,7 @@ size_t qmm_matmul_workspace_size(const qmm_qtensor *w, int64_t m);
  * where the workspace is of 0 bytes). m = 1..8 runs the decode
  * GEMV (replaces launch_mmvq_gguf_quantize_q8_1_f32 + launch_mmvq_gguf_*_f32_plain);
  * larger m runs the GEMM path (replaces launch_mmq_gguf_*). An MXFP4 weight takes
- * any m and n and k <= 2^21 (a multiple of 32) on kernels of its own. */
+ * m and k up to 2^21 (k a multiple of 32) and any n, on kernels of its own. */
 int qmm_matmul(const qmm_qtensor *w, const float *x, int64_t m, int64_t ldx, float *y, int64_t ldy,
                void *ws, size_t ws_bytes, void *stream);
 
@@ -203,14 +203,16 @@ int qmm_matmul_multi(const qmm_qtensor *const *w, int count, const float *x, int
 /* Bytes of workspace the pre-quantized entry points below need for m
  * activation rows: 0 for m <= 8 (the GEMV reads the GGML blocks as they are);
  * for m > 8 the GEMM's activation planes plus, when the weight's output tiles
- * cover fewer than half the CUs, f32 split-K partials. The workspace is the
+ * cover fewer than half the CUs, f32 split-K partials; of an MXFP4 weight the
+ * rows' digits at any m, on a 16-byte boundary. The workspace is the
  * caller's: calls on different streams need different workspaces. */
 size_t qmm_matmul_q_workspace_size(const qmm_qtensor *w, int64_t m);
 
 /* The same with activations already quantized (xq: m rows of vec-dot blocks,
  * as produced by qmm_quantize_rows). For m > 8 the rows are rearranged for
  * the GEMM into `ws` (qmm_matmul_q_workspace_size(w, m) bytes; NULL allowed
- * for m <= 8). A workspace smaller than the planes is an error; one that holds
+ * for m <= 8, but not of an MXFP4 weight). A workspace smaller than the planes
+ * is an error; one that holds
  * the planes but not the split-K partials runs the GEMM unsplit (same block
  * dots, another f32 summation order). */
 int qmm_matmul_q(const qmm_qtensor *w, const void *xq, int64_t m, float *y, int64_t ldy, void *ws, size_t ws_bytes,
@@ -226,7 +228,7 @@ int qmm_matmul_multi_q(const qmm_qtensor *const *w, int count, const void *xq, i
                        const int64_t *ldy, void *ws, size_t ws_bytes, void *stream);
 
 /* qmm_matmul_q with an optional residual add (accumulate != 0: y += result;
- * then m <= 8). */
+ * then m <= 8, or any m of an MXFP4 weight). */
 int qmm_matmul_q_ex(const qmm_qtensor *w, const void *xq, int64_t m, float *y, int64_t ldy, int accumulate,
                     void *ws, size_t ws_bytes, void *stream);
 
@@ -263,7 +265,8 @@ int qmm_matmul_grouped(const qmm_qtensor *const *w, const int *group, int count,
  * quantization prologue for m <= 2), and when `accumulate` is set the result
  * is added to y (the residual add of llama.rs:958-975). ws: device scratch of
  * qmm_matmul_ex_workspace_size(w[j], m, norm_weight != NULL) bytes, the
- * largest over the weights (m > 2 runs one pass per dtype). */
+ * largest over the weights (m > 2 runs one pass per dtype; of MXFP4 weights
+ * the normalised rows need it at any m). */
 int qmm_matmul_ex(const qmm_qtensor *const *w, int count, const float *x, int64_t m, int64_t ldx,
                   const float *norm_weight, float eps, int accumulate, float *const *y, const int64_t *ldy,
                   void *ws, size_t ws_bytes, void *stream);
@@ -273,7 +276,9 @@ size_t qmm_matmul_ex_workspace_size(const qmm_qtensor *w, int64_t m, int normali
  * llama.rs:1385-1392, after the block's RMSNorm, nn.rs:22-31): with n = x
  * RMS-normalised by norm_weight (or x itself when norm_weight is NULL),
  * y (+)= down(silu(gate(n)) * up(n)); y may be x (the residual add). gate and
- * up share shape and k; down's k is their n; every weight Q4_K or Q6_K. At
+ * up share shape and k; down's k is their n; every weight Q4_K or Q6_K, or
+ * all three MXFP4 (silu(g) * u then becomes MXFP6X2 digits without a rounding
+ * in between, at any m in two or three launches after the norm). At
  * m > 8 the gate and up GEMMs leave their split-K partials unsummed and one
  * launch sums them (in split order), forms silu(g) * u and writes the down
  * GEMM's Q8_K planes: the same values as qmm_matmul_ex, qmm_silu_mul and
@@ -498,7 +503,8 @@ int qmm_moe_gemv(const qmm_qtensor *const *w, int count, int experts, const void
  * expert's rows go through the int8 MFMA GEMM against its weight slice.
  * max_rows bounds every count (e.g. the token count for top-k routing).
  * Outputs equal qmm_matmul's GEMM path on each expert's rows bit for bit.
- * ws: qmm_moe_gemm_workspace_size(w[0], pairs) bytes; k % 256 == 0. */
+ * ws: qmm_moe_gemm_workspace_size(w[0], pairs) bytes; k % 256 == 0 (MXFP4
+ * experts: k % 32 == 0, and up to 2^21 pairs). */
 size_t qmm_moe_gemm_workspace_size(const qmm_qtensor *w, int64_t pairs);
 int qmm_moe_gemm(const qmm_qtensor *const *w, int count, int experts, const float *x, int64_t pairs, int64_t ldx,
                  int64_t max_rows, const int32_t *counts, const int32_t *offsets, float *const *y, void *ws,
@@ -548,7 +554,10 @@ int qmm_moe_ffn_ex(const float *x, int64_t tokens, int64_t ldx, const float *log
  * silu(gate(x)) * up(x) become MXFP6X2 digits without a rounding in between; other
  * experts take f32 and qmm_moe_ffn's limits. ws:
  * qmm_moe_ffn_scored_workspace_size(...) bytes. (qmm_moe_ffn and qmm_moe_ffn_ex take
- * MXFP4 experts too, routed as score QMM_SCORE_SOFTMAX with one group.) */
+ * MXFP4 experts too, routed as score QMM_SCORE_SOFTMAX with one group.)
+ * MXFP4 experts' lists run as chunks of 32768 / topk tokens. One or two tokens (a call's,
+ * or a last chunk's) add up a token's experts in another order than more do, in f32 too:
+ * a token's row may then differ in its last bits from the same token's in a longer list. */
 size_t qmm_moe_ffn_scored_workspace_size(const qmm_qtensor *gate, const qmm_qtensor *down, int64_t tokens,
                                          int experts, int topk, const qmm_qtensor *shared_gate,
                                          const qmm_qtensor *shared_up, const qmm_qtensor *shared_down);

@@ -145,7 +145,7 @@ extern "C" {
     /// where the workspace is of 0 bytes). m = 1..8 runs the decode
     /// GEMV (replaces launch_mmvq_gguf_quantize_q8_1_f32 + launch_mmvq_gguf_*_f32_plain);
     /// larger m runs the GEMM path (replaces launch_mmq_gguf_*). An MXFP4 weight takes
-    /// any m and n and k <= 2^21 (a multiple of 32) on kernels of its own.
+    /// m and k up to 2^21 (k a multiple of 32) and any n, on kernels of its own.
     pub fn qmm_matmul(
         w: *const QmmQTensor, x: *const f32, m: i64, ldx: i64, y: *mut f32, ldy: i64, ws: *mut c_void,
         ws_bytes: usize, stream: *mut c_void
@@ -192,7 +192,7 @@ extern "C" {
     /// The same with activations already quantized (xq: m rows of vec-dot blocks,
     /// as produced by qmm_quantize_rows). For m > 8 the rows are rearranged for
     /// the GEMM into `ws` (qmm_matmul_q_workspace_size(w, m) bytes; NULL allowed
-    /// for m <= 8). A workspace smaller than the planes is an error; one that holds
+    /// for m <= 8, but not of an MXFP4 weight). A workspace smaller than the planes is an error; one that holds
     /// the planes but not the split-K partials runs the GEMM unsplit (same block
     /// dots, another f32 summation order).
     pub fn qmm_matmul_q(
@@ -212,7 +212,7 @@ extern "C" {
     ) -> c_int;
 
     /// qmm_matmul_q with an optional residual add (accumulate != 0: y += result;
-    /// then m <= 8).
+    /// then m <= 8, or any m of an MXFP4 weight).
     pub fn qmm_matmul_q_ex(
         w: *const QmmQTensor, xq: *const c_void, m: i64, y: *mut f32, ldy: i64, accumulate: c_int,
         ws: *mut c_void, ws_bytes: usize, stream: *mut c_void
@@ -239,7 +239,8 @@ extern "C" {
     /// quantization prologue for m <= 2), and when `accumulate` is set the result
     /// is added to y (the residual add of llama.rs:958-975). ws: device scratch of
     /// qmm_matmul_ex_workspace_size(w[j], m, norm_weight != NULL) bytes, the
-    /// largest over the weights (m > 2 runs one pass per dtype).
+    /// largest over the weights (m > 2 runs one pass per dtype; of MXFP4 weights
+    /// the normalised rows need it at any m).
     /// Several `QMatMul::forward` calls at m = 1 on two independent rows in one launch (results equal
     /// `qmm_matmul` on each weight bit for bit).
     pub fn qmm_matmul_grouped(
@@ -259,7 +260,8 @@ extern "C" {
     /// llama.rs:1385-1392, after the block's RMSNorm, nn.rs:22-31): with n = x
     /// RMS-normalised by norm_weight (or x itself when norm_weight is NULL),
     /// y (+)= down(silu(gate(n)) * up(n)); y may be x (the residual add). gate and
-    /// up share shape and k; down's k is their n; every weight Q4_K or Q6_K. At
+    /// up share shape and k; down's k is their n; every weight Q4_K or Q6_K, or
+    /// all three MXFP4 (kernels of their own, any m). At
     /// m > 8 the gate and up GEMMs leave their split-K partials unsummed and one
     /// launch sums them (in split order), forms silu(g) * u and writes the down
     /// GEMM's Q8_K planes: the same values as qmm_matmul_ex, qmm_silu_mul and
@@ -482,7 +484,8 @@ extern "C" {
     /// expert's rows go through the int8 MFMA GEMM against its weight slice.
     /// max_rows bounds every count (e.g. the token count for top-k routing).
     /// Outputs equal qmm_matmul's GEMM path on each expert's rows bit for bit.
-    /// ws: qmm_moe_gemm_workspace_size(w[0], pairs) bytes; k % 256 == 0.
+    /// ws: qmm_moe_gemm_workspace_size(w[0], pairs) bytes; k % 256 == 0 (MXFP4
+    /// experts: k % 32 == 0, and up to 2^21 pairs).
     pub fn qmm_moe_gemm_workspace_size(w: *const QmmQTensor, pairs: i64) -> usize;
 
     pub fn qmm_moe_gemm(

@@ -693,7 +693,8 @@ def moe_ffn(x: torch.Tensor, logits: torch.Tensor, gate: QTensor, up: QTensor, d
     tokens, the weighted outputs summed in expert order; then `shared` = (gate, up, down) QTensors of the
     always-on shared expert, added after the routed sum, scaled per token by sigmoid(x . shared_gate)
     when shared_gate (f32 [hidden]) is given. `score`, `bias` and the groups route as in moe_route; the
-    result is of out_dtype. MXFP4 experts read f16 and bf16 rows as they are and round the sum once."""
+    result is of out_dtype. MXFP4 experts read f16 and bf16 rows as they are and round the sum once; one or two
+    tokens sum their experts in another f32 order than longer lists (last bits may differ)."""
     if out_dtype not in _DENSE:
         raise QmmError(QMM_ERR_INVALID, f"moe_ffn to {out_dtype}: float32, float16 or bfloat16")
     if score is None and (bias is not None or groups != 1 or topk_groups is not None or group_top != 1):
