@@ -570,6 +570,126 @@ int qmm_moe_ffn_scored(const void *x, int x_dtype, int64_t tokens, int64_t ldx, 
                        size_t ws_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * A key/value cache in pages, for several sequences that share pages, and the
+ * operators over it. The reference engine keeps pages on the host's side of its
+ * attention (crates/llm/candle-llm/src/primitives/paged_kv_cache.rs); these calls
+ * have no counterpart there.
+ *
+ * Position j of a sequence is row j % page_size of page table[slot][j / page_size].
+ * A page may stand in several table rows; refs[p] counts the entries that name page p
+ * (a caller that holds a page for a reason of its own adds one). The entries of a row
+ * outside [0, pages) name no page (-1 by convention). Every layer uses the same ids.
+ * The lists are read on the device, by each call as it runs: nothing is read back, and
+ * a captured call replays with the lists' values then.
+ * ------------------------------------------------------------------------- */
+typedef struct qmm_kv_cache {
+    void *k, *v;      /* pools [layers][pages][kv_heads][page_size][head_dim], 16-byte aligned */
+    int32_t *table;   /* [slots][max_pages] */
+    int32_t *lens;    /* [slots]: positions of each sequence */
+    int32_t *refs;    /* [pages] */
+    int64_t pages;    /* 1 .. 2^24 */
+    int dtype;        /* QMM_F32, QMM_F16 or QMM_BF16 */
+    int layers;       /* 1 .. 1024 */
+    int kv_heads;     /* 1 .. 256 */
+    int page_size;    /* a power of two, 16 .. 1024 */
+    int head_dim;     /* 64, 128 or 256 */
+    int slots;        /* 1 .. 4096 */
+    int max_pages;    /* 1 .. 2^20, with max_pages * page_size and slots * max_pages <= 2^28 */
+} qmm_kv_cache;
+
+/* The rows of a step are packed, slot by slot: slot s has rows starts[s] .. starts[s + 1] - 1
+ * (int32 [slots + 1], on the device), which take the positions lens[s], lens[s] + 1, ... in
+ * order: one token, a run of a prompt's tokens, or the nodes of a tree of drafted tokens. rows (up to
+ * 2^20) is how many the call's arrays hold; rows that are no slot's, those behind starts[slots] among
+ * them, are not read, and their outputs stay as they are (a slot that starts outside [0, rows) has none). */
+
+/* RoPE of the rows (NeoX, as qmm_rope_kv_append_n) and their append: row j of slot s is rotated
+ * at position lens[s] + depths[row] (depths NULL: + j) by the cos / sin tables [positions][head_dim]
+ * (f32; both NULL: no rotation), k and v go to cache position lens[s] + j of the layer, rounded once
+ * to its type, and the rotated q to q_out (q NULL: none; q_out may be q). lens stays as it is.
+ * x_dtype (q, k, v, q_out): QMM_F32, QMM_F16 or QMM_BF16. A row whose position is outside the tables
+ * writes nothing; one past the slot's pages writes its q alone. Row strides in elements. */
+int qmm_kv_append(const qmm_kv_cache *cache, int layer, const void *q, const void *k, const void *v, int x_dtype,
+                  int64_t rows, int64_t ldq, int64_t ldk, int64_t ldv, const int32_t *starts, const int32_t *depths,
+                  const float *cos_t, const float *sin_t, int64_t positions, void *q_out, int64_t ldqo, int heads,
+                  void *stream);
+
+/* Attention of the rows (rotated, their keys and values appended) over their own sequence in the
+ * cache: row j of slot s sees the positions below lens[s], and position lens[s] + i where bit i of
+ * its mask is set (masks: uint64 [rows][ldm], bit i % 64 of word i / 64; i at or past 64 ldm is not
+ * seen). masks NULL: i <= j. out = softmax(q . K^T * scale) . V per head, kv head h / (heads /
+ * kv_heads); a row that sees nothing gets zeros. What a row does not see does not reach it, not an
+ * infinity or a NaN either. A position that the row sees and whose page the table does not name
+ * gives NaN. Sums and softmax are held in 32 bits; a 16-bit cache is multiplied on the 16-bit
+ * matrix cores, with q and the weights split into parts that keep their bits.
+ * heads % kv_heads == 0, heads / kv_heads <= 32. max_rows bounds the rows of a slot (rows past it
+ * are left out), at most 64 ldm with masks; max_len is about the largest lens[s] + rows of s: it
+ * sets how the positions are split over workgroups (and so the f32 summation order), longer
+ * sequences are right too. x_dtype: of q and out. ws: qmm_kv_attention_workspace_size(...) bytes on
+ * a 16-byte boundary; calls that may run at once need workspaces of their own. */
+size_t qmm_kv_attention_workspace_size(const qmm_kv_cache *cache, int64_t rows, int max_rows, int64_t max_len,
+                                       int heads);
+int qmm_kv_attention(const qmm_kv_cache *cache, int layer, const void *q, int x_dtype, int64_t rows, int64_t ldq,
+                     const int32_t *starts, const uint64_t *masks, int64_t ldm, int max_rows, int64_t max_len,
+                     int heads, float scale, void *out, int64_t ldo, void *ws, size_t ws_bytes, void *stream);
+
+/* The sequences' next generation: slot i continues what slot parents[i] holds (the same slot, another
+ * one, several slots the same one; -1, or any other id outside [0, slots): slot i is emptied), cut to
+ * min(lens[parents[i]], keep[i]) positions (keep NULL or keep[i] < 0: uncut), with pages for `reserve`
+ * further positions. Pages are shared, counted in refs and free where their count is 0. With reserve > 0
+ * a part-filled last page is about to be written: of the slots that have it as theirs, the lowest keeps it
+ * where nobody else holds it, all others get a copy (its filled rows, of every layer). New pages are the
+ * free ones with the lowest ids, in slot order, a slot's copy first.
+ * The new lists go to table_out, lens_out and refs_out, which may be the cache's own. shortage[0] (device)
+ * is 0, or the number of pages that were missing (in the pool, or in a slot's max_pages): then the lists
+ * go on unchanged and no page is written. ws: qmm_kv_fork_workspace_size(cache) bytes, 16-byte aligned. */
+size_t qmm_kv_fork_workspace_size(const qmm_kv_cache *cache);
+int qmm_kv_fork(const qmm_kv_cache *cache, const int32_t *parents, const int32_t *keep, int reserve,
+                int32_t *table_out, int32_t *lens_out, int32_t *refs_out, int32_t *shortage, void *ws,
+                size_t ws_bytes, void *stream);
+
+/* The accepted path of a step's rows: for d < counts[s], the key and value rows of position lens[s] +
+ * path[s][d] move to position lens[s] + d in every layer, and lens_out[s] (it may be the cache's lens)
+ * becomes lens[s] + counts[s]. path: int32 [slots][ld_path], increasing; a path ends early at an entry
+ * that is not above the one before, below 0, or whose page or position the slot does not have, and at
+ * ld_path, and then counts as that much shorter. path NULL: each row stays (a run whose first counts[s]
+ * rows are accepted). The pages that are written must be the slot's alone (qmm_kv_fork with a reserve). */
+int qmm_kv_accept(const qmm_kv_cache *cache, const int32_t *path, int64_t ld_path, const int32_t *counts,
+                  int32_t *lens_out, void *stream);
+
+/* Packs the pool: with U pages in use (refs != 0), those with ids from U on move, in order, to the free
+ * ids below U (whole pages, every layer); the table's entries and the counts go with them, to table_out
+ * and refs_out (they may be the cache's own). used[0] (device) = U. ws: qmm_kv_compact_workspace_size(cache)
+ * bytes, 16-byte aligned. */
+size_t qmm_kv_compact_workspace_size(const qmm_kv_cache *cache);
+int qmm_kv_compact(const qmm_kv_cache *cache, int32_t *table_out, int32_t *refs_out, int32_t *used, void *ws,
+                   size_t ws_bytes, void *stream);
+
+/* A beam search's selection: of batch searches with `beams` beams each, logits [batch * beams][vocab]
+ * (dtype QMM_F32, QMM_F16 or QMM_BF16, row stride ld) and the beams' scores (f32 sums of log
+ * probabilities), the `count` best continuations of each search by
+ *   scores[beam] + (logit - log sum exp(logits of the beam)),
+ * best first; ties: the lower beam, then the lower token. Sums and scores are held in 64 bits, each
+ * exponential to 2^-30 of its value; a beam's own continuations go by their logits. tokens, parents, out_scores: [batch][count]; a parent is a row of the
+ * logits (search * beams + beam). finished (int32 [batch * beams], or NULL): a beam whose entry is not 0
+ * has one continuation, the token eos at its own score, and its logits are not read. out_finished (or NULL): 1 where the
+ * parent was finished or the token is eos (eos -1: no token ends a beam; finished is then NULL). Where
+ * fewer continuations than count have a probability, the rest have token -1, parent -1, score -inf. A NaN
+ * logit or score counts as -inf, a +inf logit as the largest finite value. batch >= 1, beams 1 .. 64, count
+ * 1 .. 128, vocab 1 .. 2^20, batch * beams <= 65535. ws: qmm_beam_select_workspace_size(...) bytes, 16-byte aligned. */
+size_t qmm_beam_select_workspace_size(int64_t batch, int beams, int64_t vocab, int count);
+int qmm_beam_select(const void *logits, int dtype, int64_t ld, int64_t batch, int beams, int64_t vocab,
+                    const float *scores, const int32_t *finished, int eos, int count, int32_t *tokens,
+                    int32_t *parents, float *out_scores, int32_t *out_finished, void *ws, size_t ws_bytes,
+                    void *stream);
+
+/* dst row i = src row index[i] for i < rows, of row_bytes bytes (strides in bytes): the beams' texts, or
+ * any state of one row a beam. An index outside [0, src_rows) leaves the row as it is. src and dst do not
+ * overlap; rows <= 2^20. */
+int qmm_reorder_rows(const void *src, int64_t src_rows, int64_t ld_src, void *dst, int64_t ld_dst,
+                     int64_t row_bytes, const int32_t *index, int64_t rows, void *stream);
+
+/* ---------------------------------------------------------------------------
  * GGUF files (llama.cpp's single-file model container, spec v2/v3).
  * Replaces the reference's GgufFile (crates/llm/mlx-llm/src/gguf/reader.rs:
  * GgufFile::open/parse :188-278, meta/meta_str/meta_u64/meta_f64 :281-303,

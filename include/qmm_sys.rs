@@ -46,6 +46,25 @@ pub struct QmmQTensor {
     _private: [u8; 0],
 }
 
+/// A key/value cache in pages (device pointers; limits as in the C declaration).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct QmmKvCache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub table: *mut i32,
+    pub lens: *mut i32,
+    pub refs: *mut i32,
+    pub pages: i64,
+    pub dtype: c_int,
+    pub layers: c_int,
+    pub kv_heads: c_int,
+    pub page_size: c_int,
+    pub head_dim: c_int,
+    pub slots: c_int,
+    pub max_pages: c_int,
+}
+
 /// Opaque parsed GGUF file.
 #[repr(C)]
 pub struct QmmGguf {
@@ -543,6 +562,70 @@ extern "C" {
         down: *const QmmQTensor, shared_gate: *const QmmQTensor, shared_up: *const QmmQTensor,
         shared_down: *const QmmQTensor, shared_gate_weight: *const f32, out: *mut c_void, out_dtype: c_int,
         ldo: i64, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+
+    /// RoPE of a step's packed rows (slot s: rows starts[s] .. starts[s + 1] - 1) at position
+    /// lens[s] + depths[row] (null: + the row's number in its slot) and their append at cache
+    /// positions lens[s], lens[s] + 1, ...; the rotated q goes to q_out.
+    pub fn qmm_kv_append(
+        cache: *const QmmKvCache, layer: c_int, q: *const c_void, k: *const c_void, v: *const c_void,
+        x_dtype: c_int, rows: i64, ldq: i64, ldk: i64, ldv: i64, starts: *const i32, depths: *const i32,
+        cos_t: *const f32, sin_t: *const f32, positions: i64, q_out: *mut c_void, ldqo: i64, heads: c_int,
+        stream: *mut c_void
+    ) -> c_int;
+
+    /// Attention of a step's rows over their own sequences: row j sees the positions below lens[s]
+    /// and lens[s] + i where bit i of its mask is set (null: i <= j). A row that sees nothing is zeros.
+    pub fn qmm_kv_attention_workspace_size(
+        cache: *const QmmKvCache, rows: i64, max_rows: c_int, max_len: i64, heads: c_int
+    ) -> usize;
+
+    pub fn qmm_kv_attention(
+        cache: *const QmmKvCache, layer: c_int, q: *const c_void, x_dtype: c_int, rows: i64, ldq: i64,
+        starts: *const i32, masks: *const u64, ldm: i64, max_rows: c_int, max_len: i64, heads: c_int, scale: f32,
+        out: *mut c_void, ldo: i64, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+
+    /// The sequences' next generation: slot i continues slot parents[i] (outside [0, slots): emptied),
+    /// cut to keep[i] positions, with pages for `reserve` more. Part-filled pages that several slots
+    /// would write are copied. shortage[0]: 0, or the pages that were missing (nothing changes then).
+    pub fn qmm_kv_fork_workspace_size(cache: *const QmmKvCache) -> usize;
+
+    pub fn qmm_kv_fork(
+        cache: *const QmmKvCache, parents: *const i32, keep: *const i32, reserve: c_int, table_out: *mut i32,
+        lens_out: *mut i32, refs_out: *mut i32, shortage: *mut i32, ws: *mut c_void, ws_bytes: usize,
+        stream: *mut c_void
+    ) -> c_int;
+
+    /// The accepted path of a step's rows: position lens[s] + path[s][d] moves to lens[s] + d in every
+    /// layer for d < counts[s]; lens_out[s] = lens[s] + counts[s].
+    pub fn qmm_kv_accept(
+        cache: *const QmmKvCache, path: *const i32, ld_path: i64, counts: *const i32, lens_out: *mut i32,
+        stream: *mut c_void
+    ) -> c_int;
+
+    /// Moves the pages in use to the lowest ids; used[0]: how many they are.
+    pub fn qmm_kv_compact_workspace_size(cache: *const QmmKvCache) -> usize;
+
+    pub fn qmm_kv_compact(
+        cache: *const QmmKvCache, table_out: *mut i32, refs_out: *mut i32, used: *mut i32, ws: *mut c_void,
+        ws_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+
+    /// The `count` best continuations (beam score + log softmax) of each of `batch` searches, best first,
+    /// ties to the lower beam and token.
+    pub fn qmm_beam_select_workspace_size(batch: i64, beams: c_int, vocab: i64, count: c_int) -> usize;
+
+    pub fn qmm_beam_select(
+        logits: *const c_void, dtype: c_int, ld: i64, batch: i64, beams: c_int, vocab: i64, scores: *const f32,
+        finished: *const i32, eos: c_int, count: c_int, tokens: *mut i32, parents: *mut i32,
+        out_scores: *mut f32, out_finished: *mut i32, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+
+    /// dst row i = src row index[i] (strides in bytes); an index outside [0, src_rows) leaves the row.
+    pub fn qmm_reorder_rows(
+        src: *const c_void, src_rows: i64, ld_src: i64, dst: *mut c_void, ld_dst: i64, row_bytes: i64,
+        index: *const i32, rows: i64, stream: *mut c_void
     ) -> c_int;
 
     /// Open a file (memory-mapped, read only) or an in-memory image (copied).

@@ -2,7 +2,8 @@
 
 The compute lives in ``inference_amd/_lib/libqmm.so`` (C ABI: ``include/qmm.h``),
 built from ``inference_amd/csrc`` for gfx950. ``inference_amd.qmm`` mirrors the
-reference engine's QTensor / QMatMul / QuantizedLinear surface over it.
+reference engine's QTensor / QMatMul / QuantizedLinear surface over it;
+``inference_amd.paged`` has the cache in pages and the beam search's selection.
 """
 from .qmm import (  # noqa: F401
     GgmlDType,
@@ -22,3 +23,4 @@ from .qmm import (  # noqa: F401
     matmul_q,
     quantize_rows,
 )
+from .paged import PagedKVCache, beam_select, reorder_rows  # noqa: F401

@@ -20,6 +20,7 @@
 extern "C" const unsigned char qmm_code_object_start[];
 extern "C" const unsigned char qmm_code_object_end[];
 extern "C" const unsigned char qmm_mx_code_object_start[];
+extern "C" const unsigned char qmm_kv_code_object_start[];
 
 namespace {
 
@@ -79,6 +80,7 @@ constexpr int kKernelSlots = 8192;  // > 4x the kernels of the code object
 
 struct Device {
   hipModule_t module = nullptr, mx_module = nullptr;  // mx: kernels named qmm_mx_* and qmm_route_*
+  hipModule_t kv_module = nullptr;                    // kernels named qmm_kv_* and qmm_beam_*
   std::atomic<const KernelEntry*> slots[kKernelSlots];
   int max_lds = 0;
   int num_cu = 0;
@@ -183,11 +185,20 @@ int current_device(Device** out) {
       return fail(QMM_ERR_NO_KERNEL, "hipModuleLoadData(second gfx950 code object) on device %d: %s", dev,
                   hipGetErrorString(e));
     }
+    e = hipModuleLoadData(&d->kv_module, qmm_kv_code_object_start);
+    if (e != hipSuccess) {
+      (void)hipModuleUnload(d->module);
+      (void)hipModuleUnload(d->mx_module);
+      delete d;
+      return fail(QMM_ERR_NO_KERNEL, "hipModuleLoadData(third gfx950 code object) on device %d: %s", dev,
+                  hipGetErrorString(e));
+    }
     e = hipDeviceGetAttribute(&d->max_lds, hipDeviceAttributeMaxSharedMemoryPerBlock, dev);
     if (e == hipSuccess) e = hipDeviceGetAttribute(&d->num_cu, hipDeviceAttributeMultiprocessorCount, dev);
     if (e != hipSuccess) {
       (void)hipModuleUnload(d->module);
       (void)hipModuleUnload(d->mx_module);
+      (void)hipModuleUnload(d->kv_module);
       delete d;
       return fail(QMM_ERR_HIP, "hipDeviceGetAttribute: %s", hipGetErrorString(e));
     }
@@ -227,7 +238,8 @@ int kernel(Device* d, const char* name, hipFunction_t* f) {
   if (i == kKernelSlots) return fail(QMM_ERR_NO_KERNEL, "kernel table full looking up %s", name);
   hipFunction_t fn = nullptr;
   const bool mx = !strncmp(name, "qmm_mx_", 7) || !strncmp(name, "qmm_route_", 10);
-  hipError_t err = hipModuleGetFunction(&fn, mx ? d->mx_module : d->module, name);
+  const bool kv = !strncmp(name, "qmm_kv_", 7) || !strncmp(name, "qmm_beam_", 9);
+  hipError_t err = hipModuleGetFunction(&fn, mx ? d->mx_module : kv ? d->kv_module : d->module, name);
   if (err != hipSuccess || !fn) {
     // The failed lookup also sets the runtime's last error; clear it so the
     // caller's next unrelated HIP call (e.g. a graph capture) does not report it.
@@ -260,6 +272,7 @@ struct qmm_qtensor {
 };
 
 #include "qmm_mx_host.h"
+#include "qmm_kv_host.h"
 
 extern "C" {
 

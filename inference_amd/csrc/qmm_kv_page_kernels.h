@@ -1,0 +1,440 @@
+// The rows of a step appended to a cache in pages, and what moves its pages: forks of
+// sequences with copies of the pages that two of them would write, the accepted rows of a
+// drafted tree, and the packing of the pool.
+#pragma once
+
+#include "qmm_kv_common.h"
+
+namespace qmm {
+
+struct KvAppend {
+  KvCache c;
+  KvRows r;
+  const void *q, *k, *v;
+  const int32_t* depths;
+  const float *cos_t, *sin_t;
+  void* q_out;
+  long long ldq, ldk, ldv, ldqo;
+  int layer, x_type, heads, positions, wide;
+};
+
+// Rounds a count up to whole pages.
+__device__ __forceinline__ int kv_pages_of(int positions, int page_log) {
+  return (positions + (1 << page_log) - 1) >> page_log;
+}
+__device__ __forceinline__ int agent_load(const int* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void agent_store(int* p, int v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void agent_add(int* p, int v) {
+  (void)__hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// A barrier after which agent_load sees what the workgroup's agent stores and adds before it left.
+__device__ __forceinline__ void agent_barrier() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+}  // namespace qmm
+
+// x cos + rotate_half(x) sin of the rows, k and v to their pages. A thread has four values
+// of a head's first half and the four of the second that turn with them; head_dim / 8
+// threads a head, q's heads first, then k's, then v's. Bound by the rows' bytes.
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_append_rows(qmm::KvAppend a) {
+#pragma clang fp contract(off)
+  using namespace qmm;
+  __shared__ int lds4[4];
+  const int per = a.c.head_dim / 8, group = 256 / per;
+  const int nq = a.q ? a.heads : 0, units = nq + 2 * a.c.kv_heads, blocks = (units + group - 1) / group;
+  const int row = blockIdx.x / blocks, u = blockIdx.x % blocks * group + threadIdx.x / per;
+  const int s = kv_slot_of(a.r, a.c.slots, row, lds4);
+  if (s < 0 || u >= units) return;
+  const KvSpan sp = kv_span(a.r, s);
+  const int j = row - sp.first, base = a.c.length(s), half = a.c.head_dim / 2;
+  const int i = 4 * (threadIdx.x % per);
+  // (64 bits: a depth is the caller's)
+  const long long p = (long long)base + (a.depths ? a.depths[row] : j);
+  if (a.cos_t && (p < 0 || p >= a.positions)) return;
+  const bool is_q = u < nq, is_v = u >= nq + a.c.kv_heads;
+  const int h = is_q ? u : is_v ? u - nq - a.c.kv_heads : u - nq;
+  const void* src = is_q ? a.q : is_v ? a.v : a.k;
+  const long long ld = is_q ? a.ldq : is_v ? a.ldv : a.ldk;
+  const long long at = row * ld + (long long)h * a.c.head_dim + i;
+  float x[4], y[4];
+  load4_typed(x, src, at, a.x_type, a.wide);
+  load4_typed(y, src, at + half, a.x_type, a.wide);
+  if (a.cos_t && !is_v) {
+    float c0[4], c1[4], s0[4], s1[4];
+    load4_typed(c0, a.cos_t, p * a.c.head_dim + i, kTypeF32, a.wide);
+    load4_typed(c1, a.cos_t, p * a.c.head_dim + i + half, kTypeF32, a.wide);
+    load4_typed(s0, a.sin_t, p * a.c.head_dim + i, kTypeF32, a.wide);
+    load4_typed(s1, a.sin_t, p * a.c.head_dim + i + half, kTypeF32, a.wide);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float xe = x[e], ye = y[e];
+      x[e] = xe * c0[e] + -ye * s0[e];
+      y[e] = ye * c1[e] + xe * s1[e];
+    }
+  }
+  if (is_q) {
+    const long long o = row * a.ldqo + (long long)h * a.c.head_dim + i;
+    store4_typed(a.q_out, o, a.x_type, a.wide, x);
+    store4_typed(a.q_out, o + half, a.x_type, a.wide, y);
+    return;
+  }
+  const int t = base + j;
+  if (t >= a.c.capacity()) return;
+  const int page = a.c.page(s, t >> a.c.page_log);
+  if (page < 0) return;
+  void* pool = is_v ? a.c.v : a.c.k;
+  const long long o = a.c.row(a.layer, page, h, t & ((1 << a.c.page_log) - 1)) + i;
+  store4_typed(pool, o, a.c.dtype, true, x);
+  store4_typed(pool, o + half, a.c.dtype, true, y);
+}
+
+// ---------------------------------------------------------------------------
+// fork
+// ---------------------------------------------------------------------------
+namespace qmm {
+
+struct KvFork {
+  KvCache c;
+  const int32_t *parents, *keep;
+  int32_t *table_out, *lens_out, *refs_out, *shortage;
+  int reserve;
+  // workspace
+  int32_t *refs, *writers, *first;  // [pages]: counts, slots that would write the page, the lowest of them
+  int32_t *free_ids;                // [pages]: free pages, the lowest first
+  int32_t *table;                   // [slots][max_pages]: the old table
+  int32_t *lens, *at, *parent;      // [slots]: new length, first of the slot's new pages in free_ids, parent or -1
+  int32_t *copy;                    // [slots]: whether the slot's last page is copied
+  int32_t *moves;                   // [1 + 3 slots]: number of copies; source, destination, rows of each
+};
+
+// A slot's new length in positions, whole and part-filled pages of it, and those with the reserve.
+struct KvGrow {
+  int len, held, total;
+  bool part;  // its last page is filled in part and will be written
+};
+__device__ __forceinline__ KvGrow kv_grow(const KvFork& f, int s) {
+  const int len = agent_load(f.lens + s), lg = f.c.page_log;
+  KvGrow g = {len, kv_pages_of(len, lg), 0, false};
+  g.total = agent_load(f.parent + s) < 0 ? 0 : f.reserve ? kv_pages_of(len + f.reserve, lg) : g.held;
+  g.part = f.reserve > 0 && (len & ((1 << lg) - 1)) != 0;
+  return g;
+}
+
+// The phases, over `n` threads (t is this one) or `n` waves; a phase reads what the one
+// before has written.
+__device__ __forceinline__ void kv_fork_begin(const KvFork& f, long long t, long long n) {
+  for (long long p = t; p < f.c.pages; p += n) {
+    agent_store(f.refs + p, f.c.refs[p]);
+    agent_store(f.writers + p, 0);
+    agent_store(f.first + p, 0x7fffffff);
+  }
+  const long long cells = (long long)f.c.slots * f.c.max_pages;
+  for (long long i = t; i < cells; i += n) {
+    const int p = f.c.table[i];
+    agent_store(f.table + i, p >= 0 && p < f.c.pages ? p : -1);
+  }
+  for (long long s = t; s < f.c.slots; s += n) {
+    const int p = f.parents[s];
+    const bool ok = p >= 0 && p < f.c.slots;
+    int len = ok ? f.c.length(p) : 0;
+    if (f.keep && f.keep[s] >= 0) len = min(len, f.keep[s]);
+    agent_store(f.lens + s, len);
+    agent_store(f.parent + s, ok ? p : -1);
+  }
+}
+
+// The counts without the old rows and with the new ones, before any new page.
+__device__ __forceinline__ void kv_fork_count(const KvFork& f, long long w, long long waves, int lane) {
+  for (long long s = w; s < f.c.slots; s += waves) {
+    const long long row = s * f.c.max_pages;
+    for (int j = lane; j < f.c.max_pages; j += 64) {
+      const int p = agent_load(f.table + row + j);
+      if (p >= 0) agent_add(f.refs + p, -1);
+    }
+    const int from = agent_load(f.parent + s);
+    if (from < 0) continue;
+    const KvGrow g = kv_grow(f, (int)s);
+    for (int j = lane; j < min(g.held, f.c.max_pages); j += 64) {
+      const int p = agent_load(f.table + (long long)from * f.c.max_pages + j);
+      if (p < 0) continue;
+      agent_add(f.refs + p, 1);
+      if (g.part && j == g.held - 1) {
+        agent_add(f.writers + p, 1);
+        (void)__hip_atomic_fetch_min(f.first + p, (int)s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+  }
+}
+
+// Exclusive sums of v over the 1024 threads of a workgroup, and the whole sum.
+__device__ __forceinline__ int block_sums(int v, int* lds, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // (the last call's values are read no more)
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int y = lds[i];
+    before += i < wave ? y : 0;
+    all += y;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// One workgroup: which slots copy their last page, how many pages each takes, and which.
+__device__ __forceinline__ void kv_fork_plan(const KvFork& f, int* lds) {
+  const int t = threadIdx.x, per = (f.c.slots + 1023) / 1024;
+  int need = 0, over = 0, copies = 0;
+  for (int i = 0; i < per; ++i) {
+    const int s = t * per + i;
+    if (s >= f.c.slots) break;
+    const KvGrow g = kv_grow(f, s);
+    int copy = -1;
+    if (g.part && agent_load(f.parent + s) >= 0) {
+      const int p = agent_load(f.table + (long long)agent_load(f.parent + s) * f.c.max_pages + g.held - 1);
+      if (p >= 0 && !(agent_load(f.refs + p) == agent_load(f.writers + p) && agent_load(f.first + p) == s)) copy = p;
+    }
+    agent_store(f.copy + s, copy);
+    copies += copy >= 0;
+    need += (copy >= 0) + max(min(g.total, f.c.max_pages) - g.held, 0);
+    over += max(g.total - f.c.max_pages, 0);
+  }
+  int total, none, slots_over;
+  int at = block_sums(need, lds, &total);
+  (void)block_sums(over, lds, &slots_over);
+  int move = block_sums(copies, lds, &none);
+  // the free pages, until there are enough
+  int found = 0;
+  for (long long p0 = 0; p0 < f.c.pages && found < total; p0 += 1024) {
+    const long long p = p0 + t;
+    const bool free = p < f.c.pages && agent_load(f.refs + p) == 0;
+    int here;
+    const int i = block_sums(free ? 1 : 0, lds, &here);
+    if (free && found + i < total) agent_store(f.free_ids + found + i, (int)p);
+    found += here;
+  }
+  const int missing = max(total - found, 0) + slots_over;
+  agent_barrier();
+  if (t == 0) {
+    agent_store(f.shortage, missing);
+    agent_store(f.moves, missing ? 0 : none);
+  }
+  if (missing) return;
+  for (int i = 0; i < per; ++i) {
+    const int s = t * per + i;
+    if (s >= f.c.slots) break;
+    const KvGrow g = kv_grow(f, s);
+    const int p = agent_load(f.copy + s);
+    agent_store(f.at + s, at);
+    if (p >= 0) {
+      agent_add(f.refs + p, -1);
+      agent_store(f.moves + 1 + 3 * move, p);
+      agent_store(f.moves + 2 + 3 * move, agent_load(f.free_ids + at));
+      agent_store(f.moves + 3 + 3 * move, g.len & ((1 << f.c.page_log) - 1));
+      ++move;
+    }
+    at += (p >= 0) + max(g.total - g.held, 0);
+  }
+  for (int i = t; i < total; i += 1024) agent_store(f.refs + agent_load(f.free_ids + i), 1);
+}
+
+__device__ __forceinline__ void kv_fork_commit(const KvFork& f, long long t, long long n) {
+  const bool ok = agent_load(f.shortage) == 0;
+  // (refs_out and table_out may be the cache's own: without room they get back what they held)
+  for (long long p = t; p < f.c.pages; p += n) f.refs_out[p] = ok ? agent_load(f.refs + p) : f.c.refs[p];
+  const long long cells = (long long)f.c.slots * f.c.max_pages;
+  for (long long i = t; i < cells; i += n) {
+    if (!ok) {
+      f.table_out[i] = f.c.table[i];
+      continue;
+    }
+    const int s = (int)(i / f.c.max_pages), j = (int)(i % f.c.max_pages);
+    const int from = agent_load(f.parent + s);
+    int p = -1;
+    if (from >= 0) {
+      const KvGrow g = kv_grow(f, s);
+      const int copy = agent_load(f.copy + s) >= 0;
+      if (j < g.held)
+        p = copy && j == g.held - 1 ? agent_load(f.free_ids + agent_load(f.at + s))
+                                    : agent_load(f.table + (long long)from * f.c.max_pages + j);
+      else if (j < g.total)
+        p = agent_load(f.free_ids + agent_load(f.at + s) + copy + j - g.held);
+    }
+    f.table_out[i] = p;
+  }
+  for (long long s = t; s < f.c.slots; s += n) f.lens_out[s] = ok ? agent_load(f.lens + s) : f.c.lens[s];
+}
+}  // namespace qmm
+
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_fork_begin(qmm::KvFork f) {
+  qmm::kv_fork_begin(f, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
+}
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_fork_count(qmm::KvFork f) {
+  qmm::kv_fork_count(f, blockIdx.x * 4LL + (threadIdx.x >> 6), gridDim.x * 4LL, threadIdx.x & 63);
+}
+extern "C" __global__ void __launch_bounds__(1024) qmm_kv_fork_plan(qmm::KvFork f) {
+  __shared__ int lds[16];
+  qmm::kv_fork_plan(f, lds);
+}
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_fork_commit(qmm::KvFork f) {
+  qmm::kv_fork_commit(f, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
+}
+
+// The listed pages' first rows (a whole page: rows = page size) to other pages, in every
+// layer and of every kv head. Sources and destinations are disjoint. Bound by the bytes.
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_copy_pages(qmm::KvCache c, const int* moves) {
+  using namespace qmm;
+  const int count = moves[0];
+  const long long items = (long long)count * c.layers * 2 * c.kv_heads;
+  for (long long i = blockIdx.x; i < items; i += gridDim.x) {
+    const int g = (int)(i % c.kv_heads), side = (int)(i / c.kv_heads % 2);
+    const int layer = (int)(i / (2 * c.kv_heads) % c.layers);
+    const int* m = moves + 1 + 3 * (i / (2LL * c.kv_heads * c.layers));
+    char* pool = (char*)(side ? c.v : c.k);
+    const uint4* src = (const uint4*)(pool + (c.row(layer, m[0], g, 0) << c.esize_log()));
+    uint4* dst = (uint4*)(pool + (c.row(layer, m[1], g, 0) << c.esize_log()));
+    const int n = (m[2] * c.head_dim << c.esize_log()) / 16;
+    for (int x = threadIdx.x; x < n; x += 256) dst[x] = src[x];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// accept
+// ---------------------------------------------------------------------------
+namespace qmm {
+struct KvAccept {
+  KvCache c;
+  const int32_t *path, *counts;
+  int32_t* lens_out;
+  long long ld_path;
+  int max_path;
+};
+
+// Entry d of the slot's path where it goes on: above `last`, its position and its place in
+// pages of the slot; -1 where the path ends.
+__device__ __forceinline__ int kv_path(const KvAccept& a, int s, int base, int d, int last) {
+  const int to = a.path[s * a.ld_path + d];
+  if (to <= last || to >= a.c.capacity() - base) return -1;
+  if (a.c.page(s, (base + to) >> a.c.page_log) < 0 || a.c.page(s, (base + d) >> a.c.page_log) < 0) return -1;
+  return to;
+}
+}  // namespace qmm
+
+// Position base + path[d] to base + d, a thread a 16-byte column of a layer's, side's and
+// head's rows, in order: path[d] >= d and rises, so no row is overwritten before it is read.
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_accept_rows(qmm::KvAccept a) {
+  using namespace qmm;
+  const KvCache& c = a.c;
+  const int s = blockIdx.y, base = c.length(s), n = min(a.counts[s], a.max_path);
+  const int per = (c.head_dim << c.esize_log()) / 16;
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  if (i >= 2LL * c.layers * c.kv_heads * per) return;
+  const int x = (int)(i % per), g = (int)(i / per % c.kv_heads), side = (int)(i / per / c.kv_heads % 2);
+  const int layer = (int)(i / per / c.kv_heads / 2);
+  char* pool = (char*)(side ? c.v : c.k);
+  const int low = (1 << c.page_log) - 1;
+  auto at = [&](int t) {
+    return (uint4*)(pool + (c.row(layer, c.page(s, t >> c.page_log), g, t & low) << c.esize_log())) + x;
+  };
+  int last = -1;
+  for (int d = 0; d < n; ++d) {
+    last = kv_path(a, s, base, d, last);
+    if (last < 0) break;
+    if (last != d) *at(base + d) = *at(base + last);
+  }
+}
+
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_accept_lens(qmm::KvAccept a) {
+  using namespace qmm;
+  const int s = blockIdx.x * 256 + threadIdx.x;
+  if (s >= a.c.slots) return;
+  const int base = a.c.length(s);
+  int d = 0;
+  if (a.path) {
+    const int n = min(a.counts[s], a.max_path);
+    for (int last = -1; d < n; ++d) {
+      last = kv_path(a, s, base, d, last);
+      if (last < 0) break;
+    }
+  } else {  // page by page
+    const int n = min(max(a.counts[s], 0), a.c.capacity() - base);
+    while (d < n && a.c.page(s, (base + d) >> a.c.page_log) >= 0)
+      d = min(((((base + d) >> a.c.page_log) + 1) << a.c.page_log) - base, n);
+  }
+  a.lens_out[s] = base + d;
+}
+
+// ---------------------------------------------------------------------------
+// compact
+// ---------------------------------------------------------------------------
+namespace qmm {
+struct KvCompact {
+  KvCache c;
+  int32_t *table_out, *refs_out, *used;
+  // workspace
+  int32_t *map, *refs;  // [pages]: where a page goes, the new counts
+  int32_t* moves;       // [1 + 3 pages / 2], as a fork's
+};
+}  // namespace qmm
+
+// One workgroup: the pages in use, then the i-th of those behind their number to the i-th
+// free one below it.
+extern "C" __global__ void __launch_bounds__(1024) qmm_kv_compact_plan(qmm::KvCompact k) {
+  using namespace qmm;
+  __shared__ int lds[16];
+  const int t = threadIdx.x, pages = k.c.pages;
+  int mine = 0, used;
+  for (int p = t; p < pages; p += 1024) mine += k.c.refs[p] != 0;
+  (void)block_sums(mine, lds, &used);
+  int src = 0, dst = 0;
+  for (int p0 = 0; p0 < pages; p0 += 1024) {
+    const int p = p0 + t;
+    const int refs = p < pages ? k.c.refs[p] : 0;
+    const bool from = p < pages && refs != 0 && p >= used, to = p < used && refs == 0;
+    int ns, nd;
+    const int i = block_sums(from, lds, &ns), j = block_sums(to, lds, &nd);
+    if (from) agent_store(k.moves + 1 + 3 * (src + i), p);
+    if (to) agent_store(k.moves + 2 + 3 * (dst + j), p);
+    if (p < pages) {
+      agent_store(k.map + p, p);
+      agent_store(k.refs + p, p < used ? refs : 0);
+    }
+    src += ns;
+    dst += nd;
+  }
+  agent_barrier();
+  if (t == 0) {
+    agent_store(k.moves, src);
+    k.used[0] = used;
+  }
+  for (int i = t; i < src; i += 1024) {
+    const int a = agent_load(k.moves + 1 + 3 * i), b = agent_load(k.moves + 2 + 3 * i);
+    agent_store(k.moves + 3 + 3 * i, 1 << k.c.page_log);
+    agent_store(k.map + a, b);
+    agent_store(k.refs + b, k.c.refs[a]);
+  }
+}
+
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_compact_commit(qmm::KvCompact k) {
+  using namespace qmm;
+  const long long n = gridDim.x * 256LL, t = blockIdx.x * 256LL + threadIdx.x;
+  for (long long p = t; p < k.c.pages; p += n) k.refs_out[p] = k.refs[p];
+  const long long cells = (long long)k.c.slots * k.c.max_pages;
+  for (long long i = t; i < cells; i += n) {
+    const int p = k.c.table[i];
+    k.table_out[i] = p >= 0 && p < k.c.pages ? k.map[p] : p;
+  }
+}

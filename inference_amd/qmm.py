@@ -66,6 +66,9 @@ EXPORTS = (
     "qmm_decode_rope_attention_warm", "qmm_matmul_grouped",
     "qmm_qtensor_quantize_from", "qmm_linear", "qmm_linear_workspace_size", "qmm_moe_route_scored",
     "qmm_moe_route_scored_workspace_size", "qmm_moe_ffn_scored", "qmm_moe_ffn_scored_workspace_size",
+    "qmm_kv_append", "qmm_kv_attention_workspace_size", "qmm_kv_attention", "qmm_kv_fork_workspace_size",
+    "qmm_kv_fork", "qmm_kv_accept", "qmm_kv_compact_workspace_size", "qmm_kv_compact",
+    "qmm_beam_select_workspace_size", "qmm_beam_select", "qmm_reorder_rows",
 )
 
 
@@ -181,6 +184,19 @@ def lib() -> ctypes.CDLL:
             "qmm_moe_ffn_scored": ([vp, i32, i64, i64, vp, i32, i32, i32, vp, i32, i32, i32, i32, ctypes.c_float, vp,
                                     vp, vp, vp, vp, vp, vp, vp, i32, i64, vp, sz, vp], i32),
             "qmm_moe_ffn_scored_workspace_size": ([vp, vp, i64, i32, i32, vp, vp, vp], sz),
+            "qmm_kv_append": ([vp, i32, vp, vp, vp, i32, i64, i64, i64, i64, vp, vp, vp, vp, i64, vp, i64, i32, vp],
+                              i32),
+            "qmm_kv_attention_workspace_size": ([vp, i64, i32, i64, i32], sz),
+            "qmm_kv_attention": ([vp, i32, vp, i32, i64, i64, vp, vp, i64, i32, i64, i32, ctypes.c_float, vp, i64, vp,
+                                  sz, vp], i32),
+            "qmm_kv_fork_workspace_size": ([vp], sz),
+            "qmm_kv_fork": ([vp, vp, vp, i32, vp, vp, vp, vp, vp, sz, vp], i32),
+            "qmm_kv_accept": ([vp, vp, i64, vp, vp, vp], i32),
+            "qmm_kv_compact_workspace_size": ([vp], sz),
+            "qmm_kv_compact": ([vp, vp, vp, vp, vp, sz, vp], i32),
+            "qmm_beam_select_workspace_size": ([i64, i32, i64, i32], sz),
+            "qmm_beam_select": ([vp, i32, i64, i64, i32, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp, sz, vp], i32),
+            "qmm_reorder_rows": ([vp, i64, i64, vp, i64, i64, vp, i64, vp], i32),
             "qmm_stream_read": ([vp, ctypes.c_size_t, vp, i32, i32, vp], i32),
         }
         for name, (args, res) in sig.items():
