@@ -59,8 +59,11 @@ __device__ __forceinline__ int kv_slot_of(const KvRows& r, int slots, int i, int
   return i >= sp.first && i < sp.first + sp.n ? s : -1;
 }
 
+// (both conversions and a choice: a branch between loads would have each wait for the last)
 __device__ __forceinline__ float from_half(uint16_t v, int type) {
-  return type == kTypeF16 ? (float)__builtin_bit_cast(_Float16, v) : __builtin_bit_cast(float, (uint32_t)v << 16);
+  const uint32_t h = __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(_Float16, v)), b = (uint32_t)v << 16;
+  const uint32_t m = type == kTypeF16 ? ~0u : 0u;
+  return __builtin_bit_cast(float, (h & m) | (b & ~m));
 }
 // (rounded to nearest even)
 __device__ __forceinline__ uint16_t to_half(float v, int type) {

@@ -100,10 +100,35 @@ struct KvAttn {
   const void* q;
   const uint64_t* masks;
   void* out;
+  float *part, *state;
   long long ldq, ldm, ldo;
-  int layer, x_type, heads;
+  int layer, x_type, heads, wide, splits, chunk, tiles;
   float scale;
 };
+
+constexpr int64_t kKvWorkgroups = 2048;
+
+// How an attention's positions are split: `splits` chunks of a slot at most, of `chunk` positions
+// (a multiple of 128, a key tile for each of four waves) or more. The chip has 256 CUs that hold
+// two workgroups each; `tiles` of 32 columns a slot.
+struct KvSplit {
+  int tiles, splits, chunk;
+  size_t parts;  // bytes of the partial outputs, a multiple of 256
+  size_t bytes;
+};
+KvSplit kv_split(const qmm_kv_cache* c, int64_t rows, int max_rows, int64_t max_len, int heads) {
+  KvSplit p;
+  const int64_t per = 32 / (heads / c->kv_heads);
+  p.tiles = (int)ceil_div(std::min<int64_t>(max_rows, std::max<int64_t>(rows, 1)), per);
+  const int64_t most = std::min<int64_t>(max_len, (int64_t)c->max_pages * c->page_size);
+  const int64_t units = (int64_t)c->slots * c->kv_heads * p.tiles;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kKvWorkgroups / units, ceil_div(most, 128)));
+  p.chunk = (int)ceil_div(ceil_div(most, p.splits), 128) * 128;
+  const size_t records = p.splits > 1 ? (size_t)rows * heads * p.splits : 0;
+  p.parts = kv_align(records * c->head_dim * 4);
+  p.bytes = p.parts + kv_align(records * 8);
+  return p;
+}
 
 struct KvFork {
   KvCache c;
@@ -206,7 +231,7 @@ static int kv_check_attention(const qmm_kv_cache* cache, int64_t rows, int max_r
 size_t qmm_kv_attention_workspace_size(const qmm_kv_cache* cache, int64_t rows, int max_rows, int64_t max_len,
                                        int heads) {
   if (kv_check_attention(cache, rows, max_rows, max_len, heads) != QMM_OK) return 0;
-  return 0;
+  return kv_split(cache, rows, max_rows, max_len, heads).bytes;
 }
 
 int qmm_kv_attention(const qmm_kv_cache* cache, int layer, const void* q, int x_dtype, int64_t rows, int64_t ldq,
@@ -226,11 +251,33 @@ int qmm_kv_attention(const qmm_kv_cache* cache, int layer, const void* q, int x_
   if (rows == 0) return QMM_OK;
   Device* d;
   QMM_TRY(current_device(&d));
+  const KvSplit p = kv_split(cache, rows, max_rows, max_len, heads);
+  const int64_t units = (int64_t)cache->slots * p.splits * cache->kv_heads;
+  if ((units + 7) / 8 * 8 * p.tiles >= (1LL << 24)) return fail(QMM_ERR_INVALID, "%d slots of up to %d rows are too many at once", cache->slots, max_rows);
+  const size_t four = 4 * kv_esize(x_dtype);
   a.r = {starts, (int)rows, max_rows};
   a.q = q, a.masks = masks, a.out = out, a.ldq = ldq, a.ldm = ldm, a.ldo = ldo;
+  a.part = (float*)ws, a.state = ws ? (float*)((uint8_t*)ws + p.parts) : nullptr;
   a.layer = layer, a.x_type = x_dtype, a.heads = heads, a.scale = scale;
+  a.wide = (uintptr_t)q % four == 0 && ldq % 4 == 0;
+  a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles;
+  // parts that hold the bits of q (24, 11, 8) in the cache's type, and of the weights
+  int qp = 1, pp = 1;
+  if (cache->dtype == QMM_BF16) {
+    qp = x_dtype == QMM_F32 ? 3 : x_dtype == QMM_F16 ? 2 : 1;
+    pp = x_dtype == QMM_F32 ? 3 : 2;
+  } else if (cache->dtype == QMM_F16) {
+    qp = x_dtype == QMM_F32 ? 2 : 1;
+    pp = 2;
+  }
+  char name[64];
+  snprintf(name, sizeof(name), "qmm_kv_attn_%s_d%d_q%d_p%d", mx_type_name(cache->dtype), cache->head_dim, qp, pp);
+  const unsigned threads = cache->dtype == QMM_F32 && cache->head_dim == 256 ? 128 : 256;
+  const hipStream_t s = (hipStream_t)stream;
   void* args[] = {&a};
-  return kv_launch(d, "qmm_kv_attn_rows", (unsigned)rows, (unsigned)ceil_div(heads, 4), 256, (hipStream_t)stream, args);
+  QMM_TRY(kv_launch(d, name, (unsigned)((units + 7) / 8 * 8 * p.tiles), 1, threads, s, args));
+  if (p.splits == 1) return QMM_OK;
+  return kv_launch(d, "qmm_kv_attn_join", (unsigned)rows, ceil_div((int64_t)heads * cache->head_dim, 256), 256, s, args);
 }
 
 size_t qmm_kv_fork_workspace_size(const qmm_kv_cache* cache) {
