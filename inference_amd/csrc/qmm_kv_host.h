@@ -102,27 +102,34 @@ struct KvAttn {
   void* out;
   float *part, *state;
   long long ldq, ldm, ldo;
-  int layer, x_type, heads, wide, splits, chunk, tiles;
+  int layer, x_type, heads, wide, splits, chunk;
+  int tiles, group_rows, join_lanes;
   float scale;
 };
 
-constexpr int64_t kKvWorkgroups = 2048;
-
-// How an attention's positions are split: `splits` chunks of a slot at most, of `chunk` positions
-// (a multiple of 128, a key tile for each of four waves) or more. The chip has 256 CUs that hold
-// two workgroups each; `tiles` of 32 columns a slot.
+// How an attention's rows and positions are split. form 0, 1: one tile of 16 or 32 columns (rows
+// x heads of a kv head) a slot, 2: groups of four tiles of 32. `splits` chunks of a slot's
+// positions at most, of `chunk` (a multiple of 128) or more.
 struct KvSplit {
-  int tiles, splits, chunk;
+  int form, tiles, group_rows, splits, chunk;
   size_t parts;  // bytes of the partial outputs, a multiple of 256
   size_t bytes;
 };
 KvSplit kv_split(const qmm_kv_cache* c, int64_t rows, int max_rows, int64_t max_len, int heads) {
   KvSplit p;
-  const int64_t per = 32 / (heads / c->kv_heads);
-  p.tiles = (int)ceil_div(std::min<int64_t>(max_rows, std::max<int64_t>(rows, 1)), per);
+  const int64_t G = heads / c->kv_heads, per = 32 / G, most_rows = std::min<int64_t>(max_rows, std::max<int64_t>(rows, 1));
+  p.form = most_rows * G <= 16 ? 0 : most_rows <= per ? 1 : 2;
+  p.group_rows = (int)(p.form == 0 ? 16 / G : p.form == 1 ? per : 4 * per);
+  p.tiles = (int)ceil_div(most_rows, p.group_rows);
   const int64_t most = std::min<int64_t>(max_len, (int64_t)c->max_pages * c->page_size);
   const int64_t units = (int64_t)c->slots * c->kv_heads * p.tiles;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kKvWorkgroups / units, ceil_div(most, 128)));
+  // Few columns: a chunk's record is small, so many short chunks even out sequences of different lengths (24 of up to
+  // 8000 positions: 86.7 us with 10 chunks, 89.5 with 4), but not so short that the chip is full of their beginnings
+  // (64 of up to 1000: 28 us whole, 34 in two; one of 30000: 28 us with chunks of 256, 34 of 128). More columns: a
+  // chunk writes and reads 0.5 KB a column (8 trees of up to 26 nodes over up to 4000 positions: 50 us with 12 chunks
+  // of at least 384, 58 with 32).
+  const int64_t wgs = p.form == 0 ? (units < 64 ? 1024 : 2048) : 768, least = p.form == 0 ? 128 * ceil_div(units, 64) : 384;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(wgs / units, ceil_div(most, least)));
   p.chunk = (int)ceil_div(ceil_div(most, p.splits), 128) * 128;
   const size_t records = p.splits > 1 ? (size_t)rows * heads * p.splits : 0;
   p.parts = kv_align(records * c->head_dim * 4);
@@ -260,7 +267,10 @@ int qmm_kv_attention(const qmm_kv_cache* cache, int layer, const void* q, int x_
   a.part = (float*)ws, a.state = ws ? (float*)((uint8_t*)ws + p.parts) : nullptr;
   a.layer = layer, a.x_type = x_dtype, a.heads = heads, a.scale = scale;
   a.wide = (uintptr_t)q % four == 0 && ldq % 4 == 0;
-  a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles;
+  a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles, a.group_rows = p.group_rows;
+  // (a thread has four chunks' loads in flight)
+  a.join_lanes = 1;
+  while (4 * a.join_lanes < p.splits && a.join_lanes < 1024 / cache->head_dim) a.join_lanes *= 2;
   // parts that hold the bits of q (24, 11, 8) in the cache's type, and of the weights
   int qp = 1, pp = 1;
   if (cache->dtype == QMM_BF16) {
@@ -271,13 +281,14 @@ int qmm_kv_attention(const qmm_kv_cache* cache, int layer, const void* q, int x_
     pp = 2;
   }
   char name[64];
-  snprintf(name, sizeof(name), "qmm_kv_attn_%s_d%d_q%d_p%d", mx_type_name(cache->dtype), cache->head_dim, qp, pp);
-  const unsigned threads = cache->dtype == QMM_F32 && cache->head_dim == 256 ? 128 : 256;
+  const char* const forms[] = {"n16", "n32", "wide"};
+  snprintf(name, sizeof(name), "qmm_kv_attn_%s_d%d_%s_q%d_p%d", mx_type_name(cache->dtype), cache->head_dim, forms[p.form], qp, pp);
+  const unsigned threads = cache->dtype == QMM_F32 && cache->head_dim == 256 && p.form != 2 ? 128 : 256;
   const hipStream_t s = (hipStream_t)stream;
   void* args[] = {&a};
   QMM_TRY(kv_launch(d, name, (unsigned)((units + 7) / 8 * 8 * p.tiles), 1, threads, s, args));
   if (p.splits == 1) return QMM_OK;
-  return kv_launch(d, "qmm_kv_attn_join", (unsigned)rows, ceil_div((int64_t)heads * cache->head_dim, 256), 256, s, args);
+  return kv_launch(d, "qmm_kv_attn_join", (unsigned)rows, ceil_div(heads, 1024 / (cache->head_dim * a.join_lanes)), 256, s, args);
 }
 
 size_t qmm_kv_fork_workspace_size(const qmm_kv_cache* cache) {
