@@ -33,21 +33,22 @@ struct BeamArgs {
   int type, beams, vocab, count, eos, slices, wide;
 };
 
-// 2^x for x <= 0, to 2^-31 of its value: the Taylor series of 2^f, |f| <= 1/2, to the
-// eighth power (its ninth term is 0.3466^9 / 9! = 2.0e-10).
-__device__ __forceinline__ double exp2_neg(double x) {
-  x = fmax(x, -1080.0);
-  const double n = rint(x), y = (x - n) * 0.69314718055994530942;
-  double r = 1.0 / 40320.0;
-  r = fma(r, y, 1.0 / 5040.0);
-  r = fma(r, y, 1.0 / 720.0);
-  r = fma(r, y, 1.0 / 120.0);
-  r = fma(r, y, 1.0 / 24.0);
-  r = fma(r, y, 1.0 / 6.0);
-  r = fma(r, y, 0.5);
-  r = fma(r, y, 1.0);
-  r = fma(r, y, 1.0);
-  return ldexp(r, (int)n);
+// e^x for x <= 0, to 2^-34 of its value (at least e^-700): x = n ln 2 + y, |y| <= ln 2 / 2, n from
+// the low bits of a sum with 1.5 2^52, e^y by the polynomial of the seventh degree whose
+// largest relative error there is least (4.0e-11; fitted), n added to the exponent's bits.
+__device__ __forceinline__ double exp_neg(double x) {
+  x = fmax(x, -700.0);
+  const double t = fma(x, 1.4426950408889634, 6755399441055744.0);
+  const double y = fma(t - 6755399441055744.0, -0.6931471805599453, x);
+  double r = 0.00019775106386756418;
+  r = fma(r, y, 0.0013948242373903435);
+  r = fma(r, y, 0.008333561543932654);
+  r = fma(r, y, 0.04166622454803521);
+  r = fma(r, y, 0.16666665121527027);
+  r = fma(r, y, 0.5000000104847449);
+  r = fma(r, y, 1.000000000244067);
+  r = fma(r, y, 0.9999999999615307);
+  return __hiloint2double(__double2hiint(r) + (__double2loint(t) << 20), __double2loint(r));
 }
 
 // A logit as the search takes it (NaN: -inf, +inf: the largest finite value, -0: 0), and
@@ -72,26 +73,67 @@ __device__ __forceinline__ bool beam_live(const BeamArgs& a, int row) {
   return s == s && s != -INFINITY && !(a.finished && a.finished[row]);
 }
 
+// Sum over the 64 lanes of a wave, the same in each: rows of 16 lanes by patterns, then the four
+// rows' (a shuffle has ten times the latency).
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  return __hiloint2double(dpp_i<CTRL>(__double2hiint(v)), dpp_i<CTRL>(__double2loint(v)));
+}
+__device__ __forceinline__ double readlane_d(double v, int l) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+  v += dpp_d<0xb1>(v);
+  v += dpp_d<0x4e>(v);
+  v += dpp_d<0x141>(v);
+  v += dpp_d<0x140>(v);
+  return (readlane_d(v, 0) + readlane_d(v, 16)) + (readlane_d(v, 32) + readlane_d(v, 48));
 }
-__device__ __forceinline__ float wave_max32(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
-}
-}  // namespace qmm
 
-// Grid slices x rows. A thread holds 16 logits. The count-th largest of the threads' own
-// maxima is a bound that the slice's count largest logits pass: `count` threads have a
-// logit at or above it and no other thread has one, so at most 16 count keys pass, and a
-// key's place is the number of larger ones among them.
-extern "C" __global__ void __launch_bounds__(256) qmm_beam_slices(qmm::BeamArgs a) {
-  using namespace qmm;
-  __shared__ uint64_t top[256];
-  __shared__ uint64_t pass[16 * 128];
+// A value as a number whose order is its own, 0 for -inf (no continuation).
+__device__ __forceinline__ uint32_t beam_order(float x) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  return x == -INFINITY ? 0 : b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+// The largest number with zeros behind its first BITS bits that k lanes of the wave are not
+// below (0 where k of them have no more): each bit is one comparison and a count of lanes.
+template <int BITS>
+__device__ __forceinline__ uint32_t wave_bound(uint32_t x, int k) {
+  uint32_t p = 0;
+#pragma unroll
+  for (int b = 31; b >= 32 - BITS; --b) {
+    const uint32_t q = p | 1u << b;
+    if (__popcll(__ballot(x >= q)) >= k) p = q;
+  }
+  return p;
+}
+// A bound that `count` of the workgroup's 256 values pass, from its four waves: a quarter of
+// them in each wave, or (ALL) all in one.
+template <int BITS, bool ALL>
+__device__ __forceinline__ uint32_t block_bound(uint32_t x, int count, uint32_t (*lds)[2]) {
+  const int wave = threadIdx.x >> 6;
+  const uint32_t part = wave_bound<BITS>(x, (count + 3) / 4), all = ALL && count <= 64 ? wave_bound<BITS>(x, count) : 0;
+  if ((threadIdx.x & 63) == 0) {
+    lds[wave][0] = part;
+    lds[wave][1] = all;
+  }
+  __syncthreads();
+  return max(min(min(lds[0][0], lds[1][0]), min(lds[2][0], lds[3][0])),
+             max(max(lds[0][1], lds[1][1]), max(lds[2][1], lds[3][1])));
+}
+constexpr int kBeamPass = 2048;  // keys that a workgroup can rank: 16 * 128
+constexpr int kBeamMany = 512;   // where a closer bound costs less than the ranking
+
+// A slice's maximum, sum of exponentials and `count` largest logits. A thread holds 16 logits;
+// a bound that the `count` largest of the threads' maxima pass is one that as many logits of the
+// slice pass. A key's place is the number of larger ones among those that do. Where more than
+// kBeamMany do (equal logits, a wave without any), the bound is the count-th largest of the threads' largest keys,
+// which no two logits share: `count` threads have a key at or above it and no other thread has.
+template <int TYPE>
+__device__ __forceinline__ void beam_slice(const BeamArgs& a) {
+  constexpr int WIDE = TYPE == kTypeF32 ? 4 : 8;  // consecutive logits of a thread (16 bytes)
+  __shared__ uint64_t pass[kBeamPass];
+  __shared__ uint32_t bounds[4][2];
   __shared__ uint64_t bound;
   __shared__ int passed;
   __shared__ float wmax[4];
@@ -99,59 +141,94 @@ extern "C" __global__ void __launch_bounds__(256) qmm_beam_slices(qmm::BeamArgs 
   const int row = blockIdx.y, sl = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
   if (!beam_live(a, row)) return;
   const int first = sl * kBeamSlice;
+  // (a last slice, which is short, is spread over the waves)
+  const bool whole = a.wide && first + kBeamSlice <= a.vocab;
+  auto token = [&](int i) { return first + (whole ? 256 * WIDE * (i / WIDE) + WIDE * t + i % WIDE : 256 * i + t); };
   float x[16];
+  if (whole) {
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int i = first + 1024 * u + 4 * t;
-    float v[4];
-    if (i + 4 <= a.vocab) {
-      load4_typed(v, a.logits, row * a.ld + i, a.type, a.wide);
-    } else {
+    for (int u = 0; u < 16 / WIDE; ++u) {
+      const long long at = row * a.ld + first + 256 * WIDE * u + WIDE * t;
+      if constexpr (TYPE == kTypeF32) {
+        const float4 v = *(const float4*)((const float*)a.logits + at);
+        x[4 * u] = v.x, x[4 * u + 1] = v.y, x[4 * u + 2] = v.z, x[4 * u + 3] = v.w;
+      } else {
+        const uint4 v = *(const uint4*)((const uint16_t*)a.logits + at);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = i + e < a.vocab ? load_typed(a.logits, row * a.ld + i + e, a.type) : -INFINITY;
+        for (int e = 0; e < 8; ++e) x[8 * u + e] = from_half((uint16_t)(w[e / 2] >> 16 * (e & 1)), TYPE);
+      }
     }
+  } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[4 * u + e] = beam_logit(v[e]);
+    for (int i = 0; i < 16; ++i) x[i] = token(i) < a.vocab ? load_typed(a.logits, row * a.ld + token(i), TYPE) : -INFINITY;
   }
-  float m = x[0];
-  uint64_t best = 0;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) odd |= !(fabsf(x[i]) < INFINITY);
+  if (__any(odd)) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = beam_logit(x[i]);
+  }
+  float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
+    x[i] += 0.0f;  // (-0 is 0)
     m = fmaxf(m, x[i]);
-    const uint64_t k = beam_key(x[i], first + 1024 * (i / 4) + 4 * t + i % 4);
-    best = k > best ? k : best;
   }
-  m = wave_max32(m);
+  const uint32_t mine = beam_order(m);
+  m = wave_max(m);
   if (lane == 0) wmax[wave] = m;
-  top[t] = best;
   if (t == 0) passed = 0;
-  __syncthreads();
+  const uint32_t least = max(block_bound<16, false>(mine, a.count, bounds), 1u);
   m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-  // (threads without a key have the key 0: the lower thread first)
-  int place = 0;
-  for (int i = 0; i < 256; ++i) place += top[i] > best || (top[i] == best && i < t) ? 1 : 0;
-  if (place == a.count - 1) bound = best;
+  if (mine >= least) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (beam_order(x[i]) >= least) {
+        const int at = atomicAdd(&passed, 1);
+        if (at < kBeamPass) pass[at] = beam_key(x[i], token(i));
+      }
+  }
   double z = 0.0;
   if (m != -INFINITY) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) z += exp2_neg(((double)x[i] - (double)m) * 1.44269504088896340736);
+    for (int i = 0; i < 16; ++i) z += exp_neg((double)x[i] - (double)m);
   }
   z = wave_sum64(z);
   if (lane == 0) wsum[wave] = z;
   __syncthreads();
-  const uint64_t least = bound ? bound : 1;
+  if (__builtin_expect(passed > kBeamMany, 0)) {
+    uint64_t best = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint64_t k = beam_key(x[i], first + 1024 * (i / 4) + 4 * t + i % 4);
-    if (k >= least) pass[atomicAdd(&passed, 1)] = k;
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t k = beam_key(x[i], token(i));
+      best = k > best ? k : best;
+    }
+    __syncthreads();
+    pass[t] = best;
+    __syncthreads();
+    // (threads without a key have the key 0: the lower thread first)
+    int place = 0;
+    for (int i = 0; i < 256; ++i) place += pass[i] > best || (pass[i] == best && i < t) ? 1 : 0;
+    if (place == a.count - 1) bound = best;
+    if (t == 0) passed = 0;
+    __syncthreads();
+    const uint64_t exact = bound ? bound : 1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t k = beam_key(x[i], token(i));
+      if (k >= exact) pass[atomicAdd(&passed, 1)] = k;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   const long long slot = (long long)row * a.slices + sl;
   uint64_t* list = a.lists + slot * a.count;
   const int n = passed;
   for (int i = t; i < n; i += 256) {
     const uint64_t k = pass[i];
     int at = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) at += pass[j] > k;
     if (at < a.count) list[at] = k;
   }
@@ -162,108 +239,165 @@ extern "C" __global__ void __launch_bounds__(256) qmm_beam_slices(qmm::BeamArgs 
   }
 }
 
-// One workgroup a search: the beams' lse, then `count` times the best head of its lists
-// (beams x slices of them, list l = beam * slices + slice; a finished beam's first list is
-// its end). A thread holds the best head of its lists.
+// A continuation: its score, and beam and key, which order equal ones (a beam past all: none).
+struct BeamBest {
+  double s;
+  uint64_t key;
+  int beam;
+  __device__ __forceinline__ bool before(const BeamBest& o) const {
+    return s > o.s || (s == o.s && (beam < o.beam || (beam == o.beam && key > o.key)));
+  }
+};
+constexpr int kBeamNone = 0x7fffffff;
+constexpr int kBeamRank = 1024;  // continuations that the merge ranks
+}  // namespace qmm
+
+// Grid slices x rows.
+extern "C" __global__ void __launch_bounds__(256) qmm_beam_slices_f32(qmm::BeamArgs a) { qmm::beam_slice<qmm::kTypeF32>(a); }
+extern "C" __global__ void __launch_bounds__(256) qmm_beam_slices_f16(qmm::BeamArgs a) { qmm::beam_slice<qmm::kTypeF16>(a); }
+extern "C" __global__ void __launch_bounds__(256) qmm_beam_slices_bf16(qmm::BeamArgs a) { qmm::beam_slice<qmm::kTypeBF16>(a); }
+
+// One workgroup a search: the beams' lse, then the best of its lists (beams x slices of them,
+// list l = beam * slices + slice; a finished beam's first list is its end). A bound that the
+// `count` best of the threads' best heads pass is one that as many continuations pass; a
+// thread takes what passes from the heads of its lists on, and places are counted as in a
+// slice. Where more than kBeamRank pass, the best head is taken `count` times.
 extern "C" __global__ void __launch_bounds__(256) qmm_beam_merge(qmm::BeamArgs a) {
   using namespace qmm;
-  __shared__ double lse[64];
-  __shared__ double wbest[2][4];
-  __shared__ uint64_t wtie[2][4];
+  __shared__ double lse[64], total[64];
+  __shared__ float score[64];  // -inf: no continuation
+  __shared__ int ended[64];
+  __shared__ uint32_t bounds[4][2];
+  __shared__ int passed;
+  __shared__ double pass_s[kBeamRank];
+  __shared__ uint64_t pass_key[kBeamRank];
+  __shared__ int pass_beam[kBeamRank];
+  __shared__ BeamBest wbest[2][4];
   __shared__ uint8_t taken[kBeamMaxLists];  // entries that each list has given
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, row0 = b * a.beams;
-  for (int w = wave; w < a.beams; w += 4) {
-    const int row = row0 + w;
-    if (!beam_live(a, row)) continue;
-    float m = -INFINITY;
-    for (int i = lane; i < a.slices; i += 64) m = fmaxf(m, a.maxima[(long long)row * a.slices + i]);
-    m = wave_max32(m);
-    double z = 0.0;
-    if (m != -INFINITY)
-      for (int i = lane; i < a.slices; i += 64) {
-        const long long at = (long long)row * a.slices + i;
-        if (a.maxima[at] != -INFINITY)
-          z += a.sums[at] * exp2_neg(((double)a.maxima[at] - (double)m) * 1.44269504088896340736);
-      }
-    z = wave_sum64(z);
-    if (lane == 0) lse[w] = (double)m + log(z);
-  }
   const int lists = a.beams * a.slices;
-  for (int l = t; l < lists; l += 256) taken[l] = 0;
-  __syncthreads();
-  // the head of list l past its first `skip` entries: score, and what orders equal ones
-  auto head = [&](int l, int skip, double& s, uint64_t& tie) {
-    s = -INFINITY;
-    tie = ~0ull;
-    const int w = l / a.slices, row = row0 + w;
-    const float score = a.scores[row];
-    if (!(score > -INFINITY)) return;
-    if (a.finished && a.finished[row]) {
-      if (l % a.slices == 0 && skip == 0) {
-        s = score;
-        tie = (uint64_t)w << 32 | (uint32_t)a.eos;
-      }
-      return;
+  // all first loads at once; of beams without a slice's results they are not used
+  const uint64_t* all = a.lists + (long long)row0 * a.slices * a.count;
+  uint64_t early[2] = {0, 0};  // the first entries of this thread's first list
+  if (t < lists) {
+    early[0] = all[(long long)t * a.count];
+    if (a.count > 1) early[1] = all[(long long)t * a.count + 1];
+  }
+  if (t < a.beams) {
+    const float s = a.scores[row0 + t];
+    score[t] = s == s ? s : -INFINITY;
+    ended[t] = a.finished ? a.finished[row0 + t] : 0;
+  }
+  if (t == 0) passed = 0;
+  for (int w0 = wave; w0 < a.beams; w0 += 16) {  // four beams a wave, their loads together
+    float m0[4];
+    double z0[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long at = (long long)(row0 + min(w0 + 4 * i, a.beams - 1)) * a.slices + min(lane, a.slices - 1);
+      m0[i] = a.maxima[at];
+      z0[i] = a.sums[at];
     }
-    if (skip >= a.count) return;
-    const uint64_t k = a.lists[((long long)row * a.slices + l % a.slices) * a.count + skip];
-    if (k == 0) return;
-    s = (double)score + ((double)beam_value(k) - lse[w]);
-    tie = (uint64_t)w << 32 | (uint32_t)beam_token(k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int w = w0 + 4 * i;
+      if (w >= a.beams) break;
+      const long long at = (long long)(row0 + w) * a.slices;
+      if (lane >= a.slices) m0[i] = -INFINITY;
+      float m = m0[i];
+      for (int j = lane + 64; j < a.slices; j += 64) m = fmaxf(m, a.maxima[at + j]);
+      m = wave_max(m);
+      double z = m0[i] > -INFINITY ? z0[i] * exp_neg((double)m0[i] - (double)m) : 0.0;
+      for (int j = lane + 64; j < a.slices; j += 64)
+        if (a.maxima[at + j] > -INFINITY) z += a.sums[at + j] * exp_neg((double)a.maxima[at + j] - (double)m);
+      z = wave_sum64(z);
+      if (lane == 0) {
+        lse[w] = (double)m;
+        total[w] = z;
+      }
+    }
+  }
+  __syncthreads();
+  if (t < a.beams) lse[t] += log(total[t]);
+  __syncthreads();
+  const BeamBest none = {-INFINITY, 0, kBeamNone};
+  // entry `skip` of list l
+  auto entry = [&](int l, int skip) {
+    const int w = l / a.slices;
+    if (!(score[w] > -INFINITY)) return none;
+    if (ended[w]) return l % a.slices == 0 && skip == 0 ? BeamBest{score[w], beam_key(0.0f, a.eos), w} : none;
+    if (skip >= a.count) return none;
+    const uint64_t k = l == t && skip < 2 ? (skip ? early[1] : early[0]) : all[(long long)l * a.count + skip];
+    if (k == 0) return none;
+    return BeamBest{(double)score[w] + ((double)beam_value(k) - lse[w]), k, w};
   };
-  double s = -INFINITY;
-  uint64_t tie = ~0ull;
+  auto put = [&](int n, const BeamBest& x) {
+    const bool no = x.beam == kBeamNone;
+    const long long o = (long long)b * a.count + n;
+    const int token = beam_token(x.key);
+    a.tokens[o] = no ? -1 : token;
+    a.parents[o] = no ? -1 : row0 + x.beam;
+    a.out_scores[o] = no ? -INFINITY : (float)x.s;
+    if (a.out_finished) a.out_finished[o] = !no && (ended[x.beam] || token == a.eos);
+  };
+  // (a rounding to f32 keeps the order, so what passes a bound as f32 holds the best)
+  float top = -INFINITY;
+  for (int l = t; l < lists; l += 256) top = fmaxf(top, (float)entry(l, 0).s);
+  const uint32_t least = max(block_bound<20, true>(beam_order(top), a.count, bounds), 1u);
+  if (beam_order(top) >= least)
+    for (int l = t; l < lists; l += 256)
+      for (int i = 0; i < a.count; ++i) {
+        const BeamBest x = entry(l, i);
+        if (beam_order((float)x.s) < least) break;
+        const int at = atomicAdd(&passed, 1);
+        if (at < kBeamRank) pass_s[at] = x.s, pass_key[at] = x.key, pass_beam[at] = x.beam;
+      }
+  __syncthreads();
+  const int n = passed;
+  if (__builtin_expect(n <= kBeamRank, 1)) {
+    for (int i = t; i < n; i += 256) {
+      const BeamBest x = {pass_s[i], pass_key[i], pass_beam[i]};
+      int at = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const double s = pass_s[j];
+        at += s > x.s;
+        if (__builtin_expect(s == x.s && j != i, 0)) at += BeamBest{s, pass_key[j], pass_beam[j]}.before(x);
+      }
+      if (at < a.count) put(at, x);
+    }
+    for (int i = n + t; i < a.count; i += 256) put(i, none);
+    return;
+  }
+  for (int l = t; l < lists; l += 256) taken[l] = 0;  // (a thread's own lists)
+  BeamBest best = none;
   int mine = 0;  // the best head of this thread's lists, and its list
   auto best_of = [&]() {
-    s = -INFINITY;
-    tie = ~0ull;
+    best = none;
     for (int l = t; l < lists; l += 256) {
-      double hs;
-      uint64_t ht;
-      head(l, taken[l], hs, ht);
-      if (hs > s || (hs == s && ht < tie)) {
-        s = hs;
-        tie = ht;
+      const BeamBest x = entry(l, taken[l]);
+      if (x.before(best)) {
+        best = x;
         mine = l;
       }
     }
   };
   best_of();
-  for (int n = 0; n < a.count; ++n) {
-    double ws = s;
-    uint64_t wt = tie;
+  for (int i = 0; i < a.count; ++i) {
+    BeamBest w = best;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-      const double os = __shfl_xor(ws, o);
-      const uint64_t ot = __shfl_xor((unsigned long long)wt, o);
-      if (os > ws || (os == ws && ot < wt)) {
-        ws = os;
-        wt = ot;
-      }
+      const BeamBest x = {__shfl_xor(w.s, o), (uint64_t)__shfl_xor((unsigned long long)w.key, o), __shfl_xor(w.beam, o)};
+      if (x.before(w)) w = x;
     }
-    if (lane == 0) {
-      wbest[n & 1][wave] = ws;
-      wtie[n & 1][wave] = wt;
-    }
+    if (lane == 0) wbest[i & 1][wave] = w;
     __syncthreads();
-    ws = wbest[n & 1][0];
-    wt = wtie[n & 1][0];
+    w = wbest[i & 1][0];
 #pragma unroll
-    for (int i = 1; i < 4; ++i)
-      if (wbest[n & 1][i] > ws || (wbest[n & 1][i] == ws && wtie[n & 1][i] < wt)) {
-        ws = wbest[n & 1][i];
-        wt = wtie[n & 1][i];
-      }
-    const bool none = wt == ~0ull;
-    const long long o = (long long)b * a.count + n;
-    const int row = row0 + (int)(wt >> 32), token = (int)(uint32_t)wt;
-    if (t == 0) {
-      a.tokens[o] = none ? -1 : token;
-      a.parents[o] = none ? -1 : row;
-      a.out_scores[o] = none ? -INFINITY : (float)ws;
-      if (a.out_finished) a.out_finished[o] = !none && ((a.finished && a.finished[row]) || token == a.eos);
-    }
-    if (!none && tie == wt) {  // (a beam and token stand in one list)
+    for (int j = 1; j < 4; ++j)
+      if (wbest[i & 1][j].before(w)) w = wbest[i & 1][j];
+    if (t == 0) put(i, w);
+    if (w.beam != kBeamNone && best.beam == w.beam && best.key == w.key) {  // (a beam and token stand in one list)
       ++taken[mine];
       best_of();
     }

@@ -398,7 +398,7 @@ int qmm_beam_select(const void* logits, int dtype, int64_t ld, int64_t batch, in
   QMM_TRY(kv_workspace(ws, ws_bytes, qmm_beam_select_workspace_size(batch, beams, vocab, count)));
   Device* d;
   QMM_TRY(current_device(&d));
-  const size_t rows = (size_t)(batch * beams), slices = ceil_div(vocab, kBeamSlice), four = 4 * kv_esize(dtype);
+  const size_t rows = (size_t)(batch * beams), slices = ceil_div(vocab, kBeamSlice);
   uint8_t* p = (uint8_t*)ws;
   BeamArgs a = {};
   a.logits = logits, a.ld = ld, a.scores = scores, a.finished = finished;
@@ -406,10 +406,10 @@ int qmm_beam_select(const void* logits, int dtype, int64_t ld, int64_t batch, in
   a.sums = kv_take<double>(p, rows * slices), a.maxima = kv_take<float>(p, rows * slices);
   a.lists = kv_take<uint64_t>(p, rows * slices * (size_t)count);
   a.type = dtype, a.beams = beams, a.vocab = (int)vocab, a.count = count, a.eos = eos, a.slices = (int)slices;
-  a.wide = (uintptr_t)logits % four == 0 && ld % 4 == 0;
+  a.wide = (uintptr_t)logits % 16 == 0 && ld * (int64_t)kv_esize(dtype) % 16 == 0;
   const hipStream_t s = (hipStream_t)stream;
   void* args[] = {&a};
-  QMM_TRY(kv_launch(d, "qmm_beam_slices", (unsigned)slices, (unsigned)rows, 256, s, args));
+  QMM_TRY(kv_launch(d, dtype == QMM_F32 ? "qmm_beam_slices_f32" : dtype == QMM_F16 ? "qmm_beam_slices_f16" : "qmm_beam_slices_bf16", (unsigned)slices, (unsigned)rows, 256, s, args));
   return kv_launch(d, "qmm_beam_merge", (unsigned)batch, 1, 256, s, args);
 }
 

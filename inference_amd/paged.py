@@ -32,10 +32,20 @@ def _bad(message: str) -> QmmError:
     return QmmError(QMM_ERR_INVALID, message)
 
 
-def _ints(t: torch.Tensor, shape: Sequence[int], dev: torch.device, what: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+def _ints(t: torch.Tensor, shape: Tuple[int, ...], dev: torch.device, what: str) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.device != dev or t.shape != shape or not t.is_contiguous():
         raise _bad(f"{what} must be contiguous int32 {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t
+
+
+def _packed(t: torch.Tensor) -> bool:
+    """Whether t's rows (along the first dimension) are contiguous and do not overlap."""
+    n = 1
+    for size, stride in zip(t.shape[:0:-1], t.stride()[:0:-1]):
+        if stride != n and size != 1:
+            return False
+        n *= size
+    return t.shape[0] <= 1 or t.stride(0) >= n
 
 
 def _run(dev: torch.device, fn, *args) -> None:
@@ -270,6 +280,9 @@ class PagedKVCache:
         return used
 
 
+_beam_ws: dict = {}  # workspace sizes by their arguments
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: int,
                 finished: Optional[torch.Tensor] = None, eos: int = -1):
     """The `count` best continuations of every search of `beams` beams: logits [batch * beams, vocab] (float32,
@@ -284,7 +297,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: i
     rows, vocab = logits.shape
     if beams < 1 or rows % beams:
         raise _bad(f"{rows} rows of logits are not whole searches of {beams} beams")
-    if scores.dtype != torch.float32 or scores.shape != (rows,) or scores.device != dev or not scores.is_contiguous():
+    if scores.dtype is not torch.float32 or scores.shape != (rows,) or scores.device != dev or not scores.is_contiguous():
         raise _bad(f"scores must be contiguous float32 [{rows}] on {dev}, got {scores.dtype} {list(scores.shape)} on "
                    f"{scores.device}")
     if finished is not None:
@@ -293,12 +306,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: i
         logits = logits.contiguous()
     batch = rows // beams
     L = lib()
-    nws = int(L.qmm_beam_select_workspace_size(batch, beams, vocab, count))
-    if nws == 0:
-        raise _bad("beam_select: " + last_error())
-    n = batch * count
-    tokens, parents, done, out = torch.empty((4, batch, count), dtype=torch.int32, device=dev).unbind()
-    out = out.view(torch.float32)
+    key = (batch, beams, vocab, count)
+    nws = _beam_ws.get(key)
+    if nws is None:
+        nws = int(L.qmm_beam_select_workspace_size(*key))
+        if nws == 0:
+            raise _bad("beam_select: " + last_error())
+        _beam_ws[key] = nws
+    out = torch.empty((batch, count), dtype=torch.float32, device=dev)
+    tokens, parents, done = torch.empty((3, batch, count), dtype=torch.int32, device=dev).unbind()
     ws = torch.empty(nws, dtype=torch.uint8, device=dev)
     _run(dev, L.qmm_beam_select, logits.data_ptr(), _DENSE[logits.dtype], logits.stride(0) if rows > 1 else vocab, batch,
          beams, vocab, scores.data_ptr(), _ptr(finished), eos, count, tokens.data_ptr(), parents.data_ptr(),
@@ -317,17 +333,16 @@ def reorder_rows(src: torch.Tensor, index: torch.Tensor, out: Optional[torch.Ten
     rows = index.shape[0]
     _ints(index, (rows,), dev, "index")
     inner = src.shape[1:]
-    if src.shape[0] > 0 and not src[0].is_contiguous() or (src.shape[0] > 1 and src.stride(0) < src[0].numel()):
+    if not _packed(src):
         src = src.contiguous()
     if out is None:
         out = torch.zeros((rows, *inner), dtype=src.dtype, device=dev)
-    if out.shape != (rows, *inner) or out.dtype != src.dtype or out.device != dev or \
-            (rows > 0 and not out[0].is_contiguous()) or (rows > 1 and out.stride(0) < out[0].numel()):
+    elif out.shape != (rows, *inner) or out.dtype != src.dtype or out.device != dev or not _packed(out):
         raise _bad(f"out must be {src.dtype} [{rows}, ...] with rows like src's on {dev}, got {out.dtype} "
                    f"{list(out.shape)} on {out.device}")
-    if rows and src.shape[0] and out[0].numel():
+    if rows and src.numel() and out.numel():
         size = src.element_size()
-        nbytes = out[0].numel() * size
+        nbytes = inner.numel() * size
         _run(dev, lib().qmm_reorder_rows, src.data_ptr(), src.shape[0],
              src.stride(0) * size if src.shape[0] > 1 else nbytes, out.data_ptr(),
              out.stride(0) * size if rows > 1 else nbytes, nbytes, index.data_ptr(), rows)
