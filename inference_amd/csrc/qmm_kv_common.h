@@ -9,6 +9,7 @@
 
 namespace qmm {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 30;  // the C ABI's tags
 
 struct KvCache {

@@ -137,6 +137,8 @@ KvSplit kv_split(const qmm_kv_cache* c, int64_t rows, int max_rows, int64_t max_
   return p;
 }
 
+// List entries up to which one workgroup does a fork (qmm::kForkLists).
+constexpr int64_t kKvForkSmall = 16384;
 struct KvFork {
   KvCache c;
   const int32_t *parents, *keep;
@@ -320,10 +322,14 @@ int qmm_kv_fork(const qmm_kv_cache* cache, const int32_t* parents, const int32_t
   const hipStream_t s = (hipStream_t)stream;
   void* args[] = {&f};
   const int64_t n = std::max<int64_t>(cells, cache->pages);
-  QMM_TRY(kv_launch(d, "qmm_kv_fork_begin", kv_grid(d, n), 1, 256, s, args));
-  QMM_TRY(kv_launch(d, "qmm_kv_fork_count", kv_grid(d, 64LL * cache->slots), 1, 256, s, args));
-  QMM_TRY(kv_launch(d, "qmm_kv_fork_plan", 1, 1, 1024, s, args));
-  QMM_TRY(kv_launch(d, "qmm_kv_fork_commit", kv_grid(d, n), 1, 256, s, args));
+  if (cells + 4 * (cache->pages + cache->slots) <= kKvForkSmall) {
+    QMM_TRY(kv_launch(d, "qmm_kv_fork_small", 1, 1, 1024, s, args));
+  } else {
+    QMM_TRY(kv_launch(d, "qmm_kv_fork_begin", kv_grid(d, n), 1, 256, s, args));
+    QMM_TRY(kv_launch(d, "qmm_kv_fork_count", kv_grid(d, 64LL * cache->slots), 1, 256, s, args));
+    QMM_TRY(kv_launch(d, "qmm_kv_fork_plan", 1, 1, 1024, s, args));
+    QMM_TRY(kv_launch(d, "qmm_kv_fork_commit", kv_grid(d, n), 1, 256, s, args));
+  }
   if (reserve == 0) return QMM_OK;  // nothing is about to be written: no copies
   return kv_copy_pages(d, f.c, f.moves, cache->slots, s);
 }
@@ -340,10 +346,15 @@ int qmm_kv_accept(const qmm_kv_cache* cache, const int32_t* path, int64_t ld_pat
   const hipStream_t s = (hipStream_t)stream;
   void* args[] = {&a};
   if (path) {
+    // (lengths that are the cache's own change behind the last read of them, in a launch of their own)
+    const bool own = lens_out == cache->lens;
+    if (own) a.lens_out = nullptr;
     const int64_t columns = 2LL * cache->layers * cache->kv_heads * ((int64_t)cache->head_dim * kv_esize(cache->dtype) / 16);
     QMM_TRY(kv_launch(d, "qmm_kv_accept_rows", ceil_div(columns, 256), (unsigned)cache->slots, 256, s, args));
+    if (!own) return QMM_OK;
+    a.lens_out = lens_out;
   }
-  return kv_launch(d, "qmm_kv_accept_lens", ceil_div(cache->slots, 256), 1, 256, s, args);
+  return kv_launch(d, "qmm_kv_accept_lens", ceil_div(cache->slots, 4), 1, 256, s, args);
 }
 
 size_t qmm_kv_compact_workspace_size(const qmm_kv_cache* cache) {

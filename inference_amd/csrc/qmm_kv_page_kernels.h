@@ -33,7 +33,7 @@ __device__ __forceinline__ void agent_add(int* p, int v) {
 }
 // A barrier after which agent_load sees what the workgroup's agent stores and adds before it left.
 __device__ __forceinline__ void agent_barrier() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
 }
 }  // namespace qmm
@@ -112,6 +112,8 @@ struct KvFork {
   int32_t *moves;                   // [1 + 3 slots]: number of copies; source, destination, rows of each
 };
 
+constexpr int kForkLists = 16384;  // entries of the lists of a small fork
+
 // A slot's new length in positions, whole and part-filled pages of it, and those with the reserve.
 struct KvGrow {
   int len, held, total;
@@ -133,8 +135,8 @@ __device__ __forceinline__ void kv_fork_begin(const KvFork& f, long long t, long
     agent_store(f.writers + p, 0);
     agent_store(f.first + p, 0x7fffffff);
   }
-  const long long cells = (long long)f.c.slots * f.c.max_pages;
-  for (long long i = t; i < cells; i += n) {
+  const unsigned cells = (unsigned)f.c.slots * (unsigned)f.c.max_pages;  // (2^28 at most)
+  for (unsigned i = (unsigned)t; i < cells; i += (unsigned)n) {
     const int p = f.c.table[i];
     agent_store(f.table + i, p >= 0 && p < f.c.pages ? p : -1);
   }
@@ -255,27 +257,26 @@ __device__ __forceinline__ void kv_fork_commit(const KvFork& f, long long t, lon
   const bool ok = agent_load(f.shortage) == 0;
   // (refs_out and table_out may be the cache's own: without room they get back what they held)
   for (long long p = t; p < f.c.pages; p += n) f.refs_out[p] = ok ? agent_load(f.refs + p) : f.c.refs[p];
-  const long long cells = (long long)f.c.slots * f.c.max_pages;
-  for (long long i = t; i < cells; i += n) {
+  const int lane = (int)(t & 63);
+  for (long long s = t >> 6; s < f.c.slots; s += n >> 6) {  // a wave a row
+    const long long row = s * f.c.max_pages;
     if (!ok) {
-      f.table_out[i] = f.c.table[i];
+      for (int j = lane; j < f.c.max_pages; j += 64) f.table_out[row + j] = f.c.table[row + j];
+      if (lane == 0) f.lens_out[s] = f.c.lens[s];
       continue;
     }
-    const int s = (int)(i / f.c.max_pages), j = (int)(i % f.c.max_pages);
-    const int from = agent_load(f.parent + s);
-    int p = -1;
-    if (from >= 0) {
-      const KvGrow g = kv_grow(f, s);
-      const int copy = agent_load(f.copy + s) >= 0;
-      if (j < g.held)
-        p = copy && j == g.held - 1 ? agent_load(f.free_ids + agent_load(f.at + s))
-                                    : agent_load(f.table + (long long)from * f.c.max_pages + j);
-      else if (j < g.total)
-        p = agent_load(f.free_ids + agent_load(f.at + s) + copy + j - g.held);
+    const int from = agent_load(f.parent + s), at = agent_load(f.at + s), copy = agent_load(f.copy + s) >= 0;
+    const KvGrow g = kv_grow(f, (int)s);
+    for (int j = lane; j < f.c.max_pages; j += 64) {
+      int p = -1;
+      if (from >= 0 && j < g.held && !(copy && j == g.held - 1))
+        p = agent_load(f.table + (long long)from * f.c.max_pages + j);
+      else if (j < g.total && (copy || j >= g.held))  // (a copied last page is the first of the slot's new ones)
+        p = agent_load(f.free_ids + at + copy + j - g.held);
+      f.table_out[row + j] = p;
     }
-    f.table_out[i] = p;
+    if (lane == 0) f.lens_out[s] = g.len;
   }
-  for (long long s = t; s < f.c.slots; s += n) f.lens_out[s] = ok ? agent_load(f.lens + s) : f.c.lens[s];
 }
 }  // namespace qmm
 
@@ -293,19 +294,47 @@ extern "C" __global__ void __launch_bounds__(256) qmm_kv_fork_commit(qmm::KvFork
   qmm::kv_fork_commit(f, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
 }
 
-// The listed pages' first rows (a whole page: rows = page size) to other pages, in every
-// layer and of every kv head. Sources and destinations are disjoint. Bound by the bytes.
+// All phases of a small fork in one workgroup, its lists in LDS: launches and round trips to
+// memory cost more than the work (with the copies, 4 slots of 64 pages 11.0 us against 15.4 in
+// four launches, 32 of 256 13.6 against 19.3; with the lists in memory 13.4 and 20.8).
+extern "C" __global__ void __launch_bounds__(1024) qmm_kv_fork_small(qmm::KvFork f) {
+  using namespace qmm;
+  __shared__ int lds[16];
+  __shared__ int32_t lists[kForkLists];
+  int32_t* at = lists;
+  auto take = [&](int n) {
+    int32_t* p = at;
+    at += n;
+    return p;
+  };
+  f.refs = take(f.c.pages), f.writers = take(f.c.pages), f.first = take(f.c.pages), f.free_ids = take(f.c.pages);
+  f.lens = take(f.c.slots), f.at = take(f.c.slots), f.parent = take(f.c.slots), f.copy = take(f.c.slots);
+  f.table = take(f.c.slots * f.c.max_pages);
+  const int t = threadIdx.x;
+  kv_fork_begin(f, t, 1024);
+  agent_barrier();
+  kv_fork_count(f, t >> 6, 16, t & 63);
+  agent_barrier();
+  kv_fork_plan(f, lds);
+  agent_barrier();
+  kv_fork_commit(f, t, 1024);
+}
+
+// The listed pages' first rows (a whole page: rows = page size) to other pages, in every layer
+// and of every kv head. Sources and destinations are disjoint. A workgroup takes a head's rows
+// of a page, side and layer at a time. Bound by the bytes: 512 of 2048 pages of 32 KB moved in 8
+// layers 105 us for 537 MB there and back (16 KB at a time over the heads, four loads a thread
+// in flight: 107, and for half-filled pages of 64 rows 41 us against 29).
 extern "C" __global__ void __launch_bounds__(256) qmm_kv_copy_pages(qmm::KvCache c, const int* moves) {
   using namespace qmm;
-  const int count = moves[0];
-  const long long items = (long long)count * c.layers * 2 * c.kv_heads;
+  const long long items = (long long)moves[0] * c.layers * 2 * c.kv_heads;
   for (long long i = blockIdx.x; i < items; i += gridDim.x) {
     const int g = (int)(i % c.kv_heads), side = (int)(i / c.kv_heads % 2);
     const int layer = (int)(i / (2 * c.kv_heads) % c.layers);
     const int* m = moves + 1 + 3 * (i / (2LL * c.kv_heads * c.layers));
     char* pool = (char*)(side ? c.v : c.k);
-    const uint4* src = (const uint4*)(pool + (c.row(layer, m[0], g, 0) << c.esize_log()));
-    uint4* dst = (uint4*)(pool + (c.row(layer, m[1], g, 0) << c.esize_log()));
+    const u32x4* src = (const u32x4*)(pool + (c.row(layer, m[0], g, 0) << c.esize_log()));
+    u32x4* dst = (u32x4*)(pool + (c.row(layer, m[1], g, 0) << c.esize_log()));
     const int n = (m[2] * c.head_dim << c.esize_log()) / 16;
     for (int x = threadIdx.x; x < n; x += 256) dst[x] = src[x];
   }
@@ -323,58 +352,95 @@ struct KvAccept {
   int max_path;
 };
 
-// Entry d of the slot's path where it goes on: above `last`, its position and its place in
-// pages of the slot; -1 where the path ends.
-__device__ __forceinline__ int kv_path(const KvAccept& a, int s, int base, int d, int last) {
-  const int to = a.path[s * a.ld_path + d];
-  if (to <= last || to >= a.c.capacity() - base) return -1;
-  if (a.c.page(s, (base + to) >> a.c.page_log) < 0 || a.c.page(s, (base + d) >> a.c.page_log) < 0) return -1;
-  return to;
+// Entries d0 .. d0 + 63 of a slot's path, one a lane of a wave: how many of them hold (each above
+// the one before, `last` before the first; its position and its place in pages of the slot), and
+// this lane's.
+struct KvStep {
+  int from, src, dst;  // the entry; the pages of its position and of its place
+};
+__device__ __forceinline__ int kv_path(const KvAccept& a, int s, int base, int d0, int n, int& last, KvStep& e) {
+  const int lane = threadIdx.x & 63, d = d0 + lane;
+  e.from = d < n ? a.path[s * a.ld_path + d] : -1;
+  int before = __shfl_up(e.from, 1);
+  if (lane == 0) before = last;
+  bool ok = d < n && e.from > before && e.from < a.c.capacity() - base;
+  if (ok) {
+    e.src = a.c.page(s, (base + e.from) >> a.c.page_log);
+    e.dst = a.c.page(s, (base + d) >> a.c.page_log);
+    ok = e.src >= 0 && e.dst >= 0;
+  }
+  last = __builtin_amdgcn_readlane(e.from, 63);
+  const uint64_t bad = ~__ballot(ok);
+  return bad ? __builtin_ctzll(bad) : 64;
 }
 }  // namespace qmm
 
 // Position base + path[d] to base + d, a thread a 16-byte column of a layer's, side's and
-// head's rows, in order: path[d] >= d and rises, so no row is overwritten before it is read.
+// head's rows. path[d] >= d and rises, so that no entry is on a row that an earlier one's goes
+// to: eight are read and then written. The lengths here too, unless another workgroup may yet
+// read them (lens_out null).
 extern "C" __global__ void __launch_bounds__(256) qmm_kv_accept_rows(qmm::KvAccept a) {
   using namespace qmm;
+  __shared__ long long from[64], to[64];
+  __shared__ int held;
   const KvCache& c = a.c;
-  const int s = blockIdx.y, base = c.length(s), n = min(a.counts[s], a.max_path);
-  const int per = (c.head_dim << c.esize_log()) / 16;
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  if (i >= 2LL * c.layers * c.kv_heads * per) return;
+  const int s = blockIdx.y, base = c.length(s), n = min(a.counts[s], a.max_path), t = threadIdx.x;
+  const int per = (c.head_dim << c.esize_log()) / 16, low = (1 << c.page_log) - 1;
+  const unsigned i = blockIdx.x * 256 + t;
+  const bool on = i < 2u * c.layers * c.kv_heads * per;
   const int x = (int)(i % per), g = (int)(i / per % c.kv_heads), side = (int)(i / per / c.kv_heads % 2);
-  const int layer = (int)(i / per / c.kv_heads / 2);
-  char* pool = (char*)(side ? c.v : c.k);
-  const int low = (1 << c.page_log) - 1;
-  auto at = [&](int t) {
-    return (uint4*)(pool + (c.row(layer, c.page(s, t >> c.page_log), g, t & low) << c.esize_log())) + x;
-  };
-  int last = -1;
-  for (int d = 0; d < n; ++d) {
-    last = kv_path(a, s, base, d, last);
-    if (last < 0) break;
-    if (last != d) *at(base + d) = *at(base + last);
+  const int layer = on ? (int)(i / per / c.kv_heads / 2) : 0;
+  u32x4* pool = (u32x4*)((char*)(side ? c.v : c.k) + (c.row(layer, 0, g, 0) << c.esize_log())) + x;
+  int last = -1, done = 0;
+  for (int d0 = 0; d0 < n; d0 += 64) {
+    if (t < 64) {
+      KvStep e;
+      const int k = kv_path(a, s, base, d0, n, last, e);
+      if (t < k) {  // (in 16-byte units from the head's rows in page 0)
+        from[t] = c.row(0, e.src, 0, (base + e.from) & low) / c.head_dim * per;
+        to[t] = c.row(0, e.dst, 0, (base + d0 + t) & low) / c.head_dim * per;
+      }
+      if (t == 0) held = k;
+    }
+    __syncthreads();
+    const int k = held;
+    if (on)
+      for (int d = 0; d < k; d += 8) {
+        u32x4 v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = pool[from[min(d + e, k - 1)]];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (d + e < k && from[d + e] != to[d + e]) pool[to[d + e]] = v[e];
+      }
+    done += k;
+    if (k < 64) break;
+    __syncthreads();
   }
+  if (a.lens_out && blockIdx.x == 0 && t == 0) a.lens_out[s] = base + done;
 }
 
+// The lengths alone, a wave a slot.
 extern "C" __global__ void __launch_bounds__(256) qmm_kv_accept_lens(qmm::KvAccept a) {
   using namespace qmm;
-  const int s = blockIdx.x * 256 + threadIdx.x;
+  const int s = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (s >= a.c.slots) return;
   const int base = a.c.length(s);
   int d = 0;
   if (a.path) {
     const int n = min(a.counts[s], a.max_path);
-    for (int last = -1; d < n; ++d) {
-      last = kv_path(a, s, base, d, last);
-      if (last < 0) break;
+    for (int last = -1; d < n;) {
+      KvStep e;
+      const int k = kv_path(a, s, base, d, n, last, e);
+      d += k;
+      if (k < 64) break;
     }
   } else {  // page by page
     const int n = min(max(a.counts[s], 0), a.c.capacity() - base);
     while (d < n && a.c.page(s, (base + d) >> a.c.page_log) >= 0)
       d = min(((((base + d) >> a.c.page_log) + 1) << a.c.page_log) - base, n);
   }
-  a.lens_out[s] = base + d;
+  if ((threadIdx.x & 63) == 0) a.lens_out[s] = base + d;
 }
 
 // ---------------------------------------------------------------------------
