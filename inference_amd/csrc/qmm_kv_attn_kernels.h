@@ -93,7 +93,7 @@ struct KvAttn {
   void* out;
   float *part, *state;  // [rows][heads][splits] records: head_dim floats; reference and sum
   long long ldq, ldm, ldo;
-  int layer, x_type, heads, wide, splits, chunk;
+  int layer, x_type, heads, wide, out_wide, splits, chunk;
   int tiles, group_rows;  // groups of a slot's rows that a workgroup takes, rows of one
   int join_lanes;
   float scale;
@@ -767,7 +767,8 @@ __device__ __forceinline__ void kv_attn_narrow(const KvAttn& a) {
       if (whole) {
         const long long to = r * a.ldo + (long long)h * S::dim + at;
 #pragma unroll
-        for (int d = 0; d < HJ; ++d) store_typed(a.out, to + d, a.x_type, lsum == 0.0f ? 0.0f : o[d] / lsum);
+        for (int d = 0; d < HJ; ++d) o[d] = lsum == 0.0f ? 0.0f : o[d] / lsum;
+        store_values<HJ>(a.out, to, a.x_type, a.out_wide, o);
       } else {
         const long long rec = kv_record<S>(a, u, r, h);
 #pragma unroll
@@ -888,8 +889,12 @@ __device__ __forceinline__ void kv_attn_wide(const KvAttn& a) {
     const long long to = row * a.ldo + (long long)head * DIM;
 #pragma unroll
     for (int r = 0; r < S::AR; ++r)
+      {
+        float o[S::DTN];
 #pragma unroll
-      for (int d = 0; d < S::DTN; ++d) store_typed(a.out, to + S::DTN * S::out_row(r, g) + d, a.x_type, l == 0.0f ? 0.0f : acc[d][r] / l);
+        for (int d = 0; d < S::DTN; ++d) o[d] = l == 0.0f ? 0.0f : acc[d][r] / l;
+        store_values<S::DTN>(a.out, to + S::DTN * S::out_row(r, g), a.x_type, a.out_wide, o);
+      }
   } else {
     const long long rec = kv_record<S>(a, u, row, head);
 #pragma unroll
@@ -996,7 +1001,8 @@ extern "C" __global__ void __launch_bounds__(256) qmm_kv_attn_join(qmm::KvAttn a
   }
   if (!on) return;
   const long long to = row * a.ldo + (long long)h * dim + 4 * x;
-  const float r[4] = {o.x, o.y, o.z, o.w};
+  float r[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) store_typed(a.out, to + e, a.x_type, l == 0.0f ? 0.0f : r[e] / l);
+  for (int e = 0; e < 4; ++e) r[e] = l == 0.0f ? 0.0f : r[e] / l;
+  store_values<4>(a.out, to, a.x_type, a.out_wide, r);
 }

@@ -109,4 +109,16 @@ __device__ __forceinline__ void store4_typed(void* p, long long i, int type, boo
   }
 }
 
+// W values from i on, four at a time where they may be (`wide`, and W does).
+template <int W>
+__device__ __forceinline__ void store_values(void* p, long long i, int type, bool wide, const float (&v)[W]) {
+  if (W % 4 == 0 && wide) {
+#pragma unroll
+    for (int e = 0; e + 3 < W; e += 4) store4_typed(p, i + e, type, true, {v[e], v[e + 1], v[e + 2], v[e + 3]});
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e) store_typed(p, i + e, type, v[e]);
+  }
+}
+
 }  // namespace qmm

@@ -102,7 +102,7 @@ struct KvAttn {
   void* out;
   float *part, *state;
   long long ldq, ldm, ldo;
-  int layer, x_type, heads, wide, splits, chunk;
+  int layer, x_type, heads, wide, out_wide, splits, chunk;
   int tiles, group_rows, join_lanes;
   float scale;
 };
@@ -127,9 +127,10 @@ KvSplit kv_split(const qmm_kv_cache* c, int64_t rows, int max_rows, int64_t max_
   // 8000 positions: 86.7 us with 10 chunks, 89.5 with 4), but not so short that the chip is full of their beginnings
   // (64 of up to 1000: 28 us whole, 34 in two; one of 30000: 28 us with chunks of 256, 34 of 128). More columns: a
   // chunk writes and reads 0.5 KB a column (8 trees of up to 26 nodes over up to 4000 positions: 50 us with 12 chunks
-  // of at least 384, 58 with 32).
-  const int64_t wgs = p.form == 0 ? (units < 64 ? 1024 : 2048) : 768, least = p.form == 0 ? 128 * ceil_div(units, 64) : 384;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(wgs / units, ceil_div(most, least)));
+  // of at least 384, 58 with 32), unless CUs would be idle (one tree over 3000 positions: 33 us with 8, 27 with 24).
+  auto splits = [&](int64_t wgs, int64_t least) { return std::max<int64_t>(1, std::min<int64_t>(wgs / units, ceil_div(most, least))); };
+  p.splits = (int)(p.form == 0 ? splits(units < 64 ? 1024 : 2048, 128 * ceil_div(units, 64))
+                               : std::max(splits(768, 384), splits(256, 128)));
   p.chunk = (int)ceil_div(ceil_div(most, p.splits), 128) * 128;
   const size_t records = p.splits > 1 ? (size_t)rows * heads * p.splits : 0;
   p.parts = kv_align(records * c->head_dim * 4);
@@ -269,6 +270,7 @@ int qmm_kv_attention(const qmm_kv_cache* cache, int layer, const void* q, int x_
   a.part = (float*)ws, a.state = ws ? (float*)((uint8_t*)ws + p.parts) : nullptr;
   a.layer = layer, a.x_type = x_dtype, a.heads = heads, a.scale = scale;
   a.wide = (uintptr_t)q % four == 0 && ldq % 4 == 0;
+  a.out_wide = (uintptr_t)out % four == 0 && ldo % 4 == 0;
   a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles, a.group_rows = p.group_rows;
   // (a thread has four chunks' loads in flight)
   a.join_lanes = 1;

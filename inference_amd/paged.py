@@ -129,6 +129,11 @@ class PagedKVCache:
     # -- a step's rows ----------------------------------------------------
     def _rows(self, x: torch.Tensor, heads: Optional[int], what: str) -> Tuple[torch.Tensor, int]:
         """x as rows [rows, heads, head_dim] whose heads are contiguous, and the row stride."""
+        # (the usual case first: a token's calls are as long as their checks)
+        shape = x.shape
+        if len(shape) == 3 and shape[2] == self.head_dim and (heads is None or shape[1] == heads) and \
+                x.device == self.device and x.dtype in _DENSE and x.is_contiguous():
+            return x, shape[1] * shape[2]
         if x.device != self.device or x.dtype not in _DENSE:
             raise _bad(f"{what} must be float32, float16 or bfloat16 on {self.device}, got {x.dtype} on {x.device}")
         dim = self.head_dim
@@ -139,6 +144,15 @@ class PagedKVCache:
         if x.stride(2) != 1 or x.stride(1) != dim or (x.shape[0] > 1 and x.stride(0) < x.shape[1] * dim):
             x = x.contiguous()
         return x, x.stride(0) if x.shape[0] > 1 else x.shape[1] * dim
+
+    def _out(self, out: Optional[torch.Tensor], q: torch.Tensor) -> Tuple[torch.Tensor, int]:
+        """Rows for a result like q (`out`, or new ones), and their stride."""
+        if out is None:
+            return torch.empty(q.shape, dtype=q.dtype, device=q.device), q.shape[1] * q.shape[2]
+        o, ld = self._rows(out, q.shape[1], "out")
+        if o.data_ptr() != out.data_ptr() or out.dtype != q.dtype or o.shape != q.shape:
+            raise _bad(f"out must be rows like q, got {list(out.shape)} {out.dtype}")
+        return out, ld
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
                q: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
@@ -162,22 +176,18 @@ class PagedKVCache:
         if (cos is None) != (sin is None):
             raise _bad("cos and sin go together")
         if cos is not None:
-            for t in (cos, sin):
-                if t.dtype != torch.float32 or t.device != dev or t.dim() != 2 or t.shape[1] != self.head_dim or \
-                        t.shape != cos.shape or not t.is_contiguous():
-                    raise _bad(f"cos and sin must be contiguous float32 [positions, {self.head_dim}] on {dev}")
             positions = cos.shape[0]
+            shape = (positions, self.head_dim)
+            for t in (cos, sin):
+                if t.shape != shape or t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous():
+                    raise _bad(f"cos and sin must be contiguous float32 [positions, {self.head_dim}] on {dev}")
         ldq = ldo = heads = 0
         if q is not None:
             q, ldq = self._rows(q, None, "q")
             heads = q.shape[1]
             if q.shape[0] != rows or q.dtype != k.dtype:
                 raise _bad(f"q must be rows like k, got {list(q.shape)} {q.dtype}")
-            if out is None:
-                out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            o, ldo = self._rows(out, heads, "out")
-            if o.data_ptr() != out.data_ptr() or out.dtype != q.dtype or o.shape != q.shape:
-                raise _bad(f"out must be rows like q, got {list(out.shape)} {out.dtype}")
+            out, ldo = self._out(out, q)
         elif out is not None:
             raise _bad("an output without q")
         _run(dev, lib().qmm_kv_append, self._p, layer, _ptr(q), k.data_ptr(), v.data_ptr(), _DENSE[k.dtype], rows, ldq,
@@ -208,11 +218,7 @@ class PagedKVCache:
         max_len = self.max_pages * self.page_size if max_len is None else max_len
         if masks is not None:
             max_rows = min(max_rows, 64 * ldm)
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        o, ldo = self._rows(out, heads, "out")
-        if o.data_ptr() != out.data_ptr() or out.dtype != q.dtype or o.shape != q.shape:
-            raise _bad(f"out must be rows like q, got {list(out.shape)} {out.dtype}")
+        out, ldo = self._out(out, q)
         L = lib()
         key = (rows, max_rows, max_len, heads)
         nws = self._sizes.get(key)
@@ -313,8 +319,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: i
         if nws == 0:
             raise _bad("beam_select: " + last_error())
         _beam_ws[key] = nws
-    out = torch.empty((batch, count), dtype=torch.float32, device=dev)
-    tokens, parents, done = torch.empty((3, batch, count), dtype=torch.int32, device=dev).unbind()
+    out = scores.new_empty((batch, count))
+    tokens = torch.empty((batch, count), dtype=torch.int32, device=dev)
+    parents, done = torch.empty_like(tokens), torch.empty_like(tokens)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev)
     _run(dev, L.qmm_beam_select, logits.data_ptr(), _DENSE[logits.dtype], logits.stride(0) if rows > 1 else vocab, batch,
          beams, vocab, scores.data_ptr(), _ptr(finished), eos, count, tokens.data_ptr(), parents.data_ptr(),
