@@ -606,7 +606,7 @@ typedef struct qmm_kv_cache {
 /* RoPE of the rows (NeoX, as qmm_rope_kv_append_n) and their append: row j of slot s is rotated
  * at position lens[s] + depths[row] (depths NULL: + j) by the cos / sin tables [positions][head_dim]
  * (f32; both NULL: no rotation), k and v go to cache position lens[s] + j of the layer, rounded once
- * to its type, and the rotated q to q_out (q NULL: none; q_out may be q). lens stays as it is.
+ * to its type, and the rotated q to q_out (q NULL: none; q_out may be q, and overlaps no row else). lens stays as it is.
  * x_dtype (q, k, v, q_out): QMM_F32, QMM_F16 or QMM_BF16. A row whose position is outside the tables
  * writes nothing; one past the slot's pages writes its q alone. Row strides in elements. */
 int qmm_kv_append(const qmm_kv_cache *cache, int layer, const void *q, const void *k, const void *v, int x_dtype,
@@ -621,7 +621,8 @@ int qmm_kv_append(const qmm_kv_cache *cache, int layer, const void *q, const voi
  * kv_heads); a row that sees nothing gets zeros. What a row does not see does not reach it, not an
  * infinity or a NaN either. A position that the row sees and whose page the table does not name
  * gives NaN. Sums and softmax are held in 32 bits; a 16-bit cache is multiplied on the 16-bit
- * matrix cores, with q and the weights split into parts that keep their bits.
+ * matrix cores, with q and the weights split into parts that keep their bits. out may be q (of one stride), and
+ * overlaps it in no other way. scale: any finite value.
  * heads % kv_heads == 0, heads / kv_heads <= 32. max_rows bounds the rows of a slot (rows past it
  * are left out), at most 64 ldm with masks; max_len is about the largest lens[s] + rows of s: it
  * sets how the positions are split over workgroups (and so the f32 summation order), longer
@@ -650,7 +651,7 @@ int qmm_kv_fork(const qmm_kv_cache *cache, const int32_t *parents, const int32_t
 
 /* The accepted path of a step's rows: for d < counts[s], the key and value rows of position lens[s] +
  * path[s][d] move to position lens[s] + d in every layer, and lens_out[s] (it may be the cache's lens)
- * becomes lens[s] + counts[s]. path: int32 [slots][ld_path], increasing; a path ends early at an entry
+ * becomes lens[s] + counts[s] (lens_out may be counts too). path: int32 [slots][ld_path], increasing; a path ends early at an entry
  * that is not above the one before, below 0, or whose page or position the slot does not have, and at
  * ld_path, and then counts as that much shorter. path NULL: each row stays (a run whose first counts[s]
  * rows are accepted). The pages that are written must be the slot's alone (qmm_kv_fork with a reserve). */

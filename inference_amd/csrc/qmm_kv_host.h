@@ -83,6 +83,18 @@ int kv_stride(int64_t rows, int64_t ld, int64_t n, const char* what) {
   return QMM_OK;
 }
 
+// Whether `rows` rows of na and nb bytes, apart by lda and ldb, share a byte (rows of one stride may lie between each
+// other; of two strides they are taken to where their ranges meet).
+bool kv_meet(const void* a, int64_t lda, int64_t na, const void* b, int64_t ldb, int64_t nb, int64_t rows) {
+  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+  const uintptr_t a1 = a0 + (uintptr_t)((rows - 1) * lda + na), b1 = b0 + (uintptr_t)((rows - 1) * ldb + nb);
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (rows == 1 || lda != ldb) return true;
+  const uintptr_t off = (b0 - a0) % (uintptr_t)lda, ld = (uintptr_t)lda;  // of b's row in one of a's strides
+  return b0 >= a0 ? off < (uintptr_t)na || off + (uintptr_t)nb > ld
+                  : kv_meet(b, ldb, nb, a, lda, na, rows);
+}
+
 struct KvAppend {
   KvCache c;
   KvRows r;
@@ -199,7 +211,7 @@ int qmm_kv_append(const qmm_kv_cache* cache, int layer, const void* q, const voi
   QMM_TRY(kv_cache(cache, &a.c));
   QMM_TRY(kv_layer(cache, layer));
   QMM_TRY(kv_check_rows(rows));
-  if (!k || !v || !starts || (!cos_t != !sin_t) || (q && !q_out)) return fail(QMM_ERR_INVALID, "null pointer");
+  if (rows && (!k || !v || !starts || (!cos_t != !sin_t) || (q && !q_out))) return fail(QMM_ERR_INVALID, "null pointer");
   if (!kv_type(x_dtype)) return fail(QMM_ERR_INVALID, "row type %d (QMM_F32, QMM_F16 or QMM_BF16)", x_dtype);
   if (q && (heads < 1 || heads > 8192)) return fail(QMM_ERR_INVALID, "%d heads (1 .. 8192)", heads);
   if (cos_t && (positions < 1 || positions > (1LL << 30))) return fail(QMM_ERR_INVALID, "tables of %lld positions", (long long)positions);
@@ -211,6 +223,12 @@ int qmm_kv_append(const qmm_kv_cache* cache, int layer, const void* q, const voi
     QMM_TRY(kv_stride(rows, ldqo, heads * dim, "q_out"));
   }
   if (rows == 0) return QMM_OK;
+  if (q) {
+    const int64_t e = (int64_t)kv_esize(x_dtype), out = heads * dim * e;
+    if ((!(q == q_out && (ldq == ldqo || rows == 1)) && kv_meet(q, ldq * e, out, q_out, ldqo * e, out, rows)) ||
+        kv_meet(k, ldk * e, width * e, q_out, ldqo * e, out, rows) || kv_meet(v, ldv * e, width * e, q_out, ldqo * e, out, rows))
+      return fail(QMM_ERR_INVALID, "q_out overlaps the rows (it may be q itself)");
+  }
   Device* d;
   QMM_TRY(current_device(&d));
   const size_t four = 4 * kv_esize(x_dtype);
@@ -251,12 +269,16 @@ int qmm_kv_attention(const qmm_kv_cache* cache, int layer, const void* q, int x_
   KvAttn a = {};
   QMM_TRY(kv_cache(cache, &a.c));
   QMM_TRY(kv_layer(cache, layer));
-  if (!q || !starts || !out) return fail(QMM_ERR_INVALID, "null pointer");
+  if (rows && (!q || !starts || !out)) return fail(QMM_ERR_INVALID, "null pointer");
+  if (!std::isfinite(scale)) return fail(QMM_ERR_INVALID, "scale %g", scale);
   if (!kv_type(x_dtype)) return fail(QMM_ERR_INVALID, "row type %d (QMM_F32, QMM_F16 or QMM_BF16)", x_dtype);
   if (masks && (ldm < 1 || ldm > (1 << 20) || (max_rows + 63) / 64 > ldm))
     return fail(QMM_ERR_INVALID, "masks of %lld words for %d rows a slot", (long long)ldm, max_rows);
   QMM_TRY(kv_stride(rows, ldq, (int64_t)heads * cache->head_dim, "q"));
   QMM_TRY(kv_stride(rows, ldo, (int64_t)heads * cache->head_dim, "out"));
+  const int64_t esize = (int64_t)kv_esize(x_dtype), row_bytes = heads * cache->head_dim * esize;
+  if (rows && !(q == out && (ldq == ldo || rows == 1)) && kv_meet(q, ldq * esize, row_bytes, out, ldo * esize, row_bytes, rows))
+    return fail(QMM_ERR_INVALID, "out overlaps q (it may be q itself)");
   QMM_TRY(kv_workspace(ws, ws_bytes, qmm_kv_attention_workspace_size(cache, rows, max_rows, max_len, heads)));
   if (rows == 0) return QMM_OK;
   Device* d;
@@ -341,15 +363,20 @@ int qmm_kv_accept(const qmm_kv_cache* cache, const int32_t* path, int64_t ld_pat
   KvAccept a = {};
   QMM_TRY(kv_cache(cache, &a.c));
   if (!counts || !lens_out) return fail(QMM_ERR_INVALID, "null pointer");
+  const uintptr_t out = (uintptr_t)lens_out, lens = 4 * (uintptr_t)cache->slots;
+  auto meets = [&](const void* p, uintptr_t n) { return p && out < (uintptr_t)p + n && (uintptr_t)p < out + lens; };
   if (path && (ld_path < 1 || ld_path > (1 << 20))) return fail(QMM_ERR_INVALID, "paths of %lld entries (1 .. 2^20)", (long long)ld_path);
+  if ((lens_out != cache->lens && meets(cache->lens, lens)) || (lens_out != counts && meets(counts, lens)) ||
+      meets(path, lens * (uintptr_t)ld_path))
+    return fail(QMM_ERR_INVALID, "lens_out overlaps the lengths, the counts (it may be either itself) or the paths");
   Device* d;
   QMM_TRY(current_device(&d));
   a.path = path, a.counts = counts, a.lens_out = lens_out, a.ld_path = ld_path, a.max_path = (int)ld_path;
   const hipStream_t s = (hipStream_t)stream;
   void* args[] = {&a};
   if (path) {
-    // (lengths that are the cache's own change behind the last read of them, in a launch of their own)
-    const bool own = lens_out == cache->lens;
+    // (lengths that stand where they or the counts are read from change behind the last read, in a launch of their own)
+    const bool own = lens_out == cache->lens || lens_out == counts;
     if (own) a.lens_out = nullptr;
     const int64_t columns = 2LL * cache->layers * cache->kv_heads * ((int64_t)cache->head_dim * kv_esize(cache->dtype) / 16);
     QMM_TRY(kv_launch(d, "qmm_kv_accept_rows", ceil_div(columns, 256), (unsigned)cache->slots, 256, s, args));
@@ -430,7 +457,7 @@ int qmm_reorder_rows(const void* src, int64_t src_rows, int64_t ld_src, void* ds
                      int64_t row_bytes, const int32_t* index, int64_t rows, void* stream) {
   if (!src || !dst || !index) return fail(QMM_ERR_INVALID, "null pointer");
   if (src_rows < 0 || rows < 0 || rows > (1LL << 20) || src_rows > INT32_MAX || row_bytes < 0 || row_bytes > (1LL << 40) ||
-      ld_src > (1LL << 40) || ld_dst > (1LL << 40) || (src_rows > 1 && ld_src < row_bytes) || (rows > 1 && ld_dst < row_bytes))
+      ld_src > (1LL << 40) || ld_dst > (1LL << 40) || (src_rows > 1 && ld_src > (1LL << 62) / src_rows) || (src_rows > 1 && ld_src < row_bytes) || (rows > 1 && ld_dst < row_bytes))
     return fail(QMM_ERR_INVALID, "reorder of %lld rows of %lld bytes out of %lld", (long long)rows, (long long)row_bytes, (long long)src_rows);
   if (rows == 0 || src_rows == 0 || row_bytes == 0) return QMM_OK;
   const uintptr_t s0 = (uintptr_t)src, d0 = (uintptr_t)dst;

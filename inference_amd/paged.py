@@ -38,6 +38,21 @@ def _ints(t: torch.Tensor, shape: Tuple[int, ...], dev: torch.device, what: str)
     return t
 
 
+def _within(v: int, low: int, high: int, what: str) -> int:
+    """v, which a C int would cut off without a word."""
+    if not low <= v <= high:
+        raise _bad(f"{what} {v} ({low} .. {high})")
+    return v
+
+
+def _kept(sizes: dict, key, size: int) -> int:
+    """A workspace size kept under its arguments (a thousand of them)."""
+    if len(sizes) >= 1024:
+        sizes.clear()
+    sizes[key] = size
+    return size
+
+
 def _packed(t: torch.Tensor) -> bool:
     """Whether t's rows (along the first dimension) are contiguous and do not overlap."""
     n = 1
@@ -99,10 +114,10 @@ class PagedKVCache:
             raise _bad(f"table must be [slots, max_pages], got {list(table.shape)}")
         slots, max_pages = table.shape
         layers, pages, kv_heads, page_size, head_dim = k.shape
-        self.k, self.v, self.device = k, v, dev
-        self.table = _ints(table, (slots, max_pages), dev, "table")
-        self.lens = _ints(lens, (slots,), dev, "lens")
-        self.refs = _ints(refs, (pages,), dev, "refs")
+        _ints(table, (slots, max_pages), dev, "table")
+        _ints(lens, (slots,), dev, "lens")
+        _ints(refs, (pages,), dev, "refs")
+        self._tensors, self.device = (k, v, table, lens, refs), dev
         self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = layers, pages, kv_heads, page_size, head_dim
         self.slots, self.max_pages = slots, max_pages
         self._c = _Cache(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), pages,
@@ -113,6 +128,13 @@ class PagedKVCache:
         if self._fork_ws == 0:
             raise _bad("paged cache: " + last_error())
         self._compact_ws = int(lib().qmm_kv_compact_workspace_size(self._p))
+
+    # (fixed: the library has their addresses)
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    table = property(lambda self: self._tensors[2])
+    lens = property(lambda self: self._tensors[3])
+    refs = property(lambda self: self._tensors[4])
 
     @classmethod
     def empty(cls, layers: int, pages: int, kv_heads: int, page_size: int, head_dim: int, slots: int, max_pages: int,
@@ -164,6 +186,7 @@ class PagedKVCache:
         is rotated at lens[s] + depths[row] (default: + j) by cos / sin (float32 [positions, head_dim]; None: not
         rotated). lens stays as it is: see ``accept``."""
         dev = self.device
+        _within(layer, 0, self.layers - 1, "layer")
         k, ldk = self._rows(k, self.kv_heads, "k")
         v, ldv = self._rows(v, self.kv_heads, "v")
         rows = k.shape[0]
@@ -201,9 +224,10 @@ class PagedKVCache:
         sequences: row j of sequence s sees the positions below lens[s], and lens[s] + i where bit i of its mask is
         set (int64 [rows, words], see tree_masks; None: i <= j). q: [rows, heads, head_dim]; the result is of its
         shape and type, a row that sees nothing is zeros (rows of no sequence are not written: a padded batch brings
-        its own `out`). max_rows bounds a sequence's rows (default: all; rows past it are left out), max_len is about the
-        longest lens + rows (default: the table's). scale: head_dim ** -0.5."""
+        its own `out`, which may be q). max_rows bounds a sequence's rows (default: all, with masks 64 * words at most; rows
+        past it are not written), max_len is about the longest lens + rows (default: the table's). scale: head_dim ** -0.5."""
         dev = self.device
+        _within(layer, 0, self.layers - 1, "layer")
         q, ldq = self._rows(q, None, "q")
         rows, heads = q.shape[0], q.shape[1]
         _ints(starts, (self.slots + 1,), dev, "starts")
@@ -214,8 +238,11 @@ class PagedKVCache:
                 raise _bad(f"masks must be contiguous int64 [{rows}, words] on {dev}, got {masks.dtype} "
                            f"{list(masks.shape)} on {masks.device}")
             ldm = masks.shape[1]
-        max_rows = max(1, rows) if max_rows is None else max_rows
-        max_len = self.max_pages * self.page_size if max_len is None else max_len
+        max_rows = max(1, rows) if max_rows is None else min(max_rows, max(1, rows))
+        most = self.max_pages * self.page_size
+        max_len = most if max_len is None else min(max_len, most)
+        if max_rows < 1 or max_len < 1:
+            raise _bad(f"max_rows {max_rows}, max_len {max_len}")
         if masks is not None:
             max_rows = min(max_rows, 64 * ldm)
         out, ldo = self._out(out, q)
@@ -223,7 +250,7 @@ class PagedKVCache:
         key = (rows, max_rows, max_len, heads)
         nws = self._sizes.get(key)
         if nws is None:
-            nws = self._sizes[key] = int(L.qmm_kv_attention_workspace_size(self._p, *key))
+            nws = _kept(self._sizes, key, int(L.qmm_kv_attention_workspace_size(self._p, *key)))
         ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
         _run(dev, L.qmm_kv_attention, self._p, layer, q.data_ptr(), _DENSE[q.dtype], rows, ldq, starts.data_ptr(),
              _ptr(masks), ldm, max_rows, max_len, heads, self.head_dim ** -0.5 if scale is None else scale,
@@ -239,6 +266,7 @@ class PagedKVCache:
         where another one holds it for good. The new lists replace table, lens and refs, or go to out = (table, lens,
         refs). Returns shortage (int32 [1]): 0, or how many pages were missing; then nothing has changed."""
         dev = self.device
+        _within(reserve, 0, self.max_pages * self.page_size, "reserve")
         _ints(parents, (self.slots,), dev, "parents")
         if keep is not None:
             _ints(keep, (self.slots,), dev, "keep")
@@ -311,6 +339,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: i
     if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
     batch = rows // beams
+    _within(count, 1, 128, "count")
+    _within(eos, -1, vocab - 1, "eos")
     L = lib()
     key = (batch, beams, vocab, count)
     nws = _beam_ws.get(key)
@@ -318,7 +348,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: i
         nws = int(L.qmm_beam_select_workspace_size(*key))
         if nws == 0:
             raise _bad("beam_select: " + last_error())
-        _beam_ws[key] = nws
+        _kept(_beam_ws, key, nws)
     out = scores.new_empty((batch, count))
     tokens = torch.empty((batch, count), dtype=torch.int32, device=dev)
     parents, done = torch.empty_like(tokens), torch.empty_like(tokens)

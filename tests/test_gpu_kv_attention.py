@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from inference_amd import PagedKVCache
+from inference_amd import PagedKVCache, QmmError
 from inference_amd.paged import tree_masks
 from oracle import paged
 
@@ -249,3 +249,96 @@ def test_streams_captures_and_repeats():
         torch.cuda.synchronize()
         assert torch.equal(out, c.attention(0, q, starts, max_rows=32, max_len=950))
     assert torch.equal(out, want)
+
+
+def test_no_rows_and_rows_in_place():
+    """A step without a row; results written over q; and over what overlaps it otherwise: refused."""
+    lens, rows = [70, 3, 400], [1, 26, 9]
+    for cache, x, n in (("f32", "f32", 26), ("bf16", "bf16", 26), ("f16", "f32", 1)):
+        c, q, starts, pools, table = step(10, lens, [min(r, n) for r in rows], 8, 2, 128, 16, x, cache)
+        want = c.attention(0, q.to(DEV), starts.to(DEV))
+        here = q.to(DEV)
+        assert c.attention(0, here, starts.to(DEV), out=here) is here and torch.equal(here, want)
+        none = torch.empty((0, 8, 128), dtype=T[x], device=DEV)
+        assert c.attention(0, none, torch.zeros(4, dtype=torch.int32, device=DEV)).shape == none.shape
+        kv = torch.empty((0, 2, 128), dtype=T[x], device=DEV)
+        assert c.append(0, kv, kv, torch.zeros(4, dtype=torch.int32, device=DEV), q=none).shape == none.shape
+    total = q.shape[0]
+    both = torch.zeros((total, 2, 8, 128), device=DEV)  # (rows between each other)
+    both[:, 0] = q.to(DEV)
+    c.attention(0, both[:, 0], starts.to(DEV), out=both[:, 1])
+    assert torch.equal(both[:, 1], want)
+    flat = torch.zeros((total + 1) * 1024, device=DEV)
+    a, b = flat[:total * 1024].view(total, 8, 128), flat[128:128 + total * 1024].view(total, 8, 128)
+    with pytest.raises(QmmError):
+        c.attention(0, a, starts.to(DEV), out=b)
+    with pytest.raises(QmmError):
+        c.append(0, a[:, :2], a[:, 2:4], starts.to(DEV), q=a[:, 4:], out=a[:, 3:7])
+    for bad in (dict(scale=float("nan")), dict(scale=float("inf")), dict(max_rows=0), dict(max_len=0)):
+        with pytest.raises(QmmError):
+            c.attention(0, q.to(DEV), starts.to(DEV), **bad)
+    for layer in (-1, 1, 2 ** 32):
+        with pytest.raises(QmmError):
+            c.attention(layer, q.to(DEV), starts.to(DEV))
+    with pytest.raises(AttributeError):
+        c.table = c.table.clone()
+
+
+@pytest.mark.parametrize("cache,x", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
+def test_scales(cache, x):
+    """Scales below 0 and 0 itself (equal weights), in each form."""
+    for rows in ([1, 1], [4, 2], [33, 1]):
+        for scale in (-0.1, 0.0, 1e-30, -3.0):
+            c, q, starts, pools, table = step(11, [50, 7], rows, 8, 2, 64, 16, x, cache)
+            check(c.attention(0, q.to(DEV), starts.to(DEV), scale=scale), q, pools, table, [50, 7], starts, None, scale)
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("part", [0, 1])
+def test_values_below_the_normal_range(cache, part):
+    """Keys (against a q as much larger), or values, that are denormal numbers of the cache's type."""
+    low = 2.0 ** (-18 if cache == "f16" else -127)
+    for rows in ([1, 1], [4, 2], [33, 1]):
+        c, q, starts, pools, table = step(12, [50, 300], rows, 8, 2, 128, 16, "f32", cache, bad=False)
+        pools[part] = (pools[part].double() * low).to(T[cache])
+        (c.v if part else c.k).copy_(pools[part].to(DEV))
+        if part == 0:
+            q = q * (1 / low if cache == "f16" else 2.0 ** 122)
+        check(c.attention(0, q.to(DEV), starts.to(DEV)), q, pools, table, [50, 300], starts, None, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("cache,x", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16")])
+def test_wide_groups_of_heads(cache, x):
+    """32 heads over one, 12 over one and 3 over one, a run of many rows; odd strides and boundaries; one chunk and many."""
+    for heads, kv, dim in ((32, 1, 64), (12, 1, 128), (3, 1, 256)):
+        for lens, rows, max_len in (([20, 0], [37, 9], 60), ([700, 0], [37, 9], None)):
+            c, q, starts, pools, table = step(13 + heads, lens, rows, heads, kv, dim, 16, x, cache, max_pages=100)
+            n = heads * dim
+            wide = torch.full((48, n + 7), float("nan"), dtype=T[x], device=DEV)
+            wide[:46, 3:3 + n] = q.to(DEV).view(46, n)
+            out = torch.full((48, n + 5), 7.0, dtype=T[x], device=DEV)
+            c.attention(0, wide[:, 3:3 + n], starts.to(DEV), max_len=max_len, out=out[:, 1:1 + n])
+            check(out[:46, 1:1 + n].unflatten(1, (heads, dim)), q, pools, table, lens, starts, None, dim ** -0.5)
+            assert (out[46:] == 7).all() and (out[:, 0] == 7).all() and (out[:, 1 + n:] == 7).all()
+
+
+def test_two_graphs():
+    """Two captured calls of different sizes, replayed in turn with eager ones between: each keeps its workspace."""
+    lens, rows = [3000, 800], [1, 40]
+    c, q, starts, pools, table = step(14, lens, rows, 8, 2, 128, 32, "bf16", "bf16")
+    q, starts = q.to(DEV), starts.to(DEV)
+    calls = [dict(max_rows=40, max_len=3000), dict(max_rows=41, max_len=100)]
+    want = [c.attention(0, q, starts, **k) for k in calls]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for k in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(c.attention(0, q, starts, **k))
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 1, 0):
+        outs[i].fill_(5.0)
+        graphs[i].replay()
+        assert torch.equal(c.attention(0, q, starts, **calls[1 - i]), want[1 - i])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want[i])

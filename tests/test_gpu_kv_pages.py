@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from inference_amd import PagedKVCache
+from inference_amd import PagedKVCache, QmmError
 from oracle import paged
 
 pytestmark = pytest.mark.gpu
@@ -312,6 +312,19 @@ def test_accept_long_paths():
     c.lens.copy_(ints([100, 3]))
     path = [sorted(rng.choice(600, 300, replace=False).tolist()) for _ in range(2)]
     check_accept(c, path, [300, 251])
+
+
+def test_accept_into_the_counts():
+    """The new lengths over the counts; over part of them or of a path: refused."""
+    c = cache_of(3, [60] * 4, 16, 40, 4)
+    c.lens.copy_(ints([10, 20, 5, 3]))
+    path, both = ints([[1, 3, 9, 11]] * 4), ints([2, 4, 0, 3, 0])
+    counts = both[:4]
+    c.accept(path, counts, out=counts)
+    assert both.tolist() == [12, 24, 5, 6, 0] and c.lens.tolist() == [10, 20, 5, 3]
+    for bad in (both[1:], path.view(-1)[:4], path.view(-1)[12:]):
+        with pytest.raises(QmmError):
+            c.accept(path, counts, out=bad)
 
 
 def test_accept_paths_that_end_early():

@@ -129,11 +129,17 @@ def check_append(so):
     c = h.cache()
     assert h.append(c) == (0, ["qmm_kv_append_rows"])
     assert h.append(c, q=None, out=None, cos=None, sin=None) == (0, ["qmm_kv_append_rows"])
-    assert h.append(c, rows=0) == (0, [])
+    assert h.append(c, rows=0) == (0, []) and h.append(c, rows=0, q=None, k=None, v=None, starts=None) == (0, [])
+    assert h.append(c, out=1 << 45)[0] == 0
+    # q, k and v of one wide row, the result in q's place or behind them all
+    whole = dict(k=(1 << 45) + 8192, v=(1 << 45) + 10240, ldq=5120, ldk=5120, ldv=5120, ldo=5120)
+    assert h.append(c, out=1 << 45, **whole)[0] == 0 and h.append(c, out=(1 << 45) + 12288, **whole)[0] == 0
+    refused(h.append(c, out=(1 << 45) + 8188, **whole), h.append(c, out=(1 << 45) + 12284, **whole),
+            h.append(c, out=(1 << 45) + 12292, **whole))
     refused(*(h.append(c, **b) for b in (
         dict(layer=-1), dict(layer=2), dict(k=None), dict(v=None), dict(starts=None), dict(cos=None), dict(sin=None),
         dict(out=None), dict(x=8), dict(heads=0), dict(heads=8193), dict(positions=0), dict(ldq=2047), dict(ldk=511),
-        dict(ldv=1), dict(ldo=100), dict(rows=-1), dict(rows=(1 << 20) + 1), dict(rows=1 << 20, heads=2048, ldq=1 << 18, ldo=1 << 18))))
+        dict(ldv=1), dict(ldo=100), dict(out=(1 << 45) + 16), dict(out=1 << 45, ldo=4096), dict(out=1 << 46), dict(out=(1 << 47) + 512), dict(rows=-1), dict(rows=(1 << 20) + 1), dict(rows=1 << 20, heads=2048, ldq=1 << 18, ldo=1 << 18))))
 
 
 def check_attention(so):
@@ -152,7 +158,10 @@ def check_attention(so):
         dict(layer=2), dict(q=None), dict(starts=None), dict(out=None), dict(x=14), dict(heads=15), dict(heads=0),
         dict(heads=4 * 33, ldq=1 << 20, ldo=1 << 20), dict(max_rows=0), dict(max_len=0), dict(ldq=2047), dict(ldo=2047),
         dict(rows=-1), dict(rows=(1 << 20) + 1), dict(masks=1 << 49, ldm=0), dict(masks=1 << 49, ldm=1, max_rows=65),
-        dict(ws=None), dict(ws_bytes=h.size(c) - 1), dict(ws=(1 << 53) + 8))))
+        dict(ws=None), dict(ws_bytes=h.size(c) - 1), dict(ws=(1 << 53) + 8), dict(scale=float("nan")),
+        dict(scale=float("-inf")), dict(out=(1 << 45) + 4), dict(out=1 << 45, ldo=4096))))
+    assert h.attention(c, out=1 << 45)[0] == 0 and h.attention(c, rows=1, out=1 << 45, ldo=1 << 30)[0] == 0
+    assert h.attention(c, rows=0, q=None, starts=None, out=None) == (0, [])
     assert h.attention(c, masks=1 << 49, ldm=2, max_rows=65)[0] == 0
     assert h.attention(c, ws_bytes=h.size(c))[0] == 0
     assert h.size(h.cache(head_dim=100)) == 0 and h.size(c, heads=3) == 0 and h.size(c, max_rows=0) == 0
@@ -184,6 +193,8 @@ def check_pages(so):
     assert h.accept(c) == (0, ["qmm_kv_accept_rows"])
     assert h.accept(c, lens=c.lens) == (0, ["qmm_kv_accept_rows", "qmm_kv_accept_lens"])
     assert h.accept(c, path=None) == (0, ["qmm_kv_accept_lens"])
+    assert h.accept(c, lens=1 << 46) == (0, ["qmm_kv_accept_rows", "qmm_kv_accept_lens"])
+    refused(h.accept(c, lens=c.lens + 4), h.accept(c, lens=(1 << 46) + 8), h.accept(c, lens=(1 << 45) + 44))
     refused(h.accept(c, counts=None), h.accept(c, lens=None), h.accept(c, ld=0), h.accept(c, ld=(1 << 20) + 1))
     need = h.L.qmm_kv_compact_workspace_size(ctypes.byref(c))
     assert h.compact(c, ws_bytes=need) == (0, ["qmm_kv_compact_plan", "qmm_kv_compact_commit", "qmm_kv_copy_pages"])
@@ -209,7 +220,7 @@ def check_beam(so):
     assert h.reorder(rows=0) == (0, []) and h.reorder(src_rows=0) == (0, []) and h.reorder(nbytes=0) == (0, [])
     refused(h.reorder(src=None), h.reorder(dst=None), h.reorder(index=None), h.reorder(rows=-1), h.reorder(src_rows=-1),
             h.reorder(nbytes=-1), h.reorder(ld_src=63), h.reorder(ld_dst=63), h.reorder(rows=(1 << 20) + 1),
-            h.reorder(dst=(1 << 45) + 639), h.reorder(src=(1 << 46) + 100, dst=1 << 46))
+            h.reorder(src_rows=1 << 30, ld_src=1 << 40), h.reorder(dst=(1 << 45) + 639), h.reorder(src=(1 << 46) + 100, dst=1 << 46))
     assert h.reorder(dst=(1 << 45) + 640)[0] == 0
 
 
