@@ -55,6 +55,8 @@ def _kept(sizes: dict, key, size: int) -> int:
 
 def _packed(t: torch.Tensor) -> bool:
     """Whether t's rows (along the first dimension) are contiguous and do not overlap."""
+    if t.is_contiguous():
+        return True
     n = 1
     for size, stride in zip(t.shape[:0:-1], t.stride()[:0:-1]):
         if stride != n and size != 1:
@@ -349,13 +351,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: i
         if nws == 0:
             raise _bad("beam_select: " + last_error())
         _kept(_beam_ws, key, nws)
-    out = scores.new_empty((batch, count))
-    tokens = torch.empty((batch, count), dtype=torch.int32, device=dev)
-    parents, done = torch.empty_like(tokens), torch.empty_like(tokens)
+    # (the four results are one allocation: four take longer than a launch)
+    block = torch.empty((4, batch, count), dtype=torch.int32, device=dev)
+    tokens, parents, done, out = block.unbind()
+    out = out.view(torch.float32)
+    first, step = block.data_ptr(), 4 * batch * count
     ws = torch.empty(nws, dtype=torch.uint8, device=dev)
     _run(dev, L.qmm_beam_select, logits.data_ptr(), _DENSE[logits.dtype], logits.stride(0) if rows > 1 else vocab, batch,
-         beams, vocab, scores.data_ptr(), _ptr(finished), eos, count, tokens.data_ptr(), parents.data_ptr(),
-         out.data_ptr(), done.data_ptr(), ws.data_ptr(), nws)
+         beams, vocab, scores.data_ptr(), _ptr(finished), eos, count, first, first + step, first + 3 * step,
+         first + 2 * step, ws.data_ptr(), nws)
     return tokens, parents, out, done
 
 
@@ -367,20 +371,19 @@ def reorder_rows(src: torch.Tensor, index: torch.Tensor, out: Optional[torch.Ten
         raise _bad("reorder_rows takes rows")
     if index.dim() != 1:
         raise _bad(f"index must be [rows], got {list(index.shape)}")
-    rows = index.shape[0]
+    rows, inner = index.shape[0], src.shape[1:]
     _ints(index, (rows,), dev, "index")
-    inner = src.shape[1:]
     if not _packed(src):
         src = src.contiguous()
     if out is None:
         out = torch.zeros((rows, *inner), dtype=src.dtype, device=dev)
-    elif out.shape != (rows, *inner) or out.dtype != src.dtype or out.device != dev or not _packed(out):
+    elif out.dim() < 1 or out.shape[0] != rows or out.shape[1:] != inner or out.dtype != src.dtype or \
+            out.device != dev or not _packed(out):
         raise _bad(f"out must be {src.dtype} [{rows}, ...] with rows like src's on {dev}, got {out.dtype} "
                    f"{list(out.shape)} on {out.device}")
-    if rows and src.numel() and out.numel():
-        size = src.element_size()
-        nbytes = inner.numel() * size
-        _run(dev, lib().qmm_reorder_rows, src.data_ptr(), src.shape[0],
-             src.stride(0) * size if src.shape[0] > 1 else nbytes, out.data_ptr(),
+    n, size = src.shape[0], src.element_size()
+    nbytes = inner.numel() * size
+    if rows and n and nbytes:
+        _run(dev, lib().qmm_reorder_rows, src.data_ptr(), n, src.stride(0) * size if n > 1 else nbytes, out.data_ptr(),
              out.stride(0) * size if rows > 1 else nbytes, nbytes, index.data_ptr(), rows)
     return out
