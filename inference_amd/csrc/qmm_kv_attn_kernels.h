@@ -12,7 +12,7 @@
 //   O^T += V^T P^T   A = V^T, B = P^T where S^T left it: the k index of a product may be
 //                    permuted freely, so V's rows are taken in P's order. Row m of V^T's
 //                    tile j is element DTN m + j (DTN = head_dim / N): a lane's values of a
-//                    key are DTN contiguous ones.
+//                    key are DTN contiguous ones (32 j + m where LDS transposes: kv_values_lds).
 // K goes straight to LDS (buffer_load ... lds, 16 bytes a lane), its 16-byte chunks XORed by
 // the key so that the keys' reads of a chunk meet distinct banks.
 //
@@ -23,6 +23,16 @@
 // flight and waits for the oldest. More columns: the four waves have a tile of columns each
 // and share the keys, K and V through LDS, two tiles deep. A sequence's chunks are joined by a
 // second launch.
+//
+// What bounds them. 32 heads over 8, head_dim 128: one token of each of 24 sequences of up to 8000
+// positions, bf16: K and V's 411 MB, 79.6 us and 5.0 for the join (the bytes alone 77 at a copy's
+// rate). One token over 1500 f32 positions: 8.6 and 3.9 us, latency (launch, page ids, K, V, join). 8
+// trees of up to 26 nodes over up to 4000 bf16 positions with f32 rows: 40 and 7 us, where the bytes
+// take 14 and the products, three times over for the parts, 12 at a large product's rate: smaller trees
+// fill their tiles in part, and a chunk's beginning counts. 4 trees of 64 nodes over 30000 f16
+// positions: 250 and 14 us, the products 180 at that rate: the matrix cores are busy 42% of the time
+// and the vector ALUs half, in turn rather than at once (two waves a SIMD are all that the registers
+// and the LDS of 64-key tiles leave).
 //
 // Pages. A tile's two halves of 16 positions each lie in one page (pages are 16 or more), so
 // a half is one buffer whose end is the last position there is: rows past it read as 0 and
@@ -404,6 +414,20 @@ __device__ __forceinline__ float kv_softmax(float (&sc)[NS], KvState& st, float 
   return w;
 }
 
+// Eight weights as the parts of a product's operand.
+template <class S, int PP>
+__device__ __forceinline__ void kv_parts(u32x4 (&p)[PP], const float* sc) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float x = sc[2 * e], y = sc[2 * e + 1];
+#pragma unroll
+    for (int q = 0; q < PP; ++q) {
+      p[q][e] = pack2<S::TYPE>(x, y);
+      x -= low_of<S::TYPE>(p[q][e]);
+      y -= high_of<S::TYPE>(p[q][e]);
+    }
+  }
+}
 // acc += V^T P^T of eight score registers and their keys' value rows; f32: acc times w first
 // (16-bit caches: kv_rescale).
 template <class S, int PP>
@@ -427,16 +451,7 @@ __device__ __forceinline__ void kv_values(typename S::Acc (&acc)[S::DTN], const 
     }
   } else {
     u32x4 p[PP];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = sc[2 * e], y = sc[2 * e + 1];
-#pragma unroll
-      for (int q = 0; q < PP; ++q) {
-        p[q][e] = pack2<S::TYPE>(x, y);
-        x -= low_of<S::TYPE>(p[q][e]);
-        y -= high_of<S::TYPE>(p[q][e]);
-      }
-    }
+    kv_parts<S, PP>(p, sc);
 #pragma unroll
     for (int d = 0; d < S::DTN; ++d) {
       u32x4 vt;  // eight keys' value d of this lane
@@ -446,6 +461,27 @@ __device__ __forceinline__ void kv_values(typename S::Acc (&acc)[S::DTN], const 
 #pragma unroll
       for (int q = PP - 1; q >= 0; --q) acc[d] = mfma_16<S>(vt, p[q], acc[d]);
     }
+  }
+}
+// The same with 16-bit V rows in LDS, transposed as they are read: 16 lanes read 16 values of four
+// rows, four values each, and lane i of them gets value i of the four. Row m of V^T's tile j is
+// element 32 j + m here. `at`: this lane's place in the tile of 16 keys, of tile 0. (Rows read as
+// they lie and interleaved by permutations: 4 trees of 64 nodes over 30000 positions 276 us, this 266.)
+__device__ __forceinline__ u32x2 read_transposed(const char* lds) {
+  typedef short i16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)lds));
+}
+template <class S, int PP>
+__device__ __forceinline__ void kv_values_lds(typename S::Acc (&acc)[S::DTN], const float* sc, const char* vb, unsigned at) {
+  u32x4 p[PP];
+  kv_parts<S, PP>(p, sc);
+#pragma unroll
+  for (int d = 0; d < S::DTN; ++d) {
+    const char* v = vb + (at ^ (64u * d));
+    const u32x2 x = read_transposed(v), y = read_transposed(v + 8 * S::RB);
+    const u32x4 vt = {x[0], x[1], y[0], y[1]};
+#pragma unroll
+    for (int q = PP - 1; q >= 0; --q) acc[d] = mfma_16<S>(vt, p[q], acc[d]);
   }
 }
 template <class S>
@@ -532,8 +568,9 @@ template <class S>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t kv_buffer(void* pool, long long at, int rows) {
   return __builtin_amdgcn_make_buffer_rsrc((char*)pool + at, 0, __builtin_amdgcn_readfirstlane(rows * S::RB), 0x00020000);
 }
-// Loads to LDS are 64 chunks, RPL rows; chunk c of row r goes to slot c ^ (r >> SH) % CH (K), or
-// c (V). A lane's byte offset in its load of K, of the rows from `row` on (a multiple of 8), of
+// Loads to LDS are 64 chunks, RPL rows; chunk c of row r goes to slot c ^ (r >> SH) % CH (K), c (V
+// in 32 bits), or c ^ 2 ((r >> SH) % min(8, CH / 2)) (V in 16: the four rows of a transposed read, 32 bytes each, in
+// banks of their own). A lane's byte offset in its load of K, of the rows from `row` on (a multiple of 8), of
 // which the load's own rows take an XOR and an addition.
 template <class S>
 __device__ __forceinline__ unsigned kv_k_lane(int row) {
@@ -543,6 +580,19 @@ __device__ __forceinline__ unsigned kv_k_lane(int row) {
 template <class S>
 __device__ __forceinline__ unsigned kv_k_load(unsigned lane, int x, int half = 0) {  // x: load within 16 rows of `half`
   return (lane ^ (16u * ((unsigned)((16 * half + S::RPL * x) >> S::SH) & (S::CH - 1)))) + 1024u * x;
+}
+template <class S>
+__device__ __forceinline__ unsigned kv_v_swap(int row) {
+  return S::F32 ? 0 : 2u * ((unsigned)(row >> S::SH) & (S::CH >= 16 ? 7 : S::CH / 2 - 1));
+}
+template <class S>
+__device__ __forceinline__ unsigned kv_v_lane(int row) {
+  const int lane = threadIdx.x & 63, r = row + lane / S::CH;
+  return (unsigned)(r & 15) * S::RB + 16u * ((unsigned)(lane % S::CH) ^ kv_v_swap<S>(r));
+}
+template <class S>
+__device__ __forceinline__ unsigned kv_v_load(unsigned lane, int x) {
+  return (lane ^ (16u * kv_v_swap<S>(S::RPL * x))) + 1024u * x;
 }
 __device__ __forceinline__ void kv_to_lds(__amdgpu_buffer_rsrc_t rs, unsigned at, char* to) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)to, 16, at, 0, 0, 0);
@@ -803,7 +853,7 @@ __device__ __forceinline__ void kv_attn_wide(const KvAttn& a) {
   pg.first = 0, pg.step = KT;
   pg.load(a, u, 0);
   bool missing = false, next_missing = false;
-  unsigned klane = kv_k_lane<S>(RW * wave), vlane = (unsigned)(RW * wave & 15) * S::RB + 16u * lane;
+  unsigned klane = kv_k_lane<S>(RW * wave), vlane = kv_v_lane<S>(RW * wave);
   auto load = [&](int i) {
     if (i && i % pg.BLOCK == 0) pg.load(a, u, i);
     asm volatile("" : "+v"(klane), "+v"(vlane));
@@ -816,7 +866,7 @@ __device__ __forceinline__ void kv_attn_wide(const KvAttn& a) {
 #pragma unroll
     for (int x = 0; x < NI; ++x) kv_to_lds(ks, kv_k_load<S>(klane, x), to + 1024 * x);
 #pragma unroll
-    for (int x = 0; x < NI; ++x) kv_to_lds(vs, vlane + 1024u * x, to + TB + 1024 * x);
+    for (int x = 0; x < NI; ++x) kv_to_lds(vs, kv_v_load<S>(vlane, x), to + TB + 1024 * x);
   };
   load(0);
   __builtin_amdgcn_sched_barrier(0);
@@ -827,6 +877,9 @@ __device__ __forceinline__ void kv_attn_wide(const KvAttn& a) {
   for (int d = 0; d < S::DTN; ++d) acc[d] = (typename S::Acc)(0.0f);
   KvState st;
   const int tiles = (u.k1 - u.k0 + KT - 1) / KT;
+  const int l16 = lane % 16;
+  const unsigned vread = (unsigned)(4 * g + l16 / 4) * S::RB + 8u * (l16 % 2) +
+                         16u * ((unsigned)(2 * (lane / 16 % 2) + l16 % 4 / 2) ^ kv_v_swap<S>(4 * g + l16 / 4));
 #pragma unroll 1
   for (int i = 0; i < tiles; ++i) {
     const int t0 = u.k0 + KT * i;
@@ -866,14 +919,18 @@ __device__ __forceinline__ void kv_attn_wide(const KvAttn& a) {
     }
     const float w = kv_softmax<S>(sc, st, c);
     kv_rescale<S>(acc, w);
-    const char* vb = kb + TB + S::DTN * S::EB * col;
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int x = 0; x < NS / 8; ++x) {
-      typename S::VRow v[8];
+      if constexpr (S::F32) {
+        const char* vb = kb + TB + S::DTN * S::EB * col;
+        typename S::VRow v[8];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] = *(const typename S::VRow*)(vb + S::key(8 * x + r, g) * S::RB);
-      kv_values<S, PP>(acc, sc + 8 * x, v, x == 0 ? w : 1.0f);
+        for (int r = 0; r < 8; ++r) v[r] = *(const typename S::VRow*)(vb + S::key(8 * x + r, g) * S::RB);
+        kv_values<S, PP>(acc, sc + 8 * x, v, x == 0 ? w : 1.0f);
+      } else {
+        kv_values_lds<S, PP>(acc, sc + 8 * x, kb + TB + 16 * x * S::RB, vread);
+      }
     }
     __builtin_amdgcn_s_setprio(0);
   }
@@ -888,19 +945,21 @@ __device__ __forceinline__ void kv_attn_wide(const KvAttn& a) {
   if (u.tl.len >= u.tl.n) {
     const long long to = row * a.ldo + (long long)head * DIM;
 #pragma unroll
-    for (int r = 0; r < S::AR; ++r)
-      {
-        float o[S::DTN];
+    for (int r = 0; r < S::AR; r += S::F32 ? 1 : 4)
 #pragma unroll
-        for (int d = 0; d < S::DTN; ++d) o[d] = l == 0.0f ? 0.0f : acc[d][r] / l;
-        store_values<S::DTN>(a.out, to + S::DTN * S::out_row(r, g), a.x_type, a.out_wide, o);
+      for (int d = 0; d < S::DTN; d += S::F32 ? S::DTN : 1) {
+        float o[S::F32 ? S::DTN : 4];
+#pragma unroll
+        for (int e = 0; e < (S::F32 ? S::DTN : 4); ++e) o[e] = l == 0.0f ? 0.0f : (S::F32 ? acc[e][r] : acc[d][r + e]) / l;
+        store_values(a.out, to + (S::F32 ? S::DTN * S::out_row(r, g) : 32 * d + S::out_row(r, g)), a.x_type, a.out_wide, o);
       }
   } else {
     const long long rec = kv_record<S>(a, u, row, head);
 #pragma unroll
-    for (int r = 0; r < S::AR; ++r)
+    for (int d = 0; d < S::DTN; ++d)
 #pragma unroll
-      for (int d = 0; d < S::DTN; ++d) a.part[rec * DIM + S::DTN * S::out_row(r, g) + d] = acc[d][r];
+      for (int r = 0; r < S::AR; ++r)
+        a.part[rec * DIM + (S::F32 ? S::DTN * S::out_row(r, g) + d : 32 * d + S::out_row(r, g))] = acc[d][r];
     if (g == 0) {
       a.state[2 * rec] = st.ref();
       a.state[2 * rec + 1] = l;

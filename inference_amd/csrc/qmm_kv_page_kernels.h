@@ -40,7 +40,8 @@ __device__ __forceinline__ void agent_barrier() {
 
 // x cos + rotate_half(x) sin of the rows, k and v to their pages. A thread has four values
 // of a head's first half and the four of the second that turn with them; head_dim / 8
-// threads a head, q's heads first, then k's, then v's. Bound by the rows' bytes.
+// threads a head, q's heads first, then k's, then v's. Bound by the rows' bytes: 2053 rows of 32
+// + 2 x 8 f32 heads of 128 into bf16 pages 19 us for 94 MB (17.6 at a copy's rate); one row 3.3 us, all of it latency.
 extern "C" __global__ void __launch_bounds__(256) qmm_kv_append_rows(qmm::KvAppend a) {
 #pragma clang fp contract(off)
   using namespace qmm;
@@ -378,7 +379,8 @@ __device__ __forceinline__ int kv_path(const KvAccept& a, int s, int base, int d
 // Position base + path[d] to base + d, a thread a 16-byte column of a layer's, side's and
 // head's rows. path[d] >= d and rises, so that no entry is on a row that an earlier one's goes
 // to: eight are read and then written. The lengths here too, unless another workgroup may yet
-// read them (lens_out null).
+// read them (lens_out null). 16 trees with 7 rows moved each in 32 layers of 8 bf16 heads of 128:
+// 5.4 us for 14.7 MB, of which the launch, the lists' round trips and one of the rows' are most.
 extern "C" __global__ void __launch_bounds__(256) qmm_kv_accept_rows(qmm::KvAccept a) {
   using namespace qmm;
   __shared__ long long from[64], to[64];
