@@ -571,9 +571,8 @@ int qmm_moe_ffn_scored(const void *x, int x_dtype, int64_t tokens, int64_t ldx, 
 
 /* ---------------------------------------------------------------------------
  * A key/value cache in pages, for several sequences that share pages, and the
- * operators over it. The reference engine keeps pages on the host's side of its
- * attention (crates/llm/candle-llm/src/primitives/paged_kv_cache.rs); these calls
- * have no counterpart there.
+ * operators over it. No kernel launcher of the reference does this (its engine has
+ * a paged cache of its own, crates/llm/candle-llm/src/primitives/paged_kv_cache.rs).
  *
  * Position j of a sequence is row j % page_size of page table[slot][j / page_size].
  * A page may stand in several table rows; refs[p] counts the entries that name page p

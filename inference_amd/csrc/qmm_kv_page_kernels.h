@@ -379,7 +379,7 @@ __device__ __forceinline__ int kv_path(const KvAccept& a, int s, int base, int d
 // Position base + path[d] to base + d, a thread a 16-byte column of a layer's, side's and
 // head's rows. path[d] >= d and rises, so that no entry is on a row that an earlier one's goes
 // to: eight are read and then written. The lengths here too, unless another workgroup may yet
-// read them (lens_out null). 16 trees with 7 rows moved each in 32 layers of 8 bf16 heads of 128:
+// read them (lens_out null). 16 trees with 8 rows accepted each in 32 layers of 8 bf16 heads of 128:
 // 5.4 us for 14.7 MB, of which the launch, the lists' round trips and one of the rows' are most.
 extern "C" __global__ void __launch_bounds__(256) qmm_kv_accept_rows(qmm::KvAccept a) {
   using namespace qmm;
