@@ -174,11 +174,10 @@ struct KvCompact {
   int32_t *map, *refs, *moves;
 };
 
-int kv_copy_pages(Device* d, KvCache c, const int32_t* moves, int64_t most, hipStream_t s) {
-  // (as many workgroups as fill the chip; how many copies there are is known on the device alone)
-  const int64_t items = most * c.layers * 2 * c.kv_heads;
-  void* args[] = {&c, &moves};
-  return kv_launch(d, "qmm_kv_copy_pages", (unsigned)std::min<int64_t>(items, 8LL * d->num_cu), 1, 256, s, args);
+// Workgroups for up to `most` page copies: as many as fill the chip (how many copies there are is known on the device
+// alone).
+unsigned kv_copy_grid(const Device* d, const KvCache& c, int64_t most) {
+  return (unsigned)std::min<int64_t>(most * c.layers * 2 * c.kv_heads, 8LL * d->num_cu);
 }
 
 // Workgroups of 256 for n elements, at most a few a CU.
@@ -348,14 +347,17 @@ int qmm_kv_fork(const qmm_kv_cache* cache, const int32_t* parents, const int32_t
   const int64_t n = std::max<int64_t>(cells, cache->pages);
   if (cells + 4 * (cache->pages + cache->slots) <= kKvForkSmall) {
     QMM_TRY(kv_launch(d, "qmm_kv_fork_small", 1, 1, 1024, s, args));
+    if (reserve == 0) return QMM_OK;  // nothing is about to be written: no copies
+    void* copy[] = {&f.c, &f.moves};
+    return kv_launch(d, "qmm_kv_copy_pages", kv_copy_grid(d, f.c, cache->slots), 1, 256, s, copy);
   } else {
     QMM_TRY(kv_launch(d, "qmm_kv_fork_begin", kv_grid(d, n), 1, 256, s, args));
     QMM_TRY(kv_launch(d, "qmm_kv_fork_count", kv_grid(d, 64LL * cache->slots), 1, 256, s, args));
     QMM_TRY(kv_launch(d, "qmm_kv_fork_plan", 1, 1, 1024, s, args));
-    QMM_TRY(kv_launch(d, "qmm_kv_fork_commit", kv_grid(d, n), 1, 256, s, args));
+    int lists = (int)kv_grid(d, n);
+    void* last[] = {&f, &lists};
+    return kv_launch(d, "qmm_kv_fork_commit", lists + (reserve ? kv_copy_grid(d, f.c, cache->slots) : 0), 1, 256, s, last);
   }
-  if (reserve == 0) return QMM_OK;  // nothing is about to be written: no copies
-  return kv_copy_pages(d, f.c, f.moves, cache->slots, s);
 }
 
 int qmm_kv_accept(const qmm_kv_cache* cache, const int32_t* path, int64_t ld_path, const int32_t* counts,
@@ -407,8 +409,9 @@ int qmm_kv_compact(const qmm_kv_cache* cache, int32_t* table_out, int32_t* refs_
   const hipStream_t s = (hipStream_t)stream;
   void* args[] = {&k};
   QMM_TRY(kv_launch(d, "qmm_kv_compact_plan", 1, 1, 1024, s, args));
-  QMM_TRY(kv_launch(d, "qmm_kv_compact_commit", kv_grid(d, std::max<int64_t>((int64_t)cache->slots * cache->max_pages, cache->pages)), 1, 256, s, args));
-  return kv_copy_pages(d, k.c, k.moves, cache->pages / 2 + 1, s);
+  int lists = (int)kv_grid(d, std::max<int64_t>((int64_t)cache->slots * cache->max_pages, cache->pages));
+  void* last[] = {&k, &lists};
+  return kv_launch(d, "qmm_kv_compact_commit", lists + kv_copy_grid(d, k.c, cache->pages / 2 + 1), 1, 256, s, last);
 }
 
 static int beam_shape(int64_t batch, int beams, int64_t vocab, int count) {

@@ -279,8 +279,29 @@ __device__ __forceinline__ void kv_fork_commit(const KvFork& f, long long t, lon
     if (lane == 0) f.lens_out[s] = g.len;
   }
 }
+// The listed pages' first rows (a whole page: rows = page size) to other pages, in every layer
+// and of every kv head. Sources and destinations are disjoint. A workgroup takes a head's rows
+// of a page, side and layer at a time. Bound by the bytes: 512 of 2048 pages of 32 KB moved in 8
+// layers 105 us for 537 MB there and back (16 KB at a time over the heads, four loads a thread
+// in flight: 107, and for half-filled pages of 64 rows 41 us against 29).
+__device__ __forceinline__ void kv_copy_pages(const KvCache& c, const int* moves, long long first, long long step) {
+  const long long items = (long long)moves[0] * c.layers * 2 * c.kv_heads;
+  for (long long i = first; i < items; i += step) {
+    const int g = (int)(i % c.kv_heads), side = (int)(i / c.kv_heads % 2);
+    const int layer = (int)(i / (2 * c.kv_heads) % c.layers);
+    const int* m = moves + 1 + 3 * (i / (2LL * c.kv_heads * c.layers));
+    char* pool = (char*)(side ? c.v : c.k);
+    const u32x4* src = (const u32x4*)(pool + (c.row(layer, m[0], g, 0) << c.esize_log()));
+    u32x4* dst = (u32x4*)(pool + (c.row(layer, m[1], g, 0) << c.esize_log()));
+    const int n = (m[2] * c.head_dim << c.esize_log()) / 16;
+    for (int x = threadIdx.x; x < n; x += 256) dst[x] = src[x];
+  }
+}
 }  // namespace qmm
 
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_copy_pages(qmm::KvCache c, const int* moves) {
+  qmm::kv_copy_pages(c, moves, blockIdx.x, gridDim.x);
+}
 extern "C" __global__ void __launch_bounds__(256) qmm_kv_fork_begin(qmm::KvFork f) {
   qmm::kv_fork_begin(f, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
 }
@@ -291,8 +312,13 @@ extern "C" __global__ void __launch_bounds__(1024) qmm_kv_fork_plan(qmm::KvFork 
   __shared__ int lds[16];
   qmm::kv_fork_plan(f, lds);
 }
-extern "C" __global__ void __launch_bounds__(256) qmm_kv_fork_commit(qmm::KvFork f) {
-  qmm::kv_fork_commit(f, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
+// The lists by the first `lists` workgroups and the copies by the others, neither of which reads
+// what the other writes (128 slots of four prompts in 8 layers 52.0 us, in two launches 55.2).
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_fork_commit(qmm::KvFork f, int lists) {
+  if (blockIdx.x < (unsigned)lists)
+    qmm::kv_fork_commit(f, blockIdx.x * 256LL + threadIdx.x, lists * 256LL);
+  else
+    qmm::kv_copy_pages(f.c, f.moves, blockIdx.x - lists, gridDim.x - lists);
 }
 
 // All phases of a small fork in one workgroup, its lists in LDS: launches and round trips to
@@ -319,26 +345,6 @@ extern "C" __global__ void __launch_bounds__(1024) qmm_kv_fork_small(qmm::KvFork
   kv_fork_plan(f, lds);
   agent_barrier();
   kv_fork_commit(f, t, 1024);
-}
-
-// The listed pages' first rows (a whole page: rows = page size) to other pages, in every layer
-// and of every kv head. Sources and destinations are disjoint. A workgroup takes a head's rows
-// of a page, side and layer at a time. Bound by the bytes: 512 of 2048 pages of 32 KB moved in 8
-// layers 105 us for 537 MB there and back (16 KB at a time over the heads, four loads a thread
-// in flight: 107, and for half-filled pages of 64 rows 41 us against 29).
-extern "C" __global__ void __launch_bounds__(256) qmm_kv_copy_pages(qmm::KvCache c, const int* moves) {
-  using namespace qmm;
-  const long long items = (long long)moves[0] * c.layers * 2 * c.kv_heads;
-  for (long long i = blockIdx.x; i < items; i += gridDim.x) {
-    const int g = (int)(i % c.kv_heads), side = (int)(i / c.kv_heads % 2);
-    const int layer = (int)(i / (2 * c.kv_heads) % c.layers);
-    const int* m = moves + 1 + 3 * (i / (2LL * c.kv_heads * c.layers));
-    char* pool = (char*)(side ? c.v : c.k);
-    const u32x4* src = (const u32x4*)(pool + (c.row(layer, m[0], g, 0) << c.esize_log()));
-    u32x4* dst = (u32x4*)(pool + (c.row(layer, m[1], g, 0) << c.esize_log()));
-    const int n = (m[2] * c.head_dim << c.esize_log()) / 16;
-    for (int x = threadIdx.x; x < n; x += 256) dst[x] = src[x];
-  }
 }
 
 // ---------------------------------------------------------------------------
@@ -496,9 +502,14 @@ extern "C" __global__ void __launch_bounds__(1024) qmm_kv_compact_plan(qmm::KvCo
   }
 }
 
-extern "C" __global__ void __launch_bounds__(256) qmm_kv_compact_commit(qmm::KvCompact k) {
+// The lists and the copies, as a fork's.
+extern "C" __global__ void __launch_bounds__(256) qmm_kv_compact_commit(qmm::KvCompact k, int lists) {
   using namespace qmm;
-  const long long n = gridDim.x * 256LL, t = blockIdx.x * 256LL + threadIdx.x;
+  if (blockIdx.x >= (unsigned)lists) {
+    kv_copy_pages(k.c, k.moves, blockIdx.x - lists, gridDim.x - lists);
+    return;
+  }
+  const long long n = lists * 256LL, t = blockIdx.x * 256LL + threadIdx.x;
   for (long long p = t; p < k.c.pages; p += n) k.refs_out[p] = k.refs[p];
   const long long cells = (long long)k.c.slots * k.c.max_pages;
   for (long long i = t; i < cells; i += n) {

@@ -184,7 +184,7 @@ def check_pages(so):
     c = h.cache()
     assert h.fork(c) == (0, ["qmm_kv_fork_small", "qmm_kv_copy_pages"])
     assert h.fork(c, reserve=0) == (0, ["qmm_kv_fork_small"])
-    assert h.fork(h.cache(pages=5000))[1][:4] == ["qmm_kv_fork_begin", "qmm_kv_fork_count", "qmm_kv_fork_plan", "qmm_kv_fork_commit"]
+    assert h.fork(h.cache(pages=5000))[1] == ["qmm_kv_fork_begin", "qmm_kv_fork_count", "qmm_kv_fork_plan", "qmm_kv_fork_commit"]
     need = h.L.qmm_kv_fork_workspace_size(ctypes.byref(c))
     assert h.fork(c, ws_bytes=need)[0] == 0
     refused(*(h.fork(c, **b) for b in (
@@ -197,7 +197,7 @@ def check_pages(so):
     refused(h.accept(c, lens=c.lens + 4), h.accept(c, lens=(1 << 46) + 8), h.accept(c, lens=(1 << 45) + 44))
     refused(h.accept(c, counts=None), h.accept(c, lens=None), h.accept(c, ld=0), h.accept(c, ld=(1 << 20) + 1))
     need = h.L.qmm_kv_compact_workspace_size(ctypes.byref(c))
-    assert h.compact(c, ws_bytes=need) == (0, ["qmm_kv_compact_plan", "qmm_kv_compact_commit", "qmm_kv_copy_pages"])
+    assert h.compact(c, ws_bytes=need) == (0, ["qmm_kv_compact_plan", "qmm_kv_compact_commit"])
     refused(h.compact(c, table=None), h.compact(c, refs=None), h.compact(c, used=None), h.compact(c, ws=None),
             h.compact(c, ws_bytes=need - 1), h.compact(c, ws=(1 << 48) + 2))
 
