@@ -607,7 +607,8 @@ typedef struct qmm_kv_cache {
  * (f32; both NULL: no rotation), k and v go to cache position lens[s] + j of the layer, rounded once
  * to its type, and the rotated q to q_out (q NULL: none; q_out may be q, and overlaps no row else). lens stays as it is.
  * x_dtype (q, k, v, q_out): QMM_F32, QMM_F16 or QMM_BF16. A row whose position is outside the tables
- * writes nothing; one past the slot's pages writes its q alone. Row strides in elements. */
+ * writes nothing; one past the slot's pages writes its q alone. Pages that are written are the slot's alone
+ * (qmm_kv_fork with a reserve sees to it). Row strides in elements. */
 int qmm_kv_append(const qmm_kv_cache *cache, int layer, const void *q, const void *k, const void *v, int x_dtype,
                   int64_t rows, int64_t ldq, int64_t ldk, int64_t ldv, const int32_t *starts, const int32_t *depths,
                   const float *cos_t, const float *sin_t, int64_t positions, void *q_out, int64_t ldqo, int heads,
@@ -659,7 +660,8 @@ int qmm_kv_accept(const qmm_kv_cache *cache, const int32_t *path, int64_t ld_pat
 
 /* Packs the pool: with U pages in use (refs != 0), those with ids from U on move, in order, to the free
  * ids below U (whole pages, every layer); the table's entries and the counts go with them, to table_out
- * and refs_out (they may be the cache's own). used[0] (device) = U. ws: qmm_kv_compact_workspace_size(cache)
+ * and refs_out (they may be the cache's own). used[0] (device) = U. A page that is counted but stands in no
+ * table row moves too, and its holder is not told: hold pages by the row of a slot. ws: qmm_kv_compact_workspace_size(cache)
  * bytes, 16-byte aligned. */
 size_t qmm_kv_compact_workspace_size(const qmm_kv_cache *cache);
 int qmm_kv_compact(const qmm_kv_cache *cache, int32_t *table_out, int32_t *refs_out, int32_t *used, void *ws,

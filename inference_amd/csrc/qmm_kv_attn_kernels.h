@@ -265,11 +265,12 @@ __device__ __forceinline__ float kv_load_q(const KvAttn& a, int row, int head, i
     a.wide ? load(four, std::true_type()) : load(four, std::false_type());
   else
     a.wide ? load(two, std::true_type()) : load(two, std::false_type());
-  if (a.scale < 0.0f) {
+  if (a.scale <= 0.0f) {  // (c = 0 would make NaN of the scores that are -inf: equal weights are products of zeros)
+    const float turn = a.scale < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
     for (int c = 0; c < S::STEPS; ++c)
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[c][e] = -x[c][e];
+      for (int e = 0; e < E; ++e) x[c][e] *= turn;
   }
   float down = 1.0f;
   if constexpr (S::TYPE == kTypeF16) {
@@ -303,7 +304,7 @@ __device__ __forceinline__ float kv_load_q(const KvAttn& a, int row, int head, i
         }
     }
   }
-  return fabsf(a.scale) * kLog2e * down;
+  return a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e * down;
 }
 
 // q where a workgroup keeps it: in registers, or in LDS (chunk c of part p of every lane).

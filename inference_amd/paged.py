@@ -182,8 +182,8 @@ class PagedKVCache:
                q: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
                sin: Optional[torch.Tensor] = None, depths: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
-        """Rotates a step's rows and appends their keys and values to the layer; returns the rotated q (`out`, which
-        may be q, or a new tensor). k, v: [rows, kv_heads, head_dim], q: [rows, heads, head_dim], one type. Sequence s
+        """Rotates a step's rows and appends their keys and values to the layer, into pages that are the slot's alone
+        (see ``fork``'s reserve); returns the rotated q (`out`, which may be q, or a new tensor). k, v: [rows, kv_heads, head_dim], q: [rows, heads, head_dim], one type. Sequence s
         has rows starts[s] .. starts[s + 1] - 1 (int32 [slots + 1]) at cache positions lens[s], lens[s] + 1, ...; row j
         is rotated at lens[s] + depths[row] (default: + j) by cos / sin (float32 [positions, head_dim]; None: not
         rotated). lens stays as it is: see ``accept``."""
@@ -303,7 +303,8 @@ class PagedKVCache:
 
     def compact(self, out=None) -> torch.Tensor:
         """Moves the pages in use to the lowest ids: afterwards pages from the returned number (int32 [1]) on are free
-        and hold nothing. table and refs follow, or go to out = (table, refs)."""
+        and hold nothing. table and refs follow, or go to out = (table, refs). A page that refs counts but no table row
+        names moves too: hold pages by the row of a slot."""
         dev = self.device
         table, refs = (self.table, self.refs) if out is None else out
         if out is not None:
