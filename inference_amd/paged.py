@@ -18,7 +18,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from .qmm import _DENSE, QMM_ERR_INVALID, QMM_OK, QmmError, _call, _device_of, _ptr, last_error, lib
+from .qmm import _DENSE, QMM_ERR_INVALID, QMM_OK, QmmError, _call, _device_of, _ptr, _raw_stream, last_error, lib
 
 
 class _Cache(ctypes.Structure):  # qmm_kv_cache
@@ -65,8 +65,13 @@ def _packed(t: torch.Tensor) -> bool:
     return t.shape[0] <= 1 or t.stride(0) >= n
 
 
+# The current device's index, which torch.cuda.current_device looks up behind a check of its own.
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _run(dev: torch.device, fn, *args) -> None:
-    status = _call(dev, fn, *args)
+    index = dev.index
+    status = fn(*args, _raw_stream(index)) if _device_now() == index else _call(dev, fn, *args)
     if status != QMM_OK:
         raise QmmError(status, last_error())
 
@@ -121,7 +126,7 @@ class PagedKVCache:
         _ints(refs, (pages,), dev, "refs")
         self._tensors, self.device = (k, v, table, lens, refs), dev
         self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = layers, pages, kv_heads, page_size, head_dim
-        self.slots, self.max_pages = slots, max_pages
+        self.slots, self.max_pages, self._starts = slots, max_pages, (slots + 1,)
         self._c = _Cache(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), pages,
                          _DENSE[k.dtype], layers, kv_heads, page_size, head_dim, slots, max_pages)
         self._p = ctypes.addressof(self._c)
@@ -172,7 +177,8 @@ class PagedKVCache:
     def _out(self, out: Optional[torch.Tensor], q: torch.Tensor) -> Tuple[torch.Tensor, int]:
         """Rows for a result like q (`out`, or new ones), and their stride."""
         if out is None:
-            return torch.empty(q.shape, dtype=q.dtype, device=q.device), q.shape[1] * q.shape[2]
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            return out, q.shape[1] * q.shape[2]
         o, ld = self._rows(out, q.shape[1], "out")
         if o.data_ptr() != out.data_ptr() or out.dtype != q.dtype or o.shape != q.shape:
             raise _bad(f"out must be rows like q, got {list(out.shape)} {out.dtype}")
@@ -188,13 +194,14 @@ class PagedKVCache:
         is rotated at lens[s] + depths[row] (default: + j) by cos / sin (float32 [positions, head_dim]; None: not
         rotated). lens stays as it is: see ``accept``."""
         dev = self.device
-        _within(layer, 0, self.layers - 1, "layer")
+        if not 0 <= layer < self.layers:
+            raise _bad(f"layer {layer} of {self.layers}")
         k, ldk = self._rows(k, self.kv_heads, "k")
         v, ldv = self._rows(v, self.kv_heads, "v")
         rows = k.shape[0]
         if v.shape[0] != rows or v.dtype != k.dtype:
             raise _bad(f"k and v must be rows of one type, got {list(k.shape)} {k.dtype}, {list(v.shape)} {v.dtype}")
-        _ints(starts, (self.slots + 1,), dev, "starts")
+        _ints(starts, self._starts, dev, "starts")
         if depths is not None:
             _ints(depths, (rows,), dev, "depths")
         positions = 0
@@ -229,10 +236,11 @@ class PagedKVCache:
         its own `out`, which may be q). max_rows bounds a sequence's rows (default: all, with masks 64 * words at most; rows
         past it are not written), max_len is about the longest lens + rows (default: the table's). scale: head_dim ** -0.5."""
         dev = self.device
-        _within(layer, 0, self.layers - 1, "layer")
+        if not 0 <= layer < self.layers:
+            raise _bad(f"layer {layer} of {self.layers}")
         q, ldq = self._rows(q, None, "q")
         rows, heads = q.shape[0], q.shape[1]
-        _ints(starts, (self.slots + 1,), dev, "starts")
+        _ints(starts, self._starts, dev, "starts")
         ldm = 0
         if masks is not None:
             if masks.dtype != torch.int64 or masks.device != dev or masks.dim() != 2 or masks.shape[0] != rows or \
@@ -278,7 +286,7 @@ class PagedKVCache:
             _ints(lens, (self.slots,), dev, "out's lens")
             _ints(refs, (self.pages,), dev, "out's refs")
         if shortage is None:
-            shortage = torch.empty(1, dtype=torch.int32, device=dev)
+            shortage = parents.new_empty(1)
         else:
             _ints(shortage, (1,), dev, "shortage")
         ws = torch.empty(self._fork_ws, dtype=torch.uint8, device=dev)
@@ -310,7 +318,7 @@ class PagedKVCache:
         if out is not None:
             _ints(table, (self.slots, self.max_pages), dev, "out's table")
             _ints(refs, (self.pages,), dev, "out's refs")
-        used = torch.empty(1, dtype=torch.int32, device=dev)
+        used = self.refs.new_empty(1)
         ws = torch.empty(self._compact_ws, dtype=torch.uint8, device=dev)
         _run(dev, lib().qmm_kv_compact, self._p, table.data_ptr(), refs.data_ptr(), used.data_ptr(), ws.data_ptr(),
              self._compact_ws)
