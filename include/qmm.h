@@ -677,7 +677,8 @@ int qmm_kv_compact(const qmm_kv_cache *cache, int32_t *table_out, int32_t *refs_
  * has one continuation, the token eos at its own score, and its logits are not read. out_finished (or NULL): 1 where the
  * parent was finished or the token is eos (eos -1: no token ends a beam; finished is then NULL). Where
  * fewer continuations than count have a probability, the rest have token -1, parent -1, score -inf. A NaN
- * logit or score counts as -inf, a +inf logit as the largest finite value. batch >= 1, beams 1 .. 64, count
+ * logit or score counts as -inf, a +inf logit as the largest finite value; a score below f32's range is chosen like
+ * any other and stored as -inf. batch >= 1, beams 1 .. 64, count
  * 1 .. 128, vocab 1 .. 2^20, batch * beams <= 65535. ws: qmm_beam_select_workspace_size(...) bytes, 16-byte aligned. */
 size_t qmm_beam_select_workspace_size(int64_t batch, int beams, int64_t vocab, int count);
 int qmm_beam_select(const void *logits, int dtype, int64_t ld, int64_t batch, int beams, int64_t vocab,

@@ -360,15 +360,17 @@ extern "C" __global__ void __launch_bounds__(256) qmm_beam_merge(qmm::BeamArgs a
     a.out_scores[o] = no ? -INFINITY : (float)x.s;
     if (a.out_finished) a.out_finished[o] = !no && (ended[x.beam] || token == a.eos);
   };
-  // (a rounding to f32 keeps the order, so what passes a bound as f32 holds the best)
+  // (a rounding to f32 keeps the order, so what passes a bound as f32 holds the best; scores below f32's range are the
+  // least of it, not none)
+  auto rounded = [&](const BeamBest& x) { return x.beam == kBeamNone ? -INFINITY : fmaxf((float)x.s, -3.402823466e38f); };
   float top = -INFINITY;
-  for (int l = t; l < lists; l += 256) top = fmaxf(top, (float)entry(l, 0).s);
+  for (int l = t; l < lists; l += 256) top = fmaxf(top, rounded(entry(l, 0)));
   const uint32_t least = max(block_bound<20, true>(beam_order(top), a.count, bounds), 1u);
   if (beam_order(top) >= least)
     for (int l = t; l < lists; l += 256)
       for (int i = 0; i < a.count; ++i) {
         const BeamBest x = entry(l, i);
-        if (beam_order((float)x.s) < least) break;
+        if (beam_order(rounded(x)) < least) break;
         const int at = atomicAdd(&passed, 1);
         if (at < kBeamRank) pass_s[at] = x.s, pass_key[at] = x.key, pass_beam[at] = x.beam;
       }

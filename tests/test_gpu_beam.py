@@ -166,3 +166,29 @@ def test_reorder_strides():
         assert torch.equal(out[:, 2:18], base[index.long(), off:off + 16]) and not out[:, :2].any() and not out[:, 18:].any()
     assert torch.equal(reorder_rows(base.t(), index), base.t()[index.long()])
     assert reorder_rows(base, index[:0]).shape == (0, 40)
+
+
+def test_scores_below_the_range_of_f32():
+    """Lowest values beside an infinite logit, or under a lowest score, have 64-bit scores below f32's: continuations all
+    the same, in both ways that a search's lists are merged (the last size here has more entries than are ranked). Their
+    f32 scores round to -inf."""
+    low, inf = torch.finfo(torch.float32).min, float("inf")
+    below = 0
+    for beams, count, vocab in ((1, 2, 2), (1, 5, 5000), (2, 9, 5000), (3, 64, 70), (1, 128, 128256)):
+        lg = torch.full((2 * beams, vocab), low)
+        lg[0, vocab // 2] = inf
+        lg[beams:, :2] = torch.tensor([1.0, 2.0])
+        for score in (-1.0, low):
+            sc = torch.full((2 * beams,), score)
+            sc[0] = -2.0
+            tokens, parents, out, _ = (x.cpu().numpy() for x in beam_select(lg.to(DEV), sc.to(DEV), beams, count))
+            want = paged.beam(lg.numpy(), sc.numpy(), beams, count)
+            np.testing.assert_array_equal(tokens, want[0])
+            np.testing.assert_array_equal(parents, want[1])
+            with np.errstate(over="ignore"):
+                near = want[2].astype(np.float32)
+            below += int((np.isneginf(near) & (tokens >= 0)).any())
+            np.testing.assert_array_equal(np.isneginf(out), np.isneginf(near))
+            fine = np.isfinite(near)
+            assert (np.abs(out[fine] - want[2][fine]) <= 2.0 ** -24 * np.abs(want[2][fine]) + 2.0 ** -29).all()
+    assert below >= 5
