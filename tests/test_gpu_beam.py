@@ -192,3 +192,18 @@ def test_scores_below_the_range_of_f32():
             fine = np.isfinite(near)
             assert (np.abs(out[fine] - want[2][fine]) <= 2.0 ** -24 * np.abs(want[2][fine]) + 2.0 ** -29).all()
     assert below >= 5
+
+
+def test_certain_tokens():
+    """A token of probability one leaves a score as it is, bit for bit: it ties with a beam that has ended."""
+    for vocab in (1, 300, 9000):
+        for value in (0.0, 5.5, -3.25, 1e30):
+            lg = torch.full((4, vocab), -float("inf"))
+            lg[:, vocab // 3] = value
+            sc = torch.tensor([-1.0, -1.0, -0.3, 0.0])
+            out = beam_select(lg.to(DEV), sc.to(DEV), 1, 1)[2]
+            assert torch.equal(out.cpu().view(-1), sc)
+            check(lg, sc, 2, 2, finished=[1, 0, 0, 0], eos=0)
+            check(lg, sc, 2, 2, finished=[0, 1, 0, 0], eos=0)
+            check(lg, torch.full((4,), -2.0), 4, 4, finished=[0, 1, 0, 1], eos=0)
+            check(lg, torch.full((4,), 0.0), 4, 3, finished=[1, 0, 0, 1], eos=0)
