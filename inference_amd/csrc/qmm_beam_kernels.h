@@ -305,7 +305,7 @@ extern "C" __global__ void __launch_bounds__(256) qmm_beam_merge(qmm::BeamArgs a
   for (int i = 0; i < 4; ++i) early[i] = all[(long long)min(t, lists - 1) * a.count + min(i, a.count - 1)];
   if (t < a.beams) {
     const float s = a.scores[row0 + t];
-    score[t] = s == s ? s : -INFINITY;
+    score[t] = s == s ? s + 0.0f : -INFINITY;  // (-0 is 0: the bound goes by bits)
     ended[t] = a.finished ? a.finished[row0 + t] : 0;
   }
   if (t == 0) passed = 0;

@@ -207,3 +207,16 @@ def test_certain_tokens():
             check(lg, sc, 2, 2, finished=[0, 1, 0, 0], eos=0)
             check(lg, torch.full((4,), -2.0), 4, 4, finished=[0, 1, 0, 1], eos=0)
             check(lg, torch.full((4,), 0.0), 4, 3, finished=[1, 0, 0, 1], eos=0)
+
+
+def test_scores_of_minus_zero():
+    """-0 and 0 are one score: the lower beam is first, whichever of them it has."""
+    lg, _ = inputs(7, 8, 300, "f32")
+    zero = torch.tensor([-0.0, 0.0, -0.0, 0.0])
+    for sc in (zero, -zero):
+        for count in (1, 2, 3, 4):
+            check(lg[:4], sc, 4, count, finished=[1] * 4, eos=3)
+            check(lg[:4], sc, 2, count, finished=[1] * 4, eos=0)
+    single = torch.zeros(4, 1)  # (one token, of probability one: scores stay as they are)
+    check(single, zero, 4, 2)
+    check(single, zero, 4, 3, finished=[1, 0, 0, 1], eos=0)
