@@ -271,7 +271,7 @@ int qmm_kv_attention(const qmm_kv_cache* cache, int layer, const void* q, int x_
   if (rows && (!q || !starts || !out)) return fail(QMM_ERR_INVALID, "null pointer");
   if (!std::isfinite(scale)) return fail(QMM_ERR_INVALID, "scale %g", scale);
   if (!kv_type(x_dtype)) return fail(QMM_ERR_INVALID, "row type %d (QMM_F32, QMM_F16 or QMM_BF16)", x_dtype);
-  if (masks && (ldm < 1 || ldm > (1 << 20) || (max_rows + 63) / 64 > ldm))
+  if (masks && (ldm < 1 || ldm > (1 << 20) || max_rows > 64 * ldm))
     return fail(QMM_ERR_INVALID, "masks of %lld words for %d rows a slot", (long long)ldm, max_rows);
   QMM_TRY(kv_stride(rows, ldq, (int64_t)heads * cache->head_dim, "q"));
   QMM_TRY(kv_stride(rows, ldo, (int64_t)heads * cache->head_dim, "out"));

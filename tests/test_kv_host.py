@@ -270,3 +270,16 @@ def test_cpu_tensors_are_refused():
         beam_select(torch.zeros(2, 10), torch.zeros(2), 2, 2)
     with pytest.raises(QmmError):
         reorder_rows(torch.zeros(2, 10), z)
+
+
+def check_masks(so):
+    h = Host(so)
+    c = h.cache()
+    for most in (2 ** 31 - 1, 2 ** 31 - 63, 2 ** 31 - 64):
+        refused(h.attention(c, masks=1 << 49, ldm=1, max_rows=most), h.attention(c, masks=1 << 49, ldm=1 << 20, max_rows=most))
+    assert h.attention(c, masks=1 << 49, ldm=1 << 20, max_rows=1 << 26)[0] == 0 and h.attention(c, max_rows=2 ** 31 - 1)[0] == 0
+
+
+@pytest.mark.parametrize("check", ["check_masks"])
+def test_host_refusals(runtime, check):
+    test_host(runtime, check)
