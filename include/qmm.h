@@ -641,7 +641,8 @@ int qmm_kv_attention(const qmm_kv_cache *cache, int layer, const void *q, int x_
  * a part-filled last page is about to be written: of the slots that have it as theirs, the lowest keeps it
  * where nobody else holds it, all others get a copy (its filled rows, of every layer). New pages are the
  * free ones with the lowest ids, in slot order, a slot's copy first.
- * The new lists go to table_out, lens_out and refs_out, which may be the cache's own. shortage[0] (device)
+ * The new lists go to table_out, lens_out and refs_out, each of which may be the cache's own list, and which overlap
+ * the cache's lists, each other, shortage and ws in no other way. shortage[0] (device)
  * is 0, or the number of pages that were missing (in the pool, or in a slot's max_pages): then the lists
  * go on unchanged and no page is written. ws: qmm_kv_fork_workspace_size(cache) bytes, 16-byte aligned. */
 size_t qmm_kv_fork_workspace_size(const qmm_kv_cache *cache);

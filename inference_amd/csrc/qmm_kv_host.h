@@ -119,6 +119,25 @@ struct KvAttn {
   float scale;
 };
 
+// Bytes that a call reads or writes (p null: none).
+struct KvBytes {
+  const void* p;
+  size_t n;
+};
+bool kv_meet(const KvBytes& a, const KvBytes& b) {
+  return a.p && b.p && (uintptr_t)a.p < (uintptr_t)b.p + b.n && (uintptr_t)b.p < (uintptr_t)a.p + a.n;
+}
+// A call's outputs lie apart from each other and from its inputs; output i may be input i itself.
+int kv_apart(std::initializer_list<KvBytes> outs, std::initializer_list<KvBytes> ins, const char* rule) {
+  for (const KvBytes* a = outs.begin(); a != outs.end(); ++a) {
+    for (const KvBytes* b = a + 1; b != outs.end(); ++b)
+      if (kv_meet(*a, *b)) return fail(QMM_ERR_INVALID, "%s", rule);
+    for (const KvBytes* b = ins.begin(); b != ins.end(); ++b)
+      if (kv_meet(*a, *b) && !(a - outs.begin() == b - ins.begin() && a->p == b->p)) return fail(QMM_ERR_INVALID, "%s", rule);
+  }
+  return QMM_OK;
+}
+
 // How an attention's rows and positions are split. form 0, 1: one tile of 16 or 32 columns (rows
 // x heads of a kv head) a slot, 2: groups of four tiles of 32. `splits` chunks of a slot's
 // positions at most, of `chunk` (a multiple of 128) or more.
@@ -330,11 +349,16 @@ int qmm_kv_fork(const qmm_kv_cache* cache, const int32_t* parents, const int32_t
   if (!parents || !table_out || !lens_out || !refs_out || !shortage) return fail(QMM_ERR_INVALID, "null pointer");
   if (reserve < 0 || reserve > cache->max_pages * cache->page_size)
     return fail(QMM_ERR_INVALID, "reserve of %d positions (0 .. max_pages * page_size)", reserve);
-  QMM_TRY(kv_workspace(ws, ws_bytes, qmm_kv_fork_workspace_size(cache)));
+  const size_t need = qmm_kv_fork_workspace_size(cache), pages = (size_t)cache->pages, slots = (size_t)cache->slots;
+  const int64_t cells = (int64_t)cache->slots * cache->max_pages;
+  QMM_TRY(kv_workspace(ws, ws_bytes, need));
+  // (parents and keep are read before any list is written, but beside the workspace)
+  const char* const rule = "fork: the new lists may be the cache's own, and overlap them, each other, shortage and the workspace in no other way";
+  QMM_TRY(kv_apart({{table_out, 4 * (size_t)cells}, {lens_out, 4 * slots}, {refs_out, 4 * pages}, {shortage, 4}, {ws, need}},
+                   {{cache->table, 4 * (size_t)cells}, {cache->lens, 4 * slots}, {cache->refs, 4 * pages}}, rule));
+  QMM_TRY(kv_apart({{ws, need}}, {{nullptr, 0}, {parents, 4 * slots}, {keep, 4 * slots}}, "fork: the workspace overlaps parents or keep"));
   Device* d;
   QMM_TRY(current_device(&d));
-  const size_t pages = (size_t)cache->pages, slots = (size_t)cache->slots;
-  const int64_t cells = (int64_t)cache->slots * cache->max_pages;
   uint8_t* p = (uint8_t*)ws;
   f.parents = parents, f.keep = keep, f.reserve = reserve;
   f.table_out = table_out, f.lens_out = lens_out, f.refs_out = refs_out, f.shortage = shortage;

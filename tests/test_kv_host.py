@@ -280,6 +280,33 @@ def check_masks(so):
     assert h.attention(c, masks=1 << 49, ldm=1 << 20, max_rows=1 << 26)[0] == 0 and h.attention(c, max_rows=2 ** 31 - 1)[0] == 0
 
 
-@pytest.mark.parametrize("check", ["check_masks"])
+def check_fork_lists(so):
+    h = Host(so)
+    c = h.cache(slots=4, max_pages=8, pages=16)
+    need = h.L.qmm_kv_fork_workspace_size(ctypes.byref(c))
+    other = dict(table=1 << 50, lens=1 << 51, refs=1 << 52, ws_bytes=need)
+    assert h.fork(c)[0] == 0 and h.fork(c, **other)[0] == 0
+    # each new list may be the cache's own, and they may differ in that; parents and keep are read first
+    for own in ("table", "lens", "refs"):
+        assert h.fork(c, **{**other, own: getattr(c, own)})[0] == 0
+    assert h.fork(c, parents=c.lens, keep=c.lens)[0] == 0 and h.fork(c, keep=1 << 51, **other)[0] == 0
+    # lists end to end
+    assert h.fork(c, table=c.table + 128, lens=c.lens + 16, refs=c.refs - 64)[0] == 0
+    for out, size in (("table", 128), ("lens", 16), ("refs", 64), ("short", 4)):
+        for name in ("table", "lens", "refs"):
+            if name != out:
+                refused(h.fork(c, **{out: getattr(c, name)}))
+            refused(h.fork(c, **{out: getattr(c, name) + 4}))
+            if size > 4:
+                refused(h.fork(c, **{out: getattr(c, name) - 4}))
+        for b, at in (("table", 1 << 50), ("lens", 1 << 51), ("refs", 1 << 52), ("short", 1 << 46), ("ws", 1 << 47)):
+            if b != out:
+                refused(h.fork(c, **{**other, "ws_bytes": need, out: at}))
+        refused(h.fork(c, **{**other, out: (1 << 47) + need - 4}))
+    for at in (c.table, c.lens, c.refs, 1 << 45, 1 << 49):
+        refused(h.fork(c, keep=1 << 49, ws=at), h.fork(c, keep=1 << 49, ws=at - 16 * (need // 16) + 16, ws_bytes=need))
+
+
+@pytest.mark.parametrize("check", ["check_masks", "check_fork_lists"])
 def test_host_refusals(runtime, check):
     test_host(runtime, check)
