@@ -661,7 +661,8 @@ int qmm_kv_accept(const qmm_kv_cache *cache, const int32_t *path, int64_t ld_pat
 
 /* Packs the pool: with U pages in use (refs != 0), those with ids from U on move, in order, to the free
  * ids below U (whole pages, every layer); the table's entries and the counts go with them, to table_out
- * and refs_out (they may be the cache's own). used[0] (device) = U. A page that is counted but stands in no
+ * and refs_out (each may be the cache's own, and overlaps the cache's lists, the other, used and ws in no other way).
+ * used[0] (device) = U. A page that is counted but stands in no
  * table row moves too, and its holder is not told: hold pages by the row of a slot. ws: qmm_kv_compact_workspace_size(cache)
  * bytes, 16-byte aligned. */
 size_t qmm_kv_compact_workspace_size(const qmm_kv_cache *cache);

@@ -423,10 +423,14 @@ int qmm_kv_compact(const qmm_kv_cache* cache, int32_t* table_out, int32_t* refs_
   KvCompact k = {};
   QMM_TRY(kv_cache(cache, &k.c));
   if (!table_out || !refs_out || !used) return fail(QMM_ERR_INVALID, "null pointer");
-  QMM_TRY(kv_workspace(ws, ws_bytes, qmm_kv_compact_workspace_size(cache)));
+  const size_t need = qmm_kv_compact_workspace_size(cache), pages = (size_t)cache->pages, slots = (size_t)cache->slots;
+  const size_t cells = slots * (size_t)cache->max_pages;
+  QMM_TRY(kv_workspace(ws, ws_bytes, need));
+  QMM_TRY(kv_apart({{table_out, 4 * cells}, {refs_out, 4 * pages}, {used, 4}, {ws, need}},
+                   {{cache->table, 4 * cells}, {cache->refs, 4 * pages}, {nullptr, 0}, {nullptr, 0}, {cache->lens, 4 * slots}},
+                   "compact: the new lists may be the cache's own, and overlap them, each other, used and the workspace in no other way"));
   Device* d;
   QMM_TRY(current_device(&d));
-  const size_t pages = (size_t)cache->pages;
   uint8_t* p = (uint8_t*)ws;
   k.table_out = table_out, k.refs_out = refs_out, k.used = used;
   k.map = kv_take<int32_t>(p, pages), k.refs = kv_take<int32_t>(p, pages), k.moves = kv_take<int32_t>(p, 1 + 3 * (pages / 2 + 1));

@@ -307,6 +307,27 @@ def check_fork_lists(so):
         refused(h.fork(c, keep=1 << 49, ws=at), h.fork(c, keep=1 << 49, ws=at - 16 * (need // 16) + 16, ws_bytes=need))
 
 
-@pytest.mark.parametrize("check", ["check_masks", "check_fork_lists"])
+def check_compact_lists(so):
+    h = Host(so)
+    c = h.cache(slots=4, max_pages=8, pages=16)
+    need = h.L.qmm_kv_compact_workspace_size(ctypes.byref(c))
+    assert h.compact(c)[0] == 0 and h.compact(c, table=c.table)[0] == 0 and h.compact(c, refs=c.refs)[0] == 0
+    assert h.compact(c, table=c.table, refs=c.refs, used=c.refs + 64, ws=(1 << 48), ws_bytes=need)[0] == 0
+    for out, size in (("table", 128), ("refs", 64), ("used", 4)):
+        for name in ("table", "lens", "refs"):
+            if name != out:
+                refused(h.compact(c, **{out: getattr(c, name)}))
+            refused(h.compact(c, **{out: getattr(c, name) + 4}))
+            if size > 4:
+                refused(h.compact(c, **{out: getattr(c, name) - 4}))
+        for b, at in (("table", 1 << 45), ("refs", 1 << 46), ("used", 1 << 47), ("ws", 1 << 48)):
+            if b != out:
+                refused(h.compact(c, ws_bytes=need, **{out: at}))
+        refused(h.compact(c, ws_bytes=need, **{out: (1 << 48) + need - 4}))
+    for at in (c.table, c.lens, c.refs):
+        refused(h.compact(c, ws=at))
+
+
+@pytest.mark.parametrize("check", ["check_masks", "check_fork_lists", "check_compact_lists"])
 def test_host_refusals(runtime, check):
     test_host(runtime, check)
