@@ -652,7 +652,7 @@ int qmm_kv_fork(const qmm_kv_cache *cache, const int32_t *parents, const int32_t
 
 /* The accepted path of a step's rows: for d < counts[s], the key and value rows of position lens[s] +
  * path[s][d] move to position lens[s] + d in every layer, and lens_out[s] (it may be the cache's lens)
- * becomes lens[s] + counts[s] (lens_out may be counts too). path: int32 [slots][ld_path], increasing; a path ends early at an entry
+ * becomes lens[s] + counts[s] (lens_out may be counts too, and overlaps no list otherwise). path: int32 [slots][ld_path], increasing; a path ends early at an entry
  * that is not above the one before, below 0, or whose page or position the slot does not have, and at
  * ld_path, and then counts as that much shorter. path NULL: each row stays (a run whose first counts[s]
  * rows are accepted). The pages that are written must be the slot's alone (qmm_kv_fork with a reserve). */

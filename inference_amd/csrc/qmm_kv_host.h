@@ -393,8 +393,9 @@ int qmm_kv_accept(const qmm_kv_cache* cache, const int32_t* path, int64_t ld_pat
   auto meets = [&](const void* p, uintptr_t n) { return p && out < (uintptr_t)p + n && (uintptr_t)p < out + lens; };
   if (path && (ld_path < 1 || ld_path > (1 << 20))) return fail(QMM_ERR_INVALID, "paths of %lld entries (1 .. 2^20)", (long long)ld_path);
   if ((lens_out != cache->lens && meets(cache->lens, lens)) || (lens_out != counts && meets(counts, lens)) ||
-      meets(path, lens * (uintptr_t)ld_path))
-    return fail(QMM_ERR_INVALID, "lens_out overlaps the lengths, the counts (it may be either itself) or the paths");
+      meets(path, lens * (uintptr_t)ld_path) || meets(cache->table, lens * (uintptr_t)cache->max_pages) ||
+      meets(cache->refs, 4 * (uintptr_t)cache->pages))
+    return fail(QMM_ERR_INVALID, "lens_out overlaps the lengths, the counts (it may be either itself), the paths or the pages' lists");
   Device* d;
   QMM_TRY(current_device(&d));
   a.path = path, a.counts = counts, a.lens_out = lens_out, a.ld_path = ld_path, a.max_path = (int)ld_path;

@@ -328,6 +328,15 @@ def check_compact_lists(so):
         refused(h.compact(c, ws=at))
 
 
-@pytest.mark.parametrize("check", ["check_masks", "check_fork_lists", "check_compact_lists"])
+def check_accept_lists(so):
+    h = Host(so)
+    c = h.cache(slots=4, max_pages=8, pages=16)
+    for path in (1 << 45, None):
+        assert h.accept(c, path=path, lens=c.table + 128)[0] == 0 and h.accept(c, path=path, lens=c.refs - 16)[0] == 0
+        refused(h.accept(c, path=path, lens=c.table), h.accept(c, path=path, lens=c.table + 124),
+                h.accept(c, path=path, lens=c.refs + 60), h.accept(c, path=path, lens=c.refs - 4))
+
+
+@pytest.mark.parametrize("check", ["check_masks", "check_fork_lists", "check_compact_lists", "check_accept_lists"])
 def test_host_refusals(runtime, check):
     test_host(runtime, check)
