@@ -681,7 +681,9 @@ int qmm_kv_compact(const qmm_kv_cache *cache, int32_t *table_out, int32_t *refs_
  * fewer continuations than count have a probability, the rest have token -1, parent -1, score -inf. A NaN
  * logit or score counts as -inf, a +inf logit as the largest finite value; a score below f32's range is chosen like
  * any other and stored as -inf. batch >= 1, beams 1 .. 64, count
- * 1 .. 128, vocab 1 .. 2^20, batch * beams <= 65535. ws: qmm_beam_select_workspace_size(...) bytes, 16-byte aligned. */
+ * 1 .. 128, vocab 1 .. 2^20, batch * beams <= 65535. The results overlap
+ * neither each other nor ws nor what is read, except that out_scores may be scores and out_finished may be finished
+ * where count == beams. ws: qmm_beam_select_workspace_size(...) bytes, 16-byte aligned. */
 size_t qmm_beam_select_workspace_size(int64_t batch, int beams, int64_t vocab, int count);
 int qmm_beam_select(const void *logits, int dtype, int64_t ld, int64_t batch, int beams, int64_t vocab,
                     const float *scores, const int32_t *finished, int eos, int count, int32_t *tokens,

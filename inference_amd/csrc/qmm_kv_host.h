@@ -467,10 +467,20 @@ int qmm_beam_select(const void* logits, int dtype, int64_t ld, int64_t batch, in
   if (eos < -1 || eos >= vocab) return fail(QMM_ERR_INVALID, "end token %d of %lld tokens (-1: none)", eos, (long long)vocab);
   if (finished && eos < 0) return fail(QMM_ERR_INVALID, "finished beams need an end token");
   QMM_TRY(kv_stride(batch * beams, ld, vocab, "logits"));
-  QMM_TRY(kv_workspace(ws, ws_bytes, qmm_beam_select_workspace_size(batch, beams, vocab, count)));
+  const size_t need = qmm_beam_select_workspace_size(batch, beams, vocab, count);
+  QMM_TRY(kv_workspace(ws, ws_bytes, need));
+  const size_t rows = (size_t)(batch * beams), slices = ceil_div(vocab, kBeamSlice), out = 4 * (size_t)batch * (size_t)count;
+  // (a search's workgroup reads its own beams' scores and ends before it writes: in place where it writes as many)
+  const bool place = count == beams;
+  const KvBytes in_scores = {scores, 4 * rows}, in_ends = {finished, 4 * rows}, none = {nullptr, 0};
+  const KvBytes in_logits = {logits, (((rows - 1) * (size_t)(rows > 1 ? ld : 0)) + (size_t)vocab) * kv_esize(dtype)};
+  const char* const rule = "beam selection: results overlap each other, the workspace or what is read (scores and ends may change in place "
+                           "where count is beams)";
+  QMM_TRY(kv_apart({{out_scores, out}, {out_finished, out}, {tokens, out}, {parents, out}, {ws, need}},
+                   {place ? in_scores : none, place ? in_ends : none, none, none, none, in_logits, in_scores.p == out_scores && place ? none : in_scores,
+                    in_ends.p == out_finished && place ? none : in_ends}, rule));
   Device* d;
   QMM_TRY(current_device(&d));
-  const size_t rows = (size_t)(batch * beams), slices = ceil_div(vocab, kBeamSlice);
   uint8_t* p = (uint8_t*)ws;
   BeamArgs a = {};
   a.logits = logits, a.ld = ld, a.scores = scores, a.finished = finished;

@@ -337,6 +337,29 @@ def check_accept_lists(so):
                 h.accept(c, path=path, lens=c.refs + 60), h.accept(c, path=path, lens=c.refs - 4))
 
 
-@pytest.mark.parametrize("check", ["check_masks", "check_fork_lists", "check_compact_lists", "check_accept_lists"])
+def check_beam_outputs(so):
+    h = Host(so)
+    base = dict(finished=1 << 51, eos=0, done=1 << 52)
+    assert h.beam(**base)[0] == 0
+    # in place where a search has as many continuations as beams
+    assert h.beam(count=4, **{**base, "out": 1 << 46, "done": 1 << 51})[0] == 0
+    refused(h.beam(**{**base, "out": 1 << 46}), h.beam(**{**base, "done": 1 << 51}))
+    need = h.L.qmm_beam_select_workspace_size(ctypes.c_int64(2), 4, ctypes.c_int64(1000), 4)
+    size = 2 * 4 * 4
+    logits = (1 << 45, 4 * 8 * 1000)
+    for out in ("tokens", "parents", "out", "done"):
+        for name, at, n in (("logits", *logits), ("scores", 1 << 46, size), ("finished", 1 << 51, size), ("tokens", 1 << 47, size),
+                            ("parents", 1 << 48, size), ("out", 1 << 49, size), ("done", 1 << 52, size), ("ws", 1 << 50, need)):
+            if name == out:
+                continue
+            for to in (at - size + 4, at + 4, at + n - 4) + (() if (out, name) in (("out", "scores"), ("done", "finished")) else (at,)):
+                refused(h.beam(count=4, **{**base, out: to}))
+            assert h.beam(count=4, ws_bytes=need, **{**base, out: at + n})[0] == 0 and h.beam(count=4, **{**base, out: at - size})[0] == 0
+    for at in (1 << 45, 1 << 46, 1 << 51, (1 << 45) + 31984):
+        refused(h.beam(count=4, **{**base, "ws": at}))
+    assert h.beam(count=4, **{**base, "ws": (1 << 45) + 32000})[0] == 0
+
+
+@pytest.mark.parametrize("check", ["check_masks", "check_fork_lists", "check_compact_lists", "check_accept_lists", "check_beam_outputs"])
 def test_host_refusals(runtime, check):
     test_host(runtime, check)
