@@ -477,8 +477,8 @@ int qmm_beam_select(const void* logits, int dtype, int64_t ld, int64_t batch, in
   const char* const rule = "beam selection: results overlap each other, the workspace or what is read (scores and ends may change in place "
                            "where count is beams)";
   QMM_TRY(kv_apart({{out_scores, out}, {out_finished, out}, {tokens, out}, {parents, out}, {ws, need}},
-                   {place ? in_scores : none, place ? in_ends : none, none, none, none, in_logits, in_scores.p == out_scores && place ? none : in_scores,
-                    in_ends.p == out_finished && place ? none : in_ends}, rule));
+                   {place ? in_scores : none, place ? in_ends : none, none, none, none, in_logits, place ? none : in_scores,
+                    place ? none : in_ends}, rule));
   Device* d;
   QMM_TRY(current_device(&d));
   uint8_t* p = (uint8_t*)ws;
