@@ -233,8 +233,9 @@ class PagedKVCache:
         sequences: row j of sequence s sees the positions below lens[s], and lens[s] + i where bit i of its mask is
         set (int64 [rows, words], see tree_masks; None: i <= j). q: [rows, heads, head_dim]; the result is of its
         shape and type, a row that sees nothing is zeros (rows of no sequence are not written: a padded batch brings
-        its own `out`, which may be q). max_rows bounds a sequence's rows (default: all, with masks 64 * words at most; rows
-        past it are not written), max_len is about the longest lens + rows (default: the table's). scale: head_dim ** -0.5."""
+        its own `out`, which may be q). max_rows bounds a sequence's rows (at most 64 * words with masks; rows past it are
+        not written; default: all, or as many as the masks have bits, and rows past those are zeros in a new result),
+        max_len is about the longest lens + rows (default: the table's). scale: head_dim ** -0.5."""
         dev = self.device
         if not 0 <= layer < self.layers:
             raise _bad(f"layer {layer} of {self.layers}")
@@ -248,13 +249,18 @@ class PagedKVCache:
                 raise _bad(f"masks must be contiguous int64 [{rows}, words] on {dev}, got {masks.dtype} "
                            f"{list(masks.shape)} on {masks.device}")
             ldm = masks.shape[1]
-        max_rows = max(1, rows) if max_rows is None else min(max_rows, max(1, rows))
+        given = max_rows
+        max_rows = max(1, rows) if given is None else min(given, max(1, rows))
         most = self.max_pages * self.page_size
         max_len = most if max_len is None else min(max_len, most)
         if max_rows < 1 or max_len < 1:
             raise _bad(f"max_rows {max_rows}, max_len {max_len}")
-        if masks is not None:
-            max_rows = min(max_rows, 64 * ldm)
+        if masks is not None and max_rows > 64 * ldm:
+            if given is not None or ldm == 0:
+                raise _bad(f"masks of {ldm} words for {max_rows} rows a sequence")
+            max_rows = 64 * ldm
+            if out is None:  # (rows past the masks' bits are left out)
+                out = torch.zeros(q.shape, dtype=q.dtype, device=dev)
         out, ldo = self._out(out, q)
         L = lib()
         key = (rows, max_rows, max_len, heads)

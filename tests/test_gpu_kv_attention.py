@@ -342,3 +342,29 @@ def test_two_graphs():
         assert torch.equal(c.attention(0, q, starts, **calls[1 - i]), want[1 - i])
         torch.cuda.synchronize()
         assert torch.equal(outs[i], want[i])
+
+
+def test_masks_narrower_than_the_step():
+    """A bound past the masks' bits is refused; without one, the rows past the bits of a sequence are zeros in a new
+    result and stay in a given one."""
+    lens, rows = [20, 6], [70, 3]
+    c, q, starts, pools, table = step(15, lens, rows, 4, 2, 64, 16, "f32", "f32")
+    masks = torch.from_numpy(np.random.default_rng(15).integers(-2 ** 63, 2 ** 63, (73, 1)))
+    args = q.to(DEV), starts.to(DEV), masks.to(DEV)
+    for most in (65, 70, 73, 1000):
+        with pytest.raises(QmmError):
+            c.attention(0, *args, max_rows=most)
+    with pytest.raises(QmmError):
+        c.attention(0, *args[:2], masks=args[2][:, :0])
+    dirty = torch.full_like(args[0], 7.0)  # (what a new result's memory held)
+    del dirty
+    got = c.attention(0, *args)
+    out = torch.full_like(args[0], 7.0)
+    c.attention(0, *args, out=out)
+    assert not got[64:70].any() and (out[64:70] == 7).all()
+    keep = [r for r in range(73) if not 64 <= r < 70]
+    assert torch.equal(got[keep], out[keep])
+    want = out.clone()
+    want[64:70] = float("nan")
+    check(want, q, pools, table, lens, starts, masks, 0.125, max_rows=64)
+    assert torch.equal(c.attention(0, *args, max_rows=64, out=out)[keep], got[keep])
