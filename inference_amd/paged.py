@@ -189,10 +189,11 @@ class PagedKVCache:
                sin: Optional[torch.Tensor] = None, depths: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """Rotates a step's rows and appends their keys and values to the layer, into pages that are the slot's alone
-        (see ``fork``'s reserve); returns the rotated q (`out`, which may be q, or a new tensor). k, v: [rows, kv_heads, head_dim], q: [rows, heads, head_dim], one type. Sequence s
-        has rows starts[s] .. starts[s + 1] - 1 (int32 [slots + 1]) at cache positions lens[s], lens[s] + 1, ...; row j
-        is rotated at lens[s] + depths[row] (default: + j) by cos / sin (float32 [positions, head_dim]; None: not
-        rotated). lens stays as it is: see ``accept``."""
+        (see ``fork``'s reserve); returns the rotated q (`out`, which may be q, or a new tensor). k, v: [rows, kv_heads,
+        head_dim], q: [rows, heads, head_dim], one type. Sequence s has rows starts[s] .. starts[s + 1] - 1 (int32
+        [slots + 1]) at cache positions lens[s], lens[s] + 1, ...; row j is rotated at lens[s] + depths[row] (default:
+        + j) by cos / sin (float32 [positions, head_dim]; None: not rotated). Rows of no sequence and rows at positions
+        past the tables are not written: a padded batch brings its own `out`. lens stays as it is: see ``accept``."""
         dev = self.device
         if not 0 <= layer < self.layers:
             raise _bad(f"layer {layer} of {self.layers}")
