@@ -170,7 +170,7 @@ class PagedKVCache:
             x = x.unflatten(1, (-1, dim))
         if x.dim() != 3 or x.shape[2] != dim or (heads is not None and x.shape[1] != heads):
             raise _bad(f"{what} must be [rows, {heads or 'heads'}, {dim}], got {list(x.shape)}")
-        if x.stride(2) != 1 or x.stride(1) != dim or (x.shape[0] > 1 and x.stride(0) < x.shape[1] * dim):
+        if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != dim) or (x.shape[0] > 1 and x.stride(0) < x.shape[1] * dim):
             x = x.contiguous()
         return x, x.stride(0) if x.shape[0] > 1 else x.shape[1] * dim
 

@@ -368,3 +368,25 @@ def test_masks_narrower_than_the_step():
     want[64:70] = float("nan")
     check(want, q, pools, table, lens, starts, masks, 0.125, max_rows=64)
     assert torch.equal(c.attention(0, *args, max_rows=64, out=out)[keep], got[keep])
+
+
+def test_one_head_of_any_stride():
+    """A dimension of one head has no stride: rows, results and what is appended with such views."""
+    lens, rows = [40, 3], [2, 5]
+    c, q, starts, pools, table = step(16, lens, rows, 1, 1, 64, 16, "f32", "f32")
+    flat = torch.full((7, 200), 7.0, device=DEV)
+    view = flat[:, None, 8:72]
+    assert view.stride(1) != 64
+    view.copy_(q.to(DEV))
+    out = torch.full((7, 200), 9.0, device=DEV)
+    got = c.attention(0, view, starts.to(DEV), out=out[:, None, 4:68])
+    check(got, q, pools, table, lens, starts, None, 0.125)
+    assert (out[:, :4] == 9).all() and (out[:, 68:] == 9).all()
+    k, v = (torch.randn((7, 90), device=DEV)[:, None, 1:65] for _ in range(2))
+    turned = torch.full((7, 200), 9.0, device=DEV)
+    c.append(0, k, v, starts.to(DEV), q=view, out=turned[:, None, 100:164])
+    assert torch.equal(turned[:, None, 100:164], view)
+    for s in range(2):
+        for j in range(rows[s]):
+            t = lens[s] + j
+            assert torch.equal(c.v[0, int(table[s, t // 16]), 0, t % 16], v[int(starts[s]) + j, 0])
