@@ -4,18 +4,24 @@
 #include <hip/hip_runtime_api.h>
 
 #include <cstdint>
+#include <cstring>
 #include <deque>
 #include <string>
 #include <vector>
 
 static std::deque<std::string> names;
 static std::vector<const std::string*> launched;
+static std::deque<std::vector<char>> kept;  // the first argument of each launch
+static size_t keep_bytes = 0;
 static uintptr_t next_address = (uintptr_t)1 << 44;
 
 extern "C" {
 int host_launches() { return (int)launched.size(); }
 const char* host_launch(int i) { return launched[i]->c_str(); }
-void host_clear() { launched.clear(); }
+// From here on the first argument of each launch is kept, which has `bytes` bytes in all of them.
+void host_keep(size_t bytes) { keep_bytes = bytes; }
+const void* host_argument(int i) { return kept[i].data(); }
+void host_clear() { launched.clear(), kept.clear(); }
 
 hipError_t hipGetDevice(int* dev) { return *dev = 0, hipSuccess; }
 hipError_t hipSetDevice(int dev) { return dev ? hipErrorInvalidDevice : hipSuccess; }
@@ -45,7 +51,9 @@ hipError_t hipModuleGetFunction(hipFunction_t* f, hipModule_t, const char* name)
 }
 
 hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned, unsigned, unsigned, unsigned, unsigned, unsigned, unsigned,
-                                 hipStream_t, void**, void**) {
+                                 hipStream_t, void** args, void**) {
+  kept.emplace_back(keep_bytes);
+  if (keep_bytes) memcpy(kept.back().data(), args[0], keep_bytes);
   launched.push_back((const std::string*)f);
   return hipSuccess;
 }

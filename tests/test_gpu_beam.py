@@ -220,3 +220,26 @@ def test_scores_of_minus_zero():
     single = torch.zeros(4, 1)  # (one token, of probability one: scores stay as they are)
     check(single, zero, 4, 2)
     check(single, zero, 4, 3, finished=[1, 0, 0, 1], eos=0)
+
+
+def test_results_in_place():
+    """The C entry point's scores and ends in place, where a search has as many continuations as beams; elsewhere: refused."""
+    from inference_amd import qmm
+    L = qmm.lib()
+    for batch, beams, count in ((5, 4, 4), (1, 1, 1), (3, 64, 64), (2, 3, 4)):
+        rows = batch * beams
+        lg, sc = inputs(8 + beams, rows, 5000, "f32")
+        end = torch.zeros(rows, dtype=torch.int32)
+        end[::3] = 1
+        lg, sc, end = lg.to(DEV), sc.to(DEV), end.to(DEV)
+        want = beam_select(lg, sc, beams, count, finished=end, eos=7)
+        size = L.qmm_beam_select_workspace_size(batch, beams, 5000, count)
+        ws = torch.empty(size, dtype=torch.uint8, device=DEV)
+        tokens, parents = torch.empty((2, batch, count), dtype=torch.int32, device=DEV)
+        rc = L.qmm_beam_select(lg.data_ptr(), 0, 5000, batch, beams, 5000, sc.data_ptr(), end.data_ptr(), 7, count,
+                               tokens.data_ptr(), parents.data_ptr(), sc.data_ptr(), end.data_ptr(), ws.data_ptr(), size,
+                               qmm._stream(DEV))
+        assert (rc == 0) == (count == beams)
+        if rc == 0:
+            for a, b in zip(want, (tokens, parents, sc, end)):
+                assert torch.equal(a.view(-1), b.view(-1))
