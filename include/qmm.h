@@ -621,7 +621,8 @@ int qmm_kv_append(const qmm_kv_cache *cache, int layer, const void *q, const voi
  * kv_heads); a row that sees nothing gets zeros. What a row does not see does not reach it, not an
  * infinity or a NaN either. A position that the row sees and whose page the table does not name
  * gives NaN. Sums and softmax are held in 32 bits; a 16-bit cache is multiplied on the 16-bit
- * matrix cores, with q and the weights split into parts that keep their bits. out may be q (of one stride), and
+ * matrix cores, with q and the weights split into parts: for f32 rows they leave out up to 2^-21 of an operand (f16) or
+ * 2^-24 (bf16), for 16-bit rows up to 2^-16 of a weight, before the output's rounding. out may be q (of one stride), and
  * overlaps it in no other way. scale: any finite value.
  * heads % kv_heads == 0, heads / kv_heads <= 32. max_rows bounds the rows of a slot (rows past it
  * are left out), at most 64 ldm with masks; max_len is about the largest lens[s] + rows of s: it
@@ -674,7 +675,7 @@ int qmm_kv_compact(const qmm_kv_cache *cache, int32_t *table_out, int32_t *refs_
  * probabilities), the `count` best continuations of each search by
  *   scores[beam] + (logit - log sum exp(logits of the beam)),
  * best first; ties: the lower beam, then the lower token. Sums and scores are held in 64 bits, each
- * exponential to 2^-30 of its value; a beam's own continuations go by their logits. tokens, parents, out_scores: [batch][count]; a parent is a row of the
+ * exponential to 2^-34 of its value (that of the largest logit exactly); a beam's own continuations go by their logits. tokens, parents, out_scores: [batch][count]; a parent is a row of the
  * logits (search * beams + beam). finished (int32 [batch * beams], or NULL): a beam whose entry is not 0
  * has one continuation, the token eos at its own score, and its logits are not read. out_finished (or NULL): 1 where the
  * parent was finished or the token is eos (eos -1: no token ends a beam; finished is then NULL). Where

@@ -7,9 +7,9 @@
 // which are sorted, by their heads.
 //
 // 16 searches of 8 beams over 128256 bf16 logits, 16 continuations: slices 22.0 us for 32.8 MB (6.1 us at a copy's rate),
-// merge 7.5. Of the slices' time 6.4 us are the exponentials, 12.5 f64 instructions each at the f32 rate,
+// merge 7.7 (medians of a kernel trace). Of the slices' time 6.4 us are the exponentials, 12.5 f64 instructions each at the f32 rate,
 // 1.7 the ranking, the rest the first loads and the bound; slices twice as long, whose threads hold 32 logits,
-// took 32 us. 4 beams: 5.6 and 5.0 us, all of it latency.
+// took 32 us. 4 beams: 5.6 and 5.4 us, all of it latency.
 //
 // Scores of different beams are compared in 64 bits: two of them lie within an f32
 // rounding of each other (2^-20 at a score of -16) once in a few thousand selections, and
@@ -283,7 +283,9 @@ extern "C" __global__ void __launch_bounds__(256, 8) qmm_beam_slices_bf16(qmm::B
 // `count` best of the threads' best heads pass is one that as many continuations pass; a
 // thread takes what passes from the heads of its lists on, and places are counted as in a
 // slice (with a branch on equal scores the launch took 12.6 us, without 7.5: bf16 logits are
-// often equal). Where more than kBeamRank pass, the best head is taken `count` times.
+// often equal). Where more than kBeamRank pass, the best head is taken `count` times, a dependent
+// round each: so it is with fewer lists than `count`, whose heads give no bound (one beam of 32 slices: 64
+// continuations 119 us, 128 233).
 extern "C" __global__ void __launch_bounds__(256) qmm_beam_merge(qmm::BeamArgs a) {
   using namespace qmm;
   __shared__ double lse[64], total[64];

@@ -24,15 +24,17 @@
 // and share the keys, K and V through LDS, two tiles deep. A sequence's chunks are joined by a
 // second launch.
 //
-// What bounds them. 32 heads over 8, head_dim 128: one token of each of 24 sequences of up to 8000
-// positions, bf16: K and V's 411 MB, 79.6 us and 5.0 for the join (the bytes alone 77 at a copy's
-// rate). One token over 1500 f32 positions: 8.6 and 3.9 us, latency (launch, page ids, K, V, join). 8
-// trees of up to 26 nodes over up to 4000 bf16 positions with f32 rows: 40 and 7 us, where the bytes
-// take 14 and the products, three times over for the parts, 12 at a large product's rate: smaller trees
-// fill their tiles in part, and a chunk's beginning counts. 4 trees of 64 nodes over 30000 f16
-// positions: 250 and 14 us, the products 180 at that rate: the matrix cores are busy 42% of the time
-// and the vector ALUs half, in turn rather than at once (two waves a SIMD are all that the registers
-// and the LDS of 64-key tiles leave).
+// What bounds them (medians of a kernel trace). 32 heads over 8, head_dim 128: one token of each of 24
+// sequences of up to 8000 positions, bf16: K and V's 411 MB, 79.7 us and 5.0 for the join (the bytes alone
+// 77 at a copy's rate). One token over 1500 f32 positions: 8.6 and 4.2 us, latency (launch, page ids, K, V,
+// join). 8 trees of up to 26 nodes over up to 4000 bf16 positions with f32 rows: 40.4 and 7.4 us, where the
+// bytes take 14 and the products, three times over for the parts, 12 at a large product's rate: smaller
+// trees fill their tiles in part, waves without a row only load, and a chunk's beginning counts. 4 trees of
+// 64 nodes over 30000 f16 positions: 292 and 17 us (248 for both in a row of passes without the trace), the
+// products 180 at that rate: of the cycles in which a CU has work the matrix cores are busy in 47% and the
+// vector ALUs in 53%, in turn rather than at once (two waves a SIMD are all that the registers and the LDS
+// of 64-key tiles leave). A prompt of 2000 rows: 101 us in 16 bits, 489 in f32, the products 30 (45 with the
+// weights' parts) and 213; the f32 matrix cores are busy in 66% of those cycles.
 //
 // Pages. A tile's two halves of 16 positions each lie in one page (pages are 16 or more), so
 // a half is one buffer whose end is the last position there is: rows past it read as 0 and
@@ -40,11 +42,13 @@
 //
 // Types. An f32 cache runs on the f32 matrix cores. A 16-bit cache runs on the 16-bit ones,
 // 16 times their rate, with the f32 operand split into parts that each have the cache's
-// type: q (QP parts: as many as hold its bits) and the weights (PP parts: 3 of bf16, 2 of
-// f16 for an f32 output, which lose 2^-24 and 2^-22 of a weight; 2 of bf16 for a 16-bit
-// output, 2^-16 of a weight against its rounding's 2^-9). For f16, whose range is small,
-// a column's q is scaled by a power of two to [2^13, 2^14) and the weights by 2^12, which
-// divides out.
+// type. q: all of its bits, but for 2^-23 of an f32 value in the two parts of f16 (QP parts: 3
+// of bf16 or 2 of f16 for f32, 2 of bf16 for f16, else 1). The weights, in PP parts: 3 of bf16
+// for f32 rows lose 2^-24 of a weight; 2 of f16 lose up to 2^-21, toward zero; 2 of bf16 for
+// 16-bit rows lose 2^-16, where the output's own rounding is 2^-8 (bf16) or 2^-11: about one bf16
+// output in 500 is rounded the other way for it (as is one in 2000 by the order of f32 sums), and
+// the third part would cost half as many products again. For f16, whose range is small, a
+// column's q is scaled by a power of two to [2^13, 2^14) and the weights by 2^12, which divides out.
 //
 // What a column does not see has the score -inf and the weight 0, but 0 times an infinity or
 // a NaN of such a value row is NaN, as is a split infinity: a workgroup whose state is not
